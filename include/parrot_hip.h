@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define PARROT_ABI_VERSION 15
+#define PARROT_ABI_VERSION 16
 
 #define PARROT_OK 0
 #define PARROT_ERR_NULL_POINTER (-1)
@@ -802,6 +802,117 @@ int parrot_grouped_experts_static_bf16(const void* x, int64_t tokens, int32_t di
                                        const void* packed_gate_up, const void* down,
                                        const void* shared_gate_up, const void* shared_down,
                                        const void* addend, void* out, void* stream);
+
+/* ---- Generation over a paged KV cache ---------------------------------- */
+
+/* What a cache's pages hold. */
+#define PARROT_PAGED_BF16 0
+#define PARROT_PAGED_E4M3 1 /* OCP e4m3 (no infinities) */
+#define PARROT_PAGED_INT8 2
+
+/* A paged KV cache (this struct lies in host memory, its pointers are device
+ * pointers).  key and value: [pages, kv_heads, page / 32, 32 head_dim] elements,
+ * 16-byte aligned, blocks of 32 positions in MFMA fragment order: K as
+ * [2][head_dim / 32][4][16][8] (position 16 n + c, dimension 32 s + 8 g + e at
+ * [n][s][g][c][e]), V as [head_dim / 16][4][16][2][4] (position 16 h + 4 g + j,
+ * dimension 16 t + c at [t][g][c][h][j]).  8-bit types: a stored q of a position
+ * and head stands for q 2^(x - 127), x the byte of key_exponent or
+ * value_exponent [pages, kv_heads, page] (4-byte aligned): the smallest power of
+ * two, 2^-100 at least, that brings the row's largest magnitude inside the type's
+ * range (448, 127); q is rounded to nearest even.  x = 255: the row held a NaN
+ * or an infinity, and reads back as NaN.  page a multiple of 32; head_dim 64, 96
+ * or 128. */
+typedef struct parrot_paged_cache {
+  void* key;
+  void* value;
+  uint8_t* key_exponent;
+  uint8_t* value_exponent;
+  int64_t pages;
+  int32_t page;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t type;
+} parrot_paged_cache;
+
+/* A batch of sequences (host memory, device pointers).  Sequence i has
+ * lengths[i] positions, its new ones included, position p in page
+ * table[i * width + p / page], and the new rows starts[i] .. starts[i + 1] - 1 of
+ * the call's operands: they are its last positions.  A page id outside the
+ * cache holds nothing: writes to it are dropped and its keys are not seen.
+ * Positions past width * page are not stored.  Rows before starts[0] and from
+ * starts[batch] on belong to no sequence.  The kernels bound every number that
+ * they read from these arrays. */
+typedef struct parrot_paged_batch {
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int32_t batch;
+  int32_t width;
+} parrot_paged_batch;
+
+/* Writes the new rows k and v, bf16 [rows, kv_heads, head_dim] with element
+ * strides k_strides / v_strides (row, head; multiples of 4, rows of unit stride,
+ * 8-byte aligned; host arrays), into their sequences' pages, quantised where the
+ * cache holds 8 bits.  A page that is written belongs to one sequence.
+ * New beside parrot_decode_attention_bf16's store into a contiguous cache
+ * (LocalGQA.decode, parrot/model.py:239-262). */
+int parrot_paged_append_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
+                             const void* k, const int64_t* k_strides, const void* v,
+                             const int64_t* v_strides, int32_t rows, void* stream);
+
+/* Reads positions 0 .. positions - 1 of every sequence back: k and v, bf16
+ * [batch, kv_heads, positions, head_dim] with element strides (sequence, head,
+ * position; multiples of 4; host arrays), zero from a sequence's length on and
+ * where no page is named.  starts is not read.  8-bit values are exact in bf16. */
+int parrot_paged_read_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
+                           int32_t positions, void* k, const int64_t* k_strides, void* v,
+                           const int64_t* v_strides, void* stream);
+
+/* Bytes of workspace that parrot_paged_attention_bf16 needs for these sizes (0
+ * where it needs none, or for sizes that it does not take). */
+size_t parrot_paged_attention_workspace_bytes(const parrot_paged_cache* cache,
+                                              const parrot_paged_batch* batch, int32_t rows,
+                                              int32_t heads, int32_t window, int32_t sinks);
+
+/* Attention of the new rows over their sequences' pages (their own keys and
+ * values already appended): out[r, h] = softmax(scale q[r, h] K^T) V, bf16
+ * [rows, heads, head_dim], over the keys j <= i with j > i - window or j < sinks,
+ * i being the row's position; window <= 0: every j <= i.  Query head h reads kv
+ * head h / (heads / kv_heads).  A row that sees no key is 0; rows of no sequence
+ * are left as they are.  What a row does not see cannot reach it, infinities and
+ * NaN included.  q bf16 [rows, heads, head_dim] with element strides q_strides
+ * (row, head; multiples of 8, 16-byte aligned; host array); out 8-byte aligned;
+ * scale finite and not 0; workspace 16-byte aligned.
+ * New beside parrot_causal_attention_bf16 and parrot_decode_attention_bf16
+ * (parrot/model.py:239-262, 264-295). */
+int parrot_paged_attention_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
+                                const void* q, const int64_t* q_strides, int32_t rows,
+                                int32_t heads, int32_t window, int32_t sinks, float scale,
+                                void* out, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/* Element types of logits. */
+#define PARROT_LOGITS_F32 0
+#define PARROT_LOGITS_BF16 1
+#define PARROT_LOGITS_F16 2
+
+/* Draws token[r] from row r of logits [rows, vocab] (stride elements apart) by
+ * the given uniform[r] in [0, 1):
+ *   w_i = exp((x_i - max x) / temperature); of the top_k largest (equal ones by
+ *   their index; top_k <= 0: all) the shortest prefix, largest first, that holds
+ *   top_p of their sum (top_p >= 1: all; never fewer than one), and of those
+ *   w_i >= min_p; the first token, by index, at which the sum of w passes uniform
+ *   times the whole.
+ * temperature <= 0: the largest, the lowest index among equal ones.  The
+ * parameters are arrays [rows], or where NULL the number beside them for every
+ * row.  A NaN logit counts as -infinity; a row of nothing else draws -1.
+ * probability (optional): the drawn token's share of the sum.  vocab <= 2^20.
+ * New beside parrot_vocab_argmax_bf16 (decode_next, parrot/model.py:927-931). */
+int parrot_sample(const void* logits, int32_t type, int64_t rows, int32_t vocab, int64_t stride,
+                  const float* uniform, const float* temperature, double temperature_all,
+                  const int32_t* top_k, int32_t top_k_all, const float* top_p, double top_p_all,
+                  const float* min_p, double min_p_all, int64_t* token, float* probability,
+                  void* stream);
 
 #ifdef __cplusplus
 }

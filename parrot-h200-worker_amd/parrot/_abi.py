@@ -13,13 +13,27 @@ from pathlib import Path
 import torch  # noqa: F401  (maps PyTorch's HIP runtime before the library)
 
 LIBRARY = Path(__file__).resolve().parent / "_lib" / "libparrot_hip.so"
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _sz = ctypes.c_size_t
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """parrot_paged_cache."""
+    _fields_ = [("key", _p), ("value", _p), ("key_exponent", _p), ("value_exponent", _p),
+                ("pages", _i64), ("page", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("type", _i32)]
+
+
+class PagedBatchStruct(ctypes.Structure):
+    """parrot_paged_batch."""
+    _fields_ = [("table", _p), ("lengths", _p), ("starts", _p), ("batch", _i32), ("width", _i32)]
+
 
 # name -> (restype, argtypes); mirrors include/parrot_hip.h
 SIGNATURES: dict[str, tuple] = {
@@ -143,6 +157,14 @@ SIGNATURES: dict[str, tuple] = {
     "parrot_route_top2_bf16": (ctypes.c_int, [_p, _p, _p, _i64, _i32, _i32, _p, _p, _p]),
     "parrot_route_top2_blocks_bf16": (
         ctypes.c_int, [_p, _p, _p, _i64, _i32, _i32, _p, _p, _p, _p]),
+    "parrot_paged_append_bf16": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _i32, _p]),
+    "parrot_paged_read_bf16": (ctypes.c_int, [_p, _p, _i32, _p, _p, _p, _p, _p]),
+    "parrot_paged_attention_workspace_bytes": (_sz, [_p, _p, _i32, _i32, _i32, _i32]),
+    "parrot_paged_attention_bf16": (
+        ctypes.c_int, [_p, _p, _p, _p, _i32, _i32, _i32, _i32, _f32, _p, _p, _sz, _p]),
+    "parrot_sample": (
+        ctypes.c_int,
+        [_p, _i32, _i64, _i32, _i64, _p, _p, _f64, _p, _i32, _p, _f64, _p, _f64, _p, _p, _p]),
     "parrot_peak_mfma_bf16": (ctypes.c_int, [_i32, _i64, _i32, _p, _p, _p]),
     "parrot_peak_copy": (ctypes.c_int, [_p, _p, _i64, _i64, _p]),
     "parrot_grouped_experts_static_bf16": (

@@ -11,6 +11,7 @@ host and never falls back to another backend: unsupported inputs raise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -36,6 +37,14 @@ MAX_DEPTH_SOURCES = 9
 
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Makes ``device`` the current one for a launch on its stream."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _require(x: Tensor, what: str, dtypes=(torch.bfloat16,)) -> None:
@@ -617,6 +626,82 @@ def vocab_argmax(h: Tensor, weight: Tensor, advance: Tensor | None = None,
                                             ptr(advance), ptr(ws), nbytes, _stream(h.device)),
                "parrot_vocab_argmax_bf16")
     return out.view(h.shape[:-1])
+
+
+_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+SAMPLE_MAX_VOCAB = 1 << 20
+
+
+def _sample_parameter(x, what: str, rows: int, device: torch.device, dtype: torch.dtype):
+    """(pointer, number) of one sampling parameter: a tensor of one value per
+    row, or a number for every row."""
+    if isinstance(x, Tensor):
+        if x.dtype != dtype or x.device != device or x.numel() != rows or not x.is_contiguous():
+            raise RuntimeError(f"{what} must be a number or a contiguous {dtype} tensor of one "
+                               "value per row on the logits' device")
+        return x.data_ptr(), 0
+    return None, x
+
+
+def sample(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor = 1.0,
+           top_k: int | Tensor = 0, top_p: float | Tensor = 1.0, min_p: float | Tensor = 0.0,
+           out: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """Draws a token per row of ``logits`` [..., vocab] (fp32, bf16 or fp16) by the
+    given ``uniform`` numbers in [0, 1) (fp32, one per row): returns int64 tokens
+    [..., 1] and their fp32 probabilities [..., 1] among the tokens that were kept.
+
+    The weights are w = exp((logits - max) / temperature).  Of the ``top_k``
+    largest (equal ones by their index; 0: all), the shortest prefix that holds
+    ``top_p`` of their sum is kept (never fewer than one), and of it the weights
+    of at least ``min_p``; the token is the first, by index, at which the sum of
+    the kept weights passes ``uniform`` times the whole.  A temperature of 0 (or
+    less) takes the largest logit, the lowest index among equal ones.  Each
+    parameter is a number or a tensor with one value per row (fp32; int32 for
+    top_k).  A NaN logit counts as -infinity; a row of nothing else gives token
+    -1 with probability 0.  ``out``: a contiguous int64 tensor of one id per row to
+    write the tokens into (a decode graph's input ids).
+
+    The arithmetic behind the borders is in 64 bits (see sample.hip), so a row's
+    token does not depend on the other rows of the call."""
+    _require(logits, "HIP sampling", tuple(_LOGIT_TYPES))
+    if logits.ndim < 1 or not 1 <= logits.shape[-1] <= SAMPLE_MAX_VOCAB:
+        raise RuntimeError(f"HIP sampling takes 1 to {SAMPLE_MAX_VOCAB} logits per row")
+    vocab = logits.shape[-1]
+    rows = logits.numel() // vocab
+    device = logits.device
+    flat = logits if logits.ndim == 2 else logits.reshape(-1, vocab)
+    if flat.stride(-1) != 1 or (rows > 1 and flat.stride(0) < vocab):
+        flat = flat.contiguous()
+    if (uniform.dtype != torch.float32 or uniform.device != device or uniform.numel() != rows or
+            not uniform.is_contiguous()):
+        raise RuntimeError("uniform must be a contiguous fp32 tensor of one number per row on the "
+                           "logits' device")
+    if not isinstance(temperature, Tensor) and not temperature >= 0:
+        raise RuntimeError("temperature must not be negative")
+    if not isinstance(top_k, Tensor) and not 0 <= top_k <= 2 ** 31 - 1:
+        raise RuntimeError("top_k must not be negative")
+    if not isinstance(top_p, Tensor) and not 0 <= top_p <= 1:
+        raise RuntimeError("top_p must lie in [0, 1]")
+    if not isinstance(min_p, Tensor) and not 0 <= min_p <= 1:
+        raise RuntimeError("min_p must lie in [0, 1]")
+    t, t_all = _sample_parameter(temperature, "temperature", rows, device, torch.float32)
+    k, k_all = _sample_parameter(top_k, "top_k", rows, device, torch.int32)
+    p, p_all = _sample_parameter(top_p, "top_p", rows, device, torch.float32)
+    m, m_all = _sample_parameter(min_p, "min_p", rows, device, torch.float32)
+    shape = (*logits.shape[:-1], 1)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int64, device=device)
+    elif (out.dtype != torch.int64 or out.device != device or not out.is_contiguous() or
+          out.numel() != rows):
+        raise RuntimeError("out must be a contiguous int64 tensor of one id per row on the "
+                           "logits' device")
+    probability = torch.empty(shape, dtype=torch.float32, device=device)
+    with _on(device):
+        _abi.check(_abi.load().parrot_sample(
+            flat.data_ptr(), _LOGIT_TYPES[logits.dtype], rows, vocab, flat.stride(0),
+            uniform.data_ptr(), t, t_all, k, k_all, p, p_all, m, m_all, out.data_ptr(),
+            probability.data_ptr(), _stream(device)), "parrot_sample")
+    return out.view(shape), probability
 
 
 # ---------------------------------------------------------------------------

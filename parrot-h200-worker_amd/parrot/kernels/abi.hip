@@ -10,6 +10,7 @@
 #include <atomic>
 
 #include "common.h"
+#include "paged.h"
 
 namespace {
 
@@ -40,6 +41,56 @@ size_t route_ws_bytes(int64_t tokens, int32_t experts) {
 int32_t* route_chunk_totals(void* workspace, int64_t tokens, int32_t experts) {
   return reinterpret_cast<int32_t*>(static_cast<char*>(workspace) +
                                     route_hist_bytes(tokens, experts));
+}
+
+int check_paged(const parrot_paged_cache* c, const parrot_paged_batch* b) {
+  if (!c || !b) return PARROT_ERR_NULL_POINTER;
+  if (c->pages < 0 || c->page <= 0 || c->kv_heads <= 0 || b->batch < 0 || b->width < 0)
+    return PARROT_ERR_BAD_SHAPE;
+  if (c->page % 32 || c->kv_heads > 65535 || b->batch > 65535 ||
+      !parrot::paged_head_dim_supported(c->head_dim))
+    return PARROT_ERR_UNSUPPORTED;
+  if (c->type != PARROT_PAGED_BF16 && c->type != PARROT_PAGED_E4M3 && c->type != PARROT_PAGED_INT8)
+    return PARROT_ERR_UNSUPPORTED;
+  // positions are 32-bit numbers
+  if (static_cast<int64_t>(b->width) * c->page > INT32_MAX - 64) return PARROT_ERR_BAD_SHAPE;
+  const bool bytes = c->type != PARROT_PAGED_BF16;
+  if (c->pages > 0 && (!c->key || !c->value || (bytes && (!c->key_exponent || !c->value_exponent))))
+    return PARROT_ERR_NULL_POINTER;
+  if (b->batch > 0 && (!b->lengths || !b->starts || (b->width > 0 && !b->table)))
+    return PARROT_ERR_NULL_POINTER;
+  if (!aligned16(c->key) || !aligned16(c->value) ||
+      (bytes && ((reinterpret_cast<uintptr_t>(c->key_exponent) |
+                  reinterpret_cast<uintptr_t>(c->value_exponent)) & 3u)))
+    return PARROT_ERR_ALIGNMENT;
+  return PARROT_OK;
+}
+
+int check_paged_rows(const void* p, const int64_t* strides, int n, int multiple, unsigned align) {
+  if (!p || !strides) return PARROT_ERR_NULL_POINTER;
+  for (int i = 0; i < n; ++i)
+    if (strides[i] % multiple) return PARROT_ERR_ALIGNMENT;
+  return reinterpret_cast<uintptr_t>(p) % align ? PARROT_ERR_ALIGNMENT : PARROT_OK;
+}
+
+// (rows x heads is also the number of a tile's rows at most, in 32 bits)
+int check_paged_heads(int32_t rows, int32_t heads, int32_t kv_heads) {
+  if (rows < 0 || heads <= 0 || heads % kv_heads) return PARROT_ERR_BAD_SHAPE;
+  return static_cast<int64_t>(rows) * heads > (int64_t{1} << 30) ? PARROT_ERR_BAD_SHAPE : PARROT_OK;
+}
+
+parrot::PagedCache paged_cache(const parrot_paged_cache* c) {
+  return {c->key, c->value, c->key_exponent, c->value_exponent, c->pages, c->page, c->kv_heads};
+}
+
+parrot::PagedBatch paged_batch(const parrot_paged_batch* b, int32_t rows) {
+  return {b->table, b->lengths, b->starts, b->batch, b->width, rows};
+}
+
+int paged_splits(const parrot_paged_cache* c, const parrot_paged_batch* b, int32_t rows,
+                 int32_t heads, int32_t window, int32_t sinks) {
+  return parrot::paged_attention_splits(b->batch, rows, heads, c->kv_heads, c->page, b->width,
+                                        window > 0 ? window : INT32_MAX, sinks);
 }
 
 struct ExpertsWorkspace {
@@ -720,6 +771,87 @@ size_t parrot_experts_workspace_bytes(int64_t tokens, int32_t dim, int32_t hidde
                                       int32_t shared_dim) {
   if (tokens < 0 || dim <= 0 || hidden_dim <= 0 || shared_dim <= 0) return 0;
   return experts_ws(nullptr, tokens, dim, hidden_dim, shared_dim).bytes;
+}
+
+int parrot_paged_append_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
+                             const void* k, const int64_t* k_strides, const void* v,
+                             const int64_t* v_strides, int32_t rows, void* stream) {
+  if (int rc = check_paged(cache, batch)) return rc;
+  if (rows < 0 || rows > (1 << 30)) return PARROT_ERR_BAD_SHAPE;
+  if (rows == 0) return PARROT_OK;
+  if (int rc = check_paged_rows(k, k_strides, 2, 4, 8)) return rc;
+  if (int rc = check_paged_rows(v, v_strides, 2, 4, 8)) return rc;
+  return status(parrot::launch_paged_append(
+      paged_cache(cache), cache->type, cache->head_dim, paged_batch(batch, rows),
+      static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_strides, v_strides,
+      as_stream(stream)));
+}
+
+int parrot_paged_read_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
+                           int32_t positions, void* k, const int64_t* k_strides, void* v,
+                           const int64_t* v_strides, void* stream) {
+  if (int rc = check_paged(cache, batch)) return rc;
+  if (positions < 0 || positions > INT32_MAX - 64) return PARROT_ERR_BAD_SHAPE;
+  if (positions == 0 || batch->batch == 0) return PARROT_OK;
+  if (int rc = check_paged_rows(k, k_strides, 3, 4, 8)) return rc;
+  if (int rc = check_paged_rows(v, v_strides, 3, 4, 8)) return rc;
+  return status(parrot::launch_paged_read(
+      paged_cache(cache), cache->type, cache->head_dim, paged_batch(batch, 0), positions,
+      static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), k_strides, v_strides,
+      as_stream(stream)));
+}
+
+size_t parrot_paged_attention_workspace_bytes(const parrot_paged_cache* cache,
+                                              const parrot_paged_batch* batch, int32_t rows,
+                                              int32_t heads, int32_t window, int32_t sinks) {
+  if (check_paged(cache, batch) || check_paged_heads(rows, heads, cache->kv_heads) || sinks < 0)
+    return 0;
+  return parrot::paged_attention_workspace_bytes(
+      paged_splits(cache, batch, rows, heads, window, sinks), rows, heads, cache->head_dim);
+}
+
+int parrot_paged_attention_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
+                                const void* q, const int64_t* q_strides, int32_t rows,
+                                int32_t heads, int32_t window, int32_t sinks, float scale,
+                                void* out, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  if (int rc = check_paged(cache, batch)) return rc;
+  if (int rc = check_paged_heads(rows, heads, cache->kv_heads)) return rc;
+  if (sinks < 0 || !(scale - scale == 0.0f) || scale == 0.0f) return PARROT_ERR_BAD_SHAPE;
+  if (rows == 0 || batch->batch == 0) return PARROT_OK;
+  if (int rc = check_paged_rows(q, q_strides, 2, 8, 16)) return rc;
+  if (!out) return PARROT_ERR_NULL_POINTER;
+  if (reinterpret_cast<uintptr_t>(out) & 7u) return PARROT_ERR_ALIGNMENT;
+  const int splits = paged_splits(cache, batch, rows, heads, window, sinks);
+  const size_t need =
+      parrot::paged_attention_workspace_bytes(splits, rows, heads, cache->head_dim);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need) return PARROT_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return PARROT_ERR_ALIGNMENT;
+  }
+  return status(parrot::launch_paged_attention(
+      paged_cache(cache), cache->type, cache->head_dim, paged_batch(batch, rows),
+      static_cast<const uint16_t*>(q), q_strides, heads, window > 0 ? window : INT32_MAX, sinks,
+      scale, splits, workspace, static_cast<uint16_t*>(out), as_stream(stream)));
+}
+
+int parrot_sample(const void* logits, int32_t type, int64_t rows, int32_t vocab, int64_t stride,
+                  const float* uniform, const float* temperature, double temperature_all,
+                  const int32_t* top_k, int32_t top_k_all, const float* top_p, double top_p_all,
+                  const float* min_p, double min_p_all, int64_t* token, float* probability,
+                  void* stream) {
+  if (rows < 0 || rows > INT32_MAX || vocab <= 0 || (rows > 1 && stride < vocab))
+    return PARROT_ERR_BAD_SHAPE;
+  if (vocab > (1 << 20) || type < PARROT_LOGITS_F32 || type > PARROT_LOGITS_F16)
+    return PARROT_ERR_UNSUPPORTED;
+  if (rows == 0) return PARROT_OK;
+  if (!logits || !uniform || !token) return PARROT_ERR_NULL_POINTER;
+  if (reinterpret_cast<uintptr_t>(logits) & (type == PARROT_LOGITS_F32 ? 3u : 1u))
+    return PARROT_ERR_ALIGNMENT;
+  return status(parrot::launch_sample(logits, type, static_cast<int>(rows), vocab, stride, uniform,
+                                      temperature, temperature_all, top_k, top_k_all, top_p,
+                                      top_p_all, min_p, min_p_all, token, probability,
+                                      as_stream(stream)));
 }
 
 }  // extern "C"

@@ -555,6 +555,15 @@ int vocab_argmax_groups(int vocab);
 hipError_t launch_vocab_argmax(const uint16_t* h, int rows, int dim, const uint16_t* w, int vocab,
                                float* part_v, int32_t* part_i, int64_t* out, int32_t* advance, hipStream_t s);
 
+// Tokens drawn from rows of logits (type 0 fp32, 1 bf16, 2 fp16) by given uniform
+// numbers (see sample.hip); each parameter per row, or one for all where its
+// pointer is null.
+hipError_t launch_sample(const void* logits, int type, int rows, int vocab, int64_t stride,
+                         const float* uniform, const float* temperature, double temperature_all,
+                         const int32_t* top_k, int32_t top_k_all, const float* top_p,
+                         double top_p_all, const float* min_p, double min_p_all, int64_t* token,
+                         float* probability, hipStream_t s);
+
 // Causal / sliding-window attention (see attention.hip).  Strides are in
 // elements: [batch, head, row] for q and k (unit stride along head_dim),
 // [batch, head, dim row] for the transposed values vt (unit stride along the

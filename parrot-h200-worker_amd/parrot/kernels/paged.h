@@ -1,0 +1,120 @@
+// A paged KV cache: its memory, and how a batch of sequences names its parts.
+//
+// A page holds `page` positions (a multiple of 32) of every kv head, in blocks
+// of 32 positions.  A block of D-wide rows is stored in the order in which the
+// attention kernels' matrix operands take it, 32 D elements of K and of V:
+//   K: [n = 2][s = D / 32][g = 4][c = 16][8]: position 16 n + c, dims 32 s + 8 g ..
+//   V: [t = D / 16][g = 4][c = 16][8]: dim 16 t + c, positions
+//      {4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3}
+// (kfrag_index / vfrag_index within one block), so an operand is one
+// contiguous piece of a wavefront's load.
+//
+// 8-bit rows are q 2^(x - 127), x one byte per position and head: the smallest
+// power of two that brings the row's largest magnitude inside the type's range.
+// A power of two, because q times one is exact in bf16: what is read back, and
+// what attention multiplies, is the stored value itself, not a rounding of it.
+// For e4m3, a floating type, the choice costs nothing but the bottom of the
+// range; for int8 half a bit on average.  Byte 255: the row held a NaN or an
+// infinity and reads back as NaN.
+#pragma once
+
+#include "common.h"
+
+namespace parrot {
+
+enum PagedType { kPagedBf16 = 0, kPagedE4m3 = 1, kPagedInt8 = 2 };
+
+constexpr int kPagedBlock = 32;  // positions of a block
+constexpr int kPagedMinExponent = -100;
+constexpr uint32_t kPagedNotFinite = 255;
+
+struct PagedCache {
+  void* key;               // [pages, kv_heads, page / 32, 32 D]
+  void* value;
+  uint8_t* key_exponent;   // [pages, kv_heads, page] (8-bit types)
+  uint8_t* value_exponent;
+  int64_t pages;
+  int page, kv_heads;
+};
+
+// Sequence i: its pages table[i, :width], its whole length lengths[i] (new
+// rows included), its new rows starts[i] .. starts[i + 1] of `rows`.
+struct PagedBatch {
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int batch, width, rows;
+};
+
+struct PagedSequence {
+  int first;   // its first new row
+  int count;   // new rows
+  int length;  // positions, as given
+  int stored;  // positions that its pages can hold
+};
+
+// Every number of it is bounded here: whatever the device tensors hold, rows
+// stay inside the operands and positions inside the table.
+__device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch& b, int page, int i) {
+  PagedSequence s;
+  s.first = min(max(b.starts[i], 0), b.rows);
+  s.count = min(max(b.starts[i + 1], s.first), b.rows) - s.first;
+  s.length = max(b.lengths[i], 0);
+  s.stored = min(s.length, b.width * page);  // width * page < 2^31, checked on the host
+  return s;
+}
+
+// The units (tiles, blocks) of the sequences in a row: which sequence unit
+// `unit` belongs to and the how manieth of it it is; false past the last.
+// Every wavefront of the workgroup calls it.  units_of(i): sequence i's number.
+template <typename F>
+__device__ __forceinline__ bool paged_locate(int batch, int unit, F units_of, int& sequence,
+                                             int& index) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int base = 0;
+  for (int c = 0; c < batch; c += kWave) {
+    const int mine = c + lane < batch ? units_of(c + lane) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+      const int before = __shfl_up(upto, d);
+      if (lane >= d) upto += before;
+    }
+    const int total = __builtin_amdgcn_readlane(upto, kWave - 1);
+    if (unit < base + total) {
+      const uint64_t hit = __ballot(unit >= base + upto - mine && unit < base + upto);
+      const int who = __builtin_ctzll(hit);
+      sequence = c + who;
+      index = unit - base - __builtin_amdgcn_readlane(upto - mine, who);
+      return true;
+    }
+    base += total;
+  }
+  return false;
+}
+
+// The page of a position's block, or -1 where the table names none.
+__device__ __forceinline__ int paged_page(const PagedBatch& b, const PagedCache& c, int sequence,
+                                          int at) {
+  const int p = b.table[static_cast<int64_t>(sequence) * b.width + at];
+  return p >= 0 && p < c.pages ? p : -1;
+}
+
+// Host side: launchers (shapes are validated by the C-ABI layer).
+bool paged_head_dim_supported(int head_dim);  // 64, 96, 128
+hipError_t launch_paged_append(const PagedCache& cache, int type, int head_dim,
+                               const PagedBatch& batch, const uint16_t* k, const uint16_t* v,
+                               const int64_t* k_strides, const int64_t* v_strides, hipStream_t s);
+hipError_t launch_paged_read(const PagedCache& cache, int type, int head_dim,
+                             const PagedBatch& batch, int positions, uint16_t* k, uint16_t* v,
+                             const int64_t* k_strides, const int64_t* v_strides, hipStream_t s);
+int paged_attention_splits(int batch, int rows, int heads, int kv_heads, int page, int width,
+                           int window, int sinks);
+size_t paged_attention_workspace_bytes(int splits, int rows, int heads, int head_dim);
+hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_dim,
+                                  const PagedBatch& batch, const uint16_t* q,
+                                  const int64_t* q_strides, int heads, int window, int sinks,
+                                  float scale, int splits, void* workspace, uint16_t* out,
+                                  hipStream_t s);
+
+}  // namespace parrot

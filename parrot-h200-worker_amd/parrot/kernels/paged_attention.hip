@@ -1,0 +1,512 @@
+// Attention of a chunk of new tokens (one, or thousands) over the pages of a
+// KV cache: key j is visible to the query at position i iff j <= i and
+// (j > i - window or j < sinks).
+//
+// The rows of a tile are (token, query head) pairs of one kv head, token-major:
+// a decode step's query heads that share a kv head are rows of one tile, so its
+// keys and values are read once for all of them.
+//
+//   S^T = K Q^T     A = 32 keys, B = 32 rows: lane l holds 16 of the block's
+//                   keys for row l % 32 (v_mfma_f32_32x32x16_bf16).
+//   O^T += V^T P^T  P^T comes straight from those registers as the B operand:
+//                   operand row i of K is key 16 j + 4 (2 s + h) + r of the block
+//                   (i = 16 s + 8 j + 4 h + r), so that the 8 scores a lane holds
+//                   per 16-key step are the keys {4 g .. + 3, 16 + 4 g .. + 3},
+//                   g = 2 s + l / 32, of one piece of V.
+//
+// 8-bit rows enter the products unrounded: K as q 2^x (exact in bf16), V as q
+// with its power of two on the probability instead (one power per key, and a
+// piece of V holds eight keys).  P is rounded to bf16 once.
+#include <algorithm>
+#include <type_traits>
+
+#include "paged.h"
+
+namespace parrot {
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;
+constexpr int kRows = 32;  // rows of a wavefront's tile
+
+struct AttendArgs {
+  PagedCache cache;
+  PagedBatch batch;
+  const uint16_t* q;
+  int64_t qs[2];  // element strides: row, head
+  int heads, rep;
+  int window;  // INT_MAX: none
+  int sinks;
+  float scale_log2;  // |scale| log2(e)
+  uint32_t q_sign;   // 0x80008000 for a negative scale (q is negated), else 0
+  int splits;
+  float* part;       // [splits][rows * heads][D], unnormalised
+  float2* part_ml;   // [splits][rows * heads]
+  uint16_t* out;     // [rows][heads][D]
+};
+
+// The key blocks that a tile's rows see, in order: the first `sinks` blocks,
+// then those from `lo` on.
+struct Blocks {
+  int sinks, lo, count;
+  __device__ __forceinline__ int at(int i) const { return i < sinks ? i : lo + i - sinks; }
+};
+
+__device__ __forceinline__ Blocks tile_blocks(int first, int last, int stored, int window,
+                                              int sinks) {
+  Blocks r{0, 0, 0};
+  last = min(last, stored - 1);
+  if (last < 0) return r;
+  // (a window past the first position reaches every key; first - window + 1 fits)
+  r.lo = first >= window ? min((first - window + 1) / kPagedBlock, last / kPagedBlock + 1) : 0;
+  // sinks > 0 only count where the window has left them
+  r.sinks = min(static_cast<int>((static_cast<int64_t>(sinks) + kPagedBlock - 1) / kPagedBlock),
+                r.lo);
+  r.count = r.sinks + last / kPagedBlock - r.lo + 1;
+  return r;
+}
+
+__device__ __forceinline__ bool visible(int key, int query, int window, int sinks) {
+  return key <= query && (query - key < window || key < sinks);
+}
+
+// A piece (8 values) of a page as bf16: K's values are times `power`, V's are
+// q itself.
+template <int TYPE>
+struct Piece {
+  using raw = uint2;
+};
+template <>
+struct Piece<kPagedBf16> {
+  using raw = uint4;
+};
+
+__device__ __forceinline__ uint32_t bits(bf16x2_t v) { return __builtin_bit_cast(uint32_t, v); }
+
+template <int TYPE>
+__device__ __forceinline__ bf16x8 piece_bf16(typename Piece<TYPE>::raw w, float power) {
+  if constexpr (TYPE == kPagedBf16) {
+    return __builtin_bit_cast(bf16x8, w);
+  } else if constexpr (TYPE == kPagedE4m3) {
+    uint4 y;
+    y.x = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, power, false));
+    y.y = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, power, true));
+    y.z = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, power, false));
+    y.w = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, power, true));
+    return __builtin_bit_cast(bf16x8, y);
+  } else {
+    uint32_t y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t half = (i < 2 ? w.x : w.y) >> (16 * (i & 1));
+      const float a = static_cast<float>(static_cast<int8_t>(half)) * power;
+      const float b = static_cast<float>(static_cast<int8_t>(half >> 8)) * power;
+      // (eight significant bits: the upper halves are the values)
+      y[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    }
+    return __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
+  }
+}
+
+__device__ __forceinline__ bool has_nonfinite(bf16x8 v) {
+  const uint4 w = __builtin_bit_cast(uint4, v);
+  auto bad = [](uint32_t x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; };
+  return bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
+}
+
+// One wavefront's running softmax state over its 32 rows: m in log2 units,
+// shared by a row's two lanes and raised only when a score passes it by more
+// than 2^8; each lane sums its own probabilities.
+template <int D>
+struct State {
+  static constexpr int DT = D / 32;
+  float m = -INFINITY, l = 0.0f;
+  f32x16 o[DT];
+};
+
+template <int D>
+__device__ __forceinline__ void clear(State<D>& st) {
+#pragma unroll
+  for (int i = 0; i < State<D>::DT; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) st.o[i][e] = 0.0f;
+}
+
+// One block of 32 keys: scores, softmax and values.
+//   kf: K operands; load_v(i, s): V operand of 32-dim tile i, 16-key step s;
+//   vpower: 2^x of the lane's 16 keys (8-bit types); k0: the block's first
+//   position; query: the lane's row's; the tile's rows are at positions first ..
+//   last, and keys < stored.
+template <int TYPE, int D, typename LoadV>
+__device__ __forceinline__ void attend_block(State<D>& st, const bf16x8 (&kf)[D / 16],
+                                             const bf16x8 (&qf)[D / 16], LoadV load_v,
+                                             const uint32_t (&vbytes)[4], int k0, int query,
+                                             int first, int last, int stored,
+                                             const AttendArgs& a) {
+  constexpr int DT = D / 32;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int half = lane >> 5, col = lane & 31;
+  constexpr float kLazy = 8.0f;
+  f32x16 sc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+#pragma unroll
+  for (int u = 0; u < D / 16; ++u)
+    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u], qf[u], sc, 0, 0, 0);
+
+  auto key_of = [&](int e) { return k0 + 16 * ((e >> 2) & 1) + 4 * (2 * (e >> 3) + half) + (e & 3); };
+  // A block that every row of the tile sees whole needs no mask.
+  const bool whole = k0 + 31 <= min(first, stored - 1) &&
+                     (last - k0 < a.window || k0 + 31 < a.sinks);
+  if (!whole) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int key = key_of(e);
+      const bool ok = key < stored && visible(key, query, a.window, a.sinks);
+      sc[e] = ok ? sc[e] : -INFINITY;
+    }
+  }
+  float t[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) t[i] = fmaxf(fmaxf(sc[3 * i], sc[3 * i + 1]), sc[3 * i + 2]);
+  float mx = fmaxf(fmaxf(fmaxf(t[0], t[1]), t[2]), fmaxf(fmaxf(t[3], t[4]), sc[15]));
+  mx *= a.scale_log2;
+  if (__ballot(mx > st.m + kLazy) != 0) {
+    const float mn = fmaxf(st.m, fmaxf(mx, __shfl_xor(mx, 32)));
+    const float alpha = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - mn);
+    st.l *= alpha;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) st.o[i][e] *= alpha;
+    st.m = mn;
+  }
+  // A row that has seen no key yet has m = -inf and only -inf scores:
+  // exp2(-inf - 0) = 0.
+  const float neg = st.m == -INFINITY ? 0.0f : -st.m;
+  float p[16], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], a.scale_log2, neg));
+    sum[e & 3] += p[e];
+  }
+  st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+
+  bf16x8 vf[2 * DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) vf[2 * i + s] = load_v(i, s);
+
+  // Values that some row must not see: times a probability of 0 an infinity or
+  // a NaN is not 0.  Such a block takes the values row by row, those of keys
+  // that the row does not see cleared.
+  bool odd = false;
+  if (!whole) {
+    bool mine = false;
+#pragma unroll
+    for (int i = 0; i < 2 * DT; ++i) mine |= has_nonfinite(vf[i]);
+    if constexpr (TYPE != kPagedBf16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mine |= ((vbytes[i] >> (8 * r)) & 0xffu) == kPagedNotFinite;
+    }
+    odd = __ballot(mine) != 0;
+  }
+  if constexpr (TYPE != kPagedBf16) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t byte = (vbytes[e >> 2] >> (8 * (e & 3))) & 0xffu;
+      const float y = p[e] * __uint_as_float(byte << 23);
+      p[e] = odd && sc[e] == -INFINITY ? 0.0f : y;
+    }
+  }
+  bf16x8 pf[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pf[s][e] = static_cast<__bf16>(p[8 * s + e]);
+
+  if (odd) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      f32x16 sums = st.o[i];
+#pragma unroll 1
+      for (int row = 0; row < kRows; ++row) {
+        const int at = __builtin_amdgcn_readlane(query, row);
+        f32x16 y = st.o[i];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          bf16x8 v = vf[2 * i + s];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int key = key_of(8 * s + e);
+            if (!(key < stored && visible(key, at, a.window, a.sinks))) v[e] = static_cast<__bf16>(0.0f);
+          }
+          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pf[s], y, 0, 0, 0);
+        }
+        if (col == row) sums = y;
+      }
+      st.o[i] = sums;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      st.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[2 * i + s], pf[s], st.o[i], 0, 0, 0);
+}
+
+// A row of a tile: its token's position, operand and output rows.
+struct TileRow {
+  int position;
+  int token;  // row of q and of the output
+  int head;
+};
+
+__device__ __forceinline__ TileRow tile_row(const PagedSequence& s, int row, int rows, int rep,
+                                            int kv_head) {
+  const int r = min(row, rows - 1);
+  const int token = r / rep;
+  return {s.length - s.count + token, s.first + token, kv_head * rep + (r - token * rep)};
+}
+
+// Every wavefront takes every fourth key block of the workgroup's share, its
+// operands straight from the pages; the four are merged in LDS.
+template <int TYPE, int D>
+__global__ __launch_bounds__(kWaves * kWave, 2) void paged_attend_kernel(AttendArgs a) {
+  constexpr int KU = D / 16, DT = D / 32;
+  using raw = typename Piece<TYPE>::raw;
+  __shared__ float o_s[kWaves][kRows][D + 4];
+  __shared__ float ml_s[kWaves][2][kRows];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const int kvh = blockIdx.y, split = blockIdx.z;
+
+  auto units_of = [&](int i) {
+    return (paged_sequence(a.batch, a.cache.page, i).count * a.rep + kRows - 1) / kRows;
+  };
+  int sequence, tile;
+  if (!paged_locate(a.batch.batch, blockIdx.x, units_of, sequence, tile)) return;
+  const PagedSequence s = paged_sequence(a.batch, a.cache.page, sequence);
+  const int rows = s.count * a.rep;
+  const int row0 = tile * kRows;
+  const TileRow mine = tile_row(s, row0 + col, rows, a.rep, kvh);
+  const int first = s.length - s.count + row0 / a.rep;
+  const int last = s.length - s.count + (min(row0 + kRows, rows) - 1) / a.rep;
+  const Blocks blocks = tile_blocks(first, last, s.stored, a.window, a.sinks);
+  // This workgroup's share of them.
+  const int share = (blocks.count + a.splits - 1) / a.splits;
+  const int begin = min(split * share, blocks.count), end = min(begin + share, blocks.count);
+
+  State<D> st;
+  clear(st);
+  if (begin < end) {
+    bf16x8 qf[KU];
+    {
+      const uint16_t* row = a.q + mine.token * a.qs[0] + mine.head * a.qs[1] + 8 * half;
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        uint4 v = *reinterpret_cast<const uint4*>(row + 16 * u);
+        v.x ^= a.q_sign;
+        v.y ^= a.q_sign;
+        v.z ^= a.q_sign;
+        v.w ^= a.q_sign;
+        qf[u] = __builtin_bit_cast(bf16x8, v);
+      }
+    }
+    const int per_page = a.cache.page / kPagedBlock;
+    const int kn = (col >> 3) & 1;
+    const int kc = 4 * (2 * (col >> 4) + ((col >> 2) & 1)) + (col & 3);
+    const int k_off = (kn * (D / 32) * 512 + half * 128 + kc * 8) / 8;  // in pieces
+    const int v_off = ((col >> 4) * 512 + half * 128 + (col & 15) * 8) / 8;
+    for (int i = begin + wave; i < end; i += kWaves) {
+      const int blk = blocks.at(i);
+      const int page = __builtin_amdgcn_readfirstlane(
+          paged_page(a.batch, a.cache, sequence, blk / per_page));
+      if (page < 0) continue;
+      const int64_t at = static_cast<int64_t>(page) * a.cache.kv_heads + kvh;
+      const int64_t off = (at * per_page + blk % per_page) * (kPagedBlock * D / 8);
+      const raw* kp = static_cast<const raw*>(a.cache.key) + off + k_off;
+      const raw* vp = static_cast<const raw*>(a.cache.value) + off + v_off;
+      raw kw[KU], vw[2 * DT];
+#pragma unroll
+      for (int u = 0; u < KU; ++u) kw[u] = kp[32 * u];
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) vw[2 * t + h] = vp[128 * t + 32 * h];
+      float kpower = 1.0f;
+      uint32_t vbytes[4] = {0, 0, 0, 0};
+      if constexpr (TYPE != kPagedBf16) {
+        const int64_t e = at * a.cache.page + (blk % per_page) * kPagedBlock;
+        kpower = __uint_as_float(static_cast<uint32_t>(a.cache.key_exponent[e + 16 * kn + kc]) << 23);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          vbytes[j] = *reinterpret_cast<const uint32_t*>(a.cache.value_exponent + e + 16 * (j & 1) +
+                                                         8 * (j >> 1) + 4 * half);
+      }
+      const int k0 = blk * kPagedBlock;
+      bf16x8 kf[KU];
+#pragma unroll
+      for (int u = 0; u < KU; ++u) kf[u] = piece_bf16<TYPE>(kw[u], kpower);
+      attend_block<TYPE, D>(
+          st, kf, qf, [&](int t, int h) { return piece_bf16<TYPE>(vw[2 * t + h], 1.0f); }, vbytes,
+          k0, mine.position, first, last, s.stored, a);
+    }
+  }
+  // Merge: every wavefront's share in its own units, then one common maximum.
+  const float l = st.l + __shfl_xor(st.l, 32);
+  if (half == 0) {
+    ml_s[wave][0][col] = st.m;
+    ml_s[wave][1][col] = l;
+  }
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<float4*>(&o_s[wave][col][32 * t + 8 * (e >> 2) + 4 * half]) =
+          make_float4(st.o[t][e], st.o[t][e + 1], st.o[t][e + 2], st.o[t][e + 3]);
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRows * (D / 4); i += kWaves * kWave) {
+    const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
+    if (row0 + r >= rows) break;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml_s[w][0][r]);
+    float sum = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float mw = ml_s[w][0][r], lw = ml_s[w][1][r];
+      // A wavefront that saw nothing adds nothing (its maximum is -inf, its sum
+      // 0; a NaN sum has to come through).
+      if (mw == -INFINITY && lw == 0.0f) continue;
+      const float f = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+      sum += lw * f;
+      const float4 x = *reinterpret_cast<const float4*>(&o_s[w][r][d]);
+      y.x += x.x * f;
+      y.y += x.y * f;
+      y.z += x.z * f;
+      y.w += x.w * f;
+    }
+    const TileRow row = tile_row(s, row0 + r, rows, a.rep, kvh);
+    const int64_t to = static_cast<int64_t>(row.token) * a.heads + row.head;
+    if (a.splits == 1) {
+      const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+      *reinterpret_cast<uint2*>(a.out + to * D + d) =
+          make_uint2(pack_bf16x2(y.x * f, y.y * f), pack_bf16x2(y.z * f, y.w * f));
+    } else {
+      const int64_t at = static_cast<int64_t>(split) * a.batch.rows * a.heads + to;
+      if (d == 0) a.part_ml[at] = make_float2(m, sum);
+      if (begin < end) *reinterpret_cast<float4*>(a.part + at * D + d) = y;
+    }
+  }
+}
+
+// Joins the shares of split tiles: D / 4 threads a row.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a) {
+  constexpr int kPer = 256 / (D / 4);
+  const int slot = threadIdx.x / (D / 4), d = 4 * (threadIdx.x - slot * (D / 4));
+  const int64_t to = static_cast<int64_t>(blockIdx.x) * kPer + slot;
+  const int64_t rows = static_cast<int64_t>(a.batch.rows) * a.heads;
+  if (slot >= kPer || to >= rows) return;
+  // Rows of no sequence stay as they are.
+  const int token = static_cast<int>(to / a.heads);
+  if (token < a.batch.starts[0] || token >= a.batch.starts[a.batch.batch]) return;
+  float m = -INFINITY;
+  for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.part_ml[i * rows + to].x);
+  float sum = 0.0f;
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i = 0; i < a.splits; ++i) {
+    const float2 ml = a.part_ml[i * rows + to];
+    if (ml.x == -INFINITY && ml.y == 0.0f) continue;
+    const float f = ml.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
+    sum += ml.y * f;
+    const float4 x = *reinterpret_cast<const float4*>(a.part + (i * rows + to) * D + d);
+    y.x += x.x * f;
+    y.y += x.y * f;
+    y.z += x.z * f;
+    y.w += x.w * f;
+  }
+  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+  *reinterpret_cast<uint2*>(a.out + to * D + d) =
+      make_uint2(pack_bf16x2(y.x * f, y.y * f), pack_bf16x2(y.z * f, y.w * f));
+}
+
+}  // namespace
+
+// Enough workgroups for the chip, each with 256 keys at least.
+int paged_attention_splits(int batch, int rows, int heads, int kv_heads, int page, int width,
+                           int window, int sinks) {
+  const int rep = heads / kv_heads;
+  const int64_t tiles = (static_cast<int64_t>(rows) * rep + kRows - 1) / kRows;
+  const int64_t units = std::max<int64_t>(tiles, std::min(batch, rows)) * kv_heads;
+  // The most keys a tile can see: its table's, or the window, the sinks and
+  // the tile's own span.
+  int64_t keys = static_cast<int64_t>(width) * page;
+  if (window < INT32_MAX) keys = std::min<int64_t>(keys, int64_t{window} + sinks + kRows + 64);
+  const int64_t want = (1024 + units - 1) / std::max<int64_t>(units, 1);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, keys / 256, 64})));
+}
+
+size_t paged_attention_workspace_bytes(int splits, int rows, int heads, int head_dim) {
+  if (splits <= 1) return 0;
+  return static_cast<size_t>(splits) * rows * heads * (head_dim + 2) * sizeof(float);
+}
+
+hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_dim,
+                                  const PagedBatch& batch, const uint16_t* q,
+                                  const int64_t* q_strides, int heads, int window, int sinks,
+                                  float scale, int splits, void* workspace, uint16_t* out,
+                                  hipStream_t s) {
+  if (batch.rows == 0 || batch.batch == 0) return hipSuccess;
+  AttendArgs a;
+  a.cache = cache;
+  a.batch = batch;
+  a.q = q;
+  a.qs[0] = q_strides[0];
+  a.qs[1] = q_strides[1];
+  a.heads = heads;
+  a.rep = heads / cache.kv_heads;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
+  a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
+  a.splits = splits;
+  a.part = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part +
+                                        static_cast<size_t>(splits) * batch.rows * heads * head_dim);
+  a.out = out;
+  // ceil(n rep / 32) tiles a sequence
+  const int64_t tiles = static_cast<int64_t>(batch.rows) * a.rep / kRows +
+                        std::min(batch.batch, batch.rows);
+  const dim3 grid(static_cast<uint32_t>(tiles), cache.kv_heads, splits);
+  auto run = [&](auto t, auto d) {
+    constexpr int TYPE = decltype(t)::value, D = decltype(d)::value;
+    paged_attend_kernel<TYPE, D><<<grid, kWaves * kWave, 0, s>>>(a);
+    if (splits > 1) {
+      constexpr int kPer = 256 / (D / 4);
+      const int64_t rows = static_cast<int64_t>(batch.rows) * heads;
+      paged_join_kernel<D><<<static_cast<uint32_t>((rows + kPer - 1) / kPer), 256, 0, s>>>(a);
+    }
+    return hipGetLastError();
+  };
+  auto by_width = [&](auto t) {
+    if (head_dim == 64) return run(t, std::integral_constant<int, 64>{});
+    if (head_dim == 96) return run(t, std::integral_constant<int, 96>{});
+    return run(t, std::integral_constant<int, 128>{});
+  };
+  if (type == kPagedBf16) return by_width(std::integral_constant<int, kPagedBf16>{});
+  if (type == kPagedE4m3) return by_width(std::integral_constant<int, kPagedE4m3>{});
+  return by_width(std::integral_constant<int, kPagedInt8>{});
+}
+
+}  // namespace parrot

@@ -1,0 +1,425 @@
+"""GPU checks of the paged KV cache (append, read) and of attention over it
+against plain forms in 64 bits (paged_cases)."""
+import itertools
+import math
+
+import pytest
+import torch
+
+from paged_cases import Plain, stored
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float8_e4m3fn, torch.int8]
+NAMES = {torch.bfloat16: "bf16", torch.float8_e4m3fn: "e4m3", torch.int8: "int8"}
+
+
+@pytest.fixture(autouse=True)
+def no_grad():
+    with torch.no_grad():
+        yield
+
+
+def _rows(g, *shape, std=1.0):
+    return (torch.randn(*shape, generator=g) * std).bfloat16()
+
+
+def _tables(g, lengths, page, spare=2):
+    """Pages in no order, and how many there are."""
+    need = [(n + page - 1) // page for n in lengths]
+    order = torch.randperm(sum(need) + spare, generator=g).tolist()
+    tables, at = [], 0
+    for n in need:
+        tables.append(order[at:at + n])
+        at += n
+    return tables, sum(need) + spare
+
+
+class Run:
+    """Sequences in a cache and in the plain form, appended to in steps."""
+
+    def __init__(self, dtype, kv_heads, d, page, steps, seed=0):
+        """steps: lists of new rows per sequence."""
+        from parrot import PagedKVCache
+        self.g = torch.Generator().manual_seed(seed)
+        self.lengths = [0] * len(steps[0])
+        total = [sum(s) for s in zip(*steps)]
+        self.tables, pages = _tables(self.g, total, page)
+        self.cache = PagedKVCache(pages, page, kv_heads, d, dtype)
+        self.plain = Plain(dtype, kv_heads, d, len(total))
+        self.kv_heads, self.d = kv_heads, d
+
+    def batch(self, new):
+        from parrot import PagedBatch
+        return PagedBatch.from_lists(self.tables, self.lengths, new)
+
+    def append(self, new, k=None, v=None):
+        n = sum(new)
+        k = _rows(self.g, n, self.kv_heads, self.d) if k is None else k
+        v = _rows(self.g, n, self.kv_heads, self.d) if v is None else v
+        self.lengths = [a + b for a, b in zip(self.lengths, new)]
+        batch = self.batch(new)
+        self.cache.append(k.cuda(), v.cuda(), batch)
+        self.plain.append(k, v, new)
+        return batch
+
+    def attend(self, heads, new, batch, scale=None, window=None, sinks=0, q=None, gone=()):
+        q = _rows(self.g, sum(new), heads, self.d, std=1.5) if q is None else q
+        scale = self.d ** -0.5 if scale is None else scale
+        got = self.cache.attend(q.cuda(), batch, scale=scale, window=window, sinks=sinks)
+        ref, bound = self.plain.attend(q, new, scale, window, sinks, gone)
+        off = (got.double().cpu() - ref).abs()
+        assert torch.isfinite(got).all()
+        worst = (off / bound.clamp_min(1e-30)).max().item() if off.numel() else 0.0
+        print(f"worst error {worst:.3f} of the bound", flush=True)
+        assert (off <= bound + 1e-30).all()
+        return got
+
+
+# ---------------------------------------------------------------------------
+# append and read
+# ---------------------------------------------------------------------------
+
+# chunk edges inside a block, at its edge and past it; a sequence without new
+# rows; single tokens; pages of one block and of several
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("kv_heads,d,page,steps", [
+    (2, 96, 64, [[1, 1], [1, 31], [1, 0], [1, 1]]),
+    (1, 64, 32, [[33, 0, 95], [32, 5, 1], [0, 64, 33]]),
+    (3, 128, 128, [[257], [1], [63], [64]]),
+    (2, 96, 96, [[100, 96, 3, 29], [1, 1, 1, 3]]),
+])
+def test_append_and_read(dtype, kv_heads, d, page, steps):
+    run = Run(dtype, kv_heads, d, page, steps)
+    for new in steps:
+        print(f"append {NAMES[dtype]} {new} after {run.lengths}", flush=True)
+        batch = run.append(new)
+    longest = max(run.lengths) + 5
+    key, value = run.cache.read(batch, longest)
+    assert key.shape == value.shape == (len(run.lengths), kv_heads, longest, d)
+    for i, n in enumerate(run.lengths):
+        for got, want in ((key[i], run.plain.k[i]), (value[i], run.plain.v[i])):
+            assert torch.equal(got[:, :n].double().cpu(), want.transpose(0, 1))
+            assert not got[:, n:].any()
+    # fewer positions than there are, into a slice of a longer cache
+    room = [torch.full((len(run.lengths), kv_heads, 2 * longest, d), 7.0, dtype=torch.bfloat16,
+                       device="cuda") for _ in range(2)]
+    run.cache.read(batch, 40, out=tuple(x[:, :, 3:43] for x in room))
+    for x, y in zip(room, (key, value)):
+        n = min(40, longest)
+        assert torch.equal(x[:, :, 3:3 + n], y[:, :, :n])
+        assert (x[:, :, :3] == 7).all() and (x[:, :, 43:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+def test_append_leaves_the_rest(dtype):
+    """Other positions, pages and rows of no sequence stay as they are; a page id
+    outside the cache and positions past the table take nothing."""
+    from parrot import PagedBatch, PagedKVCache
+    cache = PagedKVCache(6, 64, 2, 96, dtype)
+    for x in (cache.key, cache.value):
+        x.view(torch.uint8).fill_(0x31)
+    for x in (cache.key_exponent, cache.value_exponent):
+        if x is not None:
+            x.fill_(0x77)
+    g = torch.Generator().manual_seed(3)
+    k, v = _rows(g, 80, 2, 96), _rows(g, 80, 2, 96)
+    # rows 0-2 nobody's, then 40 at 30 .. 69 over pages 4 and 1, 20 on pages that
+    # are not there, 7 of which 5 lie past the table; the rest nobody's
+    def i32(x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda")
+    batch = PagedBatch(i32([[4, 1], [-1, 6], [3, -1]]), i32([70, 100, 133]), i32([3, 43, 63, 70]))
+    before = [x.clone() for x in (cache.key, cache.value)]
+    whole = cache.read(PagedBatch(i32([[0], [1], [2], [3], [4], [5]]), i32([64] * 6),
+                                  i32([0] * 7)), 64)
+    cache.append(k.cuda(), v.cuda(), batch)
+    after = cache.read(PagedBatch(i32([[0], [1], [2], [3], [4], [5]]), i32([64] * 6),
+                                  i32([0] * 7)), 64)
+    for x, y, rows in ((whole[0], after[0], k), (whole[1], after[1], v)):
+        want = x.clone()
+        new = stored(rows[3:43], dtype).transpose(0, 1).to(torch.bfloat16).cuda()
+        want[4, :, 30:] = new[:, :34]
+        want[1, :, :6] = new[:, 34:]
+        assert torch.equal(y, want)
+    for x, y in zip(before, (cache.key, cache.value)):
+        changed = (x.view(torch.uint8) != y.view(torch.uint8)).flatten(1).any(1).tolist()
+        assert changed == [False, True, False, False, True, False]
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=NAMES.get)
+def test_rows_of_every_size(dtype):
+    """Zeros, the smallest and largest numbers, halves of steps, single large
+    values, and rows that hold a NaN or an infinity."""
+    d = 64
+    g = torch.Generator().manual_seed(5)
+    rows = [torch.zeros(d), torch.full((d,), -0.0), torch.full((d,), 1e-40),
+            torch.full((d,), 3.3e38), torch.linspace(-448, 448, d), torch.linspace(-127, 127, d),
+            torch.arange(d) / 2.0, torch.arange(d) * 2.0 ** -120, 2.0 ** torch.arange(-63.0, 1)]
+    for p in range(-30, 31, 6):
+        rows.append(torch.randn(d, generator=g) * 2.0 ** p)
+    # just under and over the powers at which the scale steps
+    for top in (448.0, 449.0, 450.0, 127.0, 127.5, 128.0, 1.75, 1.7578125, 1.984375, 1.9921875):
+        x = torch.randn(d, generator=g) * 0.3 * top
+        x = x.clamp(-top, top)
+        x[7] = -top
+        rows.append(x)
+    for bad in (math.nan, math.inf, -math.inf):
+        x = torch.randn(d, generator=g)
+        x[11] = bad
+        rows.append(x)
+    rows = torch.stack(rows).bfloat16()[:, None]
+    run = Run(dtype, 1, d, 64, [[len(rows)]])
+    batch = run.append([len(rows)], rows, rows.flip(0))
+    for got, x in zip(run.cache.read(batch, len(rows)), (rows, rows.flip(0))):
+        got, want = got[0, 0].double().cpu(), stored(x, dtype)[:, 0]
+        assert torch.equal(got.isnan(), want.isnan()) and want.isnan().any()
+        assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+LAYOUTS = [(8, 2, 96), (4, 4, 64), (6, 2, 128), (16, 1, 64), (5, 1, 96)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("heads,kv_heads,d", LAYOUTS)
+@pytest.mark.parametrize("steps,window,sinks", [
+    ([[1]], None, 0),                                   # a first token alone
+    ([[31, 32, 33, 64], [1, 1, 1, 1]], None, 0),        # single tokens past block edges
+    ([[200, 7, 0, 65], [3, 0, 9, 40]], 50, 0),          # ragged chunks, one sequence idle
+    ([[300, 500], [1, 2]], 100, 5),                     # sinks far from the window
+    ([[130, 97], [33, 64]], 40, 70),                    # more sinks than window
+    ([[70]], 1, 0), ([[70]], 1, 33), ([[90]], 64, 30),  # one key; sinks that join the window
+])
+def test_attend(dtype, heads, kv_heads, d, steps, window, sinks):
+    print(f"attend {NAMES[dtype]} {heads}/{kv_heads} of {d}, {steps}, window {window} + {sinks}",
+          flush=True)
+    run = Run(dtype, kv_heads, d, 64, steps, seed=len(steps) + d)
+    for new in steps:
+        batch = run.append(new)
+        run.attend(heads, new, batch, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("steps,page,window,sinks", [
+    ([[3000, 900], [1, 1]], 32, None, 0),       # long contexts, split over workgroups
+    ([[3000, 900], [1, 6]], 256, 2048, 4),
+    ([[1500], [200]], 96, None, 0),             # a chunk over a context
+    ([[700, 333], [513, 260]], 64, 300, 40),    # hundreds of rows
+])
+def test_attend_long(dtype, steps, page, window, sinks):
+    run = Run(dtype, 2, 96, page, steps, seed=page)
+    for new in steps:
+        print(f"attend {NAMES[dtype]} {new} after {run.lengths}", flush=True)
+        batch = run.append(new)
+        run.attend(8, new, batch, window=window, sinks=sinks)
+
+
+def test_attend_scales_and_strides():
+    """Negative and large scales; rows of a packed projection, strides that the
+    kernels do not read in place, an offset that is not aligned."""
+    run = Run(torch.bfloat16, 2, 64, 32, [[77, 40]])
+    packed = _rows(run.g, 117, 10, 64).cuda()
+    run.lengths = [77, 40]
+    batch = run.batch([77, 40])
+    run.cache.append(packed[:, 6:8], packed[:, 8:], batch)
+    run.plain.append(packed[:, 6:8].cpu(), packed[:, 8:].cpu(), [77, 40])
+    for scale in (0.125, -0.125, 3.0, 1e-3):
+        q = packed[:, :6]
+        got = run.cache.attend(q, batch, scale=scale)
+        ref, bound = run.plain.attend(q.cpu(), [77, 40], scale)
+        assert ((got.double().cpu() - ref).abs() <= bound).all()
+        for other in (q.contiguous(), q.transpose(0, 1).contiguous().transpose(0, 1),
+                      torch.empty(117 * 384 + 1, dtype=q.dtype, device="cuda")[1:]
+                      .view(117, 6, 64).copy_(q)):
+            assert torch.equal(run.cache.attend(other, batch, scale=scale), got)
+
+
+def test_rows_without_keys():
+    """More new rows than positions, lengths of zero, pages that are not there: 0
+    where a row sees nothing, and rows of no sequence left as they are."""
+    from parrot import PagedBatch
+    run = Run(torch.bfloat16, 1, 64, 32, [[64, 64, 10]])
+    run.append([64, 64, 10])
+    def i32(x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda")
+    table = [run.tables[0], run.tables[1], run.tables[2] + [-1]]
+    q = _rows(run.g, 30, 2, 64)
+    for kw in ({}, {"window": 8, "sinks": 1}):
+        # 12 rows of which the last 4 have positions; 5 rows of an empty sequence;
+        # 6 whose pages are not there; 3 rows of nobody
+        table_t = i32([table[0], [9999, -7], table[2]])
+        batch = PagedBatch(table_t, i32([4, 0, 10]), i32([0, 12, 17, 23]))
+        out = torch.full((30, 128), 3.0, dtype=torch.bfloat16, device="cuda")
+        got = run.cache.attend(q.cuda(), batch, scale=0.125, out=out, **kw)
+        assert got is out
+        assert not got[:8].any() and not got[12:17].any() and (got[23:] == 3).all()
+        part = Plain(torch.bfloat16, 1, 64, 1)
+        part.k, part.v = [run.plain.k[0][:4]], [run.plain.v[0][:4]]
+        ref, bound = part.attend(q[8:12], [4], 0.125, kw.get("window"), kw.get("sinks", 0))
+        assert ((got[8:12].double().cpu() - ref).abs() <= bound).all()
+        gone = PagedBatch(i32([[9999, -7], [-1, -1]]), i32([40, 64]), i32([0, 12, 20]))
+        out.fill_(3.0)
+        run.cache.attend(q.cuda(), gone, scale=0.125, out=out, **kw)
+        assert not out[:20].any() and (out[20:] == 3).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+def test_pages_given_back(dtype):
+    """Pages that the window has left are not read: their ids may name nothing."""
+    run = Run(dtype, 2, 96, 32, [[500], [1]])
+    run.append([500])
+    batch = run.append([1])
+    q = _rows(run.g, 1, 8, 96)
+    want = run.attend(8, [1], batch, window=100, sinks=20, q=q)
+    run.tables = [[p if i < 1 or i >= 12 else -1 for i, p in enumerate(run.tables[0])]]
+    assert torch.equal(run.attend(8, [1], run.batch([1]), window=100, sinks=20, q=q), want)
+    # ... and where the window does reach them, they are not seen
+    run.tables = [[p if i != 14 else run.cache.key.shape[0] for i, p in enumerate(run.tables[0])]]
+    run.attend(8, [1], run.batch([1]), window=100, sinks=20, q=q, gone=[(0, 448, 480)])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_unseen_rows_do_not_reach_a_row(dtype, bad):
+    """Infinities and NaN among keys and values that a row does not see: later
+    positions of its own chunk, positions the window has left (in a block that it
+    still covers), and stale ones past the length."""
+    run = Run(dtype, 2, 96, 64, [[150]])
+    k, v = _rows(run.g, 150, 2, 96), _rows(run.g, 150, 2, 96)
+    k[77, 0, 5] = v[77, 0, 5] = bad
+    v[101, 1, 50] = bad
+    run.append([150], k, v)
+    q = _rows(run.g, 150, 8, 96, std=1.5)
+    batch = run.batch([150])
+    for window, sinks in ((20, 0), (20, 3)):
+        got = run.cache.attend(q.cuda(), batch, scale=0.1, window=window, sinks=sinks)
+        got = got.double().cpu().view(150, 2, 4, 96)
+        # the same without the bad rows
+        kc, vc = k.clone(), v.clone()
+        kc[77, 0], vc[77, 0], vc[101, 1] = 0, 0, 0
+        clean = Plain(dtype, 2, 96, 1)
+        clean.append(kc, vc, [150])
+        ref, bound = clean.attend(q, [150], 0.1, window, sinks)
+        ref, bound = ref.view(150, 2, 4, 96), bound.view(150, 2, 4, 96)
+        pos = torch.arange(150)
+        for head, rows in ((0, [77]), (1, [101])):
+            sees = sum(((pos >= r) & (pos < r + window)).int() for r in rows) > 0
+            assert ((got[:, head] - ref[:, head]).abs() <= bound[:, head])[~sees].all()
+            # and where a row does see it, it is not finite either (all of the
+            # row's, or that value's dimension)
+            assert not torch.isfinite(got[:, head][sees]).all(-1).any()
+    # stale rows past the length: a shorter sequence over the same pages
+    run.lengths = [70]
+    short = run.batch([70])
+    got = run.cache.attend(q[:70].cuda(), short, scale=0.1)
+    clean = Plain(dtype, 2, 96, 1)
+    clean.append(k[:70], v[:70], [70])
+    ref, bound = clean.attend(q[:70], [70], 0.1)
+    assert ((got.double().cpu() - ref).abs() <= bound).all()
+
+
+def test_far_pages():
+    """Pages past 2^31 and 2^32 elements and bytes."""
+    from parrot import PagedBatch, PagedKVCache
+    page, d = 128, 128
+    pages = (1 << 32) // (2 * page * d) + 300
+    for dtype in (torch.int8, torch.bfloat16):
+        print(f"far pages {NAMES[dtype]}", flush=True)
+        cache = PagedKVCache(pages, page, 2, d, dtype)
+        g = torch.Generator().manual_seed(1)
+        k, v, q = _rows(g, 300, 2, d), _rows(g, 300, 2, d), _rows(g, 300, 4, d)
+        tables = [[pages - 1, 0, pages // 2]]
+        batch = PagedBatch.from_lists(tables, [300], [300])
+        cache.append(k.cuda(), v.cuda(), batch)
+        plain = Plain(dtype, 2, d, 1)
+        plain.append(k, v, [300])
+        got = cache.attend(q.cuda(), batch, scale=0.1)
+        ref, bound = plain.attend(q, [300], 0.1)
+        assert ((got.double().cpu() - ref).abs() <= bound).all()
+        key, value = cache.read(batch, 300)
+        assert torch.equal(key[0].double().cpu(), plain.k[0].transpose(0, 1))
+        assert torch.equal(value[0].double().cpu(), plain.v[0].transpose(0, 1))
+        del cache
+        torch.cuda.empty_cache()
+
+
+def test_many_sequences():
+    """More sequences than a wavefront has lanes, most of them without new rows."""
+    g = torch.Generator().manual_seed(2)
+    first = torch.randint(0, 40, (150,), generator=g).tolist()
+    then = torch.randint(0, 3, (150,), generator=g).tolist()
+    run = Run(torch.float8_e4m3fn, 1, 64, 32, [first, then])
+    for new in (first, then):
+        batch = run.append(new)
+        run.attend(2, new, batch, window=17, sinks=2)
+
+
+# ---------------------------------------------------------------------------
+# streams and graphs
+# ---------------------------------------------------------------------------
+
+def test_captured_steps():
+    """Append and attention captured once, replayed for growing sequences: every
+    replay as the eager calls; two graphs at once over two caches."""
+    from parrot import PagedBatch
+    steps = [[600, 90]] + [[1, 1]] * 12
+    runs = [Run(t, 2, 96, 64, steps, seed=i) for i, t in enumerate(TYPES[:2])]
+    held = []
+    for run in runs:
+        run.append([600, 90])
+        k, v, q = (torch.empty(2, h, 96, dtype=torch.bfloat16, device="cuda") for h in (2, 2, 8))
+        lengths = torch.tensor(run.lengths, dtype=torch.int32, device="cuda")
+        batch = PagedBatch(run.batch([1, 1]).table, lengths,
+                           torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"))
+
+        def step(run=run, k=k, v=v, q=q, lengths=lengths, batch=batch):
+            lengths.add_(1)
+            run.cache.append(k, v, batch)
+            return run.cache.attend(q, batch, scale=0.1, window=400, sinks=8)
+        graph = torch.cuda.CUDAGraph()
+        for x in (k, v, q):
+            x.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            out = step()
+        held.append((graph, out, k, v, q, batch))
+    for i in range(10):
+        news = []
+        for run, (graph, out, k, v, q, _) in zip(runs, held):
+            new = [_rows(run.g, 2, h, 96) for h in (2, 2, 8)]
+            for x, y in zip((k, v, q), new):
+                x.copy_(y)
+            news.append(new)
+        for _, (graph, *_) in zip(runs, held):
+            graph.replay()
+        torch.cuda.synchronize()
+        for run, (graph, out, *_), (k, v, q) in zip(runs, held, news):
+            run.plain.append(k, v, [1, 1])
+            run.lengths = [n + 1 for n in run.lengths]
+            ref, bound = run.plain.attend(q, [1, 1], 0.1, 400, 8)
+            assert ((out.double().cpu() - ref).abs() <= bound).all(), i
+            assert torch.equal(out, run.cache.attend(q.cuda(), run.batch([1, 1]), scale=0.1,
+                                                     window=400, sinks=8))
+        torch.zeros(1 << 20, device="cuda").sum().item()  # eager work in between
+
+
+def test_two_streams():
+    """The same cache read from two streams at once gives what one stream gives."""
+    run = Run(torch.int8, 2, 96, 64, [[2500, 1800], [1, 1]])
+    run.append([2500, 1800])
+    batch = run.append([1, 1])
+    qs = [_rows(run.g, 2, 8, 96).cuda() for _ in range(2)]
+    want = [run.cache.attend(q, batch, scale=0.1) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, q in zip(streams, qs):
+            with torch.cuda.stream(s):
+                got.append(run.cache.attend(q, batch, scale=0.1))
+    torch.cuda.synchronize()
+    for y, w in zip(got, itertools.cycle(want)):
+        assert torch.equal(y, w)
