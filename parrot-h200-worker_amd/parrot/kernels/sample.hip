@@ -12,11 +12,17 @@
 //
 // A workgroup per row, which keeps the row in LDS (32768 logits; longer rows are
 // read again, from L2, in each pass).  Nothing is sorted: the border of top-k or
-// top-p is found by one histogram over the distance from the largest logit, its
-// bins as wide as to spread the row, in whole numbers (counts or weights), and
-// the order of the few logits in the border's bin by comparing each with each.
-// A bin with too many of them (equal logits, tiny temperatures) is split by its
-// range of bit patterns, 2048 parts at a time.
+// top-p is found by one histogram over the distance from the largest logit (in
+// whole numbers: counts or weights) and the order of the few logits in the
+// border's bin by comparing each with each.  A bin with too many of them (equal
+// logits) is split by its range of bit patterns, 2047 parts at a time.
+//
+// What bounds it: one CU's vector instructions, some 10 clocks per logit and pass
+// of 20 instructions, and the 64-bit exponentials.  So with a top_k of up to 512
+// the row is passed twice only: the k-th largest of the 1024 threads' maxima bounds
+// the k-th largest logit from below, and what passes it, hardly more than k, is
+// gathered in the order of indices, one logit a thread.  Without top_k each
+// exponential is made once and its weight stays in registers.
 #include <math.h>
 
 #include "common.h"
@@ -32,8 +38,27 @@ constexpr int kHeld = 32768;       // logits of a row that LDS holds
 constexpr int kBins = 2048;
 constexpr int kList = 256;         // logits compared each with each
 constexpr int kTable = 256;
+constexpr int kPairs = 128;        // logits of a list that are ordered each with each
+constexpr int kShort = 512;        // top_k for which a list is made
 
 enum LogitType { kLogitF32 = 0, kLogitBf16 = 1, kLogitF16 = 2 };
+
+// 2^(k / 256), by the exponential's series.
+struct Powers {
+  double at[kTable];
+  constexpr Powers() : at() {
+    for (int k = 0; k < kTable; ++k) {
+      const long double x = 0.693147180559945309417232121458L * k / kTable;
+      long double sum = 1.0L, term = 1.0L;
+      for (int i = 1; i < 24; ++i) {
+        term *= x / i;
+        sum += term;
+      }
+      at[k] = static_cast<double>(sum);
+    }
+  }
+};
+__device__ const Powers kPowers;
 
 struct SampleArgs {
   const void* logits;
@@ -61,10 +86,13 @@ __device__ __forceinline__ float logit(const void* row, int i) {
 }
 
 // Four logits from i on; a NaN, and what lies past the row, is -infinity.
+// aligned: the row is, and a whole number of fours: loads without a branch.
 template <int TYPE>
-__device__ __forceinline__ float4 logits4(const void* row, int i, int n, bool aligned) {
+__device__ __forceinline__ float4 logits4(const void* row, int at, int n, bool aligned) {
   float x[4];
-  if (aligned && i + 3 < n) {
+  int i = at;
+  if (aligned) {
+    i = min(at, n - 4);
     if constexpr (TYPE == kLogitF32) {
       const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + i);
       x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
@@ -84,7 +112,7 @@ __device__ __forceinline__ float4 logits4(const void* row, int i, int n, bool al
     for (int j = 0; j < 4; ++j) x[j] = i + j < n ? logit<TYPE>(row, i + j) : -INFINITY;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = x[j] == x[j] ? x[j] : -INFINITY;
+  for (int j = 0; j < 4; ++j) x[j] = x[j] == x[j] && at < n ? x[j] : -INFINITY;
   return make_float4(x[0], x[1], x[2], x[3]);
 }
 
@@ -100,34 +128,45 @@ struct Shared {
     uint64_t bins[kBins];
     Entry list[kList];
   };
+  float few[kThreads];     // a list of logits and their indices, in order
+  int few_index[kThreads];
   uint64_t wave[kWaves];
   uint64_t before;
   uint32_t low[kWaves], high[kWaves];
   int found;
   int count;
-  uint32_t edge;
+  float edge;
   int until;
 };
 
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
-  return __shfl_up(static_cast<unsigned long long>(v), d);
+// v of another lane by DPP, 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false);
+  const uint32_t hi =
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xf, false);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
-__device__ __forceinline__ uint64_t wave_total(uint64_t v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(static_cast<unsigned long long>(v), d);
-  return v;
-}
-
+// The sum of the lanes up to this one: by 1, 2, 4, 8 lanes to the right inside rows
+// of 16, then a row's last lane to the next row (rows 1, 3) and lane 31 to the upper
+// half (VALU moves; a shuffle is an LDS trip).
 __device__ __forceinline__ uint64_t wave_upto(uint64_t v) {
-  const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const uint64_t x = shfl_up64(v, d);
-    if (lane >= d) v += x;
-  }
-  return v;
+  v += dpp64<0x111, 0xf>(v);
+  v += dpp64<0x112, 0xf>(v);
+  v += dpp64<0x114, 0xf>(v);
+  v += dpp64<0x118, 0xf>(v);
+  v += dpp64<0x142, 0xa>(v);
+  return v + dpp64<0x143, 0xc>(v);
 }
+
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), kWave - 1);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), kWave - 1);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
+__device__ __forceinline__ uint64_t wave_total(uint64_t v) { return last_lane(wave_upto(v)); }
 
 // A row: `steps` times 256 consecutive logits per wavefront, so that sums over
 // wavefronts, steps, lanes and a lane's four are sums by index.
@@ -146,26 +185,132 @@ struct Row {
     if constexpr (HELD) return *reinterpret_cast<const float4*>(held + i);
     return logits4<TYPE>(at, i, n, aligned);
   }
-  // f(index, logit) for this thread's logits
+  // f(index, logit, weight if one is held) for this thread's logits
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
+#pragma unroll 2
     for (int s = 0; s < steps; ++s) {
       const int i = first(s);
-      if (i >= n) break;
+      if (i - 4 * static_cast<int>(threadIdx.x & (kWave - 1)) >= n) break;  // (the wavefront's)
       const float4 v = get(s);
-      f(i, v.x);
-      if (i + 1 < n) f(i + 1, v.y);
-      if (i + 2 < n) f(i + 2, v.z);
-      if (i + 3 < n) f(i + 3, v.w);
+      if (i < n) f(i, v.x, uint64_t{0});
+      if (i + 1 < n) f(i + 1, v.y, uint64_t{0});
+      if (i + 2 < n) f(i + 2, v.z, uint64_t{0});
+      if (i + 3 < n) f(i + 3, v.w, uint64_t{0});
     }
+  }
+  // The first index at which the sum of f passes `target` (below the whole); f's
+  // shares as total() left them.
+  template <typename F>
+  __device__ __forceinline__ int locate(F f, uint64_t target, Shared& sh) const {
+    return locate_by(
+        [&](int s, uint64_t(&w)[4]) {
+          const int i = first(s);
+          const float4 v = get(s);
+          w[0] = i < n ? f(i, v.x, uint64_t{0}) : 0;
+          w[1] = i + 1 < n ? f(i + 1, v.y, uint64_t{0}) : 0;
+          w[2] = i + 2 < n ? f(i + 2, v.z, uint64_t{0}) : 0;
+          w[3] = i + 3 < n ? f(i + 3, v.w, uint64_t{0}) : 0;
+        },
+        target, sh);
+  }
+  template <typename W>
+  __device__ __forceinline__ int locate_by(W weights, uint64_t target, Shared& sh) const {
+    const int wave = threadIdx.x >> 6;
+    uint64_t before = 0;
+    for (int w = 0; w < wave; ++w) before += sh.wave[w];
+    if (before <= target && target < before + sh.wave[wave]) {  // one wavefront
+      for (int s = 0; s < steps; ++s) {
+        uint64_t w[4];
+        weights(s, w);
+        const uint64_t mine = w[0] + w[1] + w[2] + w[3];
+        const uint64_t upto = wave_upto(mine);
+        const uint64_t all = last_lane(upto);
+        if (target < before + all) {
+          uint64_t at = before + upto - mine;
+          if (at <= target && target < at + mine) {
+            int j = 0;
+            while (target >= at + w[0]) {  // (at most three times)
+              at += w[0];
+              w[0] = w[1], w[1] = w[2], w[2] = w[3];
+              ++j;
+            }
+            sh.found = first(s) + j;
+          }
+          break;
+        }
+        before += all;
+      }
+    }
+    __syncthreads();
+    return sh.found;
+  }
+};
+
+// A held row and its weights, in registers (past its end: -infinity, of weight 0).
+template <typename R>
+struct Weights {
+  static constexpr int kSteps = kHeld / (kWaves * kStep);
+  const R row;
+  uint64_t w[kSteps][4];
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      if (s >= row.steps) break;
+      const int i = row.first(s);
+      const float4 v = row.get(s);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(i + j, x[j], w[s][j]);
+      __builtin_amdgcn_sched_barrier(0);  // (a step at a time: the weights fill the registers)
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ int locate(F f, uint64_t target, Shared& sh) const {
+    return row.locate_by(
+        [&](int s, uint64_t(&y)[4]) {
+          const int i = row.first(s);
+          const float4 v = row.get(s);
+          const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int q = 0; q < kSteps; ++q)
+            if (q == s) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) y[j] = f(i + j, x[j], w[q][j]);
+            }
+        },
+        target, sh);
+  }
+};
+
+// A list of at most one logit a thread, in the order of indices.
+struct Few {
+  int n;
+  float x;     // this thread's
+  uint64_t w;  // and its weight
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    if (static_cast<int>(threadIdx.x) < n) f(static_cast<int>(threadIdx.x), x, w);
+  }
+  template <typename F>
+  __device__ __forceinline__ int locate(F f, uint64_t target, Shared& sh) const {
+    const int t = threadIdx.x;
+    uint64_t before = 0;
+    for (int w = 0; w < (t >> 6); ++w) before += sh.wave[w];
+    const uint64_t mine = t < n ? f(t, x, w) : 0;
+    before += wave_upto(mine) - mine;
+    if (before <= target && target < before + mine) sh.found = t;
+    __syncthreads();
+    return sh.found;
   }
 };
 
 // The sum of f over the row; leaves each wavefront's share in sh.wave.
 template <typename R, typename F>
-__device__ uint64_t total(const R& row, F f, Shared& sh) {
+__device__ __forceinline__ uint64_t total(const R& row, F f, Shared& sh) {
   uint64_t t = 0;
-  row.each([&](int i, float x) { t += f(i, x); });
+  row.each([&](int i, float x, uint64_t w) { t += f(i, x, w); });
   t = wave_total(t);
   __syncthreads();
   if ((threadIdx.x & (kWave - 1)) == 0) sh.wave[threadIdx.x >> 6] = t;
@@ -174,41 +319,6 @@ __device__ uint64_t total(const R& row, F f, Shared& sh) {
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) t += sh.wave[i];
   return t;
-}
-
-// The first index at which the sum of f passes `target` (below the whole); f's
-// shares as total() left them.
-template <typename R, typename F>
-__device__ int locate(const R& row, F f, uint64_t target, Shared& sh) {
-  const int wave = threadIdx.x >> 6;
-  uint64_t before = 0;
-  for (int w = 0; w < wave; ++w) before += sh.wave[w];
-  if (before <= target && target < before + sh.wave[wave]) {  // one wavefront
-    for (int s = 0; s < row.steps; ++s) {
-      const int i = row.first(s);
-      const float4 v = row.get(s);
-      const uint64_t f0 = i < row.n ? f(i, v.x) : 0, f1 = i + 1 < row.n ? f(i + 1, v.y) : 0;
-      const uint64_t f2 = i + 2 < row.n ? f(i + 2, v.z) : 0;
-      const uint64_t f3 = i + 3 < row.n ? f(i + 3, v.w) : 0;
-      const uint64_t mine = f0 + f1 + f2 + f3;
-      const uint64_t upto = wave_upto(mine);
-      const uint64_t all = __shfl(static_cast<unsigned long long>(upto), kWave - 1);
-      if (target < before + all) {
-        uint64_t at = before + upto - mine;
-        if (at <= target && target < at + mine) {
-          int j = i;
-          if (target >= at + f0) ++j, at += f0;
-          if (j == i + 1 && target >= at + f1) ++j, at += f1;
-          if (j == i + 2 && target >= at + f2) ++j;
-          sh.found = j;
-        }
-        break;
-      }
-      before += all;
-    }
-  }
-  __syncthreads();
-  return sh.found;
 }
 
 // The first bin at which the sum over bins reaches `need`, and the sum before it;
@@ -237,40 +347,54 @@ __device__ __forceinline__ int find_bin(uint64_t need, uint64_t& before, Shared&
 }
 
 struct Edge {
-  uint32_t key;
+  float x;
   int until;
+  // (as by order_key: -0 and 0 are equal; there is no NaN)
+  __device__ __forceinline__ bool keeps(int i, float y) const {
+    return y > x || (y == x && i <= until);
+  }
 };
 
-// The last logit, in the order of size and index, that is needed for the sum of f
-// to reach `need` (1 .. the whole): its key and index.  per: bins per unit of
-// distance from `top`, the largest logit.
-template <typename R, typename F>
-__device__ Edge select(const R& row, F f, uint64_t need, float top, float per, Shared& sh) {
-  auto bin_of = [&](float x) {
-    const float d = x == top ? 0.0f : (top - x) * per;
+// The bin of a logit: by its distance from the largest, the last one for all that
+// lies further.
+struct Bins {
+  float top, per_unit;
+  __device__ __forceinline__ int operator()(float x) const {
+    const float d = x == top ? 0.0f : (top - x) * per_unit;
     return d < static_cast<float>(kBins - 1) ? static_cast<int>(d) : kBins - 1;
-  };
-  auto clear = [&] {
-    __syncthreads();
-    sh.bins[threadIdx.x] = sh.bins[threadIdx.x + kThreads] = 0;
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
-  };
-  auto add = [&](int bin, uint64_t v) {
-    if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[bin]), v);
-  };
-  clear();
-  row.each([&](int i, float x) {
-    const int b = bin_of(x);
-    if (b < kBins - 1) add(b, f(i, x));
-  });
+  }
+};
+
+__device__ __forceinline__ void clear_bins(Shared& sh) {
   __syncthreads();
+  sh.bins[threadIdx.x] = sh.bins[threadIdx.x + kThreads] = 0;
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+}
+
+__device__ __forceinline__ void add_to_bin(int bin, uint64_t v, Shared& sh) {
+  if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[bin]), v);
+}
+
+// The last logit, in the order of size and index, that is needed for the sum of f
+// to reach `need` (1 .. the whole): its key and index.  filled: the bins hold f's
+// sums already.
+template <typename R, typename F>
+__device__ __forceinline__ Edge select(const R& row, F f, uint64_t need, Bins bin_of, bool filled, Shared& sh) {
+  if (!filled) {
+    clear_bins(sh);
+    row.each([&](int i, float x, uint64_t w) {
+      const int b = bin_of(x);
+      if (b < kBins - 1) add_to_bin(b, f(i, x, w), sh);
+    });
+    __syncthreads();
+  }
   uint64_t before;
   const int bin = find_bin(need, before, sh);
   // The logits of that bin (one counter: a wavefront's in one step) and their keys'
   // range.
   uint32_t low = 0xffffffffu, high = 0;
-  row.each([&](int i, float x) {
+  row.each([&](int i, float x, uint64_t w) {
     if (bin_of(x) != bin) return;
     const uint32_t key = order_key(x);
     low = min(low, key);
@@ -280,7 +404,7 @@ __device__ Edge select(const R& row, F f, uint64_t need, float top, float per, S
     int at = 0;
     if (lane == __builtin_ctzll(who)) at = atomicAdd(&sh.count, __popcll(who));
     at = __shfl(at, __builtin_ctzll(who)) + __popcll(who & ((uint64_t{1} << lane) - 1));
-    if (at < kList) sh.list[at] = {f(i, x), key, i};
+    if (at < kList) sh.list[at] = {f(i, x, w), key, i};
   });
   __syncthreads();
   const int n = sh.count;
@@ -293,7 +417,7 @@ __device__ Edge select(const R& row, F f, uint64_t need, float top, float per, S
         if (e.key > mine.key || (e.key == mine.key && e.index < mine.index)) at += e.f;
       }
       if (at < need && need <= at + mine.f) {
-        sh.edge = mine.key;
+        sh.edge = key_value(static_cast<uint64_t>(mine.key) << 32);
         sh.until = mine.index;
       }
     }
@@ -317,10 +441,10 @@ __device__ Edge select(const R& row, F f, uint64_t need, float top, float per, S
   while (low < high) {
     int bits = 0;  // (high - low) >> bits < kBins - 1
     while (((high - low) >> bits) >= kBins - 1) ++bits;
-    clear();
-    row.each([&](int i, float x) {
+    clear_bins(sh);
+    row.each([&](int i, float x, uint64_t w) {
       const uint32_t key = order_key(x);
-      if (key >= low && key <= high) add((high - key) >> bits, f(i, x));
+      if (key >= low && key <= high) add_to_bin((high - key) >> bits, f(i, x, w), sh);
     });
     __syncthreads();
     uint64_t within;
@@ -329,9 +453,11 @@ __device__ Edge select(const R& row, F f, uint64_t need, float top, float per, S
     high -= b << bits;
     low = max(low, high - ((1u << bits) - 1));
   }
-  auto equal = [&](int i, float x) -> uint64_t { return order_key(x) == low ? f(i, x) : 0; };
+  auto equal = [&](int i, float x, uint64_t w) -> uint64_t {
+    return order_key(x) == low ? f(i, x, w) : 0;
+  };
   total(row, equal, sh);
-  return {low, locate(row, equal, need - before - 1, sh)};
+  return {key_value(static_cast<uint64_t>(low) << 32), row.locate(equal, need - before - 1, sh)};
 }
 
 template <int TYPE, bool HELD>
@@ -345,60 +471,67 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   row.held = held;
   row.n = a.vocab;
   row.steps = (a.vocab + kWaves * kStep - 1) / (kWaves * kStep);
-  row.aligned = (reinterpret_cast<uintptr_t>(row.at) & (4 * kBytes - 1)) == 0;
+  row.aligned = (reinterpret_cast<uintptr_t>(row.at) & (4 * kBytes - 1)) == 0 && row.n % 4 == 0;
   const double temperature = a.temperature ? a.temperature[r] : a.temperature_all;
   const int top_k = a.top_k ? a.top_k[r] : a.top_k_all;
   const double top_p = a.top_p ? a.top_p[r] : a.top_p_all;
   // (the largest always stays)
   const double min_p = fmin(a.min_p ? a.min_p[r] : a.min_p_all, 1.0);
-  if (t < kTable) sh.table[t] = exp2(t * (1.0 / kTable));
+  if (t < kTable) sh.table[t] = kPowers.at[t];
 
-  // The largest logit (the lowest index among equal ones), the smallest finite one.
-  uint64_t best = 0;
-  float least = INFINITY;
-  for (int s = 0; s < row.steps; ++s) {
-    const int i = row.first(s);
-    if (i >= row.n && !HELD) break;
-    const float4 v = logits4<TYPE>(row.at, i, row.n, row.aligned);
-    if constexpr (HELD) *reinterpret_cast<float4*>(&held[i]) = v;
-    const float x[4] = {v.x, v.y, v.z, v.w};
+  // This thread's and the row's largest logit.
+  float mine = -INFINITY;
+  {
+    constexpr int kAhead = kHeld / (kWaves * kStep);  // loads in flight: a held row's
+    for (int from = 0; from < row.steps; from += kAhead) {
+      float4 v[kAhead];
+      if (row.aligned) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint64_t key = expert_key(x[j], i + j);
-      best = key > best ? key : best;
-      least = x[j] > -INFINITY ? fminf(least, x[j]) : least;
+        for (int s = 0; s < kAhead; ++s)
+          v[s] = logits4<TYPE>(row.at, from + s < row.steps ? row.first(from + s) : row.n, row.n,
+                               true);
+      } else {
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s)
+          v[s] = logits4<TYPE>(row.at, from + s < row.steps ? row.first(from + s) : row.n, row.n,
+                               false);
+      }
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        if (from + s >= row.steps) break;
+        if (HELD && s < row.steps) *reinterpret_cast<float4*>(&held[row.first(s)]) = v[s];
+        mine = fmaxf(fmaxf(mine, fmaxf(v[s].x, v[s].y)), fmaxf(v[s].z, v[s].w));
+      }
     }
   }
+  float top = mine;
 #pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const uint64_t key = __shfl_xor(static_cast<unsigned long long>(best), d);
-    best = key > best ? key : best;
-    least = fminf(least, __shfl_xor(least, d));
-  }
-  if ((t & (kWave - 1)) == 0) {
-    sh.wave[t >> 6] = best;
-    sh.low[t >> 6] = __float_as_uint(least);
-  }
+  for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if ((t & (kWave - 1)) == 0) sh.low[t >> 6] = __float_as_uint(top);
   __syncthreads();
-  for (int w = 0; w < kWaves; ++w) {
-    best = sh.wave[w] > best ? sh.wave[w] : best;
-    least = fminf(least, __uint_as_float(sh.low[w]));
-  }
-  const float top = key_value(best);
-  const bool greedy = !(temperature > 0.0) || top_k == 1;
-  if (top == -INFINITY || greedy) {  // nothing to draw from; nothing to choose
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, __uint_as_float(sh.low[w]));
+  auto answer = [&](int token, double share) {
     if (t == 0) {
-      a.token[r] = top == -INFINITY ? -1 : key_expert(best);
-      if (a.probability) a.probability[r] = top == -INFINITY ? 0.0f : 1.0f;
+      a.token[r] = token;
+      if (a.probability) a.probability[r] = static_cast<float>(share);
     }
-    return;
+  };
+  if (top == -INFINITY) return answer(-1, 0.0);  // nothing to draw from
+  if (!(temperature > 0.0) || top_k == 1) {      // the first of the largest
+    auto largest = [&](int, float x, uint64_t) -> uint64_t { return x == top; };
+    total(row, largest, sh);
+    return answer(row.locate(largest, 0, sh), 1.0);
   }
 
-  // log2 w, and w 2^shift: 2^y = 2^(k / 256) e^r with k = round(256 y), r = (256 y -
-  // k) ln 2 / 256, |r| <= 0.00136, whose series to the third power is right to 2e-13.
+  // log2 w (a largest logit of infinity: 0 for it, -infinity for the others), and w
+  // 2^shift: 2^y = 2^(k / 256) e^r with k = round(256 y), r = (256 y - k) ln 2 / 256,
+  // |r| <= 0.00136, whose series to the third power is right to 2e-13.
   const double per_unit = 1.4426950408889634074 / temperature;
+  const double origin = top < INFINITY ? top : 1e300;
+  const double lowest = -(a.shift + 2);  // 2^lowest rounds to 0
   auto power = [&](float x) -> double {
-    return x == top ? 0.0 : x == -INFINITY ? -INFINITY : (static_cast<double>(x) - top) * per_unit;
+    return fmax(fmin((static_cast<double>(x) - origin) * per_unit, 0.0), lowest);
   };
   auto scaled = [&](double y, int& k) -> double {  // 2^(y - floor(k / 256))
     const double z = y * kTable, whole = rint(z);
@@ -406,53 +539,187 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     const double e = (z - whole) * (0.69314718055994530942 / kTable);
     return sh.table[k & (kTable - 1)] * fma(fma(fma(e, 1.0 / 6.0, 0.5), e, 1.0), e, 1.0);
   };
-  auto mass = [&](double y) -> uint64_t {
-    if (!(y > -(a.shift + 2))) return 0;
+  auto mass = [&](float x) -> uint64_t {
     int k;
-    const uint64_t u = __builtin_bit_cast(uint64_t, scaled(y, k));
-    const int down = 52 - a.shift - (static_cast<int>(u >> 52) - 1023 + (k >> 8));  // 2 .. 56
+    const uint64_t u = __builtin_bit_cast(uint64_t, scaled(power(x), k));
+    const int down = 52 - a.shift - (static_cast<int>(u >> 52) - 1023 + (k >> 8));  // 2 .. 55
     return (((u & ((uint64_t{1} << 52) - 1)) | (uint64_t{1} << 52)) + (uint64_t{1} << (down - 1))) >>
            down;
   };
-  // Bins: over the whole row, or the distance from which on weights round to 0 (32
-  // T: the last ones are not counted but known to be there).
-  const float range = fminf(static_cast<float>(fmin(32.0 * temperature, 1e30)), top - least);
-  const float per = range > 0.0f && top < INFINITY ? (kBins - 1.5f) / range : 0.0f;
+  // The bins reach as far as weights do (2^-46 at 32 T), but no further than 32.
+  const Bins bins{top, top < INFINITY ? (kBins - 1) / static_cast<float>(
+                                            fmax(fmin(32.0 * temperature, 32.0), 1e-30)) : 0.0f};
+  const uint64_t least_mass = static_cast<uint64_t>(ldexp(fmax(min_p, 0.0), a.shift));
+  auto needed = [&](uint64_t all) -> uint64_t {  // of the mass, for top_p
+    const uint64_t x = static_cast<uint64_t>(ceil(fmax(top_p, 0.0) * static_cast<double>(all)));
+    return x < 1 ? 1 : x > all ? all : x;
+  };
+  auto drawn = [&](uint64_t all) -> uint64_t {
+    // (u below 1: the product is below the sum but for its rounding)
+    const double u = fmax(static_cast<double>(a.uniform[r]), 0.0) * static_cast<double>(all);
+    const uint64_t x = u < static_cast<double>(all) ? static_cast<uint64_t>(u) : all - 1;
+    return x < all ? x : all - 1;
+  };
+  auto share = [&](float x, uint64_t all) -> double {
+    int k;
+    const double w = scaled(power(x), k);
+    return ldexp(w, (k >> 8) + a.shift) / static_cast<double>(all);
+  };
+  auto one = [](int, float, uint64_t) -> uint64_t { return 1; };
+  auto held_weight = [](int, float, uint64_t w) -> uint64_t { return w; };
+  const bool by_count = top_k > 0 && top_k < row.n;
 
-  Edge edge{0, a.vocab};
-  auto kept = [&](int i, float x) {
-    const uint32_t k = order_key(x);
-    return k > edge.key || (k == edge.key && i <= edge.until);
-  };
-  if (top_k > 0 && top_k < a.vocab)
-    edge = select(row, [&](int, float) { return uint64_t{1}; }, top_k, top, per, sh);
-  if (top_p < 1.0) {
-    auto f = [&](int i, float x) -> uint64_t { return kept(i, x) ? mass(power(x)) : 0; };
-    const uint64_t all = total(row, f, sh);
-    uint64_t need = static_cast<uint64_t>(ceil(fmax(top_p, 0.0) * static_cast<double>(all)));
-    need = need < 1 ? 1 : need > all ? all : need;
-    edge = select(row, f, need, top, per, sh);
-  }
-  const double floor_p = min_p > 0.0 ? log2(min_p) : -INFINITY;
-  auto f = [&](int i, float x) -> uint64_t {
-    if (!kept(i, x)) return 0;
-    const double y = power(x);
-    return y >= floor_p ? mass(y) : 0;
-  };
-  const uint64_t all = total(row, f, sh);
-  // (u below 1: the product is below the sum but for its rounding)
-  const double u = fmax(static_cast<double>(a.uniform[r]), 0.0) * static_cast<double>(all);
-  const uint64_t target = u < static_cast<double>(all) ? static_cast<uint64_t>(u) : all - 1;
-  const int token = locate(row, f, target < all ? target : all - 1, sh);
-  if (t == 0) {
-    a.token[r] = token;
-    if (a.probability) {
-      float x = logit<TYPE>(row.at, token);
-      int k;
-      const double w = scaled(power(x), k);
-      a.probability[r] =
-          static_cast<float>(ldexp(w, (k >> 8) + a.shift) / static_cast<double>(all));
+  // A list that holds the top_k: what lies in the bins of the k largest of the
+  // threads' maxima.  Or the whole of a short row.
+  int few = row.n <= kThreads ? row.n : 0;
+  if (few == 0 && by_count && top_k <= kShort) {
+    clear_bins(sh);
+    const int b = bins(mine);
+    if (b < kBins - 1) add_to_bin(b, 1, sh);
+    __syncthreads();
+    uint64_t before;
+    const int last = find_bin(top_k, before, sh);
+    if (last < kBins - 1 && top < INFINITY) {
+      // One bin further down, so that no rounding here leaves one of them out (the
+      // count says whether it did).
+      const float from = top - static_cast<float>(last + 2) / bins.per_unit;
+      const int wave = t >> 6, lane = t & (kWave - 1);
+      int n = 0;
+      for (int s = 0; s < row.steps; ++s) {
+        const float4 v = row.get(s);
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n += __popcll(__ballot(x[j] >= from));
+      }
+      if (lane == 0) sh.low[wave] = n;
+      __syncthreads();
+      int at = 0;  // where this wavefront's begin
+      n = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) at += sh.low[w];
+        n += sh.low[w];
+      }
+      if (n >= top_k && n <= kThreads) {
+        const uint64_t below = (uint64_t{1} << lane) - 1;
+        for (int s = 0; s < row.steps; ++s) {
+          const int i = row.first(s);
+          const float4 v = row.get(s);
+          const float x[4] = {v.x, v.y, v.z, v.w};
+          uint64_t who[4];
+          int to = at;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            who[j] = __ballot(x[j] >= from);
+            to += __popcll(who[j] & below);
+            at += __popcll(who[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (x[j] >= from) {
+              sh.few[to] = x[j];
+              sh.few_index[to++] = i + j;
+            }
+          }
+        }
+        few = n;
+      }
     }
+    __syncthreads();
+  } else if (few > 0) {
+    row.each([&](int i, float x, uint64_t) {
+      sh.few[i] = x;
+      sh.few_index[i] = i;
+    });
+    __syncthreads();
+  }
+  if (few > 0) {
+    Few list{few, t < few ? sh.few[t] : -INFINITY, 0};
+    if (t < few) list.w = mass(list.x);
+    if (few <= kPairs) {
+      // Each with each: how many come before it, and their mass (of which all are
+      // kept by top_k where it is).
+      if (t < few) sh.list[t] = {list.w, order_key(list.x), t};
+      __syncthreads();
+      uint64_t before = 0;
+      if (t < few) {
+        const uint32_t key = order_key(list.x);
+        int rank = 0;
+        for (int j = 0; j < few; ++j) {
+          const Entry e = sh.list[j];
+          const bool ahead = e.key > key || (e.key == key && j < t);
+          rank += ahead;
+          before += ahead ? e.f : 0;
+        }
+        if (by_count && rank >= top_k) list.w = 0;
+      }
+      if (top_p < 1.0 && before >= needed(total(list, held_weight, sh))) list.w = 0;
+      if (list.w < least_mass) list.w = 0;
+      const uint64_t all = total(list, held_weight, sh);
+      const int at = list.locate(held_weight, drawn(all), sh);
+      return answer(sh.few_index[at], share(sh.few[at], all));
+    }
+    auto cut = [&](Edge edge) {
+      if (!edge.keeps(t, list.x)) list.w = 0;
+    };
+    if (by_count && top_k < few) cut(select(list, one, top_k, bins, false, sh));
+    if (top_p < 1.0)
+      cut(select(list, held_weight, needed(total(list, held_weight, sh)), bins, false, sh));
+    if (list.w < least_mass) list.w = 0;
+    const uint64_t all = total(list, held_weight, sh);
+    const int at = list.locate(held_weight, drawn(all), sh);
+    return answer(sh.few_index[at], share(sh.few[at], all));
+  }
+
+  Edge edge{-INFINITY, row.n};
+  if (by_count) edge = select(row, one, top_k, bins, false, sh);
+  auto f = [&](int i, float x, uint64_t) -> uint64_t {
+    const uint64_t w = mass(x);
+    return edge.keeps(i, x) ? w : 0;
+  };
+  if constexpr (HELD) {
+    // Every weight once, in registers.
+    using W = Weights<Row<TYPE, HELD>>;
+    W all_of{row, {}};
+    if (top_p < 1.0) clear_bins(sh);
+#pragma unroll
+    for (int s = 0; s < W::kSteps; ++s) {
+      if (s < row.steps) {
+        const int i = row.first(s);
+        const float4 v = row.get(s);
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t w = f(i + j, x[j], 0);
+          all_of.w[s][j] = w;
+          if (top_p < 1.0) {
+            const int b = bins(x[j]);
+            if (b < kBins - 1) add_to_bin(b, w, sh);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (top_p < 1.0) {
+      const uint64_t need = needed(total(all_of, held_weight, sh));
+      __syncthreads();
+      edge = select(all_of, held_weight, need, bins, true, sh);
+    }
+    auto last = [&](int i, float x, uint64_t w) -> uint64_t {
+      return w >= least_mass && edge.keeps(i, x) ? w : 0;
+    };
+    const uint64_t all = total(all_of, last, sh);
+    const int token = all_of.locate(last, drawn(all), sh);
+    return answer(token, share(held[token], all));
+  } else {
+    if (top_p < 1.0) edge = select(row, f, needed(total(row, f, sh)), bins, false, sh);
+    auto last = [&](int i, float x, uint64_t) -> uint64_t {
+      const uint64_t w = f(i, x, 0);
+      return w < least_mass ? 0 : w;
+    };
+    const uint64_t all = total(row, last, sh);
+    const int token = row.locate(last, drawn(all), sh);
+    return answer(token, share(logit<TYPE>(row.at, token), all));
   }
 }
 
