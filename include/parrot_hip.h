@@ -850,23 +850,25 @@ typedef struct parrot_paged_batch {
   int32_t width;
 } parrot_paged_batch;
 
-/* Writes the new rows k and v, bf16 [rows, kv_heads, head_dim] with element
- * strides k_strides / v_strides (row, head; multiples of 4, rows of unit stride,
- * 8-byte aligned; host arrays), into their sequences' pages, quantised where the
- * cache holds 8 bits.  A page that is written belongs to one sequence.
+/* Writes the new rows k and v, bf16 [rows, kv_heads, head_dim] with the given
+ * element strides of rows and heads (multiples of 4; unit stride inside a row,
+ * 8-byte aligned), into their sequences' pages, quantised where the cache holds
+ * 8 bits.  A page that is written belongs to one sequence.
  * New beside parrot_decode_attention_bf16's store into a contiguous cache
  * (LocalGQA.decode, parrot/model.py:239-262). */
 int parrot_paged_append_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
-                             const void* k, const int64_t* k_strides, const void* v,
-                             const int64_t* v_strides, int32_t rows, void* stream);
+                             const void* k, int64_t k_row, int64_t k_head, const void* v,
+                             int64_t v_row, int64_t v_head, int32_t rows, void* stream);
 
 /* Reads positions 0 .. positions - 1 of every sequence back: k and v, bf16
- * [batch, kv_heads, positions, head_dim] with element strides (sequence, head,
- * position; multiples of 4; host arrays), zero from a sequence's length on and
- * where no page is named.  starts is not read.  8-bit values are exact in bf16. */
+ * [batch, kv_heads, positions, head_dim] with the given element strides of
+ * sequences, heads and positions (multiples of 4), zero from a sequence's length
+ * on and where no page is named.  starts is not read.  8-bit values are exact in
+ * bf16. */
 int parrot_paged_read_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
-                           int32_t positions, void* k, const int64_t* k_strides, void* v,
-                           const int64_t* v_strides, void* stream);
+                           int32_t positions, void* k, int64_t k_sequence, int64_t k_head,
+                           int64_t k_position, void* v, int64_t v_sequence, int64_t v_head,
+                           int64_t v_position, void* stream);
 
 /* Bytes of workspace that parrot_paged_attention_bf16 needs for these sizes (0
  * where it needs none, or for sizes that it does not take). */
@@ -880,13 +882,13 @@ size_t parrot_paged_attention_workspace_bytes(const parrot_paged_cache* cache,
  * i being the row's position; window <= 0: every j <= i.  Query head h reads kv
  * head h / (heads / kv_heads).  A row that sees no key is 0; rows of no sequence
  * are left as they are.  What a row does not see cannot reach it, infinities and
- * NaN included.  q bf16 [rows, heads, head_dim] with element strides q_strides
- * (row, head; multiples of 8, 16-byte aligned; host array); out 8-byte aligned;
+ * NaN included.  q bf16 [rows, heads, head_dim] with the given element strides of
+ * rows and heads (multiples of 8, 16-byte aligned); out 8-byte aligned;
  * scale finite and not 0; workspace 16-byte aligned.
  * New beside parrot_causal_attention_bf16 and parrot_decode_attention_bf16
  * (parrot/model.py:239-262, 264-295). */
 int parrot_paged_attention_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
-                                const void* q, const int64_t* q_strides, int32_t rows,
+                                const void* q, int64_t q_row, int64_t q_head, int32_t rows,
                                 int32_t heads, int32_t window, int32_t sinks, float scale,
                                 void* out, void* workspace, size_t workspace_bytes,
                                 void* stream);

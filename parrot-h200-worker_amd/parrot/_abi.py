@@ -157,11 +157,13 @@ SIGNATURES: dict[str, tuple] = {
     "parrot_route_top2_bf16": (ctypes.c_int, [_p, _p, _p, _i64, _i32, _i32, _p, _p, _p]),
     "parrot_route_top2_blocks_bf16": (
         ctypes.c_int, [_p, _p, _p, _i64, _i32, _i32, _p, _p, _p, _p]),
-    "parrot_paged_append_bf16": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _i32, _p]),
-    "parrot_paged_read_bf16": (ctypes.c_int, [_p, _p, _i32, _p, _p, _p, _p, _p]),
+    "parrot_paged_append_bf16": (
+        ctypes.c_int, [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _p]),
+    "parrot_paged_read_bf16": (
+        ctypes.c_int, [_p, _p, _i32, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p]),
     "parrot_paged_attention_workspace_bytes": (_sz, [_p, _p, _i32, _i32, _i32, _i32]),
     "parrot_paged_attention_bf16": (
-        ctypes.c_int, [_p, _p, _p, _p, _i32, _i32, _i32, _i32, _f32, _p, _p, _sz, _p]),
+        ctypes.c_int, [_p, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _f32, _p, _p, _sz, _p]),
     "parrot_sample": (
         ctypes.c_int,
         [_p, _i32, _i64, _i32, _i64, _p, _p, _f64, _p, _i32, _p, _f64, _p, _f64, _p, _p, _p]),

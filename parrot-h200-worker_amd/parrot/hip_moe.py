@@ -36,7 +36,8 @@ MAX_DEPTH_SOURCES = 9
 # ---------------------------------------------------------------------------
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # (torch.cuda.current_stream(device).cuda_stream without the Stream object)
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 _HERE = contextlib.nullcontext()
@@ -632,14 +633,17 @@ _LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 SAMPLE_MAX_VOCAB = 1 << 20
 
 
-def _sample_parameter(x, what: str, rows: int, device: torch.device, dtype: torch.dtype):
+def _sample_parameter(x, what: str, rows: int, device: torch.device, dtype: torch.dtype,
+                      most: float = math.inf):
     """(pointer, number) of one sampling parameter: a tensor of one value per
-    row, or a number for every row."""
+    row, or a number from 0 to ``most`` for every row."""
     if isinstance(x, Tensor):
         if x.dtype != dtype or x.device != device or x.numel() != rows or not x.is_contiguous():
             raise RuntimeError(f"{what} must be a number or a contiguous {dtype} tensor of one "
                                "value per row on the logits' device")
         return x.data_ptr(), 0
+    if not 0 <= x <= most:
+        raise RuntimeError(f"{what} must lie between 0 and {most}")
     return None, x
 
 
@@ -676,18 +680,10 @@ def sample(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor = 1.0
             not uniform.is_contiguous()):
         raise RuntimeError("uniform must be a contiguous fp32 tensor of one number per row on the "
                            "logits' device")
-    if not isinstance(temperature, Tensor) and not temperature >= 0:
-        raise RuntimeError("temperature must not be negative")
-    if not isinstance(top_k, Tensor) and not 0 <= top_k <= 2 ** 31 - 1:
-        raise RuntimeError("top_k must not be negative")
-    if not isinstance(top_p, Tensor) and not 0 <= top_p <= 1:
-        raise RuntimeError("top_p must lie in [0, 1]")
-    if not isinstance(min_p, Tensor) and not 0 <= min_p <= 1:
-        raise RuntimeError("min_p must lie in [0, 1]")
     t, t_all = _sample_parameter(temperature, "temperature", rows, device, torch.float32)
-    k, k_all = _sample_parameter(top_k, "top_k", rows, device, torch.int32)
-    p, p_all = _sample_parameter(top_p, "top_p", rows, device, torch.float32)
-    m, m_all = _sample_parameter(min_p, "min_p", rows, device, torch.float32)
+    k, k_all = _sample_parameter(top_k, "top_k", rows, device, torch.int32, 2 ** 31 - 1)
+    p, p_all = _sample_parameter(top_p, "top_p", rows, device, torch.float32, 1)
+    m, m_all = _sample_parameter(min_p, "min_p", rows, device, torch.float32, 1)
     shape = (*logits.shape[:-1], 1)
     if out is None:
         out = torch.empty(shape, dtype=torch.int64, device=device)

@@ -66,11 +66,12 @@ int check_paged(const parrot_paged_cache* c, const parrot_paged_batch* b) {
   return PARROT_OK;
 }
 
-int check_paged_rows(const void* p, const int64_t* strides, int n, int multiple, unsigned align) {
-  if (!p || !strides) return PARROT_ERR_NULL_POINTER;
-  for (int i = 0; i < n; ++i)
-    if (strides[i] % multiple) return PARROT_ERR_ALIGNMENT;
-  return reinterpret_cast<uintptr_t>(p) % align ? PARROT_ERR_ALIGNMENT : PARROT_OK;
+// Rows that are read or written in pieces of `step` bf16 values.
+int check_paged_rows(const void* p, const int64_t (&strides)[3], int step) {
+  if (!p) return PARROT_ERR_NULL_POINTER;
+  for (int64_t s : strides)
+    if (s % step) return PARROT_ERR_ALIGNMENT;
+  return reinterpret_cast<uintptr_t>(p) % (2 * step) ? PARROT_ERR_ALIGNMENT : PARROT_OK;
 }
 
 // (rows x heads is also the number of a tile's rows at most, in 32 bits)
@@ -774,13 +775,14 @@ size_t parrot_experts_workspace_bytes(int64_t tokens, int32_t dim, int32_t hidde
 }
 
 int parrot_paged_append_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
-                             const void* k, const int64_t* k_strides, const void* v,
-                             const int64_t* v_strides, int32_t rows, void* stream) {
+                             const void* k, int64_t k_row, int64_t k_head, const void* v,
+                             int64_t v_row, int64_t v_head, int32_t rows, void* stream) {
   if (int rc = check_paged(cache, batch)) return rc;
   if (rows < 0 || rows > (1 << 30)) return PARROT_ERR_BAD_SHAPE;
   if (rows == 0) return PARROT_OK;
-  if (int rc = check_paged_rows(k, k_strides, 2, 4, 8)) return rc;
-  if (int rc = check_paged_rows(v, v_strides, 2, 4, 8)) return rc;
+  const int64_t k_strides[3] = {k_row, k_head, 0}, v_strides[3] = {v_row, v_head, 0};
+  if (int rc = check_paged_rows(k, k_strides, 4)) return rc;
+  if (int rc = check_paged_rows(v, v_strides, 4)) return rc;
   return status(parrot::launch_paged_append(
       paged_cache(cache), cache->type, cache->head_dim, paged_batch(batch, rows),
       static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_strides, v_strides,
@@ -788,13 +790,16 @@ int parrot_paged_append_bf16(const parrot_paged_cache* cache, const parrot_paged
 }
 
 int parrot_paged_read_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
-                           int32_t positions, void* k, const int64_t* k_strides, void* v,
-                           const int64_t* v_strides, void* stream) {
+                           int32_t positions, void* k, int64_t k_sequence, int64_t k_head,
+                           int64_t k_position, void* v, int64_t v_sequence, int64_t v_head,
+                           int64_t v_position, void* stream) {
   if (int rc = check_paged(cache, batch)) return rc;
   if (positions < 0 || positions > INT32_MAX - 64) return PARROT_ERR_BAD_SHAPE;
   if (positions == 0 || batch->batch == 0) return PARROT_OK;
-  if (int rc = check_paged_rows(k, k_strides, 3, 4, 8)) return rc;
-  if (int rc = check_paged_rows(v, v_strides, 3, 4, 8)) return rc;
+  const int64_t k_strides[3] = {k_sequence, k_head, k_position};
+  const int64_t v_strides[3] = {v_sequence, v_head, v_position};
+  if (int rc = check_paged_rows(k, k_strides, 4)) return rc;
+  if (int rc = check_paged_rows(v, v_strides, 4)) return rc;
   return status(parrot::launch_paged_read(
       paged_cache(cache), cache->type, cache->head_dim, paged_batch(batch, 0), positions,
       static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), k_strides, v_strides,
@@ -811,7 +816,7 @@ size_t parrot_paged_attention_workspace_bytes(const parrot_paged_cache* cache,
 }
 
 int parrot_paged_attention_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
-                                const void* q, const int64_t* q_strides, int32_t rows,
+                                const void* q, int64_t q_row, int64_t q_head, int32_t rows,
                                 int32_t heads, int32_t window, int32_t sinks, float scale,
                                 void* out, void* workspace, size_t workspace_bytes,
                                 void* stream) {
@@ -819,7 +824,8 @@ int parrot_paged_attention_bf16(const parrot_paged_cache* cache, const parrot_pa
   if (int rc = check_paged_heads(rows, heads, cache->kv_heads)) return rc;
   if (sinks < 0 || !(scale - scale == 0.0f) || scale == 0.0f) return PARROT_ERR_BAD_SHAPE;
   if (rows == 0 || batch->batch == 0) return PARROT_OK;
-  if (int rc = check_paged_rows(q, q_strides, 2, 8, 16)) return rc;
+  const int64_t q_strides[3] = {q_row, q_head, 0};
+  if (int rc = check_paged_rows(q, q_strides, 8)) return rc;
   if (!out) return PARROT_ERR_NULL_POINTER;
   if (reinterpret_cast<uintptr_t>(out) & 7u) return PARROT_ERR_ALIGNMENT;
   const int splits = paged_splits(cache, batch, rows, heads, window, sinks);

@@ -64,28 +64,34 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch& b, int
   return s;
 }
 
-// The units (tiles, blocks) of the sequences in a row: which sequence unit
-// `unit` belongs to and the how manieth of it it is; false past the last.
-// Every wavefront of the workgroup calls it.  units_of(i): sequence i's number.
+// The units (tiles, blocks) of the sequences in a row: which sequence unit `unit`
+// belongs to, the how manieth of it it is, and the sequence; false past the last.
+// Every lane of a wavefront calls it.  units_of(s): sequence s's number.
 template <typename F>
-__device__ __forceinline__ bool paged_locate(int batch, int unit, F units_of, int& sequence,
-                                             int& index) {
+__device__ __forceinline__ bool paged_find(const PagedBatch& b, int page, int unit, F units_of,
+                                           int& sequence, int& index, PagedSequence& s) {
   const int lane = threadIdx.x & (kWave - 1);
   int base = 0;
-  for (int c = 0; c < batch; c += kWave) {
-    const int mine = c + lane < batch ? units_of(c + lane) : 0;
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const int before = __shfl_up(upto, d);
-      if (lane >= d) upto += before;
-    }
+  for (int c = 0; c < b.batch; c += kWave) {
+    const PagedSequence mine = paged_sequence(b, page, min(c + lane, b.batch - 1));
+    const int units = c + lane < b.batch ? units_of(mine) : 0;
+    int upto = units;  // sums by DPP: 1, 2, 4, 8 to the right in rows of 16, then across
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xf, 0xf, false);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xf, 0xf, false);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xf, 0xf, false);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, false);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x142, 0xa, 0xf, false);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x143, 0xc, 0xf, false);
     const int total = __builtin_amdgcn_readlane(upto, kWave - 1);
     if (unit < base + total) {
-      const uint64_t hit = __ballot(unit >= base + upto - mine && unit < base + upto);
+      const uint64_t hit = __ballot(unit >= base + upto - units && unit < base + upto);
       const int who = __builtin_ctzll(hit);
       sequence = c + who;
-      index = unit - base - __builtin_amdgcn_readlane(upto - mine, who);
+      index = unit - base - __builtin_amdgcn_readlane(upto - units, who);
+      s.first = __builtin_amdgcn_readlane(mine.first, who);
+      s.count = __builtin_amdgcn_readlane(mine.count, who);
+      s.length = __builtin_amdgcn_readlane(mine.length, who);
+      s.stored = __builtin_amdgcn_readlane(mine.stored, who);
       return true;
     }
     base += total;

@@ -112,14 +112,13 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c, Pa
   __shared__ __attribute__((aligned(16))) E v_s[kPagedBlock][kLd];
 
   // Blocks that new rows fall into.
-  auto units_of = [&](int i) {
-    const PagedSequence s = paged_sequence(b, c.page, i);
+  auto units_of = [&](const PagedSequence& s) {
     const int from = max(s.length - s.count, 0);
     return s.stored > from ? (s.stored - 1) / kPagedBlock - from / kPagedBlock + 1 : 0;
   };
   int sequence, index;
-  if (!paged_locate(b.batch, blockIdx.x, units_of, sequence, index)) return;
-  const PagedSequence s = paged_sequence(b, c.page, sequence);
+  PagedSequence s;
+  if (!paged_find(b, c.page, blockIdx.x, units_of, sequence, index, s)) return;
   const int from = max(s.length - s.count, 0);
   const int blk = from / kPagedBlock + index;
   const int per_page = c.page / kPagedBlock;

@@ -31,6 +31,7 @@ typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4;
 constexpr int kRows = 32;  // rows of a wavefront's tile
+constexpr int kMaxSplits = kWave;
 
 struct AttendArgs {
   PagedCache cache;
@@ -43,8 +44,8 @@ struct AttendArgs {
   float scale_log2;  // |scale| log2(e)
   uint32_t q_sign;   // 0x80008000 for a negative scale (q is negated), else 0
   int splits;
-  float* part;       // [splits][rows * heads][D], unnormalised
-  float2* part_ml;   // [splits][rows * heads]
+  float* part;       // [rows * heads][splits][D], unnormalised
+  float2* part_ml;   // [rows * heads][splits]
   uint16_t* out;     // [rows][heads][D]
 };
 
@@ -276,6 +277,49 @@ __device__ __forceinline__ TileRow tile_row(const PagedSequence& s, int row, int
   return {s.length - s.count + token, s.first + token, kv_head * rep + (r - token * rep)};
 }
 
+// The four wavefronts' shares of a tile of R rows, each in the units of its own
+// maximum, joined: to the output, or to the split's partial sums.
+template <int D, int R>
+__device__ __forceinline__ void merge_tile(const AttendArgs& a, const float (&o_s)[kWaves][R][D + 4],
+                                           const float (&ml_s)[kWaves][2][R],
+                                           const PagedSequence& s, int row0, int rows, int kvh,
+                                           int split, bool any) {
+  for (int i = threadIdx.x; i < R * (D / 4); i += kWaves * kWave) {
+    const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
+    if (row0 + r >= rows) break;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml_s[w][0][r]);
+    float sum = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float mw = ml_s[w][0][r], lw = ml_s[w][1][r];
+      // A wavefront that saw nothing adds nothing (its maximum is -inf, its sum
+      // 0; a NaN sum has to come through).
+      if (mw == -INFINITY && lw == 0.0f) continue;
+      const float f = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+      sum += lw * f;
+      const float4 x = *reinterpret_cast<const float4*>(&o_s[w][r][d]);
+      y.x += x.x * f;
+      y.y += x.y * f;
+      y.z += x.z * f;
+      y.w += x.w * f;
+    }
+    const TileRow row = tile_row(s, row0 + r, rows, a.rep, kvh);
+    const int64_t to = static_cast<int64_t>(row.token) * a.heads + row.head;
+    if (a.splits == 1) {
+      const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+      *reinterpret_cast<uint2*>(a.out + to * D + d) =
+          make_uint2(pack_bf16x2(y.x * f, y.y * f), pack_bf16x2(y.z * f, y.w * f));
+    } else {
+      const int64_t at = to * a.splits + split;
+      if (d == 0) a.part_ml[at] = make_float2(m, sum);
+      if (any) *reinterpret_cast<float4*>(a.part + at * D + d) = y;
+    }
+  }
+}
+
 // Every wavefront takes every fourth key block of the workgroup's share, its
 // operands straight from the pages; the four are merged in LDS.
 template <int TYPE, int D>
@@ -289,12 +333,10 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_attend_kernel(AttendA
   const int half = lane >> 5, col = lane & 31;
   const int kvh = blockIdx.y, split = blockIdx.z;
 
-  auto units_of = [&](int i) {
-    return (paged_sequence(a.batch, a.cache.page, i).count * a.rep + kRows - 1) / kRows;
-  };
+  auto units_of = [&](const PagedSequence& s) { return (s.count * a.rep + kRows - 1) / kRows; };
   int sequence, tile;
-  if (!paged_locate(a.batch.batch, blockIdx.x, units_of, sequence, tile)) return;
-  const PagedSequence s = paged_sequence(a.batch, a.cache.page, sequence);
+  PagedSequence s;
+  if (!paged_find(a.batch, a.cache.page, blockIdx.x, units_of, sequence, tile, s)) return;
   const int rows = s.count * a.rep;
   const int row0 = tile * kRows;
   const TileRow mine = tile_row(s, row0 + col, rows, a.rep, kvh);
@@ -361,7 +403,6 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_attend_kernel(AttendA
           k0, mine.position, first, last, s.stored, a);
     }
   }
-  // Merge: every wavefront's share in its own units, then one common maximum.
   const float l = st.l + __shfl_xor(st.l, 32);
   if (half == 0) {
     ml_s[wave][0][col] = st.m;
@@ -374,71 +415,305 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_attend_kernel(AttendA
       *reinterpret_cast<float4*>(&o_s[wave][col][32 * t + 8 * (e >> 2) + 4 * half]) =
           make_float4(st.o[t][e], st.o[t][e + 1], st.o[t][e + 2], st.o[t][e + 3]);
   __syncthreads();
-  for (int i = threadIdx.x; i < kRows * (D / 4); i += kWaves * kWave) {
-    const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
-    if (row0 + r >= rows) break;
-    float m = -INFINITY;
+  merge_tile<D, kRows>(a, o_s, ml_s, s, row0, rows, kvh, split, begin < end);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows per sequence (decode steps, short chunks): tiles of 16 rows.
+//
+// What bounds it: the pages' bytes, and below some MB the chain of dependent loads
+// (starts, lengths and table, then keys).  Each wavefront takes every fourth block of
+// its workgroup's share, straight from the pages into operand registers, and loads a
+// block while it computes the one before.
+//
+//   S^T = K Q^T     v_mfma_f32_16x16x32_bf16, A = 16 keys (two per block), B = 16
+//                   rows: lane 16 g + c holds keys 4 g .. + 3 and 16 + 4 g .. + 3 of
+//                   row c, which is the order in which
+//   O^T += V^T P^T  takes P^T as its B operand (32 keys).
+// ---------------------------------------------------------------------------
+
+constexpr int kStepRows = 16;
+
+template <int TYPE, int D>
+struct StepBlock {
+  using raw = typename Piece<TYPE>::raw;
+  static constexpr int N = D / 16;  // pieces of K, and of V, per lane
+  raw k[N], v[N];
+  uint32_t kbytes[2], vbytes[2];  // exponents of the lane's key rows; of its 8 scores
+  int page;                       // -1: none
+};
+
+template <int TYPE, int D>
+struct StepState {
+  float m = -INFINITY, l = 0.0f;
+  f32x4 o[D / 16];
+};
+
+template <int TYPE, int D>
+__device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlock<TYPE, D>& b,
+                                           const bf16x8 (&qf)[D / 32], int k0, int query,
+                                           int first, int last, int stored,
+                                           const AttendArgs& a) {
+  constexpr int S = D / 32, T = D / 16;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int g = lane >> 4, col = lane & 15;
+  constexpr float kLazy = 8.0f;
+  f32x4 sc[2];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml_s[w][0][r]);
-    float sum = 0.0f;
-    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int n = 0; n < 2; ++n) {
+    sc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const float power = TYPE == kPagedBf16 ? 1.0f : __uint_as_float(b.kbytes[n] << 23);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float mw = ml_s[w][0][r], lw = ml_s[w][1][r];
-      // A wavefront that saw nothing adds nothing (its maximum is -inf, its sum
-      // 0; a NaN sum has to come through).
-      if (mw == -INFINITY && lw == 0.0f) continue;
-      const float f = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-      sum += lw * f;
-      const float4 x = *reinterpret_cast<const float4*>(&o_s[w][r][d]);
+    for (int s = 0; s < S; ++s)
+      sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(piece_bf16<TYPE>(b.k[n * S + s], power), qf[s],
+                                                      sc[n], 0, 0, 0);
+  }
+  auto key_of = [&](int e) { return k0 + 16 * (e >> 2) + 4 * g + (e & 3); };
+  const bool whole = k0 + 31 <= min(first, stored - 1) &&
+                     (last - k0 < a.window || k0 + 31 < a.sinks);
+  if (!whole) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int key = key_of(e);
+      if (!(key < stored && visible(key, query, a.window, a.sinks))) sc[e >> 2][e & 3] = -INFINITY;
+    }
+  }
+  float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                   fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+  mx *= a.scale_log2;
+  if (__ballot(mx > st.m + kLazy) != 0) {
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float mn = fmaxf(st.m, mx);
+    const float alpha = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - mn);
+    st.l *= alpha;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.o[t][e] *= alpha;
+    st.m = mn;
+  }
+  const float neg = st.m == -INFINITY ? 0.0f : -st.m;
+  float p[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e >> 2][e & 3], a.scale_log2, neg));
+  st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+
+  bf16x8 vf[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) vf[t] = piece_bf16<TYPE>(b.v[t], 1.0f);
+  bool odd = false;  // (see attend_block)
+  if (!whole) {
+    bool mine = false;
+#pragma unroll
+    for (int t = 0; t < T; ++t) mine |= has_nonfinite(vf[t]);
+    if constexpr (TYPE != kPagedBf16) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        mine |= ((b.vbytes[e >> 2] >> (8 * (e & 3))) & 0xffu) == kPagedNotFinite;
+    }
+    odd = __ballot(mine) != 0;
+  }
+  if constexpr (TYPE != kPagedBf16) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t byte = (b.vbytes[e >> 2] >> (8 * (e & 3))) & 0xffu;
+      const float y = p[e] * __uint_as_float(byte << 23);
+      p[e] = odd && sc[e >> 2][e & 3] == -INFINITY ? 0.0f : y;
+    }
+  }
+  bf16x8 pf;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) pf[e] = static_cast<__bf16>(p[e]);
+  if (odd) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      f32x4 sums = st.o[t];
+#pragma unroll 1
+      for (int row = 0; row < kStepRows; ++row) {
+        const int at = __builtin_amdgcn_readlane(query, row);
+        bf16x8 v = vf[t];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = key_of(e);
+          if (!(key < stored && visible(key, at, a.window, a.sinks))) v[e] = static_cast<__bf16>(0.0f);
+        }
+        const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf, st.o[t], 0, 0, 0);
+        if (col == row) sums = y;
+      }
+      st.o[t] = sums;
+    }
+    return;
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+    st.o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[t], pf, st.o[t], 0, 0, 0);
+}
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a) {
+  constexpr int S = D / 32, T = D / 16;
+  using raw = typename Piece<TYPE>::raw;
+  __shared__ float o_s[kWaves][kStepRows][D + 4];
+  __shared__ float ml_s[kWaves][2][kStepRows];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, col = lane & 15;
+  const int kvh = blockIdx.y, split = blockIdx.z;
+
+  auto units_of = [&](const PagedSequence& s) {
+    return (s.count * a.rep + kStepRows - 1) / kStepRows;
+  };
+  int sequence, tile;
+  PagedSequence s;
+  if (!paged_find(a.batch, a.cache.page, blockIdx.x, units_of, sequence, tile, s)) return;
+  const int rows = s.count * a.rep;
+  const int row0 = tile * kStepRows;
+  const TileRow mine = tile_row(s, row0 + col, rows, a.rep, kvh);
+  const int first = s.length - s.count + row0 / a.rep;
+  const int last = s.length - s.count + (min(row0 + kStepRows, rows) - 1) / a.rep;
+  const Blocks blocks = tile_blocks(first, last, s.stored, a.window, a.sinks);
+  const int share = (blocks.count + a.splits - 1) / a.splits;
+  const int begin = min(split * share, blocks.count), end = min(begin + share, blocks.count);
+
+  StepState<TYPE, D> st;
+#pragma unroll
+  for (int t = 0; t < T; ++t) st.o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (begin + wave < end) {
+    const int per_page = a.cache.page / kPagedBlock;
+    int ids = -1;  // lane j: the page of this wavefront's j-th block (of the last 64)
+    auto fetch = [&](int i, StepBlock<TYPE, D>& b) {
+      const int j = (i - begin) / kWaves;
+      if (j % kWave == 0) {
+        const int at = i + kWaves * lane;
+        ids = at < end ? paged_page(a.batch, a.cache, sequence, blocks.at(at) / per_page) : -1;
+      }
+      b.page = __builtin_amdgcn_readlane(ids, j % kWave);
+      if (b.page < 0) return;
+      const int in = blocks.at(i) % per_page;
+      const int64_t at = static_cast<int64_t>(b.page) * a.cache.kv_heads + kvh;
+      const int64_t off = (at * per_page + in) * (kPagedBlock * D / 8);
+      const raw* kp = static_cast<const raw*>(a.cache.key) + off;
+      const raw* vp = static_cast<const raw*>(a.cache.value) + off;
+#pragma unroll
+      for (int u = 0; u < T; ++u) b.k[u] = kp[kWave * u + lane];
+#pragma unroll
+      for (int u = 0; u < T; ++u) b.v[u] = vp[kWave * u + lane];
+      if constexpr (TYPE != kPagedBf16) {
+        const int64_t e = at * a.cache.page + in * kPagedBlock;
+        const uint8_t* ke = a.cache.key_exponent + e;
+        const uint8_t* ve = a.cache.value_exponent + e;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          b.kbytes[n] = ke[16 * n + col];
+          b.vbytes[n] = *reinterpret_cast<const uint32_t*>(ve + 16 * n + 4 * g);
+        }
+      }
+    };
+    StepBlock<TYPE, D> b0, b1;
+    fetch(begin + wave, b0);
+    bf16x8 qf[S];
+    {
+      const uint16_t* row = a.q + mine.token * a.qs[0] + mine.head * a.qs[1] + 8 * g;
+#pragma unroll
+      for (int u = 0; u < S; ++u) {
+        uint4 v = *reinterpret_cast<const uint4*>(row + 32 * u);
+        v.x ^= a.q_sign;
+        v.y ^= a.q_sign;
+        v.z ^= a.q_sign;
+        v.w ^= a.q_sign;
+        qf[u] = __builtin_bit_cast(bf16x8, v);
+      }
+    }
+    auto compute = [&](int i, const StepBlock<TYPE, D>& b) {
+      if (b.page >= 0)
+        step_block<TYPE, D>(st, b, qf, blocks.at(i) * kPagedBlock, mine.position, first, last,
+                            s.stored, a);
+    };
+    for (int i = begin + wave; i < end; i += 2 * kWaves) {
+      if (i + kWaves < end) fetch(i + kWaves, b1);
+      compute(i, b0);
+      if (i + kWaves >= end) break;
+      if (i + 2 * kWaves < end) fetch(i + 2 * kWaves, b0);
+      compute(i + kWaves, b1);
+    }
+  }
+  float l = st.l + __shfl_xor(st.l, 16);
+  l += __shfl_xor(l, 32);
+  if (g == 0) {
+    ml_s[wave][0][col] = st.m;
+    ml_s[wave][1][col] = l;
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+    *reinterpret_cast<float4*>(&o_s[wave][col][16 * t + 4 * g]) =
+        make_float4(st.o[t][0], st.o[t][1], st.o[t][2], st.o[t][3]);
+  __syncthreads();
+  merge_tile<D, kStepRows>(a, o_s, ml_s, s, row0, rows, kvh, split, begin < end);
+}
+
+// Joins the shares of split tiles: a workgroup a row, its first wavefront one split a
+// lane for their weights, then D / 4 threads for every tenth (D = 96) of them.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a) {
+  constexpr int kGroups = 256 / (D / 4);
+  __shared__ float w_s[kMaxSplits];
+  __shared__ float4 y_s[kGroups][D / 4];
+  const int64_t to = blockIdx.x;
+  // Rows of no sequence stay as they are.
+  const int token = static_cast<int>(to / a.heads);
+  if (token < a.batch.starts[0] || token >= a.batch.starts[a.batch.batch]) return;
+  if (threadIdx.x < kWave) {
+    const int i = threadIdx.x;
+    const float2 ml = i < a.splits ? a.part_ml[to * a.splits + i] : make_float2(-INFINITY, 0.0f);
+    float m = ml.x;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+    // (a share that saw nothing adds nothing; a NaN sum has to come through)
+    const bool none = ml.x == -INFINITY && ml.y == 0.0f;
+    const float f = none ? 0.0f : ml.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
+    const float sum = wave_sum(none ? 0.0f : ml.y * f);
+    // (-1: not to be read)
+    w_s[i] = none ? -1.0f : sum == 0.0f ? 0.0f : f / sum;
+  }
+  __syncthreads();
+  const int group = threadIdx.x / (D / 4), at = threadIdx.x - group * (D / 4);
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (group < kGroups) {
+    for (int i = group; i < a.splits; i += kGroups) {
+      const float f = w_s[i];
+      if (f < 0.0f) continue;
+      const float4 x = *reinterpret_cast<const float4*>(a.part + (to * a.splits + i) * D + 4 * at);
       y.x += x.x * f;
       y.y += x.y * f;
       y.z += x.z * f;
       y.w += x.w * f;
     }
-    const TileRow row = tile_row(s, row0 + r, rows, a.rep, kvh);
-    const int64_t to = static_cast<int64_t>(row.token) * a.heads + row.head;
-    if (a.splits == 1) {
-      const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-      *reinterpret_cast<uint2*>(a.out + to * D + d) =
-          make_uint2(pack_bf16x2(y.x * f, y.y * f), pack_bf16x2(y.z * f, y.w * f));
-    } else {
-      const int64_t at = static_cast<int64_t>(split) * a.batch.rows * a.heads + to;
-      if (d == 0) a.part_ml[at] = make_float2(m, sum);
-      if (begin < end) *reinterpret_cast<float4*>(a.part + at * D + d) = y;
-    }
+    y_s[group][at] = y;
   }
+  __syncthreads();
+  if (group != 0) return;
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) {
+    const float4 x = y_s[i][at];
+    y.x += x.x;
+    y.y += x.y;
+    y.z += x.z;
+    y.w += x.w;
+  }
+  *reinterpret_cast<uint2*>(a.out + to * D + 4 * at) =
+      make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
 }
 
-// Joins the shares of split tiles: D / 4 threads a row.
-template <int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a) {
-  constexpr int kPer = 256 / (D / 4);
-  const int slot = threadIdx.x / (D / 4), d = 4 * (threadIdx.x - slot * (D / 4));
-  const int64_t to = static_cast<int64_t>(blockIdx.x) * kPer + slot;
-  const int64_t rows = static_cast<int64_t>(a.batch.rows) * a.heads;
-  if (slot >= kPer || to >= rows) return;
-  // Rows of no sequence stay as they are.
-  const int token = static_cast<int>(to / a.heads);
-  if (token < a.batch.starts[0] || token >= a.batch.starts[a.batch.batch]) return;
-  float m = -INFINITY;
-  for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.part_ml[i * rows + to].x);
-  float sum = 0.0f;
-  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int i = 0; i < a.splits; ++i) {
-    const float2 ml = a.part_ml[i * rows + to];
-    if (ml.x == -INFINITY && ml.y == 0.0f) continue;
-    const float f = ml.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
-    sum += ml.y * f;
-    const float4 x = *reinterpret_cast<const float4*>(a.part + (i * rows + to) * D + d);
-    y.x += x.x * f;
-    y.y += x.y * f;
-    y.z += x.z * f;
-    y.w += x.w * f;
-  }
-  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-  *reinterpret_cast<uint2*>(a.out + to * D + d) =
-      make_uint2(pack_bf16x2(y.x * f, y.y * f), pack_bf16x2(y.z * f, y.w * f));
+}  // namespace
+
+namespace {
+
+// Tiles of 16 rows, block by block from the pages, where a sequence has no more than
+// that on average (most of a tile of 32 would be empty).
+bool few_rows(int batch, int rows, int rep) {
+  return static_cast<int64_t>(rows) * rep <= int64_t{32} * std::min(batch, rows);
 }
 
 }  // namespace
@@ -447,14 +722,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a) {
 int paged_attention_splits(int batch, int rows, int heads, int kv_heads, int page, int width,
                            int window, int sinks) {
   const int rep = heads / kv_heads;
-  const int64_t tiles = (static_cast<int64_t>(rows) * rep + kRows - 1) / kRows;
+  const int tile = few_rows(batch, rows, rep) ? kStepRows : kRows;
+  const int64_t tiles = (static_cast<int64_t>(rows) * rep + tile - 1) / tile;
   const int64_t units = std::max<int64_t>(tiles, std::min(batch, rows)) * kv_heads;
   // The most keys a tile can see: its table's, or the window, the sinks and
   // the tile's own span.
   int64_t keys = static_cast<int64_t>(width) * page;
   if (window < INT32_MAX) keys = std::min<int64_t>(keys, int64_t{window} + sinks + kRows + 64);
   const int64_t want = (1024 + units - 1) / std::max<int64_t>(units, 1);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, keys / 256, 64})));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, keys / 256, kMaxSplits})));
 }
 
 size_t paged_attention_workspace_bytes(int splits, int rows, int heads, int head_dim) {
@@ -485,17 +761,17 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   a.part_ml = reinterpret_cast<float2*>(a.part +
                                         static_cast<size_t>(splits) * batch.rows * heads * head_dim);
   a.out = out;
-  // ceil(n rep / 32) tiles a sequence
-  const int64_t tiles = static_cast<int64_t>(batch.rows) * a.rep / kRows +
+  const bool few = few_rows(batch.batch, batch.rows, a.rep);
+  // ceil(n rep / 16 or 32) tiles a sequence
+  const int64_t tiles = static_cast<int64_t>(batch.rows) * a.rep / (few ? kStepRows : kRows) +
                         std::min(batch.batch, batch.rows);
   const dim3 grid(static_cast<uint32_t>(tiles), cache.kv_heads, splits);
   auto run = [&](auto t, auto d) {
     constexpr int TYPE = decltype(t)::value, D = decltype(d)::value;
-    paged_attend_kernel<TYPE, D><<<grid, kWaves * kWave, 0, s>>>(a);
+    if (few) paged_step_kernel<TYPE, D><<<grid, kWaves * kWave, 0, s>>>(a);
+    else paged_attend_kernel<TYPE, D><<<grid, kWaves * kWave, 0, s>>>(a);
     if (splits > 1) {
-      constexpr int kPer = 256 / (D / 4);
-      const int64_t rows = static_cast<int64_t>(batch.rows) * heads;
-      paged_join_kernel<D><<<static_cast<uint32_t>((rows + kPer - 1) / kPer), 256, 0, s>>>(a);
+      paged_join_kernel<D><<<static_cast<uint32_t>(batch.rows * heads), 256, 0, s>>>(a);
     }
     return hipGetLastError();
   };

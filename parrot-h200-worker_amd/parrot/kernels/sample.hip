@@ -188,7 +188,6 @@ struct Row {
   // f(index, logit, weight if one is held) for this thread's logits
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-#pragma unroll 2
     for (int s = 0; s < steps; ++s) {
       const int i = first(s);
       if (i - 4 * static_cast<int>(threadIdx.x & (kWave - 1)) >= n) break;  // (the wavefront's)
@@ -498,7 +497,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       }
 #pragma unroll
       for (int s = 0; s < kAhead; ++s) {
-        if (from + s >= row.steps) break;
         if (HELD && s < row.steps) *reinterpret_cast<float4*>(&held[row.first(s)]) = v[s];
         mine = fmaxf(fmaxf(mine, fmaxf(v[s].x, v[s].y)), fmaxf(v[s].z, v[s].w));
       }

@@ -28,16 +28,8 @@ from .hip_moe import ATTENTION_HEAD_DIMS, _on, _require, _stream
 PAGE_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2}
 PAGE_BLOCK = 32  # a page is a whole number of blocks of so many positions
 
-_Strides2 = ctypes.c_int64 * 2
-_Strides3 = ctypes.c_int64 * 3
 
-
-def _int32(x: Tensor, what: str, device: torch.device) -> None:
-    if x.dtype != torch.int32 or x.device != device or not x.is_contiguous():
-        raise RuntimeError(f"{what} must be a contiguous int32 tensor on the cache's device")
-
-
-@dataclass
+@dataclass(frozen=True, eq=False)
 class PagedBatch:
     """Which part of a call belongs to which sequence; int32 device tensors.
 
@@ -56,6 +48,20 @@ class PagedBatch:
     table: Tensor
     lengths: Tensor
     starts: Tensor
+
+    def __post_init__(self):
+        for name in ("table", "lengths", "starts"):
+            x = getattr(self, name)
+            if x.dtype != torch.int32 or x.device != self.table.device or not x.is_contiguous():
+                raise RuntimeError(f"{name} must be a contiguous int32 tensor, all three on one "
+                                   "device")
+        if self.table.ndim != 2 or self.lengths.shape != (self.table.shape[0],) or \
+                self.starts.shape != (self.table.shape[0] + 1,):
+            raise RuntimeError("a batch is table [b, width], lengths [b] and starts [b + 1]")
+        b, width = self.table.shape
+        object.__setattr__(self, "_struct", _abi.PagedBatchStruct(
+            self.table.data_ptr(), self.lengths.data_ptr(), self.starts.data_ptr(), b, width))
+        object.__setattr__(self, "_at", ctypes.addressof(self._struct))
 
     @classmethod
     def from_lists(cls, pages: list[list[int]], lengths: list[int], new: list[int],
@@ -76,17 +82,6 @@ class PagedBatch:
         return cls(table.to(device), torch.tensor(lengths, dtype=torch.int32).to(device),
                    torch.tensor(starts, dtype=torch.int32).to(device))
 
-    def _struct(self, device: torch.device):
-        _int32(self.table, "table", device)
-        _int32(self.lengths, "lengths", device)
-        _int32(self.starts, "starts", device)
-        if self.table.ndim != 2 or self.lengths.shape != (self.table.shape[0],) or \
-                self.starts.shape != (self.table.shape[0] + 1,):
-            raise RuntimeError("a batch is table [b, width], lengths [b] and starts [b + 1]")
-        b, width = self.table.shape
-        return _abi.PagedBatchStruct(self.table.data_ptr(), self.lengths.data_ptr(),
-                                     self.starts.data_ptr(), b, width)
-
 
 class PagedKVCache:
     """Pages of keys and values of one layer.
@@ -104,15 +99,13 @@ class PagedKVCache:
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
         self._check(pages, page_size, kv_heads, head_dim, dtype)
+        def zeros(*shape):
+            return torch.zeros(shape, dtype=torch.uint8, device=device)
         shape = (pages, kv_heads, page_size // PAGE_BLOCK, PAGE_BLOCK * head_dim)
-        self.key, self.value = (torch.zeros(shape, dtype=torch.uint8, device=device).to(dtype)
-                                for _ in range(2))
-        self.key_exponent = self.value_exponent = None
-        if dtype != torch.bfloat16:
-            self.key_exponent, self.value_exponent = (
-                torch.zeros((pages, kv_heads, page_size), dtype=torch.uint8, device=device)
-                for _ in range(2))
-        self._describe()
+        rows = [zeros(*shape).to(dtype) for _ in range(2)]
+        exponents = [None, None] if dtype == torch.bfloat16 else \
+            [zeros(pages, kv_heads, page_size) for _ in range(2)]
+        self._describe(*rows, *exponents)
 
     @classmethod
     def from_pages(cls, key: Tensor, value: Tensor, key_exponent: Tensor | None = None,
@@ -134,9 +127,7 @@ class PagedKVCache:
         if any(x.device != key.device for x in (value, *exponents)):
             raise RuntimeError("a cache's tensors must be on one device")
         self = cls.__new__(cls)
-        self.key, self.value = key, value
-        self.key_exponent, self.value_exponent = exponents or (None, None)
-        self._describe()
+        self._describe(key, value, *(exponents or (None, None)))
         return self
 
     @staticmethod
@@ -149,7 +140,8 @@ class PagedKVCache:
             raise RuntimeError(f"a page is a multiple of {PAGE_BLOCK} positions of one or more "
                                "kv heads")
 
-    def _describe(self) -> None:
+    def _describe(self, *tensors: Tensor | None) -> None:
+        self._tensors = tensors
         pages, kv_heads, blocks, width = self.key.shape
         self.page_size, self.kv_heads = blocks * PAGE_BLOCK, kv_heads
         self.head_dim, self.dtype, self.device = width // PAGE_BLOCK, self.key.dtype, self.key.device
@@ -157,6 +149,30 @@ class PagedKVCache:
             self.key.data_ptr(), self.value.data_ptr(), _abi.ptr(self.key_exponent),
             _abi.ptr(self.value_exponent), pages, self.page_size, kv_heads, self.head_dim,
             PAGE_TYPES[self.dtype])
+        self._at = ctypes.addressof(self._struct)
+        self._sizes: dict[tuple, int] = {}
+
+    # The calls hand the tensors' addresses over, so they stay what they were made with.
+    key = property(lambda self: self._tensors[0])
+    value = property(lambda self: self._tensors[1])
+    key_exponent = property(lambda self: self._tensors[2])
+    value_exponent = property(lambda self: self._tensors[3])
+
+    def _workspace_bytes(self, *sizes: int) -> int:
+        """The attention's workspace for (batch, width, rows, heads, window, sinks)."""
+        nbytes = self._sizes.get(sizes)
+        if nbytes is None:
+            if len(self._sizes) >= 256:
+                self._sizes.clear()
+            b = _abi.PagedBatchStruct(self._at, self._at, self._at, *sizes[:2])  # (not read)
+            nbytes = self._sizes[sizes] = _abi.load().parrot_paged_attention_workspace_bytes(
+                self._at, ctypes.addressof(b), *sizes[2:])
+        return nbytes
+
+    def _batch(self, batch: PagedBatch) -> int:
+        if batch.table.device != self.device:
+            raise RuntimeError("the batch must be on the cache's device")
+        return batch._at
 
     def _new_rows(self, x: Tensor, heads: int, what: str, step: int) -> Tensor:
         _require(x, what)
@@ -176,13 +192,11 @@ class PagedKVCache:
         value = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
         if key.shape != value.shape:
             raise RuntimeError("as many rows of values as of keys")
-        b = batch._struct(self.device)
+        b, (kr, kh, _), (vr, vh, _) = self._batch(batch), key.stride(), value.stride()
         with _on(self.device):
             _abi.check(_abi.load().parrot_paged_append_bf16(
-                ctypes.addressof(self._struct), ctypes.addressof(b), key.data_ptr(),
-                _Strides2(key.stride(0), key.stride(1)), value.data_ptr(),
-                _Strides2(value.stride(0), value.stride(1)), key.shape[0], _stream(self.device)),
-                "parrot_paged_append_bf16")
+                self._at, b, key.data_ptr(), kr, kh, value.data_ptr(), vr, vh, key.shape[0],
+                _stream(self.device)), "parrot_paged_append_bf16")
 
     def read(self, batch: PagedBatch, positions: int,
              out: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
@@ -192,22 +206,25 @@ class PagedKVCache:
         ``LocalKVCache.key[:, :, :positions]``; strides that are multiples of 4)."""
         if torch.is_grad_enabled():
             raise RuntimeError("HIP paged read is inference-only; disable gradients")
-        b = batch._struct(self.device)
-        shape = (b.batch, self.kv_heads, positions, self.head_dim)
+        if self.device.type != "cuda":
+            raise RuntimeError(f"HIP paged read requires a ROCm (cuda) cache, got {self.device}")
+        b = self._batch(batch)
+        shape = (batch.table.shape[0], self.kv_heads, positions, self.head_dim)
         if out is None:
-            out = tuple(torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-                        for _ in range(2))
-        key, value = out
-        for x in out:
-            if x.dtype != torch.bfloat16 or x.device != self.device or x.shape != shape or \
-                    x.stride(3) != 1 or any(st % 4 for st in x.stride()[:3]) or x.data_ptr() % 8:
-                raise RuntimeError(f"out must be two bf16 tensors {list(shape)} on the cache's "
-                                   "device, strides multiples of 4")
+            key = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            value = torch.empty_like(key)
+        else:
+            key, value = out
+            for x in out:
+                if x.dtype != torch.bfloat16 or x.device != self.device or x.shape != shape or \
+                        x.stride(3) != 1 or any(st % 4 for st in x.stride()[:3]) or \
+                        x.data_ptr() % 8:
+                    raise RuntimeError(f"out must be two bf16 tensors {list(shape)} on the cache's "
+                                       "device, strides multiples of 4")
         with _on(self.device):
             _abi.check(_abi.load().parrot_paged_read_bf16(
-                ctypes.addressof(self._struct), ctypes.addressof(b), positions, key.data_ptr(),
-                _Strides3(*key.stride()[:3]), value.data_ptr(), _Strides3(*value.stride()[:3]),
-                _stream(self.device)), "parrot_paged_read_bf16")
+                self._at, b, positions, key.data_ptr(), *key.stride()[:3], value.data_ptr(),
+                *value.stride()[:3], _stream(self.device)), "parrot_paged_read_bf16")
         return key, value
 
     def attend(self, q: Tensor, batch: PagedBatch, *, scale: float, window: int | None = None,
@@ -230,24 +247,22 @@ class PagedKVCache:
         if sinks < 0:
             raise RuntimeError("sinks must not be negative")
         rows, device = q.shape[0], self.device
-        b = batch._struct(device)
-        shape = (rows, heads * self.head_dim)
+        b = self._batch(batch)
         if out is None:
-            out = torch.empty(shape, dtype=torch.bfloat16, device=device)
-        elif out.dtype != torch.bfloat16 or out.device != device or out.shape != shape or \
-                not out.is_contiguous() or out.data_ptr() % 8:
-            raise RuntimeError(f"out must be a contiguous bf16 tensor {list(shape)} on the "
-                               "cache's device")
-        lib = _abi.load()
-        cache, bp = ctypes.addressof(self._struct), ctypes.addressof(b)
+            out = torch.empty((rows, heads * self.head_dim), dtype=torch.bfloat16, device=device)
+        elif out.dtype != torch.bfloat16 or out.device != device or not out.is_contiguous() or \
+                out.shape != (rows, heads * self.head_dim) or out.data_ptr() % 8:
+            raise RuntimeError(f"out must be a contiguous bf16 tensor [{rows}, "
+                               f"{heads * self.head_dim}] on the cache's device")
         window = 0 if window is None else min(window, 2 ** 31 - 1)
         sinks = min(sinks, 2 ** 31 - 1)
-        nbytes = lib.parrot_paged_attention_workspace_bytes(cache, bp, rows, heads, window, sinks)
+        nbytes = self._workspace_bytes(*batch.table.shape, rows, heads, window, sinks)
         # a fresh one per call: calls on several streams share nothing
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        row, head, _ = q.stride()
         with _on(device):
-            _abi.check(lib.parrot_paged_attention_bf16(
-                cache, bp, q.data_ptr(), _Strides2(q.stride(0), q.stride(1)), rows, heads, window,
-                sinks, scale, out.data_ptr(), _abi.ptr(ws), nbytes, _stream(device)),
+            _abi.check(_abi.load().parrot_paged_attention_bf16(
+                self._at, b, q.data_ptr(), row, head, rows, heads, window, sinks, scale,
+                out.data_ptr(), _abi.ptr(ws), nbytes, _stream(device)),
                 "parrot_paged_attention_bf16")
         return out

@@ -32,28 +32,26 @@ BAD = [(dict(key=None), {}, -1), (dict(value_exponent=None), {}, -1), ({}, dict(
 def test_paged_arguments():
     from parrot import _abi
     lib, ref = _abi.load(), ctypes.byref
-    two, three = (ctypes.c_int64 * 2)(192, 96), (ctypes.c_int64 * 3)(19200, 9600, 96)
+    two, three = (192, 96), (19200, 9600, 96)
 
     def append(c, b, k=FAKE, ks=two, v=FAKE, vs=two, rows=4):
-        return lib.parrot_paged_append_bf16(ref(c), ref(b), k, ks, v, vs, rows, None)
+        return lib.parrot_paged_append_bf16(ref(c), ref(b), k, *ks, v, *vs, rows, None)
 
     def read(c, b, positions=100, k=FAKE, ks=three, v=FAKE, vs=three):
-        return lib.parrot_paged_read_bf16(ref(c), ref(b), positions, k, ks, v, vs, None)
+        return lib.parrot_paged_read_bf16(ref(c), ref(b), positions, k, *ks, v, *vs, None)
 
     def attend(c, b, q=FAKE, qs=two, rows=4, heads=8, window=0, sinks=0, scale=0.1, out=FAKE,
                ws=FAKE, wsb=1 << 40):
-        return lib.parrot_paged_attention_bf16(ref(c), ref(b), q, qs, rows, heads, window, sinks,
+        return lib.parrot_paged_attention_bf16(ref(c), ref(b), q, *qs, rows, heads, window, sinks,
                                                scale, out, ws, wsb, None)
     for c, b, status in BAD:
         for call in (append, read, attend):
             assert call(_cache(**c), _batch(**b)) == status, (c, b, call.__name__)
-    for call in (lib.parrot_paged_append_bf16, lib.parrot_paged_read_bf16):
-        args = (4, None) if call is lib.parrot_paged_append_bf16 else (None,)
-        first = () if call is lib.parrot_paged_append_bf16 else (100,)
-        assert call(None, ref(_batch()), *first, FAKE, two, FAKE, two, *args) == -1
+    assert lib.parrot_paged_append_bf16(None, ref(_batch()), FAKE, *two, FAKE, *two, 4, None) == -1
+    assert lib.parrot_paged_read_bf16(ref(_cache()), None, 9, FAKE, *three, FAKE, *three, None) == -1
     c, b = _cache(), _batch()
-    odd2, odd3 = (ctypes.c_int64 * 2)(192, 98), (ctypes.c_int64 * 3)(19200, 9600, 97)
-    assert append(c, b, k=None) == -1 and append(c, b, vs=None) == -1
+    odd2, odd3 = (192, 98), (19200, 9600, 97)
+    assert append(c, b, k=None) == -1 and append(c, b, v=None) == -1
     assert append(c, b, rows=-1) == -2 and append(c, b, rows=0) == 0
     assert append(c, b, ks=odd2) == -5 and append(c, b, v=FAKE + 4) == -5
     assert read(c, b, v=None) == -1 and read(c, b, positions=-1) == -2
@@ -66,7 +64,7 @@ def test_paged_arguments():
     for scale in (0.0, float("nan"), float("inf")):
         assert attend(c, b, scale=scale) == -2
     assert attend(c, b, rows=0) == 0 and attend(c, _batch(batch=0)) == 0
-    assert attend(c, b, qs=(ctypes.c_int64 * 2)(196, 96)) == -5
+    assert attend(c, b, qs=(196, 96)) == -5
     assert attend(c, b, q=FAKE + 8) == -5 and attend(c, b, out=FAKE + 4) == -5
     size = lib.parrot_paged_attention_workspace_bytes
     need = size(ref(c), ref(_batch(width=60)), 4, 8, 0, 0)
@@ -111,6 +109,13 @@ def test_cache_checks():
     for bad in (([[0]], [3], [1, 1]), ([[0]], [3], [4]), ([[0]], [3], [-1])):
         with pytest.raises(ValueError):
             PagedBatch.from_lists(*bad, device="cpu")
+    i32 = dict(dtype=torch.int32)
+    for bad in ((torch.zeros(2, 3, **i32), torch.zeros(3, **i32), torch.zeros(3, **i32)),
+                (torch.zeros(2, 3, **i32), torch.zeros(2, **i32), torch.zeros(2, **i32)),
+                (torch.zeros(2, 3), torch.zeros(2, **i32), torch.zeros(3, **i32)),
+                (torch.zeros(3, 2, **i32).t(), torch.zeros(2, **i32), torch.zeros(3, **i32))):
+        with pytest.raises(RuntimeError):
+            PagedBatch(*bad)
     b = PagedBatch.from_lists([[0, 2], [1]], [70, 3], [1, 2], device="cpu")
     assert b.table.tolist() == [[0, 2], [1, -1]] and b.starts.tolist() == [0, 1, 3]
     q = torch.zeros(3, 8, 96, dtype=torch.bfloat16)
