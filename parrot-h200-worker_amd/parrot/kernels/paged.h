@@ -99,6 +99,65 @@ __device__ __forceinline__ bool paged_find(const PagedBatch& b, int page, int un
   return false;
 }
 
+// As paged_find with the units of all sequences in rounds: the last unit of each
+// (which sees the most keys), then the last but one, and so on, so that a grid's
+// longest workgroups begin first and its shortest end it.
+template <typename F>
+__device__ __forceinline__ bool paged_find_last(const PagedBatch& b, int page, int unit, F units_of,
+                                                int& sequence, int& index, PagedSequence& s) {
+  const int lane = threadIdx.x & (kWave - 1);
+  auto sum = [](int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return __builtin_amdgcn_readlane(v, kWave - 1);
+  };
+  auto units_at = [&](int c, PagedSequence& mine) {
+    mine = paged_sequence(b, page, min(c + lane, b.batch - 1));
+    return c + lane < b.batch ? units_of(mine) : 0;
+  };
+  PagedSequence mine;
+  int units = units_at(0, mine);
+  auto first_rounds = [&](int rounds) {  // units of that many rounds
+    int all = sum(min(units, rounds));
+    for (int c = kWave; c < b.batch; c += kWave) {
+      PagedSequence other;
+      all += sum(min(units_at(c, other), rounds));
+    }
+    return all;
+  };
+  // The round: the largest number of rounds that lie before the unit.
+  int low = 0, high = unit + 1;  // first_rounds(low) <= unit; a round has one unit at least
+  if (first_rounds(high) <= unit) return false;
+  while (high - low > 1) {
+    const int mid = low + (high - low) / 2;
+    if (first_rounds(mid) <= unit) low = mid;
+    else high = mid;
+  }
+  int left = unit - first_rounds(low);
+  for (int c = 0; c < b.batch; c += kWave) {
+    if (c > 0) units = units_at(c, mine);
+    uint64_t who = __ballot(units > low);
+    const int n = __popcll(who);
+    if (left < n) {
+      for (; left > 0; --left) who &= who - 1;
+      const int at = __builtin_ctzll(who);
+      sequence = c + at;
+      index = __builtin_amdgcn_readlane(units, at) - 1 - low;
+      s.first = __builtin_amdgcn_readlane(mine.first, at);
+      s.count = __builtin_amdgcn_readlane(mine.count, at);
+      s.length = __builtin_amdgcn_readlane(mine.length, at);
+      s.stored = __builtin_amdgcn_readlane(mine.stored, at);
+      return true;
+    }
+    left -= n;
+  }
+  return false;
+}
+
 // The page of a position's block, or -1 where the table names none.
 __device__ __forceinline__ int paged_page(const PagedBatch& b, const PagedCache& c, int sequence,
                                           int at) {

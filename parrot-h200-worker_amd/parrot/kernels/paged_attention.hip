@@ -20,6 +20,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "attention_lds.h"
 #include "paged.h"
 
 namespace parrot {
@@ -582,16 +583,19 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a
   for (int t = 0; t < T; ++t) st.o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (begin + wave < end) {
     const int per_page = a.cache.page / kPagedBlock;
-    int ids = -1;  // lane j: the page of this wavefront's j-th block (of the last 64)
+    // Lane j: the page of this wavefront's j-th block (of the last 64), and which of
+    // its blocks that is.
+    int ids = -1, ins = 0;
     auto fetch = [&](int i, StepBlock<TYPE, D>& b) {
       const int j = (i - begin) / kWaves;
       if (j % kWave == 0) {
-        const int at = i + kWaves * lane;
-        ids = at < end ? paged_page(a.batch, a.cache, sequence, blocks.at(at) / per_page) : -1;
+        const int blk = blocks.at(i + kWaves * lane), at = blk / per_page;
+        ids = i + kWaves * lane < end ? paged_page(a.batch, a.cache, sequence, at) : -1;
+        ins = blk - at * per_page;
       }
       b.page = __builtin_amdgcn_readlane(ids, j % kWave);
       if (b.page < 0) return;
-      const int in = blocks.at(i) % per_page;
+      const int in = __builtin_amdgcn_readlane(ins, j % kWave);
       const int64_t at = static_cast<int64_t>(b.page) * a.cache.kv_heads + kvh;
       const int64_t off = (at * per_page + in) * (kPagedBlock * D / 8);
       const raw* kp = static_cast<const raw*>(a.cache.key) + off;
@@ -653,6 +657,361 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a
   merge_tile<D, kStepRows>(a, o_s, ml_s, s, row0, rows, kvh, split, begin < end);
 }
 
+// ---------------------------------------------------------------------------
+// Many rows per sequence (prompts and their chunks): a wavefront has 32 rows, the
+// four of a workgroup share key blocks through LDS.
+//
+// Each wavefront brings one of a stage's four matrices (K and V of two blocks) from
+// the pages into registers while the stage before is computed, and writes it to LDS
+// as bf16: an 8-bit page is converted once for 128 rows.  K's second half lies 128
+// bytes further, so that the 16 lanes of a read's phase, which take eight keys of
+// each half, fall into different banks.
+// ---------------------------------------------------------------------------
+
+constexpr int kTileRows = kWaves * kRows;
+
+// A V piece with its positions' powers of two.
+template <int TYPE>
+__device__ __forceinline__ bf16x8 value_piece(uint2 w, const float (&power)[8]) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t u = i ? w.y : w.x;
+    if constexpr (TYPE == kPagedE4m3) {
+      typedef float f32x2_t __attribute__((ext_vector_type(2)));
+      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(u), false);
+      const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(u), true);
+      x[4 * i] = lo[0], x[4 * i + 1] = lo[1], x[4 * i + 2] = hi[0], x[4 * i + 3] = hi[1];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * i + j] = static_cast<float>(static_cast<int8_t>(u >> (8 * j)));
+    }
+  }
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)  // (eight significant bits at most: the upper halves)
+    y[i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1] * power[2 * i + 1]),
+                                 __float_as_uint(x[2 * i] * power[2 * i]), 0x07060302u);
+  return __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
+}
+
+// The key of score e of a block of 32 from k0, in a 32-row tile.
+__device__ __forceinline__ int tile_key(int k0, int e) {
+  return k0 + 16 * ((e >> 2) & 1) +
+         4 * (2 * (e >> 3) + (static_cast<int>(threadIdx.x & (kWave - 1)) >> 5)) + (e & 3);
+}
+
+// Scores that the lane's row does not see become -infinity.  True where the block
+// holds a value that is not finite.
+template <int D>
+__device__ __forceinline__ bool mask_block(f32x16& sc, const bf16x8 (&vf)[D / 16], int k0,
+                                           int query, int stored, const AttendArgs& a) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int key = tile_key(k0, e);
+    const bool ok = (key < stored) & (key <= query) & ((query - key < a.window) | (key < a.sinks));
+    sc[e] = ok ? sc[e] : -INFINITY;
+  }
+  bool mine = false;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) mine |= has_nonfinite(vf[i]);
+  return __ballot(mine) != 0;
+}
+
+// Values that are not finite become 0.
+template <int N>
+__device__ __forceinline__ void clear_nonfinite(bf16x8 (&vf)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint4 v = __builtin_bit_cast(uint4, vf[i]);
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u;
+      if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0x0000ffffu;
+    }
+    vf[i] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+
+// Adds a block's values that are not finite (in the order of pages, in LDS) to the
+// rows that see their keys, as they are: any probability above 0 leaves them so.
+template <int D>
+__device__ __forceinline__ void add_nonfinite(State<D>& st, const uint16_t* v, int k0, int query,
+                                              int stored, const AttendArgs& a) {
+  const int half = static_cast<int>(threadIdx.x & (kWave - 1)) >> 5;
+#pragma unroll 1
+  for (int i = 0; i < kPagedBlock; ++i) {
+    const int key = k0 + i;
+    if (key >= stored || !visible(key, query, a.window, a.sinks)) continue;
+    const uint16_t* const from = v + ((i >> 2) & 3) * 128 + 4 * (i >> 4) + (i & 3);
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int dim = 32 * t + 8 * (e >> 2) + 4 * half + (e & 3);
+        const uint16_t x = from[(dim >> 4) * 512 + (dim & 15) * 8];
+        if ((x & 0x7f80u) == 0x7f80u) st.o[t][e] += bf16_to_f32(x);
+      }
+  }
+}
+
+// P of 16 scores as two B operands, rounded to bf16 once; l takes the sums before
+// the rounding.
+template <int D>
+__device__ __forceinline__ void probabilities(State<D>& st, const f32x16& sc, float scale_log2,
+                                              bf16x8 (&pf)[2]) {
+  // A row that has seen no key yet has m = -inf and only -inf scores:
+  // exp2(-inf - 0) = 0.
+  const float neg = st.m == -INFINITY ? 0.0f : -st.m;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + e], scale_log2, neg));
+      sum[e & 3] += p;
+      pf[s][e] = static_cast<__bf16>(p);
+    }
+  st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// Raises the running maximum to this lane's largest score where one passes it by
+// more than 2^8.
+template <int D>
+__device__ __forceinline__ void raise(State<D>& st, const f32x16& sc, float scale_log2) {
+  float t[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) t[i] = fmaxf(fmaxf(sc[3 * i], sc[3 * i + 1]), sc[3 * i + 2]);
+  float mx = fmaxf(fmaxf(fmaxf(t[0], t[1]), t[2]), fmaxf(fmaxf(t[3], t[4]), sc[15]));
+  mx *= scale_log2;
+  if (__ballot(mx > st.m + 8.0f) != 0) {
+    const float mn = fmaxf(st.m, fmaxf(mx, __shfl_xor(mx, 32)));
+    const float alpha = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - mn);
+    st.l *= alpha;
+#pragma unroll
+    for (int i = 0; i < State<D>::DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) st.o[i][e] *= alpha;
+    st.m = mn;
+  }
+}
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArgs a) {
+  constexpr int KU = D / 16, DT = D / 32, S = D / 32;
+  constexpr int kHalf = 64;                                  // elements between K's halves
+  constexpr int kK = kPagedBlock * D + kHalf;                // elements of K, then of V
+  constexpr int kBlock = kK + kPagedBlock * D;
+  constexpr int kBytes = TYPE == kPagedBf16 ? 2 : 1;
+  constexpr int kLoads = kPagedBlock * D * kBytes / (16 * kWave);  // 1 KB pieces of a matrix
+  __shared__ __attribute__((aligned(16))) uint16_t stage[2][2][kBlock];  // [buffer][block]
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const int unit = blockIdx.x / a.cache.kv_heads, kvh = blockIdx.x - unit * a.cache.kv_heads;
+  const int split = blockIdx.z;
+
+  auto units_of = [&](const PagedSequence& s) {
+    return (s.count * a.rep + kTileRows - 1) / kTileRows;
+  };
+  int sequence, tile;
+  PagedSequence s;
+  if (!paged_find_last(a.batch, a.cache.page, unit, units_of, sequence, tile, s)) return;
+  const int rows = s.count * a.rep;
+  const int tile0 = tile * kTileRows, row0 = tile0 + wave * kRows;
+  const TileRow mine = tile_row(s, row0 + col, rows, a.rep, kvh);
+  const int before = s.length - s.count;
+  const Blocks blocks = tile_blocks(before + tile0 / a.rep,
+                                    before + (min(tile0 + kTileRows, rows) - 1) / a.rep, s.stored,
+                                    a.window, a.sinks);
+  const int share = (blocks.count + a.splits - 1) / a.splits;
+  const int begin = min(split * share, blocks.count), end = min(begin + share, blocks.count);
+  // This wavefront's own rows (none: it only brings blocks).
+  const bool has = row0 < rows;
+  const int first = before + row0 / a.rep;
+  const int last = before + (min(row0 + kRows, rows) - 1) / a.rep;
+
+  State<D> st;
+  clear(st);
+  if (begin < end) {
+    bf16x8 qf[KU];
+    {
+      const uint16_t* row = a.q + mine.token * a.qs[0] + mine.head * a.qs[1] + 8 * half;
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        uint4 v = *reinterpret_cast<const uint4*>(row + 16 * u);
+        v.x ^= a.q_sign;
+        v.y ^= a.q_sign;
+        v.z ^= a.q_sign;
+        v.w ^= a.q_sign;
+        qf[u] = __builtin_bit_cast(bf16x8, v);
+      }
+    }
+    const int per_page = a.cache.page / kPagedBlock;
+    const int which = wave >> 1;       // block of a stage, and matrix, that this wavefront brings
+    const bool brings_v = wave & 1;
+    // Lane j: the page of the share's j-th block (of the last 64), and which of its
+    // blocks that is.
+    int ids = -1, ins = 0;
+    int page0 = -1, page1 = -1;        // of the stage that is brought
+    uint4 got[kLoads];                 // 8-bit types
+    uint32_t bytes[2] = {0, 0};
+    auto bring = [&](int i, int buf) {  // blocks i and i + 1
+      const int j = (i - begin) % kWave;
+      if (j == 0) {
+        const int blk = blocks.at(i + lane), at = blk / per_page;
+        ids = i + lane < end ? paged_page(a.batch, a.cache, sequence, at) : -1;
+        ins = blk - at * per_page;
+      }
+      page0 = __builtin_amdgcn_readlane(ids, j);
+      page1 = __builtin_amdgcn_readlane(ids, j + 1);
+      const int page = which ? page1 : page0;
+      if (page < 0) return;
+      const int in = __builtin_amdgcn_readlane(ins, j + which);
+      const int64_t at = static_cast<int64_t>(page) * a.cache.kv_heads + kvh;
+      const char* from = static_cast<const char*>(brings_v ? a.cache.value : a.cache.key) +
+                         (at * per_page + in) * (kPagedBlock * D * kBytes);
+      if constexpr (TYPE == kPagedBf16) {
+        const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(from, kPagedBlock * D * kBytes);
+        uint16_t* to = &stage[buf][which][brings_v ? kK : 0];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+          buffer_to_lds16(rsrc, to + 512 * u + (!brings_v && u >= S ? kHalf : 0), lane * 16u,
+                          1024u * u);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+          got[u] = reinterpret_cast<const uint4*>(from)[kWave * u + lane];
+        const int64_t e = at * a.cache.page + in * kPagedBlock;
+        if (brings_v) {  // positions 4 g .. + 3 and 16 + 4 g .. + 3 of the lane's pieces
+          const uint8_t* x = a.cache.value_exponent + e + 4 * ((lane >> 3) & 3);
+          bytes[0] = *reinterpret_cast<const uint32_t*>(x);
+          bytes[1] = *reinterpret_cast<const uint32_t*>(x + 16);
+        } else {  // keys c, c + 1 of either half
+          const uint8_t* x = a.cache.key_exponent + e + ((2 * lane) & 15);
+          bytes[0] = *reinterpret_cast<const uint16_t*>(x);
+          bytes[1] = *reinterpret_cast<const uint16_t*>(x + 16);
+        }
+      }
+    };
+    auto put = [&](int buf) {  // 8-bit types: what was brought, as bf16
+      if constexpr (TYPE != kPagedBf16) {
+        if ((which ? page1 : page0) < 0) return;
+        uint16_t* const to = &stage[buf][which][brings_v ? kK : 0];
+        if (brings_v) {
+          float power[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            power[e] = __uint_as_float(((bytes[e >> 2] >> (8 * (e & 3))) & 0xffu) << 23);
+#pragma unroll
+          for (int u = 0; u < kLoads; ++u) {
+            bf16x8* const p = reinterpret_cast<bf16x8*>(to + (kWave * u + lane) * 16);
+            p[0] = value_piece<TYPE>(make_uint2(got[u].x, got[u].y), power);
+            p[1] = value_piece<TYPE>(make_uint2(got[u].z, got[u].w), power);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < kLoads; ++u) {
+            const int at = (kWave * u + lane) * 16;
+            const uint32_t b = at >= 16 * D ? bytes[1] : bytes[0];
+            bf16x8* const p = reinterpret_cast<bf16x8*>(to + at + (at >= 16 * D ? kHalf : 0));
+            p[0] = piece_bf16<TYPE>(make_uint2(got[u].x, got[u].y), __uint_as_float((b & 0xffu) << 23));
+            p[1] = piece_bf16<TYPE>(make_uint2(got[u].z, got[u].w), __uint_as_float((b >> 8) << 23));
+          }
+        }
+      }
+    };
+
+    const int kn = (col >> 3) & 1;
+    const int kc = 4 * (2 * (col >> 4) + ((col >> 2) & 1)) + (col & 3);
+    const uint32_t k_off = static_cast<uint32_t>(kn * (S * 1024 + 2 * kHalf) + half * 256 + kc * 16);
+    const uint32_t v_off =
+        static_cast<uint32_t>(2 * kK + (col >> 4) * 1024 + half * 256 + (col & 15) * 16);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) const uint16_t*)&stage[0][0][0]));
+    auto block = [&](uint32_t lds, const uint16_t* v, int k0) {
+      bf16x8 kf[KU], vf[2 * DT], pf[2];
+      lds_frags<0, 512>(lds + k_off, kf);
+      f32x16 sc;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u], qf[u], sc, 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      read_values<0>(lds + v_off, vf);
+      // A block that every row of the tile sees whole needs no mask.
+      const bool whole = k0 + 31 <= min(first, s.stored - 1) &&
+                         (last - k0 < a.window || k0 + 31 < a.sinks);
+      bool odd = false;
+      if (!whole) {
+        odd = mask_block<D>(sc, vf, k0, mine.position, s.stored, a);
+      }
+      raise(st, sc, a.scale_log2);
+      probabilities(st, sc, a.scale_log2, pf);
+      // Values that some row must not see: times a probability of 0 an infinity or a
+      // NaN is not 0.
+      if (odd) clear_nonfinite(vf);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+          st.o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[2 * t + h], pf[h], st.o[t], 0, 0, 0);
+      if (odd) add_nonfinite<D>(st, v, k0, mine.position, s.stored, a);
+    };
+    bring(begin, 0);
+    for (int i = begin, buf = 0; i < end; i += 2, buf ^= 1) {
+      const int now0 = page0, now1 = page1;
+      if constexpr (TYPE == kPagedBf16) {
+        // This wavefront's copies have landed; past the barrier everybody's have, and
+        // nobody reads the other buffer any more.
+        wait_vm_barrier<0>();
+      } else {
+        put(buf);
+        __syncthreads();
+      }
+      if (i + 2 < end) bring(i + 2, buf ^ 1);
+      if (!has) continue;
+      // Blocks without a page, and those that none of this wavefront's rows sees, are
+      // left out.
+      auto seen = [&](int k0) {
+        return k0 <= last && (first - (k0 + 31) < a.window || k0 < a.sinks);
+      };
+#pragma unroll 1
+      for (int b = 0; b < 2; ++b) {
+        const int k0 = blocks.at(i + b) * kPagedBlock;
+        if ((b ? now1 : now0) >= 0 && seen(k0))
+          block(lds0 + (2 * buf + b) * (2 * kBlock), &stage[buf][b][kK], k0);
+      }
+    }
+  }
+  const float l = st.l + __shfl_xor(st.l, 32);
+  if (row0 + col >= rows) return;
+  const int64_t to = static_cast<int64_t>(mine.token) * a.heads + mine.head;
+  if (a.splits == 1) {
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<uint2*>(a.out + to * D + 32 * t + 8 * (e >> 2) + 4 * half) =
+            make_uint2(pack_bf16x2(st.o[t][e] * f, st.o[t][e + 1] * f),
+                       pack_bf16x2(st.o[t][e + 2] * f, st.o[t][e + 3] * f));
+  } else {
+    const int64_t at = to * a.splits + split;
+    if (half == 0) a.part_ml[at] = make_float2(st.m, l);
+    if (begin < end) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<float4*>(a.part + at * D + 32 * t + 8 * (e >> 2) + 4 * half) =
+              make_float4(st.o[t][e], st.o[t][e + 1], st.o[t][e + 2], st.o[t][e + 3]);
+    }
+  }
+}
+
 // Joins the shares of split tiles: a workgroup a row, its first wavefront one split a
 // lane for their weights, then D / 4 threads for every tenth (D = 96) of them.
 template <int D>
@@ -710,10 +1069,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a) {
 
 namespace {
 
-// Tiles of 16 rows, block by block from the pages, where a sequence has no more than
-// that on average (most of a tile of 32 would be empty).
-bool few_rows(int batch, int rows, int rep) {
-  return static_cast<int64_t>(rows) * rep <= int64_t{32} * std::min(batch, rows);
+// Rows of a workgroup's tile: 16 where a sequence has no more than 32 on average
+// (most of a larger tile would be empty), 128 from 96 on.
+int tile_rows(int batch, int rows, int rep) {
+  const int64_t all = static_cast<int64_t>(rows) * rep, n = std::min(batch, rows);
+  return all <= 32 * n ? kStepRows : all < 96 * n ? kRows : kTileRows;
 }
 
 }  // namespace
@@ -722,13 +1082,13 @@ bool few_rows(int batch, int rows, int rep) {
 int paged_attention_splits(int batch, int rows, int heads, int kv_heads, int page, int width,
                            int window, int sinks) {
   const int rep = heads / kv_heads;
-  const int tile = few_rows(batch, rows, rep) ? kStepRows : kRows;
+  const int tile = tile_rows(batch, rows, rep);
   const int64_t tiles = (static_cast<int64_t>(rows) * rep + tile - 1) / tile;
   const int64_t units = std::max<int64_t>(tiles, std::min(batch, rows)) * kv_heads;
   // The most keys a tile can see: its table's, or the window, the sinks and
   // the tile's own span.
   int64_t keys = static_cast<int64_t>(width) * page;
-  if (window < INT32_MAX) keys = std::min<int64_t>(keys, int64_t{window} + sinks + kRows + 64);
+  if (window < INT32_MAX) keys = std::min<int64_t>(keys, int64_t{window} + sinks + tile + 64);
   const int64_t want = (1024 + units - 1) / std::max<int64_t>(units, 1);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, keys / 256, kMaxSplits})));
 }
@@ -761,15 +1121,17 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   a.part_ml = reinterpret_cast<float2*>(a.part +
                                         static_cast<size_t>(splits) * batch.rows * heads * head_dim);
   a.out = out;
-  const bool few = few_rows(batch.batch, batch.rows, a.rep);
-  // ceil(n rep / 16 or 32) tiles a sequence
-  const int64_t tiles = static_cast<int64_t>(batch.rows) * a.rep / (few ? kStepRows : kRows) +
+  const int tile = tile_rows(batch.batch, batch.rows, a.rep);
+  // ceil(n rep / tile) tiles a sequence
+  const int64_t tiles = static_cast<int64_t>(batch.rows) * a.rep / tile +
                         std::min(batch.batch, batch.rows);
   const dim3 grid(static_cast<uint32_t>(tiles), cache.kv_heads, splits);
+  const dim3 tile_grid(static_cast<uint32_t>(tiles * cache.kv_heads), 1, splits);
   auto run = [&](auto t, auto d) {
     constexpr int TYPE = decltype(t)::value, D = decltype(d)::value;
-    if (few) paged_step_kernel<TYPE, D><<<grid, kWaves * kWave, 0, s>>>(a);
-    else paged_attend_kernel<TYPE, D><<<grid, kWaves * kWave, 0, s>>>(a);
+    if (tile == kStepRows) paged_step_kernel<TYPE, D><<<grid, kWaves * kWave, 0, s>>>(a);
+    else if (tile == kRows) paged_attend_kernel<TYPE, D><<<grid, kWaves * kWave, 0, s>>>(a);
+    else paged_tile_kernel<TYPE, D><<<tile_grid, kWaves * kWave, 0, s>>>(a);
     if (splits > 1) {
       paged_join_kernel<D><<<static_cast<uint32_t>(batch.rows * heads), 256, 0, s>>>(a);
     }

@@ -283,7 +283,9 @@ def test_pages_given_back(dtype):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_unseen_rows_do_not_reach_a_row(dtype, bad):
+@pytest.mark.parametrize("last", [73, 100, 110, 118, 150])
+@pytest.mark.parametrize("n", [1, 6, 15, 73])  # tiles of 16, 32 and 128 rows
+def test_unseen_rows_do_not_reach_a_row(dtype, bad, last, n):
     """Infinities and NaN among keys and values that a row does not see: later
     positions of its own chunk, positions the window has left (in a block that it
     still covers), and stale ones past the length."""
@@ -292,33 +294,29 @@ def test_unseen_rows_do_not_reach_a_row(dtype, bad):
     k[77, 0, 5] = v[77, 0, 5] = bad
     v[101, 1, 50] = bad
     run.append([150], k, v)
-    q = _rows(run.g, 150, 8, 96, std=1.5)
-    batch = run.batch([150])
-    for window, sinks in ((20, 0), (20, 3)):
+    # a sequence of the first `last` positions, of which n are its new rows
+    run.lengths = [last]
+    batch = run.batch([n])
+    q = _rows(run.g, n, 8, 96, std=1.5)
+    for window, sinks in ((20, 0), (20, 3), (None, 0)):
         got = run.cache.attend(q.cuda(), batch, scale=0.1, window=window, sinks=sinks)
-        got = got.double().cpu().view(150, 2, 4, 96)
+        got = got.double().cpu().view(n, 2, 4, 96)
         # the same without the bad rows
-        kc, vc = k.clone(), v.clone()
-        kc[77, 0], vc[77, 0], vc[101, 1] = 0, 0, 0
+        kc, vc = k[:last].clone(), v[:last].clone()
+        for head, row in ((0, 77), (1, 101)):
+            if row < last:
+                kc[row, head], vc[row, head] = 0 if row == 77 else kc[row, head], 0
         clean = Plain(dtype, 2, 96, 1)
-        clean.append(kc, vc, [150])
-        ref, bound = clean.attend(q, [150], 0.1, window, sinks)
-        ref, bound = ref.view(150, 2, 4, 96), bound.view(150, 2, 4, 96)
-        pos = torch.arange(150)
-        for head, rows in ((0, [77]), (1, [101])):
-            sees = sum(((pos >= r) & (pos < r + window)).int() for r in rows) > 0
+        clean.append(kc, vc, [last])
+        ref, bound = clean.attend(q, [n], 0.1, window, sinks)
+        ref, bound = ref.view(n, 2, 4, 96), bound.view(n, 2, 4, 96)
+        pos = torch.arange(last - n, last)
+        for head, row in ((0, 77), (1, 101)):
+            sees = (pos >= row) & (pos < row + (window or last))
             assert ((got[:, head] - ref[:, head]).abs() <= bound[:, head])[~sees].all()
             # and where a row does see it, it is not finite either (all of the
             # row's, or that value's dimension)
             assert not torch.isfinite(got[:, head][sees]).all(-1).any()
-    # stale rows past the length: a shorter sequence over the same pages
-    run.lengths = [70]
-    short = run.batch([70])
-    got = run.cache.attend(q[:70].cuda(), short, scale=0.1)
-    clean = Plain(dtype, 2, 96, 1)
-    clean.append(k[:70], v[:70], [70])
-    ref, bound = clean.attend(q[:70], [70], 0.1)
-    assert ((got.double().cpu() - ref).abs() <= bound).all()
 
 
 def test_far_pages():
