@@ -71,8 +71,46 @@ __device__ __forceinline__ Blocks tile_blocks(int first, int last, int stored, i
   return r;
 }
 
-__device__ __forceinline__ bool visible(int key, int query, int window, int sinks) {
-  return key <= query && (query - key < window || key < sinks);
+// The key blocks of a split: at least kMinShare, and as many as the sequence's last
+// rows (which see the most) need for `splits` of them.  A tile that one share covers
+// writes its output itself; its partial sums say so (kWhole).
+constexpr int kMinShare = 8;
+constexpr float kWhole = -1.0f;  // in place of a sum
+
+struct Share {
+  int begin, end;
+  bool whole;
+};
+
+__device__ __forceinline__ Share split_share(const PagedSequence& s, int rows, int tile, int rep,
+                                             const Blocks& blocks, int split, int splits,
+                                             int window, int sinks) {
+  if (splits == 1) return {0, blocks.count, true};
+  const int row0 = (rows - 1) / tile * tile;
+  const Blocks most = tile_blocks(s.length - s.count + row0 / rep, s.length - 1, s.stored, window,
+                                  sinks);
+  const int share = max((most.count + splits - 1) / splits, kMinShare);
+  const int begin = min(split * share, blocks.count);
+  return {begin, min(begin + share, blocks.count), blocks.count <= share};
+}
+
+// The keys that a row sees: those of its window, and the first `sinks` up to itself.
+struct Visible {
+  int first;       // of the window
+  uint32_t count;  // in the window
+  int sinks;       // keys below this are seen too
+  __device__ __forceinline__ bool window(int key) const {
+    return static_cast<uint32_t>(key - first) < count;
+  }
+  __device__ __forceinline__ bool operator()(int key) const {
+    return window(key) | (key < sinks);
+  }
+};
+
+__device__ __forceinline__ Visible visible_to(int query, int stored, int window, int sinks) {
+  const int last = min(query, stored - 1);
+  const int first = query >= window ? query - window + 1 : 0;
+  return {first, static_cast<uint32_t>(max(last - first + 1, 0)), min(sinks, last + 1)};
 }
 
 // A piece (8 values) of a page as bf16: K's values are times `power`, V's are
@@ -88,6 +126,18 @@ struct Piece<kPagedBf16> {
 
 __device__ __forceinline__ uint32_t bits(bf16x2_t v) { return __builtin_bit_cast(uint32_t, v); }
 
+// 128 + the eight int8 values, each by one instruction (an unsigned byte to float).
+__device__ __forceinline__ void int8_values(uint2 w, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t u = (i ? w.y : w.x) ^ 0x80808080u;
+    x[4 * i] = static_cast<float>(u & 0xffu);
+    x[4 * i + 1] = static_cast<float>((u >> 8) & 0xffu);
+    x[4 * i + 2] = static_cast<float>((u >> 16) & 0xffu);
+    x[4 * i + 3] = static_cast<float>(u >> 24);
+  }
+}
+
 template <int TYPE>
 __device__ __forceinline__ bf16x8 piece_bf16(typename Piece<TYPE>::raw w, float power) {
   if constexpr (TYPE == kPagedBf16) {
@@ -100,23 +150,33 @@ __device__ __forceinline__ bf16x8 piece_bf16(typename Piece<TYPE>::raw w, float 
     y.w = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, power, true));
     return __builtin_bit_cast(bf16x8, y);
   } else {
+    const float shift = -128.0f * power;
+    float x[8];
+    int8_values(w, x);
     uint32_t y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t half = (i < 2 ? w.x : w.y) >> (16 * (i & 1));
-      const float a = static_cast<float>(static_cast<int8_t>(half)) * power;
-      const float b = static_cast<float>(static_cast<int8_t>(half >> 8)) * power;
-      // (eight significant bits: the upper halves are the values)
-      y[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-    }
+    for (int i = 0; i < 4; ++i)  // (eight significant bits: the upper halves are the values)
+      y[i] = __builtin_amdgcn_perm(__float_as_uint(__builtin_fmaf(x[2 * i + 1], power, shift)),
+                                   __float_as_uint(__builtin_fmaf(x[2 * i], power, shift)),
+                                   0x07060302u);
     return __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
   }
 }
 
-__device__ __forceinline__ bool has_nonfinite(bf16x8 v) {
-  const uint4 w = __builtin_bit_cast(uint4, v);
-  auto bad = [](uint32_t x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; };
-  return bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
+// Whether any value is an infinity or a NaN: by the largest of their magnitudes' bits.
+template <int N>
+__device__ __forceinline__ bool has_nonfinite(const bf16x8 (&v)[N]) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 most = {0, 0};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint4 w = __builtin_bit_cast(uint4, v[i]);
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[j] & 0x7fff7fffu));
+  }
+  return (most[0] >= 0x7f80) | (most[1] >= 0x7f80);
 }
 
 // One wavefront's running softmax state over its 32 rows: m in log2 units,
@@ -164,12 +224,9 @@ __device__ __forceinline__ void attend_block(State<D>& st, const bf16x8 (&kf)[D 
   const bool whole = k0 + 31 <= min(first, stored - 1) &&
                      (last - k0 < a.window || k0 + 31 < a.sinks);
   if (!whole) {
+    const Visible sees = visible_to(query, stored, a.window, a.sinks);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int key = key_of(e);
-      const bool ok = key < stored && visible(key, query, a.window, a.sinks);
-      sc[e] = ok ? sc[e] : -INFINITY;
-    }
+    for (int e = 0; e < 16; ++e) sc[e] = sees(key_of(e)) ? sc[e] : -INFINITY;
   }
   float t[5];
 #pragma unroll
@@ -208,9 +265,7 @@ __device__ __forceinline__ void attend_block(State<D>& st, const bf16x8 (&kf)[D 
   // that the row does not see cleared.
   bool odd = false;
   if (!whole) {
-    bool mine = false;
-#pragma unroll
-    for (int i = 0; i < 2 * DT; ++i) mine |= has_nonfinite(vf[i]);
+    bool mine = has_nonfinite(vf);
     if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -239,16 +294,15 @@ __device__ __forceinline__ void attend_block(State<D>& st, const bf16x8 (&kf)[D 
       f32x16 sums = st.o[i];
 #pragma unroll 1
       for (int row = 0; row < kRows; ++row) {
-        const int at = __builtin_amdgcn_readlane(query, row);
+        const Visible sees = visible_to(__builtin_amdgcn_readlane(query, row), stored, a.window,
+                                        a.sinks);
         f32x16 y = st.o[i];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           bf16x8 v = vf[2 * i + s];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int key = key_of(8 * s + e);
-            if (!(key < stored && visible(key, at, a.window, a.sinks))) v[e] = static_cast<__bf16>(0.0f);
-          }
+          for (int e = 0; e < 8; ++e)
+            if (!sees(key_of(8 * s + e))) v[e] = static_cast<__bf16>(0.0f);
           y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pf[s], y, 0, 0, 0);
         }
         if (col == row) sums = y;
@@ -284,7 +338,7 @@ template <int D, int R>
 __device__ __forceinline__ void merge_tile(const AttendArgs& a, const float (&o_s)[kWaves][R][D + 4],
                                            const float (&ml_s)[kWaves][2][R],
                                            const PagedSequence& s, int row0, int rows, int kvh,
-                                           int split, bool any) {
+                                           int split, const Share& share) {
   for (int i = threadIdx.x; i < R * (D / 4); i += kWaves * kWave) {
     const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
     if (row0 + r >= rows) break;
@@ -309,14 +363,15 @@ __device__ __forceinline__ void merge_tile(const AttendArgs& a, const float (&o_
     }
     const TileRow row = tile_row(s, row0 + r, rows, a.rep, kvh);
     const int64_t to = static_cast<int64_t>(row.token) * a.heads + row.head;
-    if (a.splits == 1) {
+    if (share.whole) {
       const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
       *reinterpret_cast<uint2*>(a.out + to * D + d) =
           make_uint2(pack_bf16x2(y.x * f, y.y * f), pack_bf16x2(y.z * f, y.w * f));
+      if (a.splits > 1 && d == 0) a.part_ml[to * a.splits] = make_float2(0.0f, kWhole);
     } else {
       const int64_t at = to * a.splits + split;
       if (d == 0) a.part_ml[at] = make_float2(m, sum);
-      if (any) *reinterpret_cast<float4*>(a.part + at * D + d) = y;
+      if (share.begin < share.end) *reinterpret_cast<float4*>(a.part + at * D + d) = y;
     }
   }
 }
@@ -344,9 +399,10 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_attend_kernel(AttendA
   const int first = s.length - s.count + row0 / a.rep;
   const int last = s.length - s.count + (min(row0 + kRows, rows) - 1) / a.rep;
   const Blocks blocks = tile_blocks(first, last, s.stored, a.window, a.sinks);
-  // This workgroup's share of them.
-  const int share = (blocks.count + a.splits - 1) / a.splits;
-  const int begin = min(split * share, blocks.count), end = min(begin + share, blocks.count);
+  const Share share = split_share(s, rows, kRows, a.rep, blocks, split, a.splits, a.window,
+                                  a.sinks);
+  if (share.whole && split > 0) return;
+  const int begin = share.begin, end = share.end;
 
   State<D> st;
   clear(st);
@@ -416,7 +472,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_attend_kernel(AttendA
       *reinterpret_cast<float4*>(&o_s[wave][col][32 * t + 8 * (e >> 2) + 4 * half]) =
           make_float4(st.o[t][e], st.o[t][e + 1], st.o[t][e + 2], st.o[t][e + 3]);
   __syncthreads();
-  merge_tile<D, kRows>(a, o_s, ml_s, s, row0, rows, kvh, split, begin < end);
+  merge_tile<D, kRows>(a, o_s, ml_s, s, row0, rows, kvh, split, share);
 }
 
 // ---------------------------------------------------------------------------
@@ -473,11 +529,10 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
   const bool whole = k0 + 31 <= min(first, stored - 1) &&
                      (last - k0 < a.window || k0 + 31 < a.sinks);
   if (!whole) {
+    const Visible sees = visible_to(query, stored, a.window, a.sinks);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int key = key_of(e);
-      if (!(key < stored && visible(key, query, a.window, a.sinks))) sc[e >> 2][e & 3] = -INFINITY;
-    }
+    for (int e = 0; e < 8; ++e)
+      sc[e >> 2][e & 3] = sees(key_of(e)) ? sc[e >> 2][e & 3] : -INFINITY;
   }
   float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                    fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
@@ -506,9 +561,7 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
   for (int t = 0; t < T; ++t) vf[t] = piece_bf16<TYPE>(b.v[t], 1.0f);
   bool odd = false;  // (see attend_block)
   if (!whole) {
-    bool mine = false;
-#pragma unroll
-    for (int t = 0; t < T; ++t) mine |= has_nonfinite(vf[t]);
+    bool mine = has_nonfinite(vf);
     if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -533,13 +586,12 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
       f32x4 sums = st.o[t];
 #pragma unroll 1
       for (int row = 0; row < kStepRows; ++row) {
-        const int at = __builtin_amdgcn_readlane(query, row);
+        const Visible sees = visible_to(__builtin_amdgcn_readlane(query, row), stored, a.window,
+                                        a.sinks);
         bf16x8 v = vf[t];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int key = key_of(e);
-          if (!(key < stored && visible(key, at, a.window, a.sinks))) v[e] = static_cast<__bf16>(0.0f);
-        }
+        for (int e = 0; e < 8; ++e)
+          if (!sees(key_of(e))) v[e] = static_cast<__bf16>(0.0f);
         const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf, st.o[t], 0, 0, 0);
         if (col == row) sums = y;
       }
@@ -575,8 +627,10 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a
   const int first = s.length - s.count + row0 / a.rep;
   const int last = s.length - s.count + (min(row0 + kStepRows, rows) - 1) / a.rep;
   const Blocks blocks = tile_blocks(first, last, s.stored, a.window, a.sinks);
-  const int share = (blocks.count + a.splits - 1) / a.splits;
-  const int begin = min(split * share, blocks.count), end = min(begin + share, blocks.count);
+  const Share share = split_share(s, rows, kStepRows, a.rep, blocks, split, a.splits, a.window,
+                                  a.sinks);
+  if (share.whole && split > 0) return;
+  const int begin = share.begin, end = share.end;
 
   StepState<TYPE, D> st;
 #pragma unroll
@@ -654,7 +708,7 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a
     *reinterpret_cast<float4*>(&o_s[wave][col][16 * t + 4 * g]) =
         make_float4(st.o[t][0], st.o[t][1], st.o[t][2], st.o[t][3]);
   __syncthreads();
-  merge_tile<D, kStepRows>(a, o_s, ml_s, s, row0, rows, kvh, split, begin < end);
+  merge_tile<D, kStepRows>(a, o_s, ml_s, s, row0, rows, kvh, split, share);
 }
 
 // ---------------------------------------------------------------------------
@@ -670,28 +724,31 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a
 
 constexpr int kTileRows = kWaves * kRows;
 
-// A V piece with its positions' powers of two.
+// A V piece with its positions' powers of two (int8: shift = -128 times the power).
 template <int TYPE>
-__device__ __forceinline__ bf16x8 value_piece(uint2 w, const float (&power)[8]) {
+__device__ __forceinline__ bf16x8 value_piece(uint2 w, const float (&power)[8],
+                                              const float (&shift)[8]) {
   float x[8];
+  if constexpr (TYPE == kPagedE4m3) {
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t u = i ? w.y : w.x;
-    if constexpr (TYPE == kPagedE4m3) {
-      typedef float f32x2_t __attribute__((ext_vector_type(2)));
-      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(u), false);
-      const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(u), true);
-      x[4 * i] = lo[0], x[4 * i + 1] = lo[1], x[4 * i + 2] = hi[0], x[4 * i + 3] = hi[1];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * i + j] = static_cast<float>(static_cast<int8_t>(u >> (8 * j)));
+    for (int i = 0; i < 2; ++i) {
+      const int u = static_cast<int>(i ? w.y : w.x);
+      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(u, false);
+      const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8(u, true);
+      x[4 * i] = lo[0] * power[4 * i], x[4 * i + 1] = lo[1] * power[4 * i + 1];
+      x[4 * i + 2] = hi[0] * power[4 * i + 2], x[4 * i + 3] = hi[1] * power[4 * i + 3];
     }
+  } else {
+    int8_values(w, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(x[e], power[e], shift[e]);
   }
   uint32_t y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)  // (eight significant bits at most: the upper halves)
-    y[i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1] * power[2 * i + 1]),
-                                 __float_as_uint(x[2 * i] * power[2 * i]), 0x07060302u);
+    y[i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]),
+                                 0x07060302u);
   return __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
 }
 
@@ -706,16 +763,15 @@ __device__ __forceinline__ int tile_key(int k0, int e) {
 template <int D>
 __device__ __forceinline__ bool mask_block(f32x16& sc, const bf16x8 (&vf)[D / 16], int k0,
                                            int query, int stored, const AttendArgs& a) {
+  const Visible sees = visible_to(query, stored, a.window, a.sinks);
+  if (k0 < a.sinks) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int key = tile_key(k0, e);
-    const bool ok = (key < stored) & (key <= query) & ((query - key < a.window) | (key < a.sinks));
-    sc[e] = ok ? sc[e] : -INFINITY;
+    for (int e = 0; e < 16; ++e) sc[e] = sees(tile_key(k0, e)) ? sc[e] : -INFINITY;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = sees.window(tile_key(k0, e)) ? sc[e] : -INFINITY;
   }
-  bool mine = false;
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) mine |= has_nonfinite(vf[i]);
-  return __ballot(mine) != 0;
+  return __ballot(has_nonfinite(vf)) != 0;
 }
 
 // Values that are not finite become 0.
@@ -740,10 +796,10 @@ template <int D>
 __device__ __forceinline__ void add_nonfinite(State<D>& st, const uint16_t* v, int k0, int query,
                                               int stored, const AttendArgs& a) {
   const int half = static_cast<int>(threadIdx.x & (kWave - 1)) >> 5;
+  const Visible sees = visible_to(query, stored, a.window, a.sinks);
 #pragma unroll 1
   for (int i = 0; i < kPagedBlock; ++i) {
-    const int key = k0 + i;
-    if (key >= stored || !visible(key, query, a.window, a.sinks)) continue;
+    if (!sees(k0 + i)) continue;
     const uint16_t* const from = v + ((i >> 2) & 3) * 128 + 4 * (i >> 4) + (i & 3);
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
@@ -825,8 +881,10 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
   const Blocks blocks = tile_blocks(before + tile0 / a.rep,
                                     before + (min(tile0 + kTileRows, rows) - 1) / a.rep, s.stored,
                                     a.window, a.sinks);
-  const int share = (blocks.count + a.splits - 1) / a.splits;
-  const int begin = min(split * share, blocks.count), end = min(begin + share, blocks.count);
+  const Share share = split_share(s, rows, kTileRows, a.rep, blocks, split, a.splits, a.window,
+                                  a.sinks);
+  if (share.whole && split > 0) return;
+  const int begin = share.begin, end = share.end;
   // This wavefront's own rows (none: it only brings blocks).
   const bool has = row0 < rows;
   const int first = before + row0 / a.rep;
@@ -900,15 +958,17 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
         if ((which ? page1 : page0) < 0) return;
         uint16_t* const to = &stage[buf][which][brings_v ? kK : 0];
         if (brings_v) {
-          float power[8];
+          float power[8], shift[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
+          for (int e = 0; e < 8; ++e) {
             power[e] = __uint_as_float(((bytes[e >> 2] >> (8 * (e & 3))) & 0xffu) << 23);
+            shift[e] = -128.0f * power[e];
+          }
 #pragma unroll
           for (int u = 0; u < kLoads; ++u) {
             bf16x8* const p = reinterpret_cast<bf16x8*>(to + (kWave * u + lane) * 16);
-            p[0] = value_piece<TYPE>(make_uint2(got[u].x, got[u].y), power);
-            p[1] = value_piece<TYPE>(make_uint2(got[u].z, got[u].w), power);
+            p[0] = value_piece<TYPE>(make_uint2(got[u].x, got[u].y), power, shift);
+            p[1] = value_piece<TYPE>(make_uint2(got[u].z, got[u].w), power, shift);
           }
         } else {
 #pragma unroll
@@ -930,7 +990,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
         static_cast<uint32_t>(2 * kK + (col >> 4) * 1024 + half * 256 + (col & 15) * 16);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) const uint16_t*)&stage[0][0][0]));
-    auto block = [&](uint32_t lds, const uint16_t* v, int k0) {
+    // True where values that are not finite were left out.
+    auto block = [&](uint32_t lds, int k0) -> bool {
       bf16x8 kf[KU], vf[2 * DT], pf[2];
       lds_frags<0, 512>(lds + k_off, kf);
       f32x16 sc;
@@ -944,21 +1005,21 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
       // A block that every row of the tile sees whole needs no mask.
       const bool whole = k0 + 31 <= min(first, s.stored - 1) &&
                          (last - k0 < a.window || k0 + 31 < a.sinks);
+      // Values that some row must not see: times a probability of 0 an infinity or a
+      // NaN is not 0.
       bool odd = false;
       if (!whole) {
         odd = mask_block<D>(sc, vf, k0, mine.position, s.stored, a);
+        if (odd) clear_nonfinite(vf);
       }
       raise(st, sc, a.scale_log2);
       probabilities(st, sc, a.scale_log2, pf);
-      // Values that some row must not see: times a probability of 0 an infinity or a
-      // NaN is not 0.
-      if (odd) clear_nonfinite(vf);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int t = 0; t < DT; ++t)
           st.o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[2 * t + h], pf[h], st.o[t], 0, 0, 0);
-      if (odd) add_nonfinite<D>(st, v, k0, mine.position, s.stored, a);
+      return odd;
     };
     bring(begin, 0);
     for (int i = begin, buf = 0; i < end; i += 2, buf ^= 1) {
@@ -978,18 +1039,22 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
       auto seen = [&](int k0) {
         return k0 <= last && (first - (k0 + 31) < a.window || k0 < a.sinks);
       };
+      const uint32_t lds = lds0 + buf * (4 * kBlock);
+      const int k0 = blocks.at(i) * kPagedBlock, k1 = blocks.at(i + 1) * kPagedBlock;
+      uint32_t odd = 0;
+      if (now0 >= 0 && seen(k0)) odd = block(lds, k0);
+      if (now1 >= 0 && seen(k1)) odd |= 2 * block(lds + 2 * kBlock, k1);
 #pragma unroll 1
-      for (int b = 0; b < 2; ++b) {
-        const int k0 = blocks.at(i + b) * kPagedBlock;
-        if ((b ? now1 : now0) >= 0 && seen(k0))
-          block(lds0 + (2 * buf + b) * (2 * kBlock), &stage[buf][b][kK], k0);
-      }
+      for (int b = 0; odd != 0; ++b, odd >>= 1)
+        if (odd & 1)
+          add_nonfinite<D>(st, &stage[buf][b][kK], b ? k1 : k0, mine.position, s.stored, a);
     }
   }
   const float l = st.l + __shfl_xor(st.l, 32);
   if (row0 + col >= rows) return;
   const int64_t to = static_cast<int64_t>(mine.token) * a.heads + mine.head;
-  if (a.splits == 1) {
+  if (share.whole) {
+    if (a.splits > 1 && half == 0) a.part_ml[to * a.splits] = make_float2(0.0f, kWhole);
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -1012,29 +1077,68 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
   }
 }
 
-// Joins the shares of split tiles: a workgroup a row, its first wavefront one split a
-// lane for their weights, then D / 4 threads for every tenth (D = 96) of them.
+// A share's part in the joined row: in units of the largest maximum; -1 where it saw
+// nothing (a NaN sum has to come through).
+__device__ __forceinline__ float share_weight(float2 ml, float m) {
+  if (ml.x == -INFINITY) return ml.y == 0.0f ? -1.0f : 1.0f;
+  return __builtin_amdgcn_exp2f(ml.x - m);
+}
+
+// Rows of no sequence, and those that one share wrote whole, stay as they are.
+__device__ __forceinline__ bool joined_already(const AttendArgs& a, int64_t to) {
+  const int64_t token = to / a.heads;
+  return token >= a.batch.rows || token < a.batch.starts[0] ||
+         token >= a.batch.starts[a.batch.batch] || a.part_ml[to * a.splits].y == kWhole;
+}
+
+// Joins the shares of split tiles where there are many rows: D / 4 threads a row, one
+// share after the other.
 template <int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256) void paged_join_rows_kernel(AttendArgs a) {
+  constexpr int kPer = 256 / (D / 4);
+  const int slot = threadIdx.x / (D / 4), at = threadIdx.x - slot * (D / 4);
+  const int64_t to = static_cast<int64_t>(blockIdx.x) * kPer + slot;
+  if (slot >= kPer || joined_already(a, to)) return;
+  const float2* const ml = a.part_ml + to * a.splits;
+  const float4* const part = reinterpret_cast<const float4*>(a.part) + to * a.splits * (D / 4) + at;
+  float m = -INFINITY, sum = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < a.splits; ++i) m = fmaxf(m, ml[i].x);
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int i = 0; i < a.splits; ++i) {
+    const float f = share_weight(ml[i], m);
+    if (f < 0.0f) continue;
+    sum += ml[i].y * f;
+    const float4 x = part[i * (D / 4)];
+    y.x += x.x * f;
+    y.y += x.y * f;
+    y.z += x.z * f;
+    y.w += x.w * f;
+  }
+  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+  *reinterpret_cast<uint2*>(a.out + to * D + 4 * at) =
+      make_uint2(pack_bf16x2(y.x * f, y.y * f), pack_bf16x2(y.z * f, y.w * f));
+}
+
+// ... and where there are few: a workgroup a row, one share a lane for their weights,
+// then D / 4 threads for every tenth share (D = 96).
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_shares_kernel(AttendArgs a) {
   constexpr int kGroups = 256 / (D / 4);
   __shared__ float w_s[kMaxSplits];
   __shared__ float4 y_s[kGroups][D / 4];
   const int64_t to = blockIdx.x;
-  // Rows of no sequence stay as they are.
-  const int token = static_cast<int>(to / a.heads);
-  if (token < a.batch.starts[0] || token >= a.batch.starts[a.batch.batch]) return;
+  if (joined_already(a, to)) return;
   if (threadIdx.x < kWave) {
     const int i = threadIdx.x;
     const float2 ml = i < a.splits ? a.part_ml[to * a.splits + i] : make_float2(-INFINITY, 0.0f);
     float m = ml.x;
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-    // (a share that saw nothing adds nothing; a NaN sum has to come through)
-    const bool none = ml.x == -INFINITY && ml.y == 0.0f;
-    const float f = none ? 0.0f : ml.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
-    const float sum = wave_sum(none ? 0.0f : ml.y * f);
-    // (-1: not to be read)
-    w_s[i] = none ? -1.0f : sum == 0.0f ? 0.0f : f / sum;
+    const float f = share_weight(ml, m);
+    const float sum = wave_sum(f < 0.0f ? 0.0f : ml.y * f);
+    w_s[i] = f < 0.0f ? -1.0f : sum == 0.0f ? 0.0f : f / sum;
   }
   __syncthreads();
   const int group = threadIdx.x / (D / 4), at = threadIdx.x - group * (D / 4);
@@ -1133,7 +1237,10 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
     else if (tile == kRows) paged_attend_kernel<TYPE, D><<<grid, kWaves * kWave, 0, s>>>(a);
     else paged_tile_kernel<TYPE, D><<<tile_grid, kWaves * kWave, 0, s>>>(a);
     if (splits > 1) {
-      paged_join_kernel<D><<<static_cast<uint32_t>(batch.rows * heads), 256, 0, s>>>(a);
+      constexpr int kPer = 256 / (D / 4);
+      const uint32_t rows = static_cast<uint32_t>(batch.rows * heads);
+      if (rows < 2048) paged_join_shares_kernel<D><<<rows, 256, 0, s>>>(a);
+      else paged_join_rows_kernel<D><<<(rows + kPer - 1) / kPer, 256, 0, s>>>(a);
     }
     return hipGetLastError();
   };
