@@ -838,7 +838,7 @@ int parrot_paged_attention_bf16(const parrot_paged_cache* cache, const parrot_pa
   return status(parrot::launch_paged_attention(
       paged_cache(cache), cache->type, cache->head_dim, paged_batch(batch, rows),
       static_cast<const uint16_t*>(q), q_strides, heads, window > 0 ? window : INT32_MAX, sinks,
-      scale, splits, workspace, static_cast<uint16_t*>(out), as_stream(stream)));
+      scale, workspace, static_cast<uint16_t*>(out), as_stream(stream)));
 }
 
 int parrot_sample(const void* logits, int32_t type, int64_t rows, int32_t vocab, int64_t stride,

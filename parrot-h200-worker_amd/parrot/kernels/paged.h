@@ -179,7 +179,6 @@ size_t paged_attention_workspace_bytes(int splits, int rows, int heads, int head
 hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_dim,
                                   const PagedBatch& batch, const uint16_t* q,
                                   const int64_t* q_strides, int heads, int window, int sinks,
-                                  float scale, int splits, void* workspace, uint16_t* out,
-                                  hipStream_t s);
+                                  float scale, void* workspace, uint16_t* out, hipStream_t s);
 
 }  // namespace parrot

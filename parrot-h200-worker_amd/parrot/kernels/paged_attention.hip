@@ -44,7 +44,7 @@ struct AttendArgs {
   int sinks;
   float scale_log2;  // |scale| log2(e)
   uint32_t q_sign;   // 0x80008000 for a negative scale (q is negated), else 0
-  int splits;
+  int splits, whole;
   float* part;       // [rows * heads][splits][D], unnormalised
   float2* part_ml;   // [rows * heads][splits]
   uint16_t* out;     // [rows][heads][D]
@@ -72,8 +72,9 @@ __device__ __forceinline__ Blocks tile_blocks(int first, int last, int stored, i
 }
 
 // The key blocks of a split: at least kMinShare, and as many as the sequence's last
-// rows (which see the most) need for `splits` of them.  A tile that one share covers
-// writes its output itself; its partial sums say so (kWhole).
+// rows (which see the most) need for `splits` of them; all, where those see no more
+// than `whole`.  A tile that one share covers writes its output itself; its partial
+// sums say so (kWhole).
 constexpr int kMinShare = 8;
 constexpr float kWhole = -1.0f;  // in place of a sum
 
@@ -84,12 +85,12 @@ struct Share {
 
 __device__ __forceinline__ Share split_share(const PagedSequence& s, int rows, int tile, int rep,
                                              const Blocks& blocks, int split, int splits,
-                                             int window, int sinks) {
+                                             int whole, int window, int sinks) {
   if (splits == 1) return {0, blocks.count, true};
   const int row0 = (rows - 1) / tile * tile;
   const Blocks most = tile_blocks(s.length - s.count + row0 / rep, s.length - 1, s.stored, window,
                                   sinks);
-  const int share = max((most.count + splits - 1) / splits, kMinShare);
+  const int share = most.count <= whole ? most.count : max((most.count + splits - 1) / splits, kMinShare);
   const int begin = min(split * share, blocks.count);
   return {begin, min(begin + share, blocks.count), blocks.count <= share};
 }
@@ -177,6 +178,22 @@ __device__ __forceinline__ bool has_nonfinite(const bf16x8 (&v)[N]) {
       most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[j] & 0x7fff7fffu));
   }
   return (most[0] >= 0x7f80) | (most[1] >= 0x7f80);
+}
+
+// Values that are not finite become 0.
+template <int N>
+__device__ __forceinline__ void clear_nonfinite(bf16x8 (&vf)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint4 v = __builtin_bit_cast(uint4, vf[i]);
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u;
+      if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0x0000ffffu;
+    }
+    vf[i] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+  }
 }
 
 // One wavefront's running softmax state over its 32 rows: m in log2 units,
@@ -399,8 +416,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_attend_kernel(AttendA
   const int first = s.length - s.count + row0 / a.rep;
   const int last = s.length - s.count + (min(row0 + kRows, rows) - 1) / a.rep;
   const Blocks blocks = tile_blocks(first, last, s.stored, a.window, a.sinks);
-  const Share share = split_share(s, rows, kRows, a.rep, blocks, split, a.splits, a.window,
-                                  a.sinks);
+  const Share share = split_share(s, rows, kRows, a.rep, blocks, split, a.splits, a.whole,
+                                  a.window, a.sinks);
   if (share.whole && split > 0) return;
   const int begin = share.begin, end = share.end;
 
@@ -480,8 +497,9 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_attend_kernel(AttendA
 //
 // What bounds it: the pages' bytes, and below some MB the chain of dependent loads
 // (starts, lengths and table, then keys).  Each wavefront takes every fourth block of
-// its workgroup's share, straight from the pages into operand registers, and loads a
-// block while it computes the one before.
+// its workgroup's share, straight from the pages into operand registers: the next
+// block's keys once its scores are made, the next values once these are added, so that
+// a block's registers are never empty and there are few of them.
 //
 //   S^T = K Q^T     v_mfma_f32_16x16x32_bf16, A = 16 keys (two per block), B = 16
 //                   rows: lane 16 g + c holds keys 4 g .. + 3 and 16 + 4 g .. + 3 of
@@ -506,14 +524,16 @@ struct StepState {
   f32x4 o[D / 16];
 };
 
-template <int TYPE, int D>
+// One block: scores, softmax and values.  then(): called where the block's keys are no
+// longer needed.
+template <int TYPE, int D, typename F>
 __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlock<TYPE, D>& b,
                                            const bf16x8 (&qf)[D / 32], int k0, int query,
                                            int first, int last, int stored,
-                                           const AttendArgs& a) {
+                                           const AttendArgs& a, uint16_t* v_s, F then) {
   constexpr int S = D / 32, T = D / 16;
   const int lane = threadIdx.x & (kWave - 1);
-  const int g = lane >> 4, col = lane & 15;
+  const int g = lane >> 4;
   constexpr float kLazy = 8.0f;
   f32x4 sc[2];
 #pragma unroll
@@ -525,6 +545,7 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
       sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(piece_bf16<TYPE>(b.k[n * S + s], power), qf[s],
                                                       sc[n], 0, 0, 0);
   }
+  then();
   auto key_of = [&](int e) { return k0 + 16 * (e >> 2) + 4 * g + (e & 3); };
   const bool whole = k0 + 31 <= min(first, stored - 1) &&
                      (last - k0 < a.window || k0 + 31 < a.sinks);
@@ -559,56 +580,67 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
   bf16x8 vf[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) vf[t] = piece_bf16<TYPE>(b.v[t], 1.0f);
-  bool odd = false;  // (see attend_block)
+  uint32_t bytes[2] = {b.vbytes[0], b.vbytes[1]};
+  auto byte_of = [&](int e) { return (bytes[e >> 2] >> (8 * (e & 3))) & 0xffu; };
+  // Values that some row must not see: times a probability of 0 an infinity or a NaN
+  // is not 0.  They are left out and added to the rows that see them.
+  bool odd = false;
   if (!whole) {
     bool mine = has_nonfinite(vf);
     if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        mine |= ((b.vbytes[e >> 2] >> (8 * (e & 3))) & 0xffu) == kPagedNotFinite;
+      for (int e = 0; e < 8; ++e) mine |= byte_of(e) == kPagedNotFinite;
     }
     odd = __ballot(mine) != 0;
-  }
-  if constexpr (TYPE != kPagedBf16) {
+    if (odd) {
+      if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t byte = (b.vbytes[e >> 2] >> (8 * (e & 3))) & 0xffu;
-      const float y = p[e] * __uint_as_float(byte << 23);
-      p[e] = odd && sc[e >> 2][e & 3] == -INFINITY ? 0.0f : y;
+        for (int e = 0; e < 8; ++e) {
+          if (byte_of(e) == kPagedNotFinite) {  // (such an int8 row holds zeros)
+            bytes[e >> 2] &= ~(0xffu << (8 * (e & 3)));
+#pragma unroll
+            for (int t = 0; t < T; ++t) vf[t][e] = __builtin_bit_cast(__bf16, uint16_t{0x7fc0});
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < T; ++t) *reinterpret_cast<bf16x8*>(v_s + (kWave * t + lane) * 8) = vf[t];
+      clear_nonfinite(vf);
     }
   }
   bf16x8 pf;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) pf[e] = static_cast<__bf16>(p[e]);
-  if (odd) {
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      f32x4 sums = st.o[t];
-#pragma unroll 1
-      for (int row = 0; row < kStepRows; ++row) {
-        const Visible sees = visible_to(__builtin_amdgcn_readlane(query, row), stored, a.window,
-                                        a.sinks);
-        bf16x8 v = vf[t];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (!sees(key_of(e))) v[e] = static_cast<__bf16>(0.0f);
-        const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf, st.o[t], 0, 0, 0);
-        if (col == row) sums = y;
-      }
-      st.o[t] = sums;
-    }
-    return;
+  for (int e = 0; e < 8; ++e) {
+    const float y = TYPE == kPagedBf16 ? p[e] : p[e] * __uint_as_float(byte_of(e) << 23);
+    pf[e] = static_cast<__bf16>(y);
   }
 #pragma unroll
   for (int t = 0; t < T; ++t)
     st.o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[t], pf, st.o[t], 0, 0, 0);
+  if (odd) {
+    const Visible sees = visible_to(query, stored, a.window, a.sinks);
+#pragma unroll 1
+    for (int i = 0; i < kPagedBlock; ++i) {
+      if (!sees(k0 + i)) continue;
+      const uint16_t* const from = v_s + ((i >> 2) & 3) * 128 + 4 * (i >> 4) + (i & 3);
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint16_t x = from[t * 512 + (4 * g + e) * 8];
+          if ((x & 0x7f80u) == 0x7f80u) st.o[t][e] += bf16_to_f32(x);
+        }
+    }
+  }
 }
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kWaves * kWave, D < 128 ? 3 : 2) void paged_step_kernel(AttendArgs a) {
   constexpr int S = D / 32, T = D / 16;
   using raw = typename Piece<TYPE>::raw;
-  __shared__ float o_s[kWaves][kStepRows][D + 4];
+  // (a wavefront's part takes a block's values before the merge, if any is not finite)
+  __shared__ __attribute__((aligned(16))) float o_s[kWaves][kStepRows][D + 4];
+  static_assert(kStepRows * (D + 4) * 4 >= kPagedBlock * D * 2, "a block's values fit");
   __shared__ float ml_s[kWaves][2][kStepRows];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -627,8 +659,8 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a
   const int first = s.length - s.count + row0 / a.rep;
   const int last = s.length - s.count + (min(row0 + kStepRows, rows) - 1) / a.rep;
   const Blocks blocks = tile_blocks(first, last, s.stored, a.window, a.sinks);
-  const Share share = split_share(s, rows, kStepRows, a.rep, blocks, split, a.splits, a.window,
-                                  a.sinks);
+  const Share share = split_share(s, rows, kStepRows, a.rep, blocks, split, a.splits, a.whole,
+                                  a.window, a.sinks);
   if (share.whole && split > 0) return;
   const int begin = share.begin, end = share.end;
 
@@ -640,7 +672,10 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a
     // Lane j: the page of this wavefront's j-th block (of the last 64), and which of
     // its blocks that is.
     int ids = -1, ins = 0;
-    auto fetch = [&](int i, StepBlock<TYPE, D>& b) {
+    StepBlock<TYPE, D> b = {};
+    int64_t at = 0;  // the page and head that are loaded, and the block
+    int in = 0;
+    auto find = [&](int i) {
       const int j = (i - begin) / kWaves;
       if (j % kWave == 0) {
         const int blk = blocks.at(i + kWaves * lane), at = blk / per_page;
@@ -648,29 +683,33 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a
         ins = blk - at * per_page;
       }
       b.page = __builtin_amdgcn_readlane(ids, j % kWave);
+      in = __builtin_amdgcn_readlane(ins, j % kWave);
+      at = static_cast<int64_t>(max(b.page, 0)) * a.cache.kv_heads + kvh;
+    };
+    auto load = [&](const void* pages, const uint8_t* exponents, raw(&to)[T], uint32_t(&bytes)[2],
+                    auto key) {
       if (b.page < 0) return;
-      const int in = __builtin_amdgcn_readlane(ins, j % kWave);
-      const int64_t at = static_cast<int64_t>(b.page) * a.cache.kv_heads + kvh;
-      const int64_t off = (at * per_page + in) * (kPagedBlock * D / 8);
-      const raw* kp = static_cast<const raw*>(a.cache.key) + off;
-      const raw* vp = static_cast<const raw*>(a.cache.value) + off;
+      const raw* from = static_cast<const raw*>(pages) + (at * per_page + in) * (kPagedBlock * D / 8);
 #pragma unroll
-      for (int u = 0; u < T; ++u) b.k[u] = kp[kWave * u + lane];
-#pragma unroll
-      for (int u = 0; u < T; ++u) b.v[u] = vp[kWave * u + lane];
+      for (int u = 0; u < T; ++u) to[u] = from[kWave * u + lane];
       if constexpr (TYPE != kPagedBf16) {
-        const int64_t e = at * a.cache.page + in * kPagedBlock;
-        const uint8_t* ke = a.cache.key_exponent + e;
-        const uint8_t* ve = a.cache.value_exponent + e;
+        const uint8_t* e = exponents + at * a.cache.page + in * kPagedBlock;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          b.kbytes[n] = ke[16 * n + col];
-          b.vbytes[n] = *reinterpret_cast<const uint32_t*>(ve + 16 * n + 4 * g);
+          if constexpr (decltype(key)::value) bytes[n] = e[16 * n + col];
+          else bytes[n] = *reinterpret_cast<const uint32_t*>(e + 16 * n + 4 * g);
         }
       }
     };
-    StepBlock<TYPE, D> b0, b1;
-    fetch(begin + wave, b0);
+    auto load_keys = [&] {
+      load(a.cache.key, a.cache.key_exponent, b.k, b.kbytes, std::true_type{});
+    };
+    auto load_values = [&] {
+      load(a.cache.value, a.cache.value_exponent, b.v, b.vbytes, std::false_type{});
+    };
+    find(begin + wave);
+    load_keys();
+    load_values();
     bf16x8 qf[S];
     {
       const uint16_t* row = a.q + mine.token * a.qs[0] + mine.head * a.qs[1] + 8 * g;
@@ -684,17 +723,17 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_step_kernel(AttendArgs a
         qf[u] = __builtin_bit_cast(bf16x8, v);
       }
     }
-    auto compute = [&](int i, const StepBlock<TYPE, D>& b) {
-      if (b.page >= 0)
-        step_block<TYPE, D>(st, b, qf, blocks.at(i) * kPagedBlock, mine.position, first, last,
-                            s.stored, a);
-    };
-    for (int i = begin + wave; i < end; i += 2 * kWaves) {
-      if (i + kWaves < end) fetch(i + kWaves, b1);
-      compute(i, b0);
-      if (i + kWaves >= end) break;
-      if (i + 2 * kWaves < end) fetch(i + 2 * kWaves, b0);
-      compute(i + kWaves, b1);
+    for (int i = begin + wave; i < end; i += kWaves) {
+      const bool more = i + kWaves < end;
+      // (of a block without a page no row sees a key)
+      step_block<TYPE, D>(st, b, qf, blocks.at(i) * kPagedBlock, mine.position, first, last,
+                          b.page >= 0 ? s.stored : 0, a,
+                          reinterpret_cast<uint16_t*>(&o_s[wave][0][0]), [&] {
+                            if (!more) return;
+                            find(i + kWaves);
+                            load_keys();
+                          });
+      if (more) load_values();
     }
   }
   float l = st.l + __shfl_xor(st.l, 16);
@@ -772,22 +811,6 @@ __device__ __forceinline__ bool mask_block(f32x16& sc, const bf16x8 (&vf)[D / 16
     for (int e = 0; e < 16; ++e) sc[e] = sees.window(tile_key(k0, e)) ? sc[e] : -INFINITY;
   }
   return __ballot(has_nonfinite(vf)) != 0;
-}
-
-// Values that are not finite become 0.
-template <int N>
-__device__ __forceinline__ void clear_nonfinite(bf16x8 (&vf)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const uint4 v = __builtin_bit_cast(uint4, vf[i]);
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u;
-      if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0x0000ffffu;
-    }
-    vf[i] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
-  }
 }
 
 // Adds a block's values that are not finite (in the order of pages, in LDS) to the
@@ -881,8 +904,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
   const Blocks blocks = tile_blocks(before + tile0 / a.rep,
                                     before + (min(tile0 + kTileRows, rows) - 1) / a.rep, s.stored,
                                     a.window, a.sinks);
-  const Share share = split_share(s, rows, kTileRows, a.rep, blocks, split, a.splits, a.window,
-                                  a.sinks);
+  const Share share = split_share(s, rows, kTileRows, a.rep, blocks, split, a.splits, a.whole,
+                                  a.window, a.sinks);
   if (share.whole && split > 0) return;
   const int begin = share.begin, end = share.end;
   // This wavefront's own rows (none: it only brings blocks).
@@ -1182,19 +1205,41 @@ int tile_rows(int batch, int rows, int rep) {
 
 }  // namespace
 
-// Enough workgroups for the chip, each with 256 keys at least.
-int paged_attention_splits(int batch, int rows, int heads, int kv_heads, int page, int width,
-                           int window, int sinks) {
+namespace {
+
+struct Plan {
+  int tile, splits, whole;
+};
+
+// Splits: enough workgroups for the chip, each with 256 keys at least, where a tile may
+// see more keys than are faster without the join's launch: 768 for 16 and 32 rows
+// (one sequence, 8 heads on 2 of 96, one launch / split, us: 512 keys 6.0 / 8.4, 768
+// 7.1 / 8.1, 1024 8.2 / 8.3, 1536 10.4 / 8.4; 64 sequences of 8 kv heads of 64 in int8
+// 768 17.3 / 18.1, 1024 21.3 / 21.1), and for 128 rows the more the more workgroups
+// there are without (16: 384 12.8 / 14.2, 512 15.6 / 14.2; 104: 768 21.4 / 23.0, 1024
+// 27.0 / 26.4).
+Plan plan(int batch, int rows, int heads, int kv_heads, int page, int width, int window,
+          int sinks) {
   const int rep = heads / kv_heads;
   const int tile = tile_rows(batch, rows, rep);
   const int64_t tiles = (static_cast<int64_t>(rows) * rep + tile - 1) / tile;
-  const int64_t units = std::max<int64_t>(tiles, std::min(batch, rows)) * kv_heads;
+  const int64_t units = std::max<int64_t>({tiles, std::min(batch, rows), 1}) * kv_heads;
   // The most keys a tile can see: its table's, or the window, the sinks and
   // the tile's own span.
   int64_t keys = static_cast<int64_t>(width) * page;
   if (window < INT32_MAX) keys = std::min<int64_t>(keys, int64_t{window} + sinks + tile + 64);
-  const int64_t want = (1024 + units - 1) / std::max<int64_t>(units, 1);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, keys / 256, kMaxSplits})));
+  const int64_t line = tile == kTileRows ? std::min<int64_t>(384 + 4 * units, 1024) : 768;
+  const int64_t want = (1024 + units - 1) / units;
+  const int64_t splits =
+      keys <= line ? 1 : std::min<int64_t>({want, (keys + 255) / 256, kMaxSplits});
+  return {tile, static_cast<int>(splits), static_cast<int>(line / kPagedBlock)};
+}
+
+}  // namespace
+
+int paged_attention_splits(int batch, int rows, int heads, int kv_heads, int page, int width,
+                           int window, int sinks) {
+  return plan(batch, rows, heads, kv_heads, page, width, window, sinks).splits;
 }
 
 size_t paged_attention_workspace_bytes(int splits, int rows, int heads, int head_dim) {
@@ -1205,8 +1250,7 @@ size_t paged_attention_workspace_bytes(int splits, int rows, int heads, int head
 hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_dim,
                                   const PagedBatch& batch, const uint16_t* q,
                                   const int64_t* q_strides, int heads, int window, int sinks,
-                                  float scale, int splits, void* workspace, uint16_t* out,
-                                  hipStream_t s) {
+                                  float scale, void* workspace, uint16_t* out, hipStream_t s) {
   if (batch.rows == 0 || batch.batch == 0) return hipSuccess;
   AttendArgs a;
   a.cache = cache;
@@ -1220,12 +1264,15 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   a.sinks = sinks;
   a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
+  a.out = out;
+  const Plan p = plan(batch.batch, batch.rows, heads, cache.kv_heads, cache.page, batch.width,
+                      window, sinks);
+  const int tile = p.tile, splits = p.splits;
   a.splits = splits;
+  a.whole = p.whole;
   a.part = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part +
                                         static_cast<size_t>(splits) * batch.rows * heads * head_dim);
-  a.out = out;
-  const int tile = tile_rows(batch.batch, batch.rows, a.rep);
   // ceil(n rep / tile) tiles a sequence
   const int64_t tiles = static_cast<int64_t>(batch.rows) * a.rep / tile +
                         std::min(batch.batch, batch.rows);
