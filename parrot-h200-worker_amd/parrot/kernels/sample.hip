@@ -8,7 +8,8 @@
 // Weights are 64-bit whole numbers (w 2^shift, rounded; a row's sum fits): their
 // sums do not depend on an order, so a row's token does not depend on how the work
 // is split, and a border between two tokens lies where it does in 64-bit arithmetic
-// up to the rounding of single weights (2^-47 of the largest at 32768 tokens).
+// up to the errors of single weights (1e-10 of a weight, and its rounding, 2^-47 of
+// the largest at 32768 tokens).
 //
 // A workgroup per row, which keeps the row in LDS (32768 logits; longer rows are
 // read again, from L2, in each pass).  Nothing is sorted: the border of top-k or
@@ -37,7 +38,7 @@ constexpr int kStep = 4 * kWave;   // logits of a wavefront's step, four a lane
 constexpr int kHeld = 32768;       // logits of a row that LDS holds
 constexpr int kBins = 2048;
 constexpr int kList = 256;         // logits compared each with each
-constexpr int kTable = 256;
+constexpr int kTableBits = 8, kTable = 1 << kTableBits;
 constexpr int kPairs = 128;        // logits of a list that are ordered each with each
 constexpr int kShort = 512;        // top_k for which a list is made
 
@@ -116,6 +117,12 @@ __device__ __forceinline__ float4 logits4(const void* row, int at, int n, bool a
   return make_float4(x[0], x[1], x[2], x[3]);
 }
 
+// A row whose largest logit is an infinity: only the infinities are drawn from, alike.
+__device__ __forceinline__ float4 finite_of(float4 v) {
+  auto f = [](float x) { return x == INFINITY ? 0.0f : -INFINITY; };
+  return make_float4(f(v.x), f(v.y), f(v.z), f(v.w));
+}
+
 struct Entry {
   uint64_t f;
   uint32_t key;
@@ -131,6 +138,8 @@ struct Shared {
   float few[kThreads];     // a list of logits and their indices, in order
   int few_index[kThreads];
   uint64_t wave[kWaves];
+  uint64_t ahead[kList];  // of a list's logits: the mass before each
+  int rank[kList];         // ... and their number
   uint64_t before;
   uint32_t low[kWaves], high[kWaves];
   int found;
@@ -176,6 +185,7 @@ struct Row {
   const float* held;
   int n, steps;
   bool aligned;
+  bool infinite;  // infinities are 0 and everything else is left out (-infinity)
   __device__ __forceinline__ int first(int step) const {
     return (static_cast<int>(threadIdx.x >> 6) * steps + step) * kStep +
            4 * static_cast<int>(threadIdx.x & (kWave - 1));
@@ -183,7 +193,8 @@ struct Row {
   __device__ __forceinline__ float4 get(int step) const {
     const int i = first(step);
     if constexpr (HELD) return *reinterpret_cast<const float4*>(held + i);
-    return logits4<TYPE>(at, i, n, aligned);
+    float4 v = logits4<TYPE>(at, i, n, aligned);
+    return infinite ? finite_of(v) : v;
   }
   // f(index, logit, weight if one is held) for this thread's logits
   template <typename F>
@@ -281,6 +292,61 @@ struct Weights {
         },
         target, sh);
   }
+  // Leaves out what f does not keep.
+  template <typename F>
+  __device__ __forceinline__ void keep(F f) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      if (s >= row.steps) break;
+      const int i = row.first(s);
+      const float4 v = row.get(s);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[s][j] = f(i + j, x[j], w[s][j]) ? w[s][j] : 0;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // The sum of the weights; leaves each wavefront's share in sh.wave.
+  __device__ __forceinline__ uint64_t sum(Shared& sh) const {
+    uint64_t all = 0;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) all += (w[s][0] + w[s][1]) + (w[s][2] + w[s][3]);
+    all = wave_total(all);
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) sh.wave[threadIdx.x >> 6] = all;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) all += sh.wave[i];
+    return all;
+  }
+  // The first index at which the sum of the weights passes `target`.
+  __device__ __forceinline__ int locate(uint64_t target, Shared& sh) const {
+    const int wave = threadIdx.x >> 6;
+    uint64_t before = 0;
+    for (int i = 0; i < wave; ++i) before += sh.wave[i];
+    if (before <= target && target < before + sh.wave[wave]) {  // one wavefront
+      bool found = false;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        if (found) continue;
+        const uint64_t mine = (w[s][0] + w[s][1]) + (w[s][2] + w[s][3]);
+        const uint64_t upto = before + wave_upto(mine);
+        before = last_lane(upto);
+        found = target < before;  // one step
+        uint64_t at = upto - mine;
+        if (found && at <= target && target < at + mine) {
+          int j = 0;
+          if (target >= at + w[s][0]) at += w[s][0], j = 1;
+          if (j == 1 && target >= at + w[s][1]) at += w[s][1], j = 2;
+          if (j == 2 && target >= at + w[s][2]) j = 3;
+          sh.found = row.first(s) + j;
+        }
+      }
+    }
+    __syncthreads();
+    return sh.found;
+  }
 };
 
 // A list of at most one logit a thread, in the order of indices.
@@ -350,7 +416,7 @@ struct Edge {
   int until;
   // (as by order_key: -0 and 0 are equal; there is no NaN)
   __device__ __forceinline__ bool keeps(int i, float y) const {
-    return y > x || (y == x && i <= until);
+    return (y > x) | ((y == x) & (i <= until));
   }
 };
 
@@ -358,9 +424,14 @@ struct Edge {
 // lies further.
 struct Bins {
   float top, per_unit;
+  __device__ __forceinline__ float distance(float x) const { return (top - x) * per_unit; }
   __device__ __forceinline__ int operator()(float x) const {
-    const float d = x == top ? 0.0f : (top - x) * per_unit;
-    return d < static_cast<float>(kBins - 1) ? static_cast<int>(d) : kBins - 1;
+    return static_cast<int>(fminf(distance(x), static_cast<float>(kBins - 1)));
+  }
+  // Whether the logit is in the bin.
+  __device__ __forceinline__ bool in(float x, float bin) const {
+    const float d = distance(x);
+    return d >= bin && (d < bin + 1.0f || bin == static_cast<float>(kBins - 1));
   }
 };
 
@@ -373,6 +444,37 @@ __device__ __forceinline__ void clear_bins(Shared& sh) {
 
 __device__ __forceinline__ void add_to_bin(int bin, uint64_t v, Shared& sh) {
   if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[bin]), v);
+}
+
+// Of the n <= kList logits in sh.list: how many of them come before each (in the order
+// of size and index), and their sum, to sh.rank and sh.ahead.  Each is compared with
+// each, by as many threads a logit as there are.
+__device__ __forceinline__ void order_list(int n, Shared& sh) {
+  const int t = threadIdx.x;
+  const int width = n <= 64 ? 64 : n <= 128 ? 128 : kList;
+  const int i = t & (width - 1), parts = kThreads / width, part = t / width;
+  if (t < kList) {
+    sh.ahead[t] = 0;
+    sh.rank[t] = 0;
+  }
+  __syncthreads();
+  if (i < n) {
+    const Entry mine = sh.list[i];
+    uint64_t sum = 0;
+    int rank = 0;
+#pragma unroll 4
+    for (int j = part; j < n; j += parts) {
+      const Entry e = sh.list[j];
+      const bool before = (e.key > mine.key) | ((e.key == mine.key) & (e.index < mine.index));
+      rank += before;
+      sum += before ? e.f : 0;
+    }
+    if (rank) {
+      atomicAdd(&sh.rank[i], rank);
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.ahead[i]), sum);
+    }
+  }
+  __syncthreads();
 }
 
 // The last logit, in the order of size and index, that is needed for the sum of f
@@ -394,7 +496,7 @@ __device__ __forceinline__ Edge select(const R& row, F f, uint64_t need, Bins bi
   // range.
   uint32_t low = 0xffffffffu, high = 0;
   row.each([&](int i, float x, uint64_t w) {
-    if (bin_of(x) != bin) return;
+    if (!bin_of.in(x, static_cast<float>(bin))) return;
     const uint32_t key = order_key(x);
     low = min(low, key);
     high = max(high, key);
@@ -408,13 +510,10 @@ __device__ __forceinline__ Edge select(const R& row, F f, uint64_t need, Bins bi
   __syncthreads();
   const int n = sh.count;
   if (n <= kList) {
+    order_list(n, sh);
     if (static_cast<int>(threadIdx.x) < n) {
       const Entry mine = sh.list[threadIdx.x];
-      uint64_t at = before;
-      for (int j = 0; j < n; ++j) {
-        const Entry e = sh.list[j];
-        if (e.key > mine.key || (e.key == mine.key && e.index < mine.index)) at += e.f;
-      }
+      const uint64_t at = before + sh.ahead[threadIdx.x];
       if (at < need && need <= at + mine.f) {
         sh.edge = key_value(static_cast<uint64_t>(mine.key) << 32);
         sh.until = mine.index;
@@ -471,7 +570,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   row.n = a.vocab;
   row.steps = (a.vocab + kWaves * kStep - 1) / (kWaves * kStep);
   row.aligned = (reinterpret_cast<uintptr_t>(row.at) & (4 * kBytes - 1)) == 0 && row.n % 4 == 0;
-  const double temperature = a.temperature ? a.temperature[r] : a.temperature_all;
+  row.infinite = false;
+  // (logits are finite numbers: at 1e30 all that are not -infinity are alike)
+  const double temperature = fmin(a.temperature ? a.temperature[r] : a.temperature_all, 1e30);
   const int top_k = a.top_k ? a.top_k[r] : a.top_k_all;
   const double top_p = a.top_p ? a.top_p[r] : a.top_p_all;
   // (the largest always stays)
@@ -516,37 +617,47 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     }
   };
   if (top == -INFINITY) return answer(-1, 0.0);  // nothing to draw from
-  if (!(temperature > 0.0) || top_k == 1) {      // the first of the largest
+  if (!(temperature > 0.0) || top_k == 1) {  // the first of the largest
     auto largest = [&](int, float x, uint64_t) -> uint64_t { return x == top; };
     total(row, largest, sh);
     return answer(row.locate(largest, 0, sh), 1.0);
   }
 
-  // log2 w (a largest logit of infinity: 0 for it, -infinity for the others), and w
-  // 2^shift: 2^y = 2^(k / 256) e^r with k = round(256 y), r = (256 y - k) ln 2 / 256,
-  // |r| <= 0.00136, whose series to the third power is right to 2e-13.
-  const double per_unit = 1.4426950408889634074 / temperature;
-  const double origin = top < INFINITY ? top : 1e300;
-  const double lowest = -(a.shift + 2);  // 2^lowest rounds to 0
-  auto power = [&](float x) -> double {
-    return fmax(fmin((static_cast<double>(x) - origin) * per_unit, 0.0), lowest);
+  if (top == INFINITY) {
+    row.infinite = true;
+    if constexpr (HELD) {
+      __syncthreads();
+      for (int s = 0; s < row.steps; ++s) {
+        float4* const v = reinterpret_cast<float4*>(&held[row.first(s)]);
+        *v = finite_of(*v);
+      }
+      __syncthreads();
+    }
+    mine = mine == INFINITY ? 0.0f : -INFINITY;
+    top = 0.0f;
+  }
+
+  // w 2^shift: w = 2^(k / 256) e^r with k = round(256 log2 w), |r| <= ln 2 / 512, and
+  // e^r - 1 <= 0.00136 to the third power in 32 bits: w is right to 1e-10.
+  const double per_unit = kTable * 1.4426950408889634074 / temperature;
+  const double origin = top;
+  const double lowest = -kTable * (a.shift + 2);  // rounds to 0
+  auto weight = [&](float x, int scale) -> double {  // w 2^scale
+    const double z = fmax((static_cast<double>(x) - origin) * per_unit, lowest);
+    const double whole = rint(z);
+    const int k = static_cast<int>(whole);
+    const float r = static_cast<float>(z - whole) * (0.693147180559945309f / kTable);
+    const float more = __builtin_fmaf(__builtin_fmaf(r, 1.0f / 6.0f, 0.5f) * r, r, r);
+    const double at = sh.table[k & (kTable - 1)];
+    return ldexp(fma(at, static_cast<double>(more), at), (k >> kTableBits) + scale);
   };
-  auto scaled = [&](double y, int& k) -> double {  // 2^(y - floor(k / 256))
-    const double z = y * kTable, whole = rint(z);
-    k = static_cast<int>(whole);
-    const double e = (z - whole) * (0.69314718055994530942 / kTable);
-    return sh.table[k & (kTable - 1)] * fma(fma(fma(e, 1.0 / 6.0, 0.5), e, 1.0), e, 1.0);
-  };
+  // (rounded to a whole number where 2^52 is added to it)
   auto mass = [&](float x) -> uint64_t {
-    int k;
-    const uint64_t u = __builtin_bit_cast(uint64_t, scaled(power(x), k));
-    const int down = 52 - a.shift - (static_cast<int>(u >> 52) - 1023 + (k >> 8));  // 2 .. 55
-    return (((u & ((uint64_t{1} << 52) - 1)) | (uint64_t{1} << 52)) + (uint64_t{1} << (down - 1))) >>
-           down;
+    return __builtin_bit_cast(uint64_t, weight(x, a.shift) + 0x1p52) - (uint64_t{1075} << 52);
   };
   // The bins reach as far as weights do (2^-46 at 32 T), but no further than 32.
-  const Bins bins{top, top < INFINITY ? (kBins - 1) / static_cast<float>(
-                                            fmax(fmin(32.0 * temperature, 32.0), 1e-30)) : 0.0f};
+  const Bins bins{top, (kBins - 1) / static_cast<float>(
+                                         fmax(fmin(32.0 * temperature, 32.0), 1e-30))};
   const uint64_t least_mass = static_cast<uint64_t>(ldexp(fmax(min_p, 0.0), a.shift));
   auto needed = [&](uint64_t all) -> uint64_t {  // of the mass, for top_p
     const uint64_t x = static_cast<uint64_t>(ceil(fmax(top_p, 0.0) * static_cast<double>(all)));
@@ -559,9 +670,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     return x < all ? x : all - 1;
   };
   auto share = [&](float x, uint64_t all) -> double {
-    int k;
-    const double w = scaled(power(x), k);
-    return ldexp(w, (k >> 8) + a.shift) / static_cast<double>(all);
+    return weight(x, a.shift) / static_cast<double>(all);
   };
   auto one = [](int, float, uint64_t) -> uint64_t { return 1; };
   auto held_weight = [](int, float, uint64_t w) -> uint64_t { return w; };
@@ -577,7 +686,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     __syncthreads();
     uint64_t before;
     const int last = find_bin(top_k, before, sh);
-    if (last < kBins - 1 && top < INFINITY) {
+    if (last < kBins - 1) {
       // One bin further down, so that no rounding here leaves one of them out (the
       // count says whether it did).
       const float from = top - static_cast<float>(last + 2) / bins.per_unit;
@@ -635,21 +744,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     Few list{few, t < few ? sh.few[t] : -INFINITY, 0};
     if (t < few) list.w = mass(list.x);
     if (few <= kPairs) {
-      // Each with each: how many come before it, and their mass (of which all are
-      // kept by top_k where it is).
+      // (all that come before a logit that top_k keeps are kept by it)
       if (t < few) sh.list[t] = {list.w, order_key(list.x), t};
       __syncthreads();
+      order_list(few, sh);
       uint64_t before = 0;
       if (t < few) {
-        const uint32_t key = order_key(list.x);
-        int rank = 0;
-        for (int j = 0; j < few; ++j) {
-          const Entry e = sh.list[j];
-          const bool ahead = e.key > key || (e.key == key && j < t);
-          rank += ahead;
-          before += ahead ? e.f : 0;
-        }
-        if (by_count && rank >= top_k) list.w = 0;
+        before = sh.ahead[t];
+        if (by_count && sh.rank[t] >= top_k) list.w = 0;
       }
       if (top_p < 1.0 && before >= needed(total(list, held_weight, sh))) list.w = 0;
       if (list.w < least_mass) list.w = 0;
@@ -691,23 +793,22 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
           const uint64_t w = f(i + j, x[j], 0);
           all_of.w[s][j] = w;
           if (top_p < 1.0) {
-            const int b = bins(x[j]);
-            if (b < kBins - 1) add_to_bin(b, w, sh);
+            const float d = bins.distance(x[j]);
+            if (d < static_cast<float>(kBins - 1)) add_to_bin(static_cast<int>(d), w, sh);
           }
         }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     if (top_p < 1.0) {
-      const uint64_t need = needed(total(all_of, held_weight, sh));
+      const uint64_t need = needed(all_of.sum(sh));
       __syncthreads();
       edge = select(all_of, held_weight, need, bins, true, sh);
     }
-    auto last = [&](int i, float x, uint64_t w) -> uint64_t {
-      return w >= least_mass && edge.keeps(i, x) ? w : 0;
-    };
-    const uint64_t all = total(all_of, last, sh);
-    const int token = all_of.locate(last, drawn(all), sh);
+    if (top_p < 1.0 || least_mass > 0)
+      all_of.keep([&](int i, float x, uint64_t w) { return (w >= least_mass) & edge.keeps(i, x); });
+    const uint64_t all = all_of.sum(sh);
+    const int token = all_of.locate(drawn(all), sh);
     return answer(token, share(held[token], all));
   } else {
     if (top_p < 1.0) edge = select(row, f, needed(total(row, f, sh)), bins, false, sh);
@@ -717,7 +818,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     };
     const uint64_t all = total(row, last, sh);
     const int token = row.locate(last, drawn(all), sh);
-    return answer(token, share(logit<TYPE>(row.at, token), all));
+    const float x = logit<TYPE>(row.at, token);
+    return answer(token, share(row.infinite ? 0.0f : x, all));
   }
 }
 
@@ -739,7 +841,7 @@ hipError_t launch_sample(const void* logits, int type, int rows, int vocab, int6
                temperature_all, top_p_all, min_p_all, top_k_all, 0, token, probability};
   int bits = 0;
   while ((int64_t{1} << bits) < vocab) ++bits;
-  a.shift = bits > 12 ? 62 - bits : 50;  // (a row's sum fits 63 bits)
+  a.shift = bits > 12 ? 62 - bits : 50;  // (a row's sum fits 63 bits, a weight 52)
   if (type == kLogitF32) launch<kLogitF32>(a, rows, s);
   else if (type == kLogitBf16) launch<kLogitBf16>(a, rows, s);
   else launch<kLogitF16>(a, rows, s);
