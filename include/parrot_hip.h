@@ -860,6 +860,21 @@ int parrot_paged_append_bf16(const parrot_paged_cache* cache, const parrot_paged
                              const void* k, int64_t k_row, int64_t k_head, const void* v,
                              int64_t v_row, int64_t v_head, int32_t rows, void* stream);
 
+/* As above with RoPE: the keys are rotated by their positions (interleaved pairs by
+ * the fp32 tables cos and sin [positions, head_dim / 2], positions past them by the
+ * last) and rounded to bf16 before they are stored, and the query rows q, bf16
+ * [rows, heads, head_dim] with the given element strides (multiples of 4), go to
+ * q_out [rows, heads, head_dim] in the same way (8-byte aligned; not in place).
+ * Rows of q_out that no sequence has, or that lie before its position 0, are left as
+ * they are.  New beside parrot_rope_qkv_bf16 (LocalGQA._project, parrot/model.py:206-262),
+ * whose rows have one first position. */
+int parrot_paged_append_rope_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
+                                  const void* k, int64_t k_row, int64_t k_head, const void* v,
+                                  int64_t v_row, int64_t v_head, int32_t rows, const float* cos,
+                                  const float* sin, int32_t positions, const void* q,
+                                  int64_t q_row, int64_t q_head, int32_t heads, void* q_out,
+                                  void* stream);
+
 /* Reads positions 0 .. positions - 1 of every sequence back: k and v, bf16
  * [batch, kv_heads, positions, head_dim] with the given element strides of
  * sequences, heads and positions (multiples of 4), zero from a sequence's length

@@ -159,6 +159,9 @@ SIGNATURES: dict[str, tuple] = {
         ctypes.c_int, [_p, _p, _p, _i64, _i32, _i32, _p, _p, _p, _p]),
     "parrot_paged_append_bf16": (
         ctypes.c_int, [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _p]),
+    "parrot_paged_append_rope_bf16": (
+        ctypes.c_int, [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _i32, _p, _i64, _i64,
+                       _i32, _p, _p]),
     "parrot_paged_read_bf16": (
         ctypes.c_int, [_p, _p, _i32, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p]),
     "parrot_paged_attention_workspace_bytes": (_sz, [_p, _p, _i32, _i32, _i32, _i32]),

@@ -45,17 +45,27 @@ class DecodeGraph:
     ``decode_step`` do.  The state must stay with this object: eager decode
     steps on it in between are allowed (they advance both positions
     consistently).
+
+    With ``sampling`` (a dict of hip_moe.sample's parameters, numbers or tensors of
+    one value per sequence that every replay reads) the tokens are drawn, by the
+    numbers ``uniform`` [batch] that each ``step(ids, uniform)`` brings, exactly as
+    ``model.decode_sample`` would.
     """
 
     @torch.inference_mode()
-    def __init__(self, model: Parrot, state: GenerationState, logits: bool = False):
+    def __init__(self, model: Parrot, state: GenerationState, logits: bool = False,
+                 sampling: dict | None = None):
         if state.position_device is None:
             raise RuntimeError("DecodeGraph needs a generation state from a HIP-backend prefill")
         if model.training:
             raise RuntimeError("DecodeGraph requires model.eval()")
+        if logits and sampling is not None:
+            raise RuntimeError("a DecodeGraph returns either logits or drawn tokens")
         self.model, self.state, self.logits = model, state, logits
         device = state.position_device.device
         self.ids = torch.zeros((state.batch_size, 1), dtype=torch.long, device=device)
+        self.sampling = None if sampling is None else dict(sampling)
+        self.uniform = torch.zeros(state.batch_size, device=device)
         start = state.position
         limit = model.config.max_seq_len
         if start >= limit:
@@ -128,8 +138,9 @@ class DecodeGraph:
         else:
             # The tokens land in the input buffer, read by the next replay's
             # first launch (the embedding gather), after this step's reads.
+            draw = None if self.sampling is None else (self.uniform, self.sampling)
             out, _ = self.model.decode_step(self.ids, self.state, _next_token_only=True,
-                                            _out=self.ids)
+                                            _out=self.ids, _draw=draw)
         return out
 
     def _rewind(self, position: int) -> None:
@@ -137,13 +148,19 @@ class DecodeGraph:
         self.state.position_device.fill_(position)
 
     @torch.inference_mode()
-    def step(self, input_ids: Tensor) -> Tensor:
+    def step(self, input_ids: Tensor, uniform: Tensor | None = None) -> Tensor:
         if input_ids.shape != self.ids.shape:
             raise ValueError("decode input must be [cached batch, 1]")
+        if (uniform is None) != (self.sampling is None):
+            raise ValueError("a step takes uniform numbers where the graph draws its tokens")
+        if uniform is not None and uniform.shape != self.uniform.shape:
+            raise ValueError("uniform must be [cached batch]")
         if self.state.position >= self.model.config.max_seq_len:
             raise ValueError("Generation state has reached max_seq_len")
         if input_ids.data_ptr() != self.ids.data_ptr():
             self.ids.copy_(input_ids)
+        if uniform is not None and uniform.data_ptr() != self.uniform.data_ptr():
+            self.uniform.copy_(uniform)
         self.graph.replay()
         self.state.position += 1
         return self.out

@@ -774,19 +774,51 @@ size_t parrot_experts_workspace_bytes(int64_t tokens, int32_t dim, int32_t hidde
   return experts_ws(nullptr, tokens, dim, hidden_dim, shared_dim).bytes;
 }
 
+namespace {
+
+int paged_append(const parrot_paged_cache* cache, const parrot_paged_batch* batch, const void* k,
+                 int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
+                 int32_t rows, const parrot::PagedRope& rope, void* stream) {
+  const int64_t k_strides[3] = {k_row, k_head, 0}, v_strides[3] = {v_row, v_head, 0};
+  if (int rc = check_paged_rows(k, k_strides, 4)) return rc;
+  if (int rc = check_paged_rows(v, v_strides, 4)) return rc;
+  return status(parrot::launch_paged_append(
+      paged_cache(cache), cache->type, cache->head_dim, paged_batch(batch, rows),
+      static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_strides, v_strides, rope,
+      as_stream(stream)));
+}
+
+}  // namespace
+
 int parrot_paged_append_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
                              const void* k, int64_t k_row, int64_t k_head, const void* v,
                              int64_t v_row, int64_t v_head, int32_t rows, void* stream) {
   if (int rc = check_paged(cache, batch)) return rc;
   if (rows < 0 || rows > (1 << 30)) return PARROT_ERR_BAD_SHAPE;
   if (rows == 0) return PARROT_OK;
-  const int64_t k_strides[3] = {k_row, k_head, 0}, v_strides[3] = {v_row, v_head, 0};
-  if (int rc = check_paged_rows(k, k_strides, 4)) return rc;
-  if (int rc = check_paged_rows(v, v_strides, 4)) return rc;
-  return status(parrot::launch_paged_append(
-      paged_cache(cache), cache->type, cache->head_dim, paged_batch(batch, rows),
-      static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_strides, v_strides,
-      as_stream(stream)));
+  return paged_append(cache, batch, k, k_row, k_head, v, v_row, v_head, rows, parrot::PagedRope{},
+                      stream);
+}
+
+int parrot_paged_append_rope_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
+                                  const void* k, int64_t k_row, int64_t k_head, const void* v,
+                                  int64_t v_row, int64_t v_head, int32_t rows, const float* cos,
+                                  const float* sin, int32_t positions, const void* q,
+                                  int64_t q_row, int64_t q_head, int32_t heads, void* q_out,
+                                  void* stream) {
+  if (int rc = check_paged(cache, batch)) return rc;
+  if (int rc = check_paged_heads(rows, heads, cache->kv_heads)) return rc;
+  if (positions <= 0) return PARROT_ERR_BAD_SHAPE;
+  if (rows == 0) return PARROT_OK;
+  if (!cos || !sin || !q_out) return PARROT_ERR_NULL_POINTER;
+  const int64_t q_strides[3] = {q_row, q_head, 0};
+  if (int rc = check_paged_rows(q, q_strides, 4)) return rc;
+  if ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin) |
+       reinterpret_cast<uintptr_t>(q_out)) & 7u)
+    return PARROT_ERR_ALIGNMENT;
+  const parrot::PagedRope rope{cos, sin, positions, heads, static_cast<const uint16_t*>(q),
+                               {q_row, q_head}, static_cast<uint16_t*>(q_out)};
+  return paged_append(cache, batch, k, k_row, k_head, v, v_row, v_head, rows, rope, stream);
 }
 
 int parrot_paged_read_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,

@@ -46,6 +46,17 @@ struct PagedBatch {
   int batch, width, rows;
 };
 
+// Rotation of keys, and of query rows (q may be null), by their positions' angles
+// (those past the tables by the last).  cos null: none.
+struct PagedRope {
+  const float* cos;  // [positions, D / 2]
+  const float* sin;
+  int positions, heads;
+  const uint16_t* q;
+  int64_t qs[2];  // element strides: row, head
+  uint16_t* out;  // [rows, heads, D]
+};
+
 struct PagedSequence {
   int first;   // its first new row
   int count;   // new rows
@@ -169,7 +180,8 @@ __device__ __forceinline__ int paged_page(const PagedBatch& b, const PagedCache&
 bool paged_head_dim_supported(int head_dim);  // 64, 96, 128
 hipError_t launch_paged_append(const PagedCache& cache, int type, int head_dim,
                                const PagedBatch& batch, const uint16_t* k, const uint16_t* v,
-                               const int64_t* k_strides, const int64_t* v_strides, hipStream_t s);
+                               const int64_t* k_strides, const int64_t* v_strides,
+                               const PagedRope& rope, hipStream_t s);
 hipError_t launch_paged_read(const PagedCache& cache, int type, int head_dim,
                              const PagedBatch& batch, int positions, uint16_t* k, uint16_t* v,
                              const int64_t* k_strides, const int64_t* v_strides, hipStream_t s);

@@ -101,9 +101,20 @@ struct Rows {
   const uint16_t* k;
   const uint16_t* v;
   int64_t ks[2], vs[2];  // element strides: row, head
+  PagedRope rope;        // (ROPE)
 };
 
-template <int TYPE, int D>
+// Four values of a row from dimension `dim` on, rotated by the angles of its position.
+__device__ __forceinline__ uint2 rotated(uint2 w, const PagedRope& r, int64_t angles, int dim) {
+  const float2 c = *reinterpret_cast<const float2*>(r.cos + angles + dim / 2);
+  const float2 s = *reinterpret_cast<const float2*>(r.sin + angles + dim / 2);
+  const float e0 = lo_bf16(w.x), o0 = hi_bf16(w.x), e1 = lo_bf16(w.y), o1 = hi_bf16(w.y);
+  return make_uint2(pack_bf16x2(rope_even(e0, o0, c.x, s.x), rope_odd(e0, o0, c.x, s.x)),
+                    pack_bf16x2(rope_even(e1, o1, c.y, s.y), rope_odd(e1, o1, c.y, s.y)));
+}
+
+// ROPE: keys, and the query heads that share the kv head, are rotated first.
+template <int TYPE, int D, bool ROPE>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c, PagedBatch b,
                                                                 Rows rows) {
   using E = typename Stored<TYPE>::type;
@@ -113,8 +124,8 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c, Pa
 
   // Blocks that new rows fall into.
   auto units_of = [&](const PagedSequence& s) {
-    const int from = max(s.length - s.count, 0);
-    return s.stored > from ? (s.stored - 1) / kPagedBlock - from / kPagedBlock + 1 : 0;
+    const int from = max(s.length - s.count, 0), to = ROPE ? s.length : s.stored;
+    return to > from ? (to - 1) / kPagedBlock - from / kPagedBlock + 1 : 0;
   };
   int sequence, index;
   PagedSequence s;
@@ -122,15 +133,33 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c, Pa
   const int from = max(s.length - s.count, 0);
   const int blk = from / kPagedBlock + index;
   const int per_page = c.page / kPagedBlock;
-  const int page = paged_page(b, c, sequence, blk / per_page);
-  if (page < 0) return;
+  const int page = blk / per_page < b.width ? paged_page(b, c, sequence, blk / per_page) : -1;
+  if (!ROPE && page < 0) return;
   const int head = blockIdx.y;
+  const int p = threadIdx.x >> 3, part = threadIdx.x & 7;
+  const int position = blk * kPagedBlock + p;
+  const int64_t row = s.first + (position - (s.length - s.count));
+  int64_t angles = 0;
+  if constexpr (ROPE) {
+    const PagedRope& r = rows.rope;
+    angles = static_cast<int64_t>(min(position, r.positions - 1)) * (D / 2);
+    if (position >= from && position < s.length && r.q != nullptr) {
+      const int rep = r.heads / c.kv_heads;
+      for (int h = head * rep; h < (head + 1) * rep; ++h) {
+        const uint16_t* const qr = r.q + row * r.qs[0] + h * r.qs[1] + 4 * part;
+        uint16_t* const to = r.out + (row * r.heads + h) * D + 4 * part;
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+          *reinterpret_cast<uint2*>(to + 32 * j) = rotated(
+              *reinterpret_cast<const uint2*>(qr + 32 * j), r, angles, 32 * j + 4 * part);
+      }
+    }
+    if (page < 0) return;
+  }
   const int64_t at = static_cast<int64_t>(page) * c.kv_heads + head;
   E* const kp = static_cast<E*>(c.key) + (at * per_page + blk % per_page) * (kPagedBlock * D);
   E* const vp = static_cast<E*>(c.value) + (at * per_page + blk % per_page) * (kPagedBlock * D);
 
-  const int p = threadIdx.x >> 3, part = threadIdx.x & 7;
-  const int position = blk * kPagedBlock + p;
   // Rows lo .. hi of the block are new.
   const int lo = max(from - blk * kPagedBlock, 0);
   const int hi = min(s.stored - blk * kPagedBlock, kPagedBlock);
@@ -139,13 +168,16 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c, Pa
 #pragma unroll
   for (int j = 0; j < S; ++j) kw[j] = vw[j] = make_uint2(0, 0);
   if (fresh) {
-    const int64_t row = s.first + (position - (s.length - s.count));
     const uint16_t* const kr = rows.k + row * rows.ks[0] + head * rows.ks[1] + 4 * part;
     const uint16_t* const vr = rows.v + row * rows.vs[0] + head * rows.vs[1] + 4 * part;
 #pragma unroll
     for (int j = 0; j < S; ++j) {
       kw[j] = *reinterpret_cast<const uint2*>(kr + 32 * j);
       vw[j] = *reinterpret_cast<const uint2*>(vr + 32 * j);
+    }
+    if constexpr (ROPE) {
+#pragma unroll
+      for (int j = 0; j < S; ++j) kw[j] = rotated(kw[j], rows.rope, angles, 32 * j + 4 * part);
     }
   }
   uint32_t kb = 0, vb = 0;
@@ -314,15 +346,20 @@ bool paged_head_dim_supported(int head_dim) {
 
 hipError_t launch_paged_append(const PagedCache& cache, int type, int head_dim,
                                const PagedBatch& batch, const uint16_t* k, const uint16_t* v,
-                               const int64_t* k_strides, const int64_t* v_strides, hipStream_t s) {
-  if (batch.rows == 0 || batch.batch == 0 || batch.width == 0) return hipSuccess;
-  const Rows rows{k, v, {k_strides[0], k_strides[1]}, {v_strides[0], v_strides[1]}};
+                               const int64_t* k_strides, const int64_t* v_strides,
+                               const PagedRope& rope, hipStream_t s) {
+  if (batch.rows == 0 || batch.batch == 0) return hipSuccess;
+  const Rows rows{k, v, {k_strides[0], k_strides[1]}, {v_strides[0], v_strides[1]}, rope};
   // n rows touch at most (n + 30) / 32 + 1 blocks
   const dim3 grid(batch.rows / kPagedBlock + 2 * std::min(batch.batch, batch.rows), cache.kv_heads);
   auto run = [&](auto t) {
     constexpr int TYPE = decltype(t)::value;
     return by_width(head_dim, [&](auto d) {
-      paged_append_kernel<TYPE, decltype(d)::value><<<grid, kThreads, 0, s>>>(cache, batch, rows);
+      constexpr int D = decltype(d)::value;
+      if (rope.cos != nullptr)
+        paged_append_kernel<TYPE, D, true><<<grid, kThreads, 0, s>>>(cache, batch, rows);
+      else
+        paged_append_kernel<TYPE, D, false><<<grid, kThreads, 0, s>>>(cache, batch, rows);
     });
   };
   if (type == kPagedBf16) return run(std::integral_constant<int, kPagedBf16>{});

@@ -2,7 +2,7 @@
 
 Public API mirrors the reference package (parrot/__init__.py, parrot/model.py):
 ``ModelConfig``, ``Parrot`` (``forward``, ``prefill``, ``decode_step``,
-``decode_next``, ``parameter_counts``), ``ModelOutput``, ``GenerationState``.
+``decode_next``, ``decode_sample``, ``parameter_counts``), ``ModelOutput``, ``GenerationState``.
 
 Backends
   * ``moe_backend="pytorch"`` / ``depth_backend="pytorch"``: plain PyTorch on
@@ -23,12 +23,15 @@ Parrot(cfg)`` draws the same weights.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Literal
+from typing import TYPE_CHECKING, Literal
 
 import torch
 from torch import Tensor, nn
 from torch.nn import functional as F
 from torch.utils.checkpoint import checkpoint
+
+if TYPE_CHECKING:
+    from .paged import PagedBatch, PagedKVCache
 
 _ROPE_TABLES: dict[tuple, tuple[Tensor, Tensor]] = {}
 _WINDOW_MASKS: dict[tuple, list[Tensor]] = {}
@@ -509,6 +512,33 @@ class LocalGQA(nn.Module):
         result = self.out(y.transpose(1, 2).reshape(b, 1, -1))
         return result if addend is None else addend + result
 
+    def extend(self, x: Tensor, cache: "PagedKVCache", batch: "PagedBatch",
+               addend: Tensor | None = None, sinks: int = 0) -> Tensor:
+        """out(attention(x)) [+ addend] for the new rows x [rows, dim] of a batch of
+        sequences of their own lengths, over a paged cache that the rows' keys and
+        values are appended to (one token or a chunk of a prompt per sequence; a
+        window's first ``sinks`` positions stay visible).  HIP backend only.  Rows
+        of no sequence hold anything."""
+        c = self.cfg
+        if not self._hip(x) or x.ndim != 2:
+            raise RuntimeError("a paged extension takes bf16 rows [rows, dim] on the HIP backend")
+        if (cache.kv_heads, cache.head_dim) != (c.n_kv_heads, c.head_dim):
+            raise RuntimeError("the cache's heads do not match the layer's")
+        from . import hip_moe
+        if x.shape[0] == 0:
+            return x if addend is None else addend
+        width, kv = c.n_heads * c.head_dim, c.n_kv_heads * c.head_dim
+        if hip_moe.proj_supported(c.dim, width + 2 * kv):
+            qkv = hip_moe.proj(x, self._qkv_fragments(), width + 2 * kv)
+        else:
+            qkv = F.linear(x, self._packed_qkv())
+        qkv = qkv.view(-1, c.n_heads + 2 * c.n_kv_heads, c.head_dim)
+        q, k, v = qkv.split((c.n_heads, c.n_kv_heads, c.n_kv_heads), dim=1)
+        cos, sin = _rope_tables(c, x.new_empty(0, dtype=torch.float32))
+        q = cache.append_rope(q, k, v, batch, cos, sin)
+        y = cache.attend(q, batch, scale=c.head_dim ** -0.5, window=c.window_size, sinks=sinks)
+        return self._project_out(y, addend)
+
 
 class GlobalMLA(nn.Module):
     """NoPE attention over a joint KV latent (reference parrot/model.py:331-432).
@@ -836,6 +866,43 @@ class MoE(nn.Module):
             return result.view_as(x), mixed.view_as(x)
         result = self.inference(x, direct=False, addend=addend)
         return result, depth.normalized(sources + [result], output_norm)
+
+
+def sample_torch(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor = 1.0,
+                 top_k: int | Tensor = 0, top_p: float | Tensor = 1.0,
+                 min_p: float | Tensor = 0.0) -> tuple[Tensor, Tensor]:
+    """hip_moe.sample in plain PyTorch, for the pytorch backend: (tokens, their
+    probabilities) [..., 1]."""
+    vocab = logits.shape[-1]
+    x = logits.reshape(-1, vocab).double()
+    rows = x.shape[0]
+
+    def column(v):
+        v = torch.as_tensor(v, device=x.device)
+        return v.double().reshape(-1, 1).expand(rows, 1)
+    t, k, p, m = (column(v) for v in (temperature, top_k, top_p, min_p))
+    x = torch.where(x.isnan(), -float("inf"), x)
+    x, order = torch.sort(x, dim=-1, descending=True, stable=True)
+    top = x[:, :1]
+    greedy = ~(t > 0)
+    w = torch.exp((x - top) / torch.where(greedy, 1.0, t))
+    w = torch.where(x == top, 1.0, torch.where(w.isnan(), 0.0, w))
+    rank = torch.arange(vocab, device=x.device)
+    k = torch.where(greedy, 1.0, torch.where(k > 0, k, float(vocab)))
+    w = torch.where(rank < k, w, 0.0)
+    before = torch.cumsum(w, -1) - w
+    w = torch.where((before < p * w.sum(-1, keepdim=True)) | (p >= 1) | (rank == 0), w, 0.0)
+    w = torch.where(w >= m.clamp_max(1.0), w, 0.0)
+    w = torch.zeros_like(w).scatter_(1, order, w)
+    reach = torch.cumsum(w, -1)
+    total = reach[:, -1:]
+    target = uniform.reshape(-1, 1).double() * total
+    token = torch.searchsorted(reach, target, right=True).clamp_max(vocab - 1)
+    none = top == -float("inf")
+    prob = torch.where(none, 0.0, w.gather(1, token) / total)
+    token = torch.where(none, -1, token)
+    shape = (*logits.shape[:-1], 1)
+    return token.view(shape), prob.float().view(shape)
 
 
 class Block(nn.Module):
@@ -1285,11 +1352,12 @@ class Parrot(nn.Module):
 
     @torch.inference_mode()
     def decode_step(self, input_ids: Tensor, state: GenerationState, *,
-                    _next_token_only: bool = False,
-                    _out: Tensor | None = None) -> tuple[Tensor, GenerationState]:
+                    _next_token_only: bool = False, _out: Tensor | None = None,
+                    _draw: tuple[Tensor, dict] | None = None) -> tuple[Tensor, GenerationState]:
         """Append one token per sequence to an existing generation state.
         ``_out``: the tensor that the logits, or (with ``_next_token_only``,
-        int64 [batch, 1]) the greedy tokens, are written into and returned as."""
+        int64 [batch, 1]) the greedy tokens, are written into and returned as.
+        ``_draw``: uniform numbers and parameters to draw the tokens by instead."""
         cfg = self.config
         if self.training:
             raise RuntimeError("decode_step requires model.eval()")
@@ -1346,7 +1414,8 @@ class Parrot(nn.Module):
         else:
             h = self.final_norm(x)
         advanced = False
-        if _next_token_only and state.position_device is not None and h.shape[0] <= 16:
+        if _next_token_only and _draw is None and state.position_device is not None and \
+                h.shape[0] <= 16:
             # Greedy token straight from fp32 logits, never materialised
             # (cf. vocab_argmax_partials/reduce_bf16, moe_bf16.metal:1541-1621);
             # the same launch advances the device position.
@@ -1354,6 +1423,13 @@ class Parrot(nn.Module):
             output = hip_moe.vocab_argmax(h, self.embedding.weight, advance=state.position_device,
                                           out=_out)
             advanced = True
+        elif _draw is not None:
+            logits = self._head(h)[:, -1]
+            if self.config.uses_hip and _hip_inference(h):
+                from . import hip_moe
+                output = hip_moe.sample(logits, _draw[0], out=_out, **_draw[1])[0]
+            else:
+                output = sample_torch(logits, _draw[0], **_draw[1])[0]
         else:
             logits = self._head(h, None if _next_token_only else _out)
             output = logits.argmax(-1) if _next_token_only else logits
@@ -1369,6 +1445,16 @@ class Parrot(nn.Module):
                     state: GenerationState) -> tuple[Tensor, GenerationState]:
         """Append one token and return the next greedy token without logits."""
         return self.decode_step(input_ids, state, _next_token_only=True)
+
+    @torch.inference_mode()
+    def decode_sample(self, input_ids: Tensor, state: GenerationState, uniform: Tensor, *,
+                      temperature: float | Tensor = 1.0, top_k: int | Tensor = 0,
+                      top_p: float | Tensor = 1.0,
+                      min_p: float | Tensor = 0.0) -> tuple[Tensor, GenerationState]:
+        """Append one token and draw the next [batch, 1] by the given numbers
+        ``uniform`` [batch] in [0, 1) (see hip_moe.sample for the parameters)."""
+        kw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        return self.decode_step(input_ids, state, _next_token_only=True, _draw=(uniform, kw))
 
     def parameter_counts(self) -> dict[str, int]:
         total = sum(p.numel() for p in self.parameters())

@@ -198,6 +198,36 @@ class PagedKVCache:
                 self._at, b, key.data_ptr(), kr, kh, value.data_ptr(), vr, vh, key.shape[0],
                 _stream(self.device)), "parrot_paged_append_bf16")
 
+    def append_rope(self, q: Tensor, key: Tensor, value: Tensor, batch: PagedBatch, cos: Tensor,
+                    sin: Tensor) -> Tensor:
+        """``append`` of keys that RoPE rotates first by their positions (interleaved
+        pairs; fp32 tables [positions, head_dim / 2], past them by the last row), in
+        the same launch.  Returns the query rows q [rows, heads, head_dim] rotated in
+        the same way, a new tensor.  Rows of no sequence hold anything in it."""
+        key = self._new_rows(key, self.kv_heads, "HIP paged append", 4)
+        value = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
+        heads = q.shape[1] if q.ndim == 3 else 0
+        if heads < 1 or heads % self.kv_heads:
+            raise RuntimeError("HIP paged append takes query rows [rows, heads, head_dim] of a "
+                               "multiple of the cache's kv heads")
+        q = self._new_rows(q, heads, "HIP paged append", 4)
+        if not key.shape[0] == value.shape[0] == q.shape[0]:
+            raise RuntimeError("as many rows of queries and values as of keys")
+        for x in (cos, sin):
+            if x.dtype != torch.float32 or x.device != self.device or not x.is_contiguous() or \
+                    x.ndim != 2 or x.shape != (cos.shape[0], self.head_dim // 2) or not len(x):
+                raise RuntimeError("RoPE tables must be contiguous fp32 [positions, head_dim / 2] "
+                                   "on the cache's device")
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        b = self._batch(batch)
+        (kr, kh, _), (vr, vh, _), (qr, qh, _) = key.stride(), value.stride(), q.stride()
+        with _on(self.device):
+            _abi.check(_abi.load().parrot_paged_append_rope_bf16(
+                self._at, b, key.data_ptr(), kr, kh, value.data_ptr(), vr, vh, key.shape[0],
+                cos.data_ptr(), sin.data_ptr(), cos.shape[0], q.data_ptr(), qr, qh, heads,
+                out.data_ptr(), _stream(self.device)), "parrot_paged_append_rope_bf16")
+        return out
+
     def read(self, batch: PagedBatch, positions: int,
              out: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
         """Keys and values of positions 0 .. positions - 1 of every sequence, bf16

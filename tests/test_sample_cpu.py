@@ -1,0 +1,82 @@
+"""Sampling on the pytorch backend against the definition written out in numpy, and
+generation that draws its tokens (no GPU)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import tiny_model_config
+
+
+def _draw(x, u, t=1.0, k=0, p=1.0, m=0.0):
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    if x.max() == -np.inf:
+        return -1, 0.0
+    if not t > 0:
+        return int(x.argmax()), 1.0
+    with np.errstate(invalid="ignore"):
+        w = np.where(x == x.max(), 1.0, np.exp((x - x.max()) / t))
+    kept = np.argsort(-x, kind="stable")
+    if 0 < k < len(x):
+        kept = kept[:k]
+    if p < 1:
+        mass = np.cumsum(w[kept])
+        before = np.concatenate(([0.0], mass[:-1]))
+        kept = kept[(before < p * mass[-1]) | (np.arange(len(kept)) == 0)]
+    kept = np.sort(kept[w[kept] >= min(m, 1.0)])
+    reach = np.cumsum(w[kept])
+    i = min(int(np.searchsorted(reach, u * reach[-1], side="right")), len(kept) - 1)
+    return int(kept[i]), w[kept[i]] / reach[-1]
+
+
+def test_sample_torch():
+    from parrot.model import sample_torch
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(40, 300, generator=g) * 3
+    x[3, ::2] = -math.inf
+    x[4] = -math.inf
+    x[5, ::3] = math.nan
+    x[6] = torch.randint(0, 3, (300,), generator=g).float()
+    x[7, [4, 9]] = math.inf
+    u = torch.rand(40, generator=g)
+    pick = lambda v: torch.tensor(v)[torch.randint(0, len(v), (40,), generator=g)]  # noqa: E731
+    for kw in (dict(), dict(temperature=0.5, top_k=7, top_p=0.8, min_p=0.05),
+               dict(temperature=pick([0.0, 0.7, 2.0]), top_k=pick([0, 1, 5, 500]).int(),
+                    top_p=pick([1.0, 0.9, 0.0]), min_p=pick([0.0, 0.1, 1.0]))):
+        token, prob = sample_torch(x, u, **kw)
+        for r in range(40):
+            value = lambda n, v: (  # noqa: E731
+                kw[n][r].item() if isinstance(kw.get(n), torch.Tensor) else kw.get(n, v))
+            args = dict(t=value("temperature", 1.0), k=value("top_k", 0), p=value("top_p", 1.0),
+                        m=value("min_p", 0.0))
+            want, share = _draw(x[r].numpy(), u[r].double().item(), **args)
+            assert token[r].item() == want, (r, args)
+            assert abs(prob[r].item() - share) <= 1e-6
+
+
+def test_decode_sample_on_the_pytorch_backend():
+    from parrot import Parrot
+    from parrot.model import sample_torch
+    torch.manual_seed(0)
+    model = Parrot(tiny_model_config()).eval()
+    ids = torch.randint(0, model.config.vocab_size, (2, 9))
+    u = torch.rand(5, 2)
+    _, state = model.prefill(ids)
+    _, other = model.prefill(ids)
+    token = ids[:, -1:]
+    for i in range(5):
+        logits, other = model.decode_step(token, other)
+        want = sample_torch(logits[:, -1], u[i], temperature=0.8, top_k=10, top_p=0.9)[0]
+        token, state = model.decode_sample(token, state, u[i], temperature=0.8, top_k=10,
+                                           top_p=0.9)
+        assert token.shape == (2, 1) and torch.equal(token, want)
+    greedy, _ = model.decode_sample(token, state, u[0], temperature=0.0)
+    best, _ = model.decode_next(token, other)
+    assert torch.equal(greedy, best)
+
+
+def test_hip_sample_refuses_cpu_tensors():
+    from parrot import hip_moe
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        hip_moe.sample(torch.zeros(2, 5), torch.zeros(2))
