@@ -1,0 +1,278 @@
+// Paged attention of many rows per sequence (prompts and their chunks): a wavefront has 32 rows, the
+// four of a workgroup share key blocks through LDS.
+//
+// Each wavefront brings one of a stage's four matrices (K and V of two blocks) from
+// the pages into registers while the stage before is computed, and writes it to LDS
+// as bf16: an 8-bit page is converted once for 128 rows.  K's second half lies 128
+// bytes further, so that the 16 lanes of a read's phase, which take eight keys of
+// each half, fall into different banks.
+#include "attention_lds.h"
+#include "paged_attention.h"
+
+namespace parrot {
+namespace paged {
+
+namespace {
+
+// A V piece with its positions' powers of two (int8: shift = -128 times the power).
+template <int TYPE>
+__device__ __forceinline__ bf16x8 value_piece(uint2 w, const float (&power)[8],
+                                              const float (&shift)[8]) {
+  float x[8];
+  if constexpr (TYPE == kPagedE4m3) {
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int u = static_cast<int>(i ? w.y : w.x);
+      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(u, false);
+      const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8(u, true);
+      x[4 * i] = lo[0] * power[4 * i], x[4 * i + 1] = lo[1] * power[4 * i + 1];
+      x[4 * i + 2] = hi[0] * power[4 * i + 2], x[4 * i + 3] = hi[1] * power[4 * i + 3];
+    }
+  } else {
+    int8_values(w, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(x[e], power[e], shift[e]);
+  }
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)  // (eight significant bits at most: the upper halves)
+    y[i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]),
+                                 0x07060302u);
+  return __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
+}
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArgs a) {
+  constexpr int KU = D / 16, DT = D / 32, S = D / 32;
+  constexpr int kHalf = 64;                                  // elements between K's halves
+  constexpr int kK = kPagedBlock * D + kHalf;                // elements of K, then of V
+  constexpr int kBlock = kK + kPagedBlock * D;
+  constexpr int kBytes = TYPE == kPagedBf16 ? 2 : 1;
+  constexpr int kLoads = kPagedBlock * D * kBytes / (16 * kWave);  // 1 KB pieces of a matrix
+  __shared__ __attribute__((aligned(16))) uint16_t stage[2][2][kBlock];  // [buffer][block]
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const int unit = blockIdx.x / a.cache.kv_heads, kvh = blockIdx.x - unit * a.cache.kv_heads;
+  const int split = blockIdx.z;
+
+  auto units_of = [&](const PagedSequence& s) {
+    return (s.count * a.rep + kTileRows - 1) / kTileRows;
+  };
+  int sequence, tile;
+  PagedSequence s;
+  if (!paged_find_last(a.batch, a.cache.page, unit, units_of, sequence, tile, s)) return;
+  const int rows = s.count * a.rep;
+  const int tile0 = tile * kTileRows, row0 = tile0 + wave * kRows;
+  const TileRow mine = tile_row(s, row0 + col, rows, a.rep, kvh);
+  const int before = s.length - s.count;
+  const Blocks blocks = tile_blocks(before + tile0 / a.rep,
+                                    before + (min(tile0 + kTileRows, rows) - 1) / a.rep, s.stored,
+                                    a.window, a.sinks);
+  const Share share = split_share(s, rows, kTileRows, a.rep, blocks, split, a.splits, a.whole,
+                                  a.window, a.sinks);
+  if (share.whole && split > 0) return;
+  const int begin = share.begin, end = share.end;
+  // This wavefront's own rows (none: it only brings blocks).
+  const bool has = row0 < rows;
+  const int first = before + row0 / a.rep;
+  const int last = before + (min(row0 + kRows, rows) - 1) / a.rep;
+
+  State<D> st;
+  clear(st);
+  if (begin < end) {
+    bf16x8 qf[KU];
+    {
+      const uint16_t* row = a.q + mine.token * a.qs[0] + mine.head * a.qs[1] + 8 * half;
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        uint4 v = *reinterpret_cast<const uint4*>(row + 16 * u);
+        v.x ^= a.q_sign;
+        v.y ^= a.q_sign;
+        v.z ^= a.q_sign;
+        v.w ^= a.q_sign;
+        qf[u] = __builtin_bit_cast(bf16x8, v);
+      }
+    }
+    const int per_page = a.cache.page / kPagedBlock;
+    const int which = wave >> 1;       // block of a stage, and matrix, that this wavefront brings
+    const bool brings_v = wave & 1;
+    // Lane j: the page of the share's j-th block (of the last 64), and which of its
+    // blocks that is.
+    int ids = -1, ins = 0;
+    int page0 = -1, page1 = -1;        // of the stage that is brought
+    uint4 got[kLoads];                 // 8-bit types
+    uint32_t bytes[2] = {0, 0};
+    auto bring = [&](int i, int buf) {  // blocks i and i + 1
+      const int j = (i - begin) % kWave;
+      if (j == 0) {
+        const int blk = blocks.at(i + lane), at = blk / per_page;
+        ids = i + lane < end ? paged_page(a.batch, a.cache, sequence, at) : -1;
+        ins = blk - at * per_page;
+      }
+      page0 = __builtin_amdgcn_readlane(ids, j);
+      page1 = __builtin_amdgcn_readlane(ids, j + 1);
+      const int page = which ? page1 : page0;
+      if (page < 0) return;
+      const int in = __builtin_amdgcn_readlane(ins, j + which);
+      const int64_t at = static_cast<int64_t>(page) * a.cache.kv_heads + kvh;
+      const char* from = static_cast<const char*>(brings_v ? a.cache.value : a.cache.key) +
+                         (at * per_page + in) * (kPagedBlock * D * kBytes);
+      if constexpr (TYPE == kPagedBf16) {
+        const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(from, kPagedBlock * D * kBytes);
+        uint16_t* to = &stage[buf][which][brings_v ? kK : 0];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+          buffer_to_lds16(rsrc, to + 512 * u + (!brings_v && u >= S ? kHalf : 0), lane * 16u,
+                          1024u * u);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+          got[u] = reinterpret_cast<const uint4*>(from)[kWave * u + lane];
+        const int64_t e = at * a.cache.page + in * kPagedBlock;
+        if (brings_v) {  // positions 4 g .. + 3 and 16 + 4 g .. + 3 of the lane's pieces
+          const uint8_t* x = a.cache.value_exponent + e + 4 * ((lane >> 3) & 3);
+          bytes[0] = *reinterpret_cast<const uint32_t*>(x);
+          bytes[1] = *reinterpret_cast<const uint32_t*>(x + 16);
+        } else {  // keys c, c + 1 of either half
+          const uint8_t* x = a.cache.key_exponent + e + ((2 * lane) & 15);
+          bytes[0] = *reinterpret_cast<const uint16_t*>(x);
+          bytes[1] = *reinterpret_cast<const uint16_t*>(x + 16);
+        }
+      }
+    };
+    auto put = [&](int buf) {  // 8-bit types: what was brought, as bf16
+      if constexpr (TYPE != kPagedBf16) {
+        if ((which ? page1 : page0) < 0) return;
+        uint16_t* const to = &stage[buf][which][brings_v ? kK : 0];
+        if (brings_v) {
+          float power[8], shift[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            power[e] = __uint_as_float(((bytes[e >> 2] >> (8 * (e & 3))) & 0xffu) << 23);
+            shift[e] = -128.0f * power[e];
+          }
+#pragma unroll
+          for (int u = 0; u < kLoads; ++u) {
+            bf16x8* const p = reinterpret_cast<bf16x8*>(to + (kWave * u + lane) * 16);
+            p[0] = value_piece<TYPE>(make_uint2(got[u].x, got[u].y), power, shift);
+            p[1] = value_piece<TYPE>(make_uint2(got[u].z, got[u].w), power, shift);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < kLoads; ++u) {
+            const int at = (kWave * u + lane) * 16;
+            const uint32_t b = at >= 16 * D ? bytes[1] : bytes[0];
+            bf16x8* const p = reinterpret_cast<bf16x8*>(to + at + (at >= 16 * D ? kHalf : 0));
+            p[0] = piece_bf16<TYPE>(make_uint2(got[u].x, got[u].y), __uint_as_float((b & 0xffu) << 23));
+            p[1] = piece_bf16<TYPE>(make_uint2(got[u].z, got[u].w), __uint_as_float((b >> 8) << 23));
+          }
+        }
+      }
+    };
+
+    const int kn = (col >> 3) & 1;
+    const int kc = 4 * (2 * (col >> 4) + ((col >> 2) & 1)) + (col & 3);
+    const uint32_t k_off = static_cast<uint32_t>(kn * (S * 1024 + 2 * kHalf) + half * 256 + kc * 16);
+    const uint32_t v_off =
+        static_cast<uint32_t>(2 * kK + (col >> 4) * 1024 + half * 256 + (col & 15) * 16);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) const uint16_t*)&stage[0][0][0]));
+    // True where values that are not finite were left out.
+    auto block = [&](uint32_t lds, int k0) -> bool {
+      bf16x8 kf[KU], vf[2 * DT], pf[2];
+      lds_frags<0, 512>(lds + k_off, kf);
+      f32x16 sc;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u], qf[u], sc, 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      read_values<0>(lds + v_off, vf);
+      // A block that every row of the tile sees whole needs no mask.
+      const bool whole = k0 + 31 <= min(first, s.stored - 1) &&
+                         (last - k0 < a.window || k0 + 31 < a.sinks);
+      // Values that some row must not see: times a probability of 0 an infinity or a
+      // NaN is not 0.
+      bool odd = false;
+      if (!whole) {
+        odd = mask_block<D>(sc, vf, k0, mine.position, s.stored, a);
+        if (odd) clear_nonfinite(vf);
+      }
+      raise(st, sc, a.scale_log2);
+      probabilities(st, sc, a.scale_log2, pf, [](float p, int) { return p; });
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+          st.o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[2 * t + h], pf[h], st.o[t], 0, 0, 0);
+      return odd;
+    };
+    bring(begin, 0);
+    for (int i = begin, buf = 0; i < end; i += 2, buf ^= 1) {
+      const int now0 = page0, now1 = page1;
+      if constexpr (TYPE == kPagedBf16) {
+        // This wavefront's copies have landed; past the barrier everybody's have, and
+        // nobody reads the other buffer any more.
+        wait_vm_barrier<0>();
+      } else {
+        put(buf);
+        __syncthreads();
+      }
+      if (i + 2 < end) bring(i + 2, buf ^ 1);
+      if (!has) continue;
+      // Blocks without a page, and those that none of this wavefront's rows sees, are
+      // left out.
+      auto seen = [&](int k0) {
+        return k0 <= last && (first - (k0 + 31) < a.window || k0 < a.sinks);
+      };
+      const uint32_t lds = lds0 + buf * (4 * kBlock);
+      const int k0 = blocks.at(i) * kPagedBlock, k1 = blocks.at(i + 1) * kPagedBlock;
+      uint32_t odd = 0;
+      if (now0 >= 0 && seen(k0)) odd = block(lds, k0);
+      if (now1 >= 0 && seen(k1)) odd |= 2 * block(lds + 2 * kBlock, k1);
+#pragma unroll 1
+      for (int b = 0; odd != 0; ++b, odd >>= 1)
+        if (odd & 1)
+          add_nonfinite<D>(st, &stage[buf][b][kK], b ? k1 : k0, mine.position, s.stored, a);
+    }
+  }
+  const float l = st.l + __shfl_xor(st.l, 32);
+  if (row0 + col >= rows) return;
+  const int64_t to = static_cast<int64_t>(mine.token) * a.heads + mine.head;
+  if (share.whole) {
+    if (a.splits > 1 && half == 0) a.part_ml[to * a.splits] = make_float2(0.0f, kWhole);
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<uint2*>(a.out + to * D + 32 * t + 8 * (e >> 2) + 4 * half) =
+            make_uint2(pack_bf16x2(st.o[t][e] * f, st.o[t][e + 1] * f),
+                       pack_bf16x2(st.o[t][e + 2] * f, st.o[t][e + 3] * f));
+  } else {
+    const int64_t at = to * a.splits + split;
+    if (half == 0) a.part_ml[at] = make_float2(st.m, l);
+    if (begin < end) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<float4*>(a.part + at * D + 32 * t + 8 * (e >> 2) + 4 * half) =
+              make_float4(st.o[t][e], st.o[t][e + 1], st.o[t][e + 2], st.o[t][e + 3]);
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_tiles(const AttendArgs& a, int type, int head_dim, dim3 grid, hipStream_t s) {
+  return by_type_and_width(type, head_dim, [&](auto t, auto d) {
+    paged_tile_kernel<decltype(t)::value, decltype(d)::value><<<grid, kWaves * kWave, 0, s>>>(a);
+  });
+}
+
+}  // namespace paged
+}  // namespace parrot
