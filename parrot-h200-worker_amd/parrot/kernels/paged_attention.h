@@ -99,9 +99,16 @@ __device__ __forceinline__ Share split_share(const PagedSequence& s, int rows, i
   return {begin, min(begin + share, blocks.count), blocks.count <= share};
 }
 
+// Which block of the cache (whose number fits 32 bits) a sequence's is, -1 where the table
+// names no page.
+__device__ __forceinline__ int cache_block(const AttendArgs& a, int sequence, int kvh, int block) {
+  const int per_page = a.cache.page / kPagedBlock, at = block / per_page;
+  const int page = paged_page(a.batch, a.cache, sequence, at);
+  return page < 0 ? -1 : (page * a.cache.kv_heads + kvh) * per_page + block - at * per_page;
+}
+
 // Where a wavefront's key blocks (every fourth of its workgroup's share) lie among the
-// cache's blocks, whose number fits 32 bits: lane j holds the j-th of the last 64, -1
-// where the table names no page.
+// cache's: lane j holds the j-th of the last 64.
 struct WaveBlocks {
   const AttendArgs& a;
   const int sequence, kvh;
@@ -115,13 +122,8 @@ struct WaveBlocks {
   __device__ __forceinline__ int find(int i) {
     const int j = (i - begin) / kWaves % kWave;
     if (j == 0) {
-      const int lane = threadIdx.x & (kWave - 1), per_page = a.cache.page / kPagedBlock;
-      held = -1;
-      if (i + kWaves * lane < end) {
-        const int blk = blocks.at(i + kWaves * lane), at = blk / per_page;
-        const int page = paged_page(a.batch, a.cache, sequence, at);
-        if (page >= 0) held = (page * a.cache.kv_heads + kvh) * per_page + blk - at * per_page;
-      }
+      const int mine = i + kWaves * static_cast<int>(threadIdx.x & (kWave - 1));
+      held = mine < end ? cache_block(a, sequence, kvh, blocks.at(mine)) : -1;
     }
     return __builtin_amdgcn_readlane(held, j);
   }
@@ -370,14 +372,17 @@ __device__ __forceinline__ void probabilities(State<D>& st, const f32x16& sc, fl
   st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// Raises the running maximum to this lane's largest score where one passes it by
-// more than 2^8.
-template <int D>
-__device__ __forceinline__ void raise(State<D>& st, const f32x16& sc, float scale_log2) {
+__device__ __forceinline__ float largest(const f32x16& sc) {
   float t[5];
 #pragma unroll
   for (int i = 0; i < 5; ++i) t[i] = fmaxf(fmaxf(sc[3 * i], sc[3 * i + 1]), sc[3 * i + 2]);
-  float mx = fmaxf(fmaxf(fmaxf(t[0], t[1]), t[2]), fmaxf(fmaxf(t[3], t[4]), sc[15]));
+  return fmaxf(fmaxf(fmaxf(t[0], t[1]), t[2]), fmaxf(fmaxf(t[3], t[4]), sc[15]));
+}
+
+// Raises the running maximum to this lane's largest score where one passes it by
+// more than 2^8.
+template <int D>
+__device__ __forceinline__ void raise(State<D>& st, float mx, float scale_log2) {
   mx *= scale_log2;
   if (__ballot(mx > st.m + 8.0f) != 0) {
     const float mn = fmaxf(st.m, fmaxf(mx, __shfl_xor(mx, 32)));

@@ -145,7 +145,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
           clear_nonfinite(vf);
         }
       }
-      raise(st, sc, a.scale_log2);
+      raise(st, largest(sc), a.scale_log2);
       bf16x8 pf[2];
       probabilities(st, sc, a.scale_log2, pf, [&](float p, int e) {
         return TYPE == kPagedBf16 ? p : p * __uint_as_float(byte_of(e) << 23);

@@ -95,42 +95,29 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
         qf[u] = __builtin_bit_cast(bf16x8, v);
       }
     }
-    const int per_page = a.cache.page / kPagedBlock;
     const int which = wave >> 1;       // block of a stage, and matrix, that this wavefront brings
     const bool brings_v = wave & 1;
-    // Lane j: the page of the share's j-th block (of the last 64), and which of its
-    // blocks that is.
-    int ids = -1, ins = 0;
-    int page0 = -1, page1 = -1;        // of the stage that is brought
+    const char* const matrix = static_cast<const char*>(brings_v ? a.cache.value : a.cache.key);
+    // Lane j: which block of the cache the share's j-th is (of the last 64), -1 for none.
+    int ids = -1;
+    int at0 = -1, at1 = -1;            // of the stage that is brought
+    __amdgpu_buffer_rsrc_t from;       // what this wavefront brings of it
     uint4 got[kLoads];                 // 8-bit types
     uint32_t bytes[2] = {0, 0};
-    auto bring = [&](int i, int buf) {  // blocks i and i + 1
+    auto aim = [&](int i) {  // at blocks i and i + 1 (past the share: at nothing)
       const int j = (i - begin) % kWave;
-      if (j == 0) {
-        const int blk = blocks.at(i + lane), at = blk / per_page;
-        ids = i + lane < end ? paged_page(a.batch, a.cache, sequence, at) : -1;
-        ins = blk - at * per_page;
+      if (j == 0 && i < end) {
+        ids = -1;
+        if (i + lane < end) ids = cache_block(a, sequence, kvh, blocks.at(i + lane));
       }
-      page0 = __builtin_amdgcn_readlane(ids, j);
-      page1 = __builtin_amdgcn_readlane(ids, j + 1);
-      const int page = which ? page1 : page0;
-      if (page < 0) return;
-      const int in = __builtin_amdgcn_readlane(ins, j + which);
-      const int64_t at = static_cast<int64_t>(page) * a.cache.kv_heads + kvh;
-      const char* from = static_cast<const char*>(brings_v ? a.cache.value : a.cache.key) +
-                         (at * per_page + in) * (kPagedBlock * D * kBytes);
-      if constexpr (TYPE == kPagedBf16) {
-        const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(from, kPagedBlock * D * kBytes);
-        uint16_t* to = &stage[buf][which][brings_v ? kK : 0];
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u)
-          buffer_to_lds16(rsrc, to + 512 * u + (!brings_v && u >= S ? kHalf : 0), lane * 16u,
-                          1024u * u);
-      } else {
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u)
-          got[u] = reinterpret_cast<const uint4*>(from)[kWave * u + lane];
-        const int64_t e = at * a.cache.page + in * kPagedBlock;
+      at0 = i < end ? __builtin_amdgcn_readlane(ids, j) : -1;
+      at1 = i < end ? __builtin_amdgcn_readlane(ids, j + 1) : -1;
+      const int at = which ? at1 : at0;
+      from = make_rsrc(matrix + int64_t{max(at, 0)} * (kPagedBlock * D * kBytes),
+                       at < 0 ? 0 : kPagedBlock * D * kBytes);
+      if constexpr (TYPE != kPagedBf16) {
+        if (at < 0) return;
+        const int64_t e = int64_t{at} * kPagedBlock;
         if (brings_v) {  // positions 4 g .. + 3 and 16 + 4 g .. + 3 of the lane's pieces
           const uint8_t* x = a.cache.value_exponent + e + 4 * ((lane >> 3) & 3);
           bytes[0] = *reinterpret_cast<const uint32_t*>(x);
@@ -142,9 +129,22 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
         }
       }
     };
+    // Pieces u0 .. u1 - 1 of what was aimed at (zeros for a block without a page).
+    auto bring = [&](int u0, int u1, int buf) {
+#pragma unroll
+      for (int u = u0; u < u1; ++u) {
+        if constexpr (TYPE == kPagedBf16)
+          buffer_to_lds16(from, &stage[buf][which][brings_v ? kK : 0] + 512 * u +
+                                    (!brings_v && u >= S ? kHalf : 0),
+                          lane * 16u, 1024u * u);
+        else
+          got[u] = __builtin_bit_cast(
+              uint4, __builtin_amdgcn_raw_buffer_load_b128(from, lane * 16u, 1024u * u, 0));
+      }
+    };
     auto put = [&](int buf) {  // 8-bit types: what was brought, as bf16
       if constexpr (TYPE != kPagedBf16) {
-        if ((which ? page1 : page0) < 0) return;
+        if ((which ? at1 : at0) < 0) return;
         uint16_t* const to = &stage[buf][which][brings_v ? kK : 0];
         if (brings_v) {
           float power[8], shift[8];
@@ -180,9 +180,11 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) const uint16_t*)&stage[0][0][0]));
     // True where values that are not finite were left out.
-    auto block = [&](uint32_t lds, int k0) -> bool {
+    // (between(n): where a quarter of the next stage is brought)
+    auto block = [&](uint32_t lds, int k0, int stored, auto between) -> bool {
       bf16x8 kf[KU], vf[2 * DT], pf[2];
       lds_frags<0, 512>(lds + k_off, kf);
+      between(0);
       f32x16 sc;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
@@ -190,19 +192,22 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
       for (int u = 0; u < KU; ++u)
         sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u], qf[u], sc, 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
+      between(1);
       read_values<0>(lds + v_off, vf);
+      between(2);
       // A block that every row of the tile sees whole needs no mask.
-      const bool whole = k0 + 31 <= min(first, s.stored - 1) &&
+      const bool whole = k0 + 31 <= min(first, stored - 1) &&
                          (last - k0 < a.window || k0 + 31 < a.sinks);
       // Values that some row must not see: times a probability of 0 an infinity or a
       // NaN is not 0.
       bool odd = false;
       if (!whole) {
-        odd = mask_block<D>(sc, vf, k0, mine.position, s.stored, a);
+        odd = mask_block<D>(sc, vf, k0, mine.position, stored, a);
         if (odd) clear_nonfinite(vf);
       }
-      raise(st, sc, a.scale_log2);
+      raise(st, largest(sc), a.scale_log2);
       probabilities(st, sc, a.scale_log2, pf, [](float p, int) { return p; });
+      between(3);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -210,9 +215,48 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
           st.o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[2 * t + h], pf[h], st.o[t], 0, 0, 0);
       return odd;
     };
-    bring(begin, 0);
-    for (int i = begin, buf = 0; i < end; i += 2, buf ^= 1) {
-      const int now0 = page0, now1 = page1;
+    // Both blocks of a stage that every row sees whole: one step of the softmax.
+    auto both = [&](uint32_t lds, auto between) {
+      bf16x8 kf[KU], vf[2 * DT], pf[2];
+      f32x16 sc[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        lds_frags<0, 512>(lds + 2 * kBlock * b + k_off, kf);
+        between(2 * b);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[b][e] = 0.0f;
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+          sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u], qf[u], sc[b], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      read_values<0>(lds + v_off, vf);
+      raise(st, fmaxf(largest(sc[0]), largest(sc[1])), a.scale_log2);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        probabilities(st, sc[b], a.scale_log2, pf, [](float p, int) { return p; });
+        between(2 * b + 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < DT; ++t)
+            st.o[t] =
+                __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[2 * t + h], pf[h], st.o[t], 0, 0, 0);
+        if (b == 0) {
+          __builtin_amdgcn_sched_barrier(0);
+          read_values<0>(lds + 2 * kBlock + v_off, vf);
+        }
+      }
+    };
+    // The share's blocks that every row of the tile sees whole: from..to - 1.
+    const int low = last >= a.window ? (last - a.window) / kPagedBlock + 1 : 0;
+    const int whole0 = blocks.sinks + max(low - blocks.lo, 0);
+    const int whole1 = min(end, blocks.sinks + (min(first + 1, s.stored)) / kPagedBlock - blocks.lo);
+    aim(begin);
+    bring(0, kLoads, 0);
+    int i = begin, buf = 0;
+    auto between = [&](int n) { bring(n * kLoads / 4, (n + 1) * kLoads / 4, buf ^ 1); };
+    auto next = [&] {  // stage i is there, and i + 2 aimed at
       if constexpr (TYPE == kPagedBf16) {
         // This wavefront's copies have landed; past the barrier everybody's have, and
         // nobody reads the other buffer any more.
@@ -221,22 +265,35 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
         put(buf);
         __syncthreads();
       }
-      if (i + 2 < end) bring(i + 2, buf ^ 1);
-      if (!has) continue;
-      // Blocks without a page, and those that none of this wavefront's rows sees, are
-      // left out.
-      auto seen = [&](int k0) {
-        return k0 <= last && (first - (k0 + 31) < a.window || k0 < a.sinks);
-      };
-      const uint32_t lds = lds0 + buf * (4 * kBlock);
-      const int k0 = blocks.at(i) * kPagedBlock, k1 = blocks.at(i + 1) * kPagedBlock;
-      uint32_t odd = 0;
-      if (now0 >= 0 && seen(k0)) odd = block(lds, k0);
-      if (now1 >= 0 && seen(k1)) odd |= 2 * block(lds + 2 * kBlock, k1);
+      aim(i + 2);
+    };
+    // Blocks without a page, and those that none of this wavefront's rows sees, are
+    // left out (but a stage's first, which brings the next).
+    auto seen = [&](int k0) {
+      return k0 <= last && (first - (k0 + 31) < a.window || k0 < a.sinks);
+    };
+    auto easy = [&] { return i >= whole0 && i + 2 <= whole1 && (at0 | at1) >= 0; };
+    while (i < end) {
 #pragma unroll 1
-      for (int b = 0; odd != 0; ++b, odd >>= 1)
-        if (odd & 1)
-          add_nonfinite<D>(st, &stage[buf][b][kK], b ? k1 : k0, mine.position, s.stored, a);
+      for (; i < end && !easy(); i += 2, buf ^= 1) {
+        const int now1 = at1, stored0 = at0 >= 0 ? s.stored : 0;
+        next();
+        const uint32_t lds = lds0 + buf * (4 * kBlock);
+        const int k0 = blocks.at(i) * kPagedBlock, k1 = blocks.at(i + 1) * kPagedBlock;
+        uint32_t odd = block(lds, k0, stored0, between);
+        if (has && now1 >= 0 && seen(k1))
+          odd |= 2 * block(lds + 2 * kBlock, k1, s.stored, [](int) {});
+#pragma unroll 1
+        for (int b = 0; odd != 0; ++b, odd >>= 1)
+          if (odd & 1)
+            add_nonfinite<D>(st, &stage[buf][b][kK], b ? k1 : k0, mine.position,
+                             b ? s.stored : stored0, a);
+      }
+#pragma unroll 1
+      for (; i < end && easy(); i += 2, buf ^= 1) {
+        next();
+        both(lds0 + buf * (4 * kBlock), between);
+      }
     }
   }
   const float l = st.l + __shfl_xor(st.l, 32);
