@@ -84,19 +84,20 @@ constexpr float kWhole = -1.0f;  // in place of a sum
 struct Share {
   int begin, end;
   bool whole;
+  int most;  // key blocks of the sequence's longest share
 };
 
 __device__ __forceinline__ Share split_share(const PagedSequence& s, int rows, int tile, int rep,
                                              const Blocks& blocks, int split, int splits,
                                              int whole, int window, int sinks) {
-  if (splits == 1) return {0, blocks.count, true};
   const int row0 = (rows - 1) / tile * tile;
   const Blocks most = tile_blocks(s.length - s.count + row0 / rep, s.length - 1, s.stored, window,
                                   sinks);
+  if (splits == 1) return {0, blocks.count, true, most.count};
   const int even = ((most.count + splits - 1) / splits + kWaves - 1) / kWaves * kWaves;
   const int share = most.count <= whole ? most.count : max(even, kMinShare);
   const int begin = min(split * share, blocks.count);
-  return {begin, min(begin + share, blocks.count), blocks.count <= share};
+  return {begin, min(begin + share, blocks.count), blocks.count <= share, min(share, most.count)};
 }
 
 // Which block of the cache (whose number fits 32 bits) a sequence's is, -1 where the table

@@ -255,6 +255,14 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
     aim(begin);
     bring(0, kLoads, 0);
     int i = begin, buf = 0;
+    // The hardware lets the oldest of equal wavefronts go first, and a CU's last workgroup
+    // would be alone at its end.  Those with little left step back for the others, and
+    // short ones go first, so that what follows them begins early.
+    const int mark1 = 3 * share.most / 8, mark0 = share.most / 6;
+    const bool little = end - begin <= 5 * share.most / 8;
+    int mark = little ? -1 : mark1;
+    if (little) __builtin_amdgcn_s_setprio(3);
+    else __builtin_amdgcn_s_setprio(2);
     auto between = [&](int n) { bring(n * kLoads / 4, (n + 1) * kLoads / 4, buf ^ 1); };
     auto next = [&] {  // stage i is there, and i + 2 aimed at
       if constexpr (TYPE == kPagedBf16) {
@@ -264,6 +272,11 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
       } else {
         put(buf);
         __syncthreads();
+      }
+      if (end - i <= mark) {
+        if (mark == mark0) __builtin_amdgcn_s_setprio(0);
+        else __builtin_amdgcn_s_setprio(1);
+        mark = mark == mark0 ? -1 : mark0;
       }
       aim(i + 2);
     };
