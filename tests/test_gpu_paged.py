@@ -319,6 +319,53 @@ def test_unseen_rows_do_not_reach_a_row(dtype, bad, last, n):
             assert not torch.isfinite(got[:, head][sees]).all(-1).any()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("n", [1, 6, 75])  # tiles of 16, 32 and 128 rows
+def test_pages_missing_inside(dtype, n):
+    """Pages that are not there between pages that are, at either block of a pair, one
+    and several at a time: their positions are not seen."""
+    run = Run(dtype, 2, 96, 32, [[900], [n]])
+    run.append([900])
+    run.append([n])
+    missing = [3, 6, 7, 12, 13, 14, 20, 25]
+    run.tables = [[-1 if i in missing else p for i, p in enumerate(run.tables[0])]]
+    gone = [(0, 32 * i, 32 * i + 32) for i in missing]
+    for window in (None, 300):
+        run.attend(8, [n], run.batch([n]), window=window, sinks=40, gone=gone)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+def test_shared_pages(dtype):
+    """Sequences that begin with the same pages."""
+    run = Run(dtype, 2, 64, 32, [[160, 0, 0], [1, 7, 100]])
+    run.append([160, 0, 0])
+    run.tables = [run.tables[0], *(run.tables[0][:5] + t for t in run.tables[1:])]
+    run.lengths = [160] * 3
+    for x in (run.plain.k, run.plain.v):
+        x[1:] = [x[0], x[0]]
+    for new in ([1, 7, 0], [0, 0, 100]):
+        batch = run.append(new)
+        run.attend(8, new, batch, window=120, sinks=33)
+    key, _ = run.cache.read(batch, 160)
+    assert torch.equal(key[0], key[1]) and torch.equal(key[0], key[2])
+
+
+@pytest.mark.parametrize("heads,kv_heads,others,new,length", [
+    (8, 2, 400, 1, 8400),    # tiles of 16 rows: 263 blocks, every fourth by one wavefront
+    (16, 2, 260, 6, 8400),   # of 32
+    (32, 32, 31, 128, 3000),  # of 128: 98 blocks
+])
+def test_shares_of_many_blocks(heads, kv_heads, others, new, length):
+    """One long sequence among so many that no tile's keys are split: more blocks than
+    are looked up at once."""
+    print(f"{length} keys, {new} new rows, {others} other sequences", flush=True)
+    steps = [[length] + [0] * others, [new] * (others + 1)]
+    run = Run(torch.int8, kv_heads, 64, 32, steps)
+    for now in steps:
+        batch = run.append(now)
+    run.attend(heads, steps[-1], batch)
+
+
 def test_far_pages():
     """Pages past 2^31 and 2^32 elements and bytes."""
     from parrot import PagedBatch, PagedKVCache
