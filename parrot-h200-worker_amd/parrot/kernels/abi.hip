@@ -93,7 +93,7 @@ parrot::PagedBatch paged_batch(const parrot_paged_batch* b, int32_t rows) {
 
 int paged_splits(const parrot_paged_cache* c, const parrot_paged_batch* b, int32_t rows,
                  int32_t heads, int32_t window, int32_t sinks) {
-  return parrot::paged_attention_splits(b->batch, rows, heads, c->kv_heads, c->page, b->width,
+  return parrot::paged_attention_splits(c->type, b->batch, rows, heads, c->kv_heads, c->page, b->width,
                                         window > 0 ? window : INT32_MAX, sinks);
 }
 

@@ -185,8 +185,8 @@ hipError_t launch_paged_append(const PagedCache& cache, int type, int head_dim,
 hipError_t launch_paged_read(const PagedCache& cache, int type, int head_dim,
                              const PagedBatch& batch, int positions, uint16_t* k, uint16_t* v,
                              const int64_t* k_strides, const int64_t* v_strides, hipStream_t s);
-int paged_attention_splits(int batch, int rows, int heads, int kv_heads, int page, int width,
-                           int window, int sinks);
+int paged_attention_splits(int type, int batch, int rows, int heads, int kv_heads, int page,
+                           int width, int window, int sinks);
 size_t paged_attention_workspace_bytes(int splits, int rows, int heads, int head_dim);
 hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_dim,
                                   const PagedBatch& batch, const uint16_t* q,

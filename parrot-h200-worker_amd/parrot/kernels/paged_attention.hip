@@ -102,17 +102,20 @@ __global__ __launch_bounds__(256) void paged_join_shares_kernel(AttendArgs a) {
       make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
 }
 
-// Rows of a workgroup's tile: 16 where a sequence has no more than 32 on average
-// (most of a larger tile would be empty), 128 from 96 on.
-int tile_rows(int batch, int rows, int rep) {
-  const int64_t all = static_cast<int64_t>(rows) * rep, n = std::min(batch, rows);
-  return all <= 32 * n ? kStepRows : all < 96 * n ? kRows : kTileRows;
-}
-
 struct Plan {
   int tile, splits, whole;
 };
 
+// Tiles: of 16 rows where a sequence has no more than 32 on average (most of a larger
+// tile would be empty).  Of 32 while there is little to do, four blocks of 32 keys for
+// each of the chip's 1024 wavefront schedulers, eight of 8-bit keys: each wavefront
+// takes its own, straight from the pages, and none waits for another.  Beyond, of 128,
+// which share what they read and convert.  32 / 128 rows, 8 heads on 2 of 96 (us):
+//   bf16: 1 sequence of 500 keys, 1024 rows per kv head (1500 blocks) 9.1 / 15.0, 4 of
+//   2000, 128 (2000) 12.6 / 14.9, 16 of 1000, 96 (3000) 17.6 / 17.8, 4 of 2000, 256 (4100)
+//   21.6 / 20.8, 1 of 4000, 1024 (8500) 28.2 / 27.1, 32 of 4000, 48 (16000) 48.8 / 34.2
+//   int8: 4 of 2000, 256 (4100) 21.5 / 23.8, 16 of 1000, 256 (8200) 27.1 / 25.2, 1 of 4000,
+//   1024 (8500) 32.4 / 29.9
 // Splits, where a tile may see more keys than are faster without the join's launch: 768
 // for 16 and 32 rows (one sequence, 8 heads on 2 of 96, one launch / split, us: 512 keys
 // 6.0 / 8.4, 768 7.1 / 8.1, 1024 8.2 / 8.3, 1536 10.4 / 8.4; 64 sequences of 8 kv heads of
@@ -123,16 +126,24 @@ struct Plan {
 // least (384: 24.5 and, of 32 rows with a window, 12.8 for 12.7); for larger tiles about
 // 1024, which evens out the causal ones (2 prompts of 4096 92.5 us, of 768 102), each with
 // 384 keys (3 chunks of 512 rows after 3500 keys 32.2 us, of 256 keys 35.5, of 512 33.2).
-Plan plan(int batch, int rows, int heads, int kv_heads, int page, int width, int window,
+Plan plan(int type, int batch, int rows, int heads, int kv_heads, int page, int width, int window,
           int sinks) {
   const int rep = heads / kv_heads;
-  const int tile = tile_rows(batch, rows, rep);
-  const int64_t tiles = (static_cast<int64_t>(rows) * rep + tile - 1) / tile;
-  const int64_t units = std::max<int64_t>({tiles, std::min(batch, rows), 1}) * kv_heads;
   // The most keys a tile can see: its table's, or the window, the sinks and
   // the tile's own span.
-  int64_t keys = static_cast<int64_t>(width) * page;
-  if (window < INT32_MAX) keys = std::min<int64_t>(keys, int64_t{window} + sinks + tile + 64);
+  auto keys_of = [&](int tile) {
+    const int64_t keys = static_cast<int64_t>(width) * page;
+    return window < INT32_MAX ? std::min<int64_t>(keys, int64_t{window} + sinks + tile + 64) : keys;
+  };
+  const int64_t all = static_cast<int64_t>(rows) * rep, n = std::max(std::min(batch, rows), 1);
+  const int64_t work = n * ((all + n * kRows - 1) / (n * kRows)) * kv_heads *
+                       ((keys_of(kRows) + kPagedBlock - 1) / kPagedBlock);
+  const int tile = all <= 2 * kStepRows * n                          ? kStepRows
+                   : work <= (type == kPagedBf16 ? 4096 : 8192) ? kRows
+                                                                     : kTileRows;
+  const int64_t keys = keys_of(tile);
+  const int64_t tiles = (static_cast<int64_t>(rows) * rep + tile - 1) / tile;
+  const int64_t units = std::max<int64_t>({tiles, std::min(batch, rows), 1}) * kv_heads;
   const int64_t line = tile == kTileRows ? std::min<int64_t>(384 + 4 * units, 1024) : 768;
   const bool step = tile == kStepRows;
   const int64_t want = step ? std::max<int64_t>(768 / units, 1) : (1024 + units - 1) / units;
@@ -144,9 +155,9 @@ Plan plan(int batch, int rows, int heads, int kv_heads, int page, int width, int
 
 }  // namespace
 
-int paged_attention_splits(int batch, int rows, int heads, int kv_heads, int page, int width,
-                           int window, int sinks) {
-  return plan(batch, rows, heads, kv_heads, page, width, window, sinks).splits;
+int paged_attention_splits(int type, int batch, int rows, int heads, int kv_heads, int page,
+                           int width, int window, int sinks) {
+  return plan(type, batch, rows, heads, kv_heads, page, width, window, sinks).splits;
 }
 
 size_t paged_attention_workspace_bytes(int splits, int rows, int heads, int head_dim) {
@@ -172,7 +183,7 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.out = out;
-  const Plan p = plan(batch.batch, batch.rows, heads, cache.kv_heads, cache.page, batch.width,
+  const Plan p = plan(type, batch.batch, batch.rows, heads, cache.kv_heads, cache.page, batch.width,
                       window, sinks);
   const int tile = p.tile, splits = p.splits;
   a.splits = splits;
@@ -192,7 +203,8 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   return by_type_and_width(type, head_dim, [&](auto, auto d) {
     constexpr int D = decltype(d)::value, kPer = 256 / (D / 4);
     const uint32_t rows = static_cast<uint32_t>(batch.rows * heads);
-    if (rows < 2048) paged_join_shares_kernel<D><<<rows, 256, 0, s>>>(a);
+    // (by rows / by shares: 2048 rows of 64 shares 46 / 9 us, 12288 rows of 6 8.4 / 13.2)
+    if (rows < 2048 || splits >= 16) paged_join_shares_kernel<D><<<rows, 256, 0, s>>>(a);
     else paged_join_rows_kernel<D><<<(rows + kPer - 1) / kPer, 256, 0, s>>>(a);
   });
 }

@@ -286,6 +286,13 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
       return k0 <= last && (first - (k0 + 31) < a.window || k0 < a.sinks);
     };
     auto easy = [&] { return i >= whole0 && i + 2 <= whole1 && (at0 | at1) >= 0; };
+    if (!has) {
+#pragma unroll 1
+      for (; i < end; i += 2, buf ^= 1) {
+        next();
+        bring(0, kLoads, buf ^ 1);
+      }
+    }
     while (i < end) {
 #pragma unroll 1
       for (; i < end && !easy(); i += 2, buf ^= 1) {
@@ -294,7 +301,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
         const uint32_t lds = lds0 + buf * (4 * kBlock);
         const int k0 = blocks.at(i) * kPagedBlock, k1 = blocks.at(i + 1) * kPagedBlock;
         uint32_t odd = block(lds, k0, stored0, between);
-        if (has && now1 >= 0 && seen(k1))
+        if (now1 >= 0 && seen(k1))
           odd |= 2 * block(lds + 2 * kBlock, k1, s.stored, [](int) {});
 #pragma unroll 1
         for (int b = 0; odd != 0; ++b, odd >>= 1)

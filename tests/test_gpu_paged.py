@@ -203,6 +203,21 @@ def test_attend(dtype, heads, kv_heads, d, steps, window, sinks):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("heads,kv_heads,d", [(32, 16, 96), (16, 16, 64), (32, 8, 128)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (50, 0), (70, 40), (1, 0)])
+def test_attend_many_rows(dtype, heads, kv_heads, d, window, sinks):
+    """Tiles of 128 rows: many sequences with ragged chunks after ragged contexts."""
+    g = torch.Generator().manual_seed(d)
+    first = torch.randint(0, 200, (24,), generator=g).tolist()
+    then = torch.randint(40, 260, (24,), generator=g).tolist()
+    then[3] = 0
+    run = Run(dtype, kv_heads, d, 64, [first, then])
+    run.append(first)
+    batch = run.append(then)
+    run.attend(heads, then, batch, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("steps,page,window,sinks", [
     ([[3000, 900], [1, 1]], 32, None, 0),       # long contexts, split over workgroups
     ([[3000, 900], [1, 6]], 256, 2048, 4),
@@ -284,11 +299,13 @@ def test_pages_given_back(dtype):
 @pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("last", [73, 100, 110, 118, 150])
-@pytest.mark.parametrize("n", [1, 6, 15, 73])  # tiles of 16, 32 and 128 rows
-def test_unseen_rows_do_not_reach_a_row(dtype, bad, last, n):
+# tiles of 16 rows, of 32, and (many sequences with many rows) of 128
+@pytest.mark.parametrize("n,copies", [(1, 1), (6, 1), (15, 1), (73, 1), (73, 128)])
+def test_unseen_rows_do_not_reach_a_row(dtype, bad, last, n, copies):
     """Infinities and NaN among keys and values that a row does not see: later
     positions of its own chunk, positions the window has left (in a block that it
-    still covers), and stale ones past the length."""
+    still covers), and stale ones past the length.  copies: sequences of the same
+    pages, to all of which the same must come out."""
     run = Run(dtype, 2, 96, 64, [[150]])
     k, v = _rows(run.g, 150, 2, 96), _rows(run.g, 150, 2, 96)
     k[77, 0, 5] = v[77, 0, 5] = bad
@@ -296,11 +313,14 @@ def test_unseen_rows_do_not_reach_a_row(dtype, bad, last, n):
     run.append([150], k, v)
     # a sequence of the first `last` positions, of which n are its new rows
     run.lengths = [last]
-    batch = run.batch([n])
+    run.tables, run.lengths = run.tables * copies, run.lengths * copies
+    batch = run.batch([n] * copies)
     q = _rows(run.g, n, 8, 96, std=1.5)
     for window, sinks in ((20, 0), (20, 3), (None, 0)):
-        got = run.cache.attend(q.cuda(), batch, scale=0.1, window=window, sinks=sinks)
-        got = got.double().cpu().view(n, 2, 4, 96)
+        got = run.cache.attend(q.cuda().repeat(copies, 1, 1), batch, scale=0.1, window=window,
+                               sinks=sinks).view(copies, n, 2, 4, 96)
+        assert torch.equal(got.view(torch.int16), got[:1].view(torch.int16).expand_as(got))
+        got = got[0].double().cpu()
         # the same without the bad rows
         kc, vc = k[:last].clone(), v[:last].clone()
         for head, row in ((0, 77), (1, 101)):
@@ -320,8 +340,8 @@ def test_unseen_rows_do_not_reach_a_row(dtype, bad, last, n):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
-@pytest.mark.parametrize("n", [1, 6, 75])  # tiles of 16, 32 and 128 rows
-def test_pages_missing_inside(dtype, n):
+@pytest.mark.parametrize("n,copies", [(1, 1), (6, 1), (75, 1), (75, 40)])  # tiles as above
+def test_pages_missing_inside(dtype, n, copies):
     """Pages that are not there between pages that are, at either block of a pair, one
     and several at a time: their positions are not seen."""
     run = Run(dtype, 2, 96, 32, [[900], [n]])
@@ -330,8 +350,20 @@ def test_pages_missing_inside(dtype, n):
     missing = [3, 6, 7, 12, 13, 14, 20, 25]
     run.tables = [[-1 if i in missing else p for i, p in enumerate(run.tables[0])]]
     gone = [(0, 32 * i, 32 * i + 32) for i in missing]
+    q = _rows(run.g, n, 8, 96)
     for window in (None, 300):
-        run.attend(8, [n], run.batch([n]), window=window, sinks=40, gone=gone)
+        want = run.attend(8, [n], run.batch([n]), window=window, sinks=40, q=q, gone=gone)
+        if copies == 1:
+            continue
+        run.tables, run.lengths = run.tables * copies, run.lengths * copies
+        got = run.cache.attend(q.cuda().repeat(copies, 1, 1), run.batch([n] * copies),
+                               scale=96 ** -0.5, window=window, sinks=40)
+        run.tables, run.lengths = run.tables[:1], run.lengths[:1]
+        got = got.double().cpu().view(copies, n, -1)
+        assert torch.equal(got, got[:1].expand_as(got))
+        ref, bound = run.plain.attend(q, [n], 96 ** -0.5, window, 40, gone)
+        assert ((got[0] - ref).abs() <= bound).all()
+        assert ((got[0] - want.double().cpu()).abs() <= 2 * bound).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
