@@ -10,6 +10,12 @@
 //                   rows: lane 16 g + c holds keys 4 g .. + 3 and 16 + 4 g .. + 3 of
 //                   row c, which is the order in which
 //   O^T += V^T P^T  takes P^T as its B operand (32 keys).
+//
+// Measured, 8 heads on 2 of 96 in e4m3: 8 sequences of 32000 keys 19.6 us for 99 MB
+// (5.1 TB/s, what a large copy reaches) and 4.6 for the join of 43 shares; 32 sequences
+// in a window of 2048 8.8 us for 23 MB and 4.2; one sequence of 129 keys 4.8 us.  Not
+// kept: registers of two blocks at a time (33 us for the first), four workgroups a CU
+// (the registers spill).
 #include "paged_attention.h"
 
 namespace parrot {

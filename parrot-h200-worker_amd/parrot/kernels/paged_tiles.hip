@@ -1,11 +1,23 @@
-// Paged attention of many rows per sequence (prompts and their chunks): a wavefront has 32 rows, the
-// four of a workgroup share key blocks through LDS.
+// Paged attention of many rows per sequence (prompts and their chunks): a wavefront has
+// 32 rows, the four of a workgroup share key blocks through LDS.
 //
 // Each wavefront brings one of a stage's four matrices (K and V of two blocks) from
-// the pages into registers while the stage before is computed, and writes it to LDS
-// as bf16: an 8-bit page is converted once for 128 rows.  K's second half lies 128
-// bytes further, so that the 16 lanes of a read's phase, which take eight keys of
-// each half, fall into different banks.
+// the pages while the stage before is computed: bf16 straight into LDS, 8-bit pages
+// into registers, from which they are written as bf16, converted once for 128 rows.
+// K's second half lies 128 bytes further, so that the 16 lanes of a read's phase, which
+// take eight keys of each half, fall into different banks.
+//
+// What bounds it: the vector instructions of the softmax (32 exponentials a lane and
+// pair of blocks, at a quarter of the rate) beside the matrix instructions, and how well
+// the three wavefronts of a SIMD overlap them.  So a pair that every row sees whole
+// takes one step of the softmax and no mask (4 prompts of 4096, 8 heads on 2 of 96 in
+// bf16, window 2048: 114 us without, 102 with), and wavefronts step back for those with
+// more left (99).  Measured there 93 us in a trace, 0.83 PFLOP/s of the visible pairs'
+// products; 2 prompts of 4096, 8 heads of 64 in int8, 78 us and 7.6 for the join; 3 chunks
+// of 512 after up to 3500 keys 21.8 and 8.4.  Not kept: two blocks' scores ahead of the
+// softmax (no change at three workgroups a CU, 130 us where registers leave two),
+// workgroups that take a second, short tile (the registers leave two a CU), odd shares in
+// reverse order (no change).
 #include "attention_lds.h"
 #include "paged_attention.h"
 

@@ -92,8 +92,8 @@ class PagedKVCache:
     rows.  8-bit rows are scaled by a power of two of their own, one byte per
     position and head in ``key_exponent`` / ``value_exponent`` [pages, kv_heads,
     page_size], so that a stored value is exact in bf16.  What that costs, for
-    normally distributed rows of 96: 2.6 % of the row's norm in e4m3 (whatever
-    the row holds: its error goes with the value), 0.8 % in int8.  A row with a
+    normally distributed rows of 96: 2.7 % of the row's norm in e4m3 (whatever
+    the row holds: its error goes with the value), 0.9 % in int8.  A row with a
     NaN or an infinity reads back as NaN."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int,
