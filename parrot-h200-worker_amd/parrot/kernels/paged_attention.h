@@ -272,9 +272,11 @@ __device__ __forceinline__ void merge_tile(const AttendArgs& a, const float (&o_
                                            const float (&ml_s)[kWaves][2][R],
                                            const PagedSequence& s, int row0, int rows, int kvh,
                                            int split, const Share& share) {
-  for (int i = threadIdx.x; i < R * (D / 4); i += kWaves * kWave) {
-    const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
-    if (row0 + r >= rows) break;
+  constexpr int kThreads = kWaves * kWave, kPieces = R * (D / 4);
+#pragma unroll
+  for (int k = 0; k < (kPieces + kThreads - 1) / kThreads; ++k) {
+    const int i = threadIdx.x + k * kThreads;
+    const int r = min(i / (D / 4), R - 1), d = 4 * (i % (D / 4));
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml_s[w][0][r]);
@@ -285,15 +287,16 @@ __device__ __forceinline__ void merge_tile(const AttendArgs& a, const float (&o_
       const float mw = ml_s[w][0][r], lw = ml_s[w][1][r];
       // A wavefront that saw nothing adds nothing (its maximum is -inf, its sum
       // 0; a NaN sum has to come through).
-      if (mw == -INFINITY && lw == 0.0f) continue;
+      const bool nothing = (mw == -INFINITY) & (lw == 0.0f);
       const float f = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-      sum += lw * f;
       const float4 x = *reinterpret_cast<const float4*>(&o_s[w][r][d]);
-      y.x += x.x * f;
-      y.y += x.y * f;
-      y.z += x.z * f;
-      y.w += x.w * f;
+      sum += nothing ? 0.0f : lw * f;
+      y.x += nothing ? 0.0f : x.x * f;
+      y.y += nothing ? 0.0f : x.y * f;
+      y.z += nothing ? 0.0f : x.z * f;
+      y.w += nothing ? 0.0f : x.w * f;
     }
+    if (i >= kPieces || row0 + r >= rows) continue;
     const TileRow row = tile_row(s, row0 + r, rows, a.rep, kvh);
     const int64_t to = static_cast<int64_t>(row.token) * a.heads + row.head;
     if (share.whole) {

@@ -25,8 +25,9 @@
 // gathered in the order of indices, one logit a thread.  Without top_k each
 // exponential is made once and its weight stays in registers.
 //
-// Measured (graph of launches): a row of 32768 fp32 logits with top_p 13.4 us, 64 rows with
-// parameters of their own 28.9 us; the bytes would take 0.1 and 1.7.
+// Measured (graph of launches): a row of 32768 fp32 logits with top_k 50 and top_p 11.0 us,
+// the largest alone 8.6, top_p alone 27.7; 64 rows with parameters of their own as their
+// slowest, 29; the bytes would take 0.1 and 1.7.
 #include <math.h>
 
 #include "common.h"
@@ -697,10 +698,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       int n = 0;
       for (int s = 0; s < row.steps; ++s) {
         const float4 v = row.get(s);
-        const float x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) n += __popcll(__ballot(x[j] >= from));
+        n += (v.x >= from) + (v.y >= from) + (v.z >= from) + (v.w >= from);
       }
+      n = static_cast<int>(wave_total(n));
       if (lane == 0) sh.low[wave] = n;
       __syncthreads();
       int at = 0;  // where this wavefront's begin
@@ -716,6 +716,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
           const int i = row.first(s);
           const float4 v = row.get(s);
           const float x[4] = {v.x, v.y, v.z, v.w};
+          // (of most steps none)
+          if (__ballot(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= from) == 0) continue;
           uint64_t who[4];
           int to = at;
 #pragma unroll
@@ -751,16 +753,34 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       if (t < few) sh.list[t] = {list.w, order_key(list.x), t};
       __syncthreads();
       order_list(few, sh);
-      uint64_t before = 0;
-      if (t < few) {
-        before = sh.ahead[t];
-        if (by_count && sh.rank[t] >= top_k) list.w = 0;
+      // The rest by one wavefront, two logits a lane, without a barrier.
+      if (t >= kWave) return;
+      static_assert(kPairs == 2 * kWave, "two a lane");
+      uint64_t w[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int e = t + kWave * h;
+        w[h] = e < few && !(by_count && sh.rank[e] >= top_k) ? sh.list[e].f : 0;
       }
-      if (top_p < 1.0 && before >= needed(total(list, held_weight, sh))) list.w = 0;
-      if (list.w < least_mass) list.w = 0;
-      const uint64_t all = total(list, held_weight, sh);
-      const int at = list.locate(held_weight, drawn(all), sh);
-      return answer(sh.few_index[at], share(sh.few[at], all));
+      if (top_p < 1.0) {
+        const uint64_t need = needed(wave_total(w[0] + w[1]));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[h] = sh.ahead[t + kWave * h] >= need ? 0 : w[h];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) w[h] = w[h] < least_mass ? 0 : w[h];
+      const uint64_t first = wave_upto(w[0]), second = last_lane(first) + wave_upto(w[1]);
+      const uint64_t all = last_lane(second), target = drawn(all);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint64_t upto = h ? second : first;
+        if (upto - w[h] <= target && target < upto) {
+          const int e = t + kWave * h;
+          a.token[r] = sh.few_index[e];
+          if (a.probability) a.probability[r] = static_cast<float>(share(sh.few[e], all));
+        }
+      }
+      return;
     }
     auto cut = [&](Edge edge) {
       if (!edge.keeps(t, list.x)) list.w = 0;
