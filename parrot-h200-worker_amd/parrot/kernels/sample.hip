@@ -26,8 +26,8 @@
 // exponential is made once and its weight stays in registers.
 //
 // Measured (graph of launches): a row of 32768 fp32 logits with top_k 50 and top_p 11.0 us,
-// the largest alone 8.6, top_p alone 27.7; 64 rows with parameters of their own as their
-// slowest, 29; the bytes would take 0.1 and 1.7.
+// the largest alone 8.6, top_p alone 24.8 (9.0 of 2000 logits); 64 rows with parameters of
+// their own as their slowest, 26; the bytes would take 0.1 and 1.7.
 #include <math.h>
 
 #include "common.h"
@@ -39,7 +39,7 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kStep = 4 * kWave;   // logits of a wavefront's step, four a lane
-constexpr int kHeld = 32768;       // logits of a row that LDS holds
+constexpr int kMost = 8;           // steps of a row that LDS holds (32768 logits)
 constexpr int kBins = 2048;
 constexpr int kList = 256;         // logits compared each with each
 constexpr int kTableBits = 8, kTable = 1 << kTableBits;
@@ -90,7 +90,8 @@ __device__ __forceinline__ float logit(const void* row, int i) {
   return x;
 }
 
-// Four logits from i on; a NaN, and what lies past the row, is -infinity.
+// Four logits from i on; a NaN is -infinity, what lies past the row a NaN (which is
+// larger or smaller than nothing, so no pass over a held row counts it).
 // aligned: the row is, and a whole number of fours: loads without a branch.
 template <int TYPE>
 __device__ __forceinline__ float4 logits4(const void* row, int at, int n, bool aligned) {
@@ -117,13 +118,16 @@ __device__ __forceinline__ float4 logits4(const void* row, int at, int n, bool a
     for (int j = 0; j < 4; ++j) x[j] = i + j < n ? logit<TYPE>(row, i + j) : -INFINITY;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = x[j] == x[j] && at < n ? x[j] : -INFINITY;
+  for (int j = 0; j < 4; ++j) {
+    const float past = at + j < n ? -INFINITY : __uint_as_float(0x7fc00000u);
+    x[j] = x[j] == x[j] && at + j < n ? x[j] : past;
+  }
   return make_float4(x[0], x[1], x[2], x[3]);
 }
 
 // A row whose largest logit is an infinity: only the infinities are drawn from, alike.
 __device__ __forceinline__ float4 finite_of(float4 v) {
-  auto f = [](float x) { return x == INFINITY ? 0.0f : -INFINITY; };
+  auto f = [](float x) { return x == INFINITY ? 0.0f : x == x ? -INFINITY : x; };
   return make_float4(f(v.x), f(v.y), f(v.z), f(v.w));
 }
 
@@ -183,7 +187,8 @@ __device__ __forceinline__ uint64_t wave_total(uint64_t v) { return last_lane(wa
 
 // A row: `steps` times 256 consecutive logits per wavefront, so that sums over
 // wavefronts, steps, lanes and a lane's four are sums by index.
-template <int TYPE, bool HELD>
+// STEPS > 0: the row is held in LDS.
+template <int TYPE, int STEPS>
 struct Row {
   const void* at;
   const float* held;
@@ -196,7 +201,7 @@ struct Row {
   }
   __device__ __forceinline__ float4 get(int step) const {
     const int i = first(step);
-    if constexpr (HELD) return *reinterpret_cast<const float4*>(held + i);
+    if constexpr (STEPS > 0) return *reinterpret_cast<const float4*>(held + i);
     float4 v = logits4<TYPE>(at, i, n, aligned);
     return infinite ? finite_of(v) : v;
   }
@@ -261,17 +266,18 @@ struct Row {
   }
 };
 
-// A held row and its weights, in registers (past its end: -infinity, of weight 0).
-template <typename R>
+// A held row and its weights, in registers (past its end 0).  Of a row of kMost steps the
+// steps past its end are left out, which also leaves the compiler fewer registers to spill
+// than passing all would (26.6 us for 31.4 at 32768); in keep it is the other way round.
+template <typename R, int kSteps>
 struct Weights {
-  static constexpr int kSteps = kHeld / (kWaves * kStep);
   const R row;
   uint64_t w[kSteps][4];
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      if (s >= row.steps) break;
+      if (kSteps == kMost && s >= row.steps) break;
       const int i = row.first(s);
       const float4 v = row.get(s);
       const float x[4] = {v.x, v.y, v.z, v.w};
@@ -301,7 +307,6 @@ struct Weights {
   __device__ __forceinline__ void keep(F f) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      if (s >= row.steps) break;
       const int i = row.first(s);
       const float4 v = row.get(s);
       const float x[4] = {v.x, v.y, v.z, v.w};
@@ -562,17 +567,18 @@ __device__ __forceinline__ Edge select(const R& row, F f, uint64_t need, Bins bi
   return {key_value(static_cast<uint64_t>(low) << 32), row.locate(equal, need - before - 1, sh)};
 }
 
-template <int TYPE, bool HELD>
+template <int TYPE, int STEPS>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
-  __shared__ __attribute__((aligned(16))) float held[HELD ? kHeld : 4];
+  constexpr bool HELD = STEPS > 0;
+  __shared__ __attribute__((aligned(16))) float held[HELD ? STEPS * kWaves * kStep : 4];
   __shared__ Shared sh;
   const int r = blockIdx.x, t = threadIdx.x;
-  Row<TYPE, HELD> row;
+  Row<TYPE, STEPS> row;
   constexpr int kBytes = TYPE == kLogitF32 ? 4 : 2;
   row.at = static_cast<const char*>(a.logits) + r * a.stride * kBytes;
   row.held = held;
   row.n = a.vocab;
-  row.steps = (a.vocab + kWaves * kStep - 1) / (kWaves * kStep);
+  row.steps = HELD && STEPS < kMost ? STEPS : (a.vocab + kWaves * kStep - 1) / (kWaves * kStep);
   row.aligned = (reinterpret_cast<uintptr_t>(row.at) & (4 * kBytes - 1)) == 0 && row.n % 4 == 0;
   row.infinite = false;
   // (logits are finite numbers: at 1e30 all that are not -infinity are alike)
@@ -586,7 +592,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   // This thread's and the row's largest logit.
   float mine = -INFINITY;
   {
-    constexpr int kAhead = kHeld / (kWaves * kStep);  // loads in flight: a held row's
+    constexpr int kAhead = HELD ? STEPS : kMost;  // loads in flight
     for (int from = 0; from < row.steps; from += kAhead) {
       float4 v[kAhead];
       if (row.aligned) {
@@ -802,11 +808,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   };
   if constexpr (HELD) {
     // Every weight once, in registers.
-    using W = Weights<Row<TYPE, HELD>>;
-    W all_of{row, {}};
+    Weights<Row<TYPE, STEPS>, STEPS> all_of{row, {}};
     if (top_p < 1.0) clear_bins(sh);
 #pragma unroll
-    for (int s = 0; s < W::kSteps; ++s) {
+    for (int s = 0; s < STEPS; ++s) {
       if (s < row.steps) {
         const int i = row.first(s);
         const float4 v = row.get(s);
@@ -846,10 +851,15 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   }
 }
 
+// (a step's 4096 logits are passed whole, so the fewest that hold the row)
 template <int TYPE>
 void launch(const SampleArgs& a, int rows, hipStream_t s) {
-  if (a.vocab <= kHeld) sample_kernel<TYPE, true><<<rows, kThreads, 0, s>>>(a);
-  else sample_kernel<TYPE, false><<<rows, kThreads, 0, s>>>(a);
+  constexpr int kOne = kWaves * kStep;
+  if (a.vocab <= kOne) sample_kernel<TYPE, 1><<<rows, kThreads, 0, s>>>(a);
+  else if (a.vocab <= 2 * kOne) sample_kernel<TYPE, 2><<<rows, kThreads, 0, s>>>(a);
+  else if (a.vocab <= 4 * kOne) sample_kernel<TYPE, 4><<<rows, kThreads, 0, s>>>(a);
+  else if (a.vocab <= kMost * kOne) sample_kernel<TYPE, kMost><<<rows, kThreads, 0, s>>>(a);
+  else sample_kernel<TYPE, 0><<<rows, kThreads, 0, s>>>(a);
 }
 
 }  // namespace

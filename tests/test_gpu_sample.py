@@ -56,7 +56,8 @@ def _check(x, u, **kw):
     return token
 
 
-@pytest.mark.parametrize("vocab", [1, 2, 63, 1000, 1025, 32768, 50001, 200000])
+@pytest.mark.parametrize("vocab", [1, 2, 63, 1000, 1025, 4096, 4099, 9000, 16381, 20000, 30001, 32768,
+                                   50001, 200000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_sample(vocab, dtype):
     g = torch.Generator().manual_seed(vocab)
@@ -86,6 +87,19 @@ def test_ties():
     _check(same, torch.rand(8, generator=g))
 
 
+@pytest.mark.parametrize("vocab", [2000, 12002, 25001])
+def test_ties_of_other_lengths(vocab):
+    """As above, and fewer logits above -infinity than are asked for."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randint(-3, 4, (12, vocab), generator=g).float()
+    x[3, 40:] = -math.inf
+    x[4, :-40] = -math.inf
+    u = torch.rand(12, generator=g)
+    for kw in ({}, {"top_k": 700}, {"top_p": 0.3}, {"top_k": 900, "top_p": 0.5, "min_p": 0.3},
+               {"top_p": 0.9999, "temperature": 0.02}, {"top_p": 0.999, "temperature": 100.0}):
+        _check(x, u, **kw)
+
+
 def test_borders_of_uniform():
     """u of 0 is the first kept token, the largest u below 1 the last."""
     g = torch.Generator().manual_seed(1)
@@ -95,9 +109,10 @@ def test_borders_of_uniform():
             _check(x, torch.full((4,), u), **kw)
 
 
-def test_infinite_and_missing_logits():
+@pytest.mark.parametrize("vocab", [777, 3001, 6000, 12001, 20002, 29000, 40001])
+def test_infinite_and_missing_logits(vocab):
     g = torch.Generator().manual_seed(2)
-    x = torch.randn(9, 777, generator=g)
+    x = torch.randn(9, vocab, generator=g)
     x[0, ::2] = -math.inf
     x[1, ::3] = math.nan
     x[2, 5:] = -math.inf
