@@ -45,7 +45,8 @@ _HERE = contextlib.nullcontext()
 
 def _on(device: torch.device):
     """Makes ``device`` the current one for a launch on its stream."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    # (torch.cuda.current_device() without its check that there is a GPU)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _require(x: Tensor, what: str, dtypes=(torch.bfloat16,)) -> None:
@@ -638,7 +639,8 @@ def _sample_parameter(x, what: str, rows: int, device: torch.device, dtype: torc
     """(pointer, number) of one sampling parameter: a tensor of one value per
     row, or a number from 0 to ``most`` for every row."""
     if isinstance(x, Tensor):
-        if x.dtype != dtype or x.device != device or x.numel() != rows or not x.is_contiguous():
+        if x.dtype is not dtype or x.device != device or x.numel() != rows or \
+                not x.is_contiguous():
             raise RuntimeError(f"{what} must be a number or a contiguous {dtype} tensor of one "
                                "value per row on the logits' device")
         return x.data_ptr(), 0
@@ -667,15 +669,17 @@ def sample(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor = 1.0
 
     The arithmetic behind the borders is in 64 bits (see sample.hip), so a row's
     token does not depend on the other rows of the call."""
-    _require(logits, "HIP sampling", tuple(_LOGIT_TYPES))
+    _require(logits, "HIP sampling", _LOGIT_TYPES)
     if logits.ndim < 1 or not 1 <= logits.shape[-1] <= SAMPLE_MAX_VOCAB:
         raise RuntimeError(f"HIP sampling takes 1 to {SAMPLE_MAX_VOCAB} logits per row")
-    vocab = logits.shape[-1]
-    rows = logits.numel() // vocab
+    *lead, vocab = logits.shape
     device = logits.device
-    flat = logits if logits.ndim == 2 else logits.reshape(-1, vocab)
-    if flat.stride(-1) != 1 or (rows > 1 and flat.stride(0) < vocab):
+    flat = logits if len(lead) == 1 else logits.reshape(-1, vocab)
+    rows = flat.shape[0]
+    row_stride, stride = flat.stride()
+    if stride != 1 or (rows > 1 and row_stride < vocab):
         flat = flat.contiguous()
+        row_stride = vocab
     if (uniform.dtype != torch.float32 or uniform.device != device or uniform.numel() != rows or
             not uniform.is_contiguous()):
         raise RuntimeError("uniform must be a contiguous fp32 tensor of one number per row on the "
@@ -684,20 +688,22 @@ def sample(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor = 1.0
     k, k_all = _sample_parameter(top_k, "top_k", rows, device, torch.int32, 2 ** 31 - 1)
     p, p_all = _sample_parameter(top_p, "top_p", rows, device, torch.float32, 1)
     m, m_all = _sample_parameter(min_p, "min_p", rows, device, torch.float32, 1)
-    shape = (*logits.shape[:-1], 1)
+    lead.append(1)
     if out is None:
-        out = torch.empty(shape, dtype=torch.int64, device=device)
+        out = token = torch.empty(lead, dtype=torch.int64, device=device)
     elif (out.dtype != torch.int64 or out.device != device or not out.is_contiguous() or
           out.numel() != rows):
         raise RuntimeError("out must be a contiguous int64 tensor of one id per row on the "
                            "logits' device")
-    probability = torch.empty(shape, dtype=torch.float32, device=device)
+    else:
+        token = out.view(lead)
+    probability = uniform.new_empty(lead)
     with _on(device):
         _abi.check(_abi.load().parrot_sample(
-            flat.data_ptr(), _LOGIT_TYPES[logits.dtype], rows, vocab, flat.stride(0),
+            flat.data_ptr(), _LOGIT_TYPES[logits.dtype], rows, vocab, row_stride,
             uniform.data_ptr(), t, t_all, k, k_all, p, p_all, m, m_all, out.data_ptr(),
             probability.data_ptr(), _stream(device)), "parrot_sample")
-    return out.view(shape), probability
+    return token, probability
 
 
 # ---------------------------------------------------------------------------

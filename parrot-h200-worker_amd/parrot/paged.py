@@ -176,7 +176,8 @@ class PagedKVCache:
 
     def _new_rows(self, x: Tensor, heads: int, what: str, step: int) -> Tensor:
         _require(x, what)
-        if x.ndim != 3 or x.shape[1:] != (heads, self.head_dim) or x.device != self.device:
+        if x.ndim != 3 or x.shape[1] != heads or x.shape[2] != self.head_dim or \
+                x.device != self.device:
             raise RuntimeError(f"{what} takes rows [rows, {heads}, {self.head_dim}] on the "
                                "cache's device")
         sr, sh, sd = x.stride()
@@ -279,7 +280,7 @@ class PagedKVCache:
         rows, device = q.shape[0], self.device
         b = self._batch(batch)
         if out is None:
-            out = torch.empty((rows, heads * self.head_dim), dtype=torch.bfloat16, device=device)
+            out = q.new_empty((rows, heads * self.head_dim))
         elif out.dtype != torch.bfloat16 or out.device != device or not out.is_contiguous() or \
                 out.shape != (rows, heads * self.head_dim) or out.data_ptr() % 8:
             raise RuntimeError(f"out must be a contiguous bf16 tensor [{rows}, "
