@@ -191,11 +191,36 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
         static_cast<uint32_t>(2 * kK + (col >> 4) * 1024 + half * 256 + (col & 15) * 16);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) const uint16_t*)&stage[0][0][0]));
+    // A block's operands.  Before every read of its own the compiler waits for all copies
+    // into LDS, the next stage's too, so with bf16 pages the reads and their waits are
+    // written out; of 8-bit types it may read early and wait late (84.4 -> 82 us for 2
+    // prompts of 4096).
+    auto read_k = [&](uint32_t lds, bf16x8(&kf)[KU]) {
+      if constexpr (TYPE == kPagedBf16) {
+        lds_frags<0, 512>(lds + k_off, kf);
+      } else {
+        const uint16_t* const from = &stage[0][0][0] + (lds - lds0 + k_off) / 2;
+#pragma unroll
+        for (int u = 0; u < KU; ++u) kf[u] = *reinterpret_cast<const bf16x8*>(from + 256 * u);
+      }
+    };
+    auto read_v = [&](uint32_t lds, bf16x8(&vf)[2 * DT]) {
+      if constexpr (TYPE == kPagedBf16) {
+        read_values<0>(lds + v_off, vf);
+      } else {
+        const uint16_t* const from = &stage[0][0][0] + (lds - lds0 + v_off) / 2;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            vf[2 * t + h] = *reinterpret_cast<const bf16x8*>(from + 1024 * t + 256 * h);
+      }
+    };
     // True where values that are not finite were left out.
     // (between(n): where a quarter of the next stage is brought)
     auto block = [&](uint32_t lds, int k0, int stored, auto between) -> bool {
       bf16x8 kf[KU], vf[2 * DT], pf[2];
-      lds_frags<0, 512>(lds + k_off, kf);
+      read_k(lds, kf);
       between(0);
       f32x16 sc;
 #pragma unroll
@@ -203,9 +228,9 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
 #pragma unroll
       for (int u = 0; u < KU; ++u)
         sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u], qf[u], sc, 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (TYPE == kPagedBf16) __builtin_amdgcn_sched_barrier(0);
       between(1);
-      read_values<0>(lds + v_off, vf);
+      read_v(lds, vf);
       between(2);
       // A block that every row of the tile sees whole needs no mask.
       const bool whole = k0 + 31 <= min(first, stored - 1) &&
@@ -233,16 +258,16 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
       f32x16 sc[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        lds_frags<0, 512>(lds + 2 * kBlock * b + k_off, kf);
+        read_k(lds + 2 * kBlock * b, kf);
         between(2 * b);
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[b][e] = 0.0f;
 #pragma unroll
         for (int u = 0; u < KU; ++u)
           sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u], qf[u], sc[b], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (TYPE == kPagedBf16) __builtin_amdgcn_sched_barrier(0);
       }
-      read_values<0>(lds + v_off, vf);
+      read_v(lds, vf);
       raise(st, fmaxf(largest(sc[0]), largest(sc[1])), a.scale_log2);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -255,8 +280,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
             st.o[t] =
                 __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[2 * t + h], pf[h], st.o[t], 0, 0, 0);
         if (b == 0) {
-          __builtin_amdgcn_sched_barrier(0);
-          read_values<0>(lds + 2 * kBlock + v_off, vf);
+          if constexpr (TYPE == kPagedBf16) __builtin_amdgcn_sched_barrier(0);
+          read_v(lds + 2 * kBlock, vf);
         }
       }
     };
