@@ -13,7 +13,7 @@
 // takes one step of the softmax and no mask (4 prompts of 4096, 8 heads on 2 of 96 in
 // bf16, window 2048: 114 us without, 102 with), and wavefronts step back for those with
 // more left (99).  Measured there 93 us in a trace, 0.83 PFLOP/s of the visible pairs'
-// products; 2 prompts of 4096, 8 heads of 64 in int8, 78 us and 7.6 for the join; 3 chunks
+// products; 2 prompts of 4096, 8 heads of 64 in int8, 75 us and 7.6 for the join; 3 chunks
 // of 512 after up to 3500 keys 21.8 and 8.4.  Not kept: two blocks' scores ahead of the
 // softmax (no change at three workgroups a CU, 130 us where registers leave two),
 // workgroups that take a second, short tile (the registers leave two a CU), odd shares in
@@ -352,6 +352,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
         both(lds0 + buf * (4 * kBlock), between);
       }
     }
+    // (the copies of the last step, of nothing, write zeros: not past the workgroup's end)
+    if constexpr (TYPE == kPagedBf16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   const float l = st.l + __shfl_xor(st.l, 32);
   if (row0 + col >= rows) return;
