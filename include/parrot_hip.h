@@ -821,7 +821,7 @@ int parrot_grouped_experts_static_bf16(const void* x, int64_t tokens, int32_t di
  * two, 2^-100 at least, that brings the row's largest magnitude inside the type's
  * range (448, 127); q is rounded to nearest even.  x = 255: the row held a NaN
  * or an infinity, and reads back as NaN.  page a multiple of 32; head_dim 64, 96
- * or 128. */
+ * or 128; pages * kv_heads * page / 32 below 2^31. */
 typedef struct parrot_paged_cache {
   void* key;
   void* value;

@@ -55,8 +55,7 @@ int check_paged(const parrot_paged_cache* c, const parrot_paged_batch* b) {
   // positions are 32-bit numbers, and so are the cache's blocks of 32 of them (which
   // are 4 KiB or more: 2^31 of them fit no memory)
   if (static_cast<int64_t>(b->width) * c->page > INT32_MAX - 64) return PARROT_ERR_BAD_SHAPE;
-  if (static_cast<int64_t>(c->pages) * c->kv_heads > INT32_MAX / (c->page / 32))
-    return PARROT_ERR_BAD_SHAPE;
+  if (c->pages > INT32_MAX / (c->page / 32) / c->kv_heads) return PARROT_ERR_BAD_SHAPE;
   const bool bytes = c->type != PARROT_PAGED_BF16;
   if (c->pages > 0 && (!c->key || !c->value || (bytes && (!c->key_exponent || !c->value_exponent))))
     return PARROT_ERR_NULL_POINTER;

@@ -23,7 +23,8 @@ def _batch(**kw):
 
 BAD = [(dict(key=None), {}, -1), (dict(value_exponent=None), {}, -1), ({}, dict(table=None), -1),
        ({}, dict(lengths=None), -1), ({}, dict(starts=None), -1), (dict(page=0), {}, -2),
-       (dict(pages=-1), {}, -2), (dict(kv_heads=0), {}, -2), ({}, dict(batch=-1), -2),
+       (dict(pages=-1), {}, -2), (dict(pages=1 << 30), {}, -2), (dict(pages=1 << 62), {}, -2),
+       (dict(kv_heads=0), {}, -2), ({}, dict(batch=-1), -2),
        ({}, dict(width=-1), -2), ({}, dict(width=1 << 26), -2), (dict(page=48), {}, -3),
        (dict(head_dim=80), {}, -3), (dict(type=3), {}, -3), (dict(type=-1), {}, -3),
        ({}, dict(batch=70000), -3), (dict(key=FAKE + 8), {}, -5), (dict(key_exponent=FAKE + 2), {}, -5)]
