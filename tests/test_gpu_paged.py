@@ -398,6 +398,33 @@ def test_shares_of_many_blocks(heads, kv_heads, others, new, length):
     run.attend(heads, steps[-1], batch)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("n,copies", [(1, 1), (6, 1), (75, 1), (75, 40)])
+def test_tables_of_no_pages_and_endless_windows(dtype, n, copies):
+    """Tables without a column hold nothing; a window and sinks as large as they get
+    hide nothing."""
+    from parrot import PagedBatch
+    run = Run(dtype, 2, 64, 32, [[90], [n]])
+    run.append([90])
+    batch = run.append([n])
+    q = _rows(run.g, n, 8, 64)
+    want = run.attend(8, [n], batch, scale=0.1, q=q)
+    many = q.cuda().repeat(copies, 1, 1)
+    batch = PagedBatch.from_lists(run.tables * copies, run.lengths * copies, [n] * copies)
+    for kw in ({"window": 2 ** 31 - 1}, {"window": 2 ** 40, "sinks": 2 ** 40},
+               {"window": 1, "sinks": 2 ** 31 - 1}):
+        got = run.cache.attend(many, batch, scale=0.1, **kw).view(copies, n, -1)
+        ref, bound = run.plain.attend(q, [n], 0.1)
+        assert ((got.double().cpu() - ref).abs() <= bound).all() and want.shape == got.shape[1:]
+    none = PagedBatch.from_lists([[]] * copies, [90 + n] * copies, [n] * copies)
+    before = [x.clone() for x in run.cache.read(run.batch([n]), 90 + n)]
+    run.cache.append(many[:, :2], many[:, 2:4], none)
+    assert not run.cache.attend(many, none, scale=0.1).any()
+    assert not any(x.any() for x in run.cache.read(none, 50))
+    for x, y in zip(before, run.cache.read(run.batch([n]), 90 + n)):
+        assert torch.equal(x, y)
+
+
 def test_far_pages():
     """Pages past 2^31 and 2^32 elements and bytes."""
     from parrot import PagedBatch, PagedKVCache
