@@ -18,39 +18,61 @@ __device__ __forceinline__ float share_weight(float2 ml, float m) {
 }
 
 // Rows of no sequence, and those that one share wrote whole, stay as they are.
-__device__ __forceinline__ bool joined_already(const AttendArgs& a, int64_t to) {
-  const int64_t token = to / a.heads;
-  return token >= a.batch.rows || token < a.batch.starts[0] ||
-         token >= a.batch.starts[a.batch.batch] || a.part_ml[to * a.splits].y == kWhole;
+__device__ __forceinline__ bool joined_already(const AttendArgs& a, int to) {
+  const int token = to / a.heads;
+  return (token < a.batch.starts[0]) | (token >= a.batch.starts[a.batch.batch]) |
+         (a.part_ml[static_cast<int64_t>(to) * a.splits].y == kWhole);
 }
 
-// Joins the shares of split tiles where there are many rows: D / 4 threads a row, one
-// share after the other.
+// Joins the shares of split tiles where there are many rows: D / 4 threads a row, eight
+// shares in flight (of a share that saw nothing the memory may hold anything).
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_rows_kernel(AttendArgs a) {
-  constexpr int kPer = 256 / (D / 4);
+  constexpr int kPer = 256 / (D / 4), kAhead = 8;
   const int slot = threadIdx.x / (D / 4), at = threadIdx.x - slot * (D / 4);
-  const int64_t to = static_cast<int64_t>(blockIdx.x) * kPer + slot;
-  if (slot >= kPer || joined_already(a, to)) return;
-  const float2* const ml = a.part_ml + to * a.splits;
-  const float4* const part = reinterpret_cast<const float4*>(a.part) + to * a.splits * (D / 4) + at;
+  const int to = static_cast<int>(blockIdx.x) * kPer + slot;  // rows * heads fit 30 bits
+  if (slot >= kPer || to >= a.batch.rows * a.heads) return;
+  const float2* const ml = a.part_ml + static_cast<int64_t>(to) * a.splits;
+  const float4* const part =
+      reinterpret_cast<const float4*>(a.part) + static_cast<int64_t>(to) * a.splits * (D / 4) + at;
+  // (of few shares many rows are whole: 2 prompts of 4096 in int8 81.9 us, asked late 82.8;
+  // of six, 3 chunks of 512 rows 30.4 us asked first, late 27.8)
+  const bool late = a.splits >= 4;
+  if (!late && joined_already(a, to)) return;
   float m = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < a.splits; ++i) m = fmaxf(m, ml[i].x);
   float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-  for (int i = 0; i < a.splits; ++i) {
-    const float f = share_weight(ml[i], m);
-    if (f < 0.0f) continue;
-    sum += ml[i].y * f;
-    const float4 x = part[i * (D / 4)];
-    y.x += x.x * f;
-    y.y += x.y * f;
-    y.z += x.z * f;
-    y.w += x.w * f;
+  for (int c = 0; c < a.splits; c += kAhead) {
+    float2 w[kAhead];
+    float4 x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      w[i] = make_float2(-INFINITY, 0.0f);
+      if (c + i >= a.splits) continue;  // (the same for all)
+      w[i] = ml[c + i];
+      x[i] = part[(c + i) * (D / 4)];
+    }
+    if (late && c == 0 && joined_already(a, to)) return;
+    float most = m;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) most = fmaxf(most, w[i].x);
+    // (what came before, in the units of the larger maximum)
+    const float back = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - most);
+    m = most;
+    sum *= back;
+    y = make_float4(y.x * back, y.y * back, y.z * back, y.w * back);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float f = share_weight(w[i], m);
+      const bool counts = !(f < 0.0f);
+      sum += counts ? w[i].y * f : 0.0f;
+      y.x += counts ? x[i].x * f : 0.0f;
+      y.y += counts ? x[i].y * f : 0.0f;
+      y.z += counts ? x[i].z * f : 0.0f;
+      y.w += counts ? x[i].w * f : 0.0f;
+    }
   }
   const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-  *reinterpret_cast<uint2*>(a.out + to * D + 4 * at) =
+  *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(to) * D + 4 * at) =
       make_uint2(pack_bf16x2(y.x * f, y.y * f), pack_bf16x2(y.z * f, y.w * f));
 }
 
@@ -61,11 +83,20 @@ __global__ __launch_bounds__(256) void paged_join_shares_kernel(AttendArgs a) {
   constexpr int kGroups = 256 / (D / 4);
   __shared__ float w_s[kMaxSplits];
   __shared__ float4 y_s[kGroups][D / 4];
-  const int64_t to = blockIdx.x;
+  const int to = blockIdx.x;
+  const int group = threadIdx.x / (D / 4), at = threadIdx.x - group * (D / 4);
+  const float4* const part =
+      reinterpret_cast<const float4*>(a.part) + static_cast<int64_t>(to) * a.splits * (D / 4) + at;
+  constexpr int kMine = (kMaxSplits + kGroups - 1) / kGroups;
+  float4 x[kMine];
+#pragma unroll
+  for (int k = 0; k < kMine; ++k)
+    if (group + k * kGroups < a.splits) x[k] = part[(group + k * kGroups) * (D / 4)];
   if (joined_already(a, to)) return;
   if (threadIdx.x < kWave) {
     const int i = threadIdx.x;
-    const float2 ml = i < a.splits ? a.part_ml[to * a.splits + i] : make_float2(-INFINITY, 0.0f);
+    const float2 ml = i < a.splits ? a.part_ml[static_cast<int64_t>(to) * a.splits + i]
+                                   : make_float2(-INFINITY, 0.0f);
     float m = ml.x;
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
@@ -74,17 +105,17 @@ __global__ __launch_bounds__(256) void paged_join_shares_kernel(AttendArgs a) {
     w_s[i] = f < 0.0f ? -1.0f : sum == 0.0f ? 0.0f : f / sum;
   }
   __syncthreads();
-  const int group = threadIdx.x / (D / 4), at = threadIdx.x - group * (D / 4);
   float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (group < kGroups) {
-    for (int i = group; i < a.splits; i += kGroups) {
-      const float f = w_s[i];
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      if (group + k * kGroups >= a.splits) continue;
+      const float f = w_s[group + k * kGroups];
       if (f < 0.0f) continue;
-      const float4 x = *reinterpret_cast<const float4*>(a.part + (to * a.splits + i) * D + 4 * at);
-      y.x += x.x * f;
-      y.y += x.y * f;
-      y.z += x.z * f;
-      y.w += x.w * f;
+      y.x += x[k].x * f;
+      y.y += x[k].y * f;
+      y.z += x[k].z * f;
+      y.w += x[k].w * f;
     }
     y_s[group][at] = y;
   }
@@ -98,7 +129,7 @@ __global__ __launch_bounds__(256) void paged_join_shares_kernel(AttendArgs a) {
     y.z += x.z;
     y.w += x.w;
   }
-  *reinterpret_cast<uint2*>(a.out + to * D + 4 * at) =
+  *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(to) * D + 4 * at) =
       make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
 }
 
@@ -203,7 +234,8 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   return by_type_and_width(type, head_dim, [&](auto, auto d) {
     constexpr int D = decltype(d)::value, kPer = 256 / (D / 4);
     const uint32_t rows = static_cast<uint32_t>(batch.rows * heads);
-    // (by rows / by shares: 2048 rows of 64 shares 46 / 9 us, 12288 rows of 6 8.4 / 13.2)
+    // (by rows / by shares, with one load in flight: 2048 rows of 64 shares 46 / 9 us, 12288
+    // rows of 6 8.4 / 13.2)
     if (rows < 2048 || splits >= 16) paged_join_shares_kernel<D><<<rows, 256, 0, s>>>(a);
     else paged_join_rows_kernel<D><<<(rows + kPer - 1) / kPer, 256, 0, s>>>(a);
   });
