@@ -12,8 +12,8 @@
 //   O^T += V^T P^T  takes P^T as its B operand (32 keys).
 //
 // Measured, 8 heads on 2 of 96 in e4m3: 8 sequences of 32000 keys 19.6 us for 99 MB
-// (5.1 TB/s, what a large copy reaches) and 4.6 for the join of 43 shares; 32 sequences
-// in a window of 2048 8.8 us for 23 MB and 4.2; one sequence of 129 keys 4.8 us.  Not
+// (5.1 TB/s, what a large copy reaches) and 3.9 for the join of 42 shares; 32 sequences
+// in a window of 2048 8.3 us for 23 MB and 3.9; one sequence of 129 keys in bf16 4.6 us.  Not
 // kept: registers of two blocks at a time (33 us for the first), four workgroups a CU
 // (the registers spill).
 #include "paged_attention.h"

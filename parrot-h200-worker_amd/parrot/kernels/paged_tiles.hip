@@ -13,8 +13,8 @@
 // takes one step of the softmax and no mask (4 prompts of 4096, 8 heads on 2 of 96 in
 // bf16, window 2048: 114 us without, 102 with), and wavefronts step back for those with
 // more left (99).  Measured there 93 us in a trace, 0.83 PFLOP/s of the visible pairs'
-// products; 2 prompts of 4096, 8 heads of 64 in int8, 75 us and 7.6 for the join; 3 chunks
-// of 512 after up to 3500 keys 21.8 and 8.4.  Not kept: two blocks' scores ahead of the
+// products; 2 prompts of 4096, 8 heads of 64 in int8, 75 us and 6.8 for the join; 3 chunks
+// of 512 after up to 3500 keys 21.9 and 5.5.  Not kept: two blocks' scores ahead of the
 // softmax (no change at three workgroups a CU, 130 us where registers leave two),
 // workgroups that take a second, short tile (the registers leave two a CU), odd shares in
 // reverse order (no change).
