@@ -234,9 +234,9 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   return by_type_and_width(type, head_dim, [&](auto, auto d) {
     constexpr int D = decltype(d)::value, kPer = 256 / (D / 4);
     const uint32_t rows = static_cast<uint32_t>(batch.rows * heads);
-    // (by rows / by shares, with one load in flight: 2048 rows of 64 shares 46 / 9 us, 12288
-    // rows of 6 8.4 / 13.2)
-    if (rows < 2048 || splits >= 16) paged_join_shares_kernel<D><<<rows, 256, 0, s>>>(a);
+    // (by rows / by shares, in all: 1024 rows after 30000 keys in 64 shares 52.7 / 49.9 us,
+    // 4096 in 16 109.4 / 112.1; the join of 12288 rows in 6 8.4 / 13.2)
+    if (rows < 2048 || splits >= 32) paged_join_shares_kernel<D><<<rows, 256, 0, s>>>(a);
     else paged_join_rows_kernel<D><<<(rows + kPer - 1) / kPer, 256, 0, s>>>(a);
   });
 }
