@@ -19,12 +19,10 @@
 #pragma once
 
 #include "common.h"
+#include "paged_share.h"
 
 namespace parrot {
 
-enum PagedType { kPagedBf16 = 0, kPagedE4m3 = 1, kPagedInt8 = 2 };
-
-constexpr int kPagedBlock = 32;  // positions of a block
 constexpr int kPagedMinExponent = -100;
 constexpr uint32_t kPagedNotFinite = 255;
 
@@ -55,13 +53,6 @@ struct PagedRope {
   const uint16_t* q;
   int64_t qs[2];  // element strides: row, head
   uint16_t* out;  // [rows, heads, D]
-};
-
-struct PagedSequence {
-  int first;   // its first new row
-  int count;   // new rows
-  int length;  // positions, as given
-  int stored;  // positions that its pages can hold
 };
 
 // Every number of it is bounded here: whatever the device tensors hold, rows

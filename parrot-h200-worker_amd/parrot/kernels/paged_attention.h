@@ -34,11 +34,7 @@ namespace paged {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;
-constexpr int kRows = 32;  // rows of a wavefront's tile
-constexpr int kMaxSplits = kWave;
-constexpr int kStepRows = 16;             // rows of a workgroup's tile, few per sequence
-constexpr int kTileRows = kWaves * kRows;  // ... many
+static_assert(kMaxSplits == kWave, "a share a lane");
 
 struct AttendArgs {
   PagedCache cache;
@@ -55,53 +51,6 @@ struct AttendArgs {
   float2* part_ml;   // [rows * heads][splits]
   uint16_t* out;     // [rows][heads][D]
 };
-
-// The key blocks that a tile's rows see, in order: the first `sinks` blocks,
-// then those from `lo` on.
-struct Blocks {
-  int sinks, lo, count;
-  __device__ __forceinline__ int at(int i) const { return i < sinks ? i : lo + i - sinks; }
-};
-
-__device__ __forceinline__ Blocks tile_blocks(int first, int last, int stored, int window,
-                                              int sinks) {
-  Blocks r{0, 0, 0};
-  last = min(last, stored - 1);
-  if (last < 0) return r;
-  // (a window past the first position reaches every key; first - window + 1 fits)
-  r.lo = first >= window ? min((first - window + 1) / kPagedBlock, last / kPagedBlock + 1) : 0;
-  // sinks > 0 only count where the window has left them
-  r.sinks = min(static_cast<int>((static_cast<int64_t>(sinks) + kPagedBlock - 1) / kPagedBlock),
-                r.lo);
-  r.count = r.sinks + last / kPagedBlock - r.lo + 1;
-  return r;
-}
-
-// The key blocks of a split: at least kMinShare, as many for each wavefront, and as many
-// as the sequence's last rows (which see the most) need for `splits` of them; all, where
-// those see no more than `whole`.  A tile that one share covers writes its output itself; its partial
-// sums say so (kWhole).
-constexpr int kMinShare = 8;
-constexpr float kWhole = -1.0f;  // in place of a sum
-
-struct Share {
-  int begin, end;
-  bool whole;
-  int most;  // key blocks of the sequence's longest share
-};
-
-__device__ __forceinline__ Share split_share(const PagedSequence& s, int rows, int tile, int rep,
-                                             const Blocks& blocks, int split, int splits,
-                                             int whole, int window, int sinks) {
-  const int row0 = (rows - 1) / tile * tile;
-  const Blocks most = tile_blocks(s.length - s.count + row0 / rep, s.length - 1, s.stored, window,
-                                  sinks);
-  if (splits == 1) return {0, blocks.count, true, most.count};
-  const int even = ((most.count + splits - 1) / splits + kWaves - 1) / kWaves * kWaves;
-  const int share = most.count <= whole ? most.count : max(even, kMinShare);
-  const int begin = min(split * share, blocks.count);
-  return {begin, min(begin + share, blocks.count), blocks.count <= share, min(share, most.count)};
-}
 
 // Which block of the cache (whose number fits 32 bits) a sequence's is, -1 where the table
 // names no page.

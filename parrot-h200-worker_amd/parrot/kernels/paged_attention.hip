@@ -133,57 +133,6 @@ __global__ __launch_bounds__(256) void paged_join_shares_kernel(AttendArgs a) {
       make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
 }
 
-struct Plan {
-  int tile, splits, whole;
-};
-
-// Tiles: of 16 rows where a sequence has no more than 32 on average (most of a larger
-// tile would be empty).  Of 32 while there is little to do, four blocks of 32 keys for
-// each of the chip's 1024 wavefront schedulers, eight of 8-bit keys: each wavefront
-// takes its own, straight from the pages, and none waits for another.  Beyond, of 128,
-// which share what they read and convert.  32 / 128 rows, 8 heads on 2 of 96 (us):
-//   bf16: 1 sequence of 500 keys, 1024 rows per kv head (1500 blocks) 9.1 / 15.0, 4 of
-//   2000, 128 (2000) 12.6 / 14.9, 16 of 1000, 96 (3000) 17.6 / 17.8, 4 of 2000, 256 (4100)
-//   21.6 / 20.8, 1 of 4000, 1024 (8500) 28.2 / 27.1, 32 of 4000, 48 (16000) 48.8 / 34.2
-//   int8: 4 of 2000, 256 (4100) 21.5 / 23.8, 16 of 1000, 256 (8200) 27.1 / 25.2, 1 of 4000,
-//   1024 (8500) 32.4 / 29.9
-// Splits, where a tile may see more keys than are faster without the join's launch: 768
-// for 16 and 32 rows (one sequence, 8 heads on 2 of 96, one launch / split, us: 512 keys
-// 6.0 / 8.4, 768 7.1 / 8.1, 1024 8.2 / 8.3, 1536 10.4 / 8.4; 64 sequences of 8 kv heads of
-// 64 in int8 768 17.3 / 18.1, 1024 21.3 / 21.1), and for 128 rows the more the more
-// workgroups there are without (16: 384 12.8 / 14.2, 512 15.6 / 14.2; 104: 768 21.4 / 23.0,
-// 1024 27.0 / 26.4).  For 16 rows no more workgroups than are resident at once, three a CU
-// (8 sequences of 32000 keys 24.5 us, of 1024 workgroups 27.2), each with 256 keys at
-// least (384: 24.5 and, of 32 rows with a window, 12.8 for 12.7); for larger tiles about
-// 1024, which evens out the causal ones (2 prompts of 4096 92.5 us, of 768 102), each with
-// 384 keys (3 chunks of 512 rows after 3500 keys 32.2 us, of 256 keys 35.5, of 512 33.2).
-Plan plan(int type, int batch, int rows, int heads, int kv_heads, int page, int width, int window,
-          int sinks) {
-  const int rep = heads / kv_heads;
-  // The most keys a tile can see: its table's, or the window, the sinks and
-  // the tile's own span.
-  auto keys_of = [&](int tile) {
-    const int64_t keys = static_cast<int64_t>(width) * page;
-    return window < INT32_MAX ? std::min<int64_t>(keys, int64_t{window} + sinks + tile + 64) : keys;
-  };
-  const int64_t all = static_cast<int64_t>(rows) * rep, n = std::max(std::min(batch, rows), 1);
-  const int64_t work = n * ((all + n * kRows - 1) / (n * kRows)) * kv_heads *
-                       ((keys_of(kRows) + kPagedBlock - 1) / kPagedBlock);
-  const int tile = all <= 2 * kStepRows * n                          ? kStepRows
-                   : work <= (type == kPagedBf16 ? 4096 : 8192) ? kRows
-                                                                     : kTileRows;
-  const int64_t keys = keys_of(tile);
-  const int64_t tiles = (static_cast<int64_t>(rows) * rep + tile - 1) / tile;
-  const int64_t units = std::max<int64_t>({tiles, std::min(batch, rows), 1}) * kv_heads;
-  const int64_t line = tile == kTileRows ? std::min<int64_t>(384 + 4 * units, 1024) : 768;
-  const bool step = tile == kStepRows;
-  const int64_t want = step ? std::max<int64_t>(768 / units, 1) : (1024 + units - 1) / units;
-  const int64_t least = step ? 256 : 384;
-  const int64_t splits =
-      keys <= line ? 1 : std::min<int64_t>({want, (keys + least - 1) / least, kMaxSplits});
-  return {tile, static_cast<int>(splits), static_cast<int>(line / kPagedBlock)};
-}
-
 }  // namespace
 
 int paged_attention_splits(int type, int batch, int rows, int heads, int kv_heads, int page,
