@@ -50,30 +50,34 @@ PARROT_EXTENT Blocks tile_blocks(int first, int last, int stored, int window, in
 }
 
 // The key blocks of a split: at least kMinShare, as many for each wavefront, and as many
-// as the sequence's last rows (which see the most) need for `splits` of them; all, where
-// those see no more than `whole`.  A tile that one share covers writes its output itself; its partial
-// sums say so (kWhole).
+// as `splits` of them need for the tile and for the sequence's last rows; all, where
+// those see no more than `whole`.  The last rows see the most without a window, which
+// makes shares of one size for a sequence's tiles.  With one, or past the table's end, a
+// tile before them may see more (the last may be short: 5 rows of 4 heads in tiles of 16
+// see 65, then 64 blocks of a window of 2048), and takes larger shares.  A tile that one
+// share covers writes its output itself; its partial sums say so (kWhole).
 constexpr int kMinShare = 8;
 constexpr float kWhole = -1.0f;  // in place of a sum
 
 struct Share {
   int begin, end;
   bool whole;
-  int most;  // key blocks of the sequence's longest share
+  int most;  // key blocks of the longest share of the tile and the sequence's last rows
 };
 
 PARROT_EXTENT Share split_share(const PagedSequence& s, int rows, int tile, int rep,
                                 const Blocks& blocks, int split, int splits, int whole,
                                 int window, int sinks) {
   const int row0 = (rows - 1) / tile * tile;
-  const Blocks most = tile_blocks(s.length - s.count + row0 / rep, s.length - 1, s.stored, window,
+  const Blocks last = tile_blocks(s.length - s.count + row0 / rep, s.length - 1, s.stored, window,
                                   sinks);
-  if (splits == 1) return {0, blocks.count, true, most.count};
-  const int even = ((most.count + splits - 1) / splits + kWaves - 1) / kWaves * kWaves;
-  const int share = most.count <= whole ? most.count : std::max(even, kMinShare);
+  const int most = std::max(last.count, blocks.count);
+  if (splits == 1) return {0, blocks.count, true, most};
+  const int even = ((most + splits - 1) / splits + kWaves - 1) / kWaves * kWaves;
+  const int share = most <= whole ? most : std::max(even, kMinShare);
   const int begin = std::min(split * share, blocks.count);
   return {begin, std::min(begin + share, blocks.count), blocks.count <= share,
-          std::min(share, most.count)};
+          std::min(share, most)};
 }
 
 struct Plan {

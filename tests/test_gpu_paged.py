@@ -461,6 +461,43 @@ def test_many_sequences():
         run.attend(2, new, batch, window=17, sinks=2)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("heads,kv_heads,d,new,length,window,sinks,copies", [
+    (8, 2, 96, 5, 4096, 2048, 0, 64), (8, 2, 96, 5, 4096, 2048, 0, 36),
+    (8, 2, 96, 1025, 4096, 2048, 0, 4), (8, 2, 96, 465, 1465, 1000, 0, 1),
+    (8, 8, 64, 337, 1337, 1024, 0, 16), (16, 2, 128, 1172, 1172, 1000, 0, 1),
+    (8, 2, 64, 1025, 3000, 1024, 70, 4),
+])
+def test_split_windows_with_short_last_tiles(dtype, heads, kv_heads, d, new, length, window, sinks,
+                                             copies):
+    """A sequence's last tile spans fewer positions than the others and sees fewer of
+    the window's blocks, in calls that split the keys.  copies: sequences of the same
+    pages, to all of which the same must come out."""
+    print(f"{copies} x {new} of {length}, {heads} on {kv_heads} of {d}, window {window} + {sinks}",
+          flush=True)
+    run = Run(dtype, kv_heads, d, 64, [[length]])
+    run.append([length])
+    q = _rows(run.g, new, heads, d, std=1.5)
+    run.tables, run.lengths = run.tables * copies, run.lengths * copies
+    got = run.cache.attend(q.cuda().repeat(copies, 1, 1), run.batch([new] * copies), scale=d ** -0.5,
+                           window=window, sinks=sinks).view(copies, new, -1)
+    assert torch.equal(got, got[:1].expand_as(got))
+    ref, bound = run.plain.attend(q, [new], d ** -0.5, window, sinks)
+    assert ((got[0].double().cpu() - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("new", [5, 40, 2000])
+@pytest.mark.parametrize("window,sinks", [(1000, 0), (1000, 5), (300, 0), (None, 0)])
+def test_tables_shorter_than_the_lengths(dtype, new, window, sinks):
+    """Positions past the table are not stored: no row sees them, and the last rows'
+    window may hold nothing else."""
+    run = Run(dtype, 2, 96, 64, [[3200]])
+    run.append([3200])
+    run.tables = [run.tables[0][:32]]
+    run.attend(8, [new], run.batch([new]), window=window, sinks=sinks, gone=[(0, 2048, 3200)])
+
+
 # ---------------------------------------------------------------------------
 # streams and graphs
 # ---------------------------------------------------------------------------
