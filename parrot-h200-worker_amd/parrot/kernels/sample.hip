@@ -649,7 +649,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
 
   // w 2^shift: w = 2^(k / 256) e^r with k = round(256 log2 w), |r| <= ln 2 / 512, and
   // e^r - 1 <= 0.00136 to the third power in 32 bits: w is right to 1e-10.
-  const double per_unit = kTable * 1.4426950408889634074 / temperature;
+  // (below 2e-306 the quotient would be infinite and the largest's own weight, by 0 times
+  // it, nothing; at 1e-300 the nearest two logits, 2^-149 apart, already differ by a weight
+  // that rounds to 0)
+  const double per_unit = kTable * 1.4426950408889634074 / fmax(temperature, 1e-300);
   const double origin = top;
   const double lowest = -kTable * (a.shift + 2);  // rounds to 0
   auto weight = [&](float x, int scale) -> double {  // w 2^scale

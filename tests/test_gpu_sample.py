@@ -128,6 +128,21 @@ def test_infinite_and_missing_logits(vocab):
         _check(x, u, **kw)
 
 
+@pytest.mark.parametrize("vocab", [100, 1000, 3001, 6000, 12001, 29000, 40001])
+@pytest.mark.parametrize("temperature", [1e-290, 1e-306, 1e-310, 5e-324])
+def test_tiny_temperatures(vocab, temperature):
+    """The smallest positive numbers: the largest logits alone are drawn from, alike."""
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(4, vocab, generator=g)
+    x[1, [1, 50, 90]] = 9.0
+    x[2] = 0.0
+    x[2, ::2] = 2.0 ** -149
+    x[3, [7, 80]] = math.inf
+    u = torch.rand(4, generator=g)
+    for kw in ({}, {"top_k": 2}, {"top_k": 600}, {"top_p": 0.4}, {"min_p": 1.0}):
+        _check(x, u, temperature=temperature, **kw)
+
+
 def test_a_row_does_not_depend_on_the_others():
     from parrot import hip_moe
     g = torch.Generator().manual_seed(3)
