@@ -923,7 +923,9 @@ int parrot_paged_attention_bf16(const parrot_paged_cache* cache, const parrot_pa
  *   times the whole.
  * temperature <= 0: the largest, the lowest index among equal ones.  The
  * parameters are arrays [rows], or where NULL the number beside them for every
- * row.  A NaN logit counts as -infinity; a row of nothing else draws -1.
+ * row.  Among them a NaN counts as a temperature of 0, a top_p of 1, a min_p of 0,
+ * a uniform number of 0; at an infinite temperature every logit but -infinity weighs 1.
+ * A NaN logit counts as -infinity; a row of nothing else draws -1.
  * probability (optional): the drawn token's share of the sum.  vocab <= 2^20.
  * New beside parrot_vocab_argmax_bf16 (decode_next, parrot/model.py:927-931). */
 int parrot_sample(const void* logits, int32_t type, int64_t rows, int32_t vocab, int64_t stride,

@@ -663,7 +663,9 @@ def sample(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor = 1.0
     the kept weights passes ``uniform`` times the whole.  A temperature of 0 (or
     less) takes the largest logit, the lowest index among equal ones.  Each
     parameter is a number or a tensor with one value per row (fp32; int32 for
-    top_k).  A NaN logit counts as -infinity; a row of nothing else gives token
+    top_k; a NaN there counts as a temperature of 0, a top_p of 1, a min_p or
+    uniform number of 0).  At an infinite temperature every logit but -infinity
+    weighs 1.  A NaN logit counts as -infinity; a row of nothing else gives token
     -1 with probability 0.  ``out``: a contiguous int64 tensor of one id per row to
     write the tokens into (a decode graph's input ids).
 

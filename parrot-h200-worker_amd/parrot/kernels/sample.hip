@@ -581,12 +581,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   row.steps = HELD && STEPS < kMost ? STEPS : (a.vocab + kWaves * kStep - 1) / (kWaves * kStep);
   row.aligned = (reinterpret_cast<uintptr_t>(row.at) & (4 * kBytes - 1)) == 0 && row.n % 4 == 0;
   row.infinite = false;
-  // (logits are finite numbers: at 1e30 all that are not -infinity are alike)
-  const double temperature = fmin(a.temperature ? a.temperature[r] : a.temperature_all, 1e30);
+  // (NaN: as 0; infinity: every logit but -infinity weighs 1)
+  const double temperature = a.temperature ? a.temperature[r] : a.temperature_all;
   const int top_k = a.top_k ? a.top_k[r] : a.top_k_all;
-  const double top_p = a.top_p ? a.top_p[r] : a.top_p_all;
-  // (the largest always stays)
-  const double min_p = fmin(a.min_p ? a.min_p[r] : a.min_p_all, 1.0);
+  const double top_p = a.top_p ? a.top_p[r] : a.top_p_all;  // (NaN: as 1)
+  // (the largest always stays; NaN: as 0)
+  const double min_p = fmin(fmax(a.min_p ? a.min_p[r] : a.min_p_all, 0.0), 1.0);
   if (t < kTable) sh.table[t] = kPowers.at[t];
 
   // This thread's and the row's largest logit.
@@ -671,13 +671,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   // The bins reach as far as weights do (2^-46 at 32 T), but no further than 32.
   const Bins bins{top, (kBins - 1) / static_cast<float>(
                                          fmax(fmin(32.0 * temperature, 32.0), 1e-30))};
-  const uint64_t least_mass = static_cast<uint64_t>(ldexp(fmax(min_p, 0.0), a.shift));
+  const uint64_t least_mass = static_cast<uint64_t>(ldexp(min_p, a.shift));
   auto needed = [&](uint64_t all) -> uint64_t {  // of the mass, for top_p
     const uint64_t x = static_cast<uint64_t>(ceil(fmax(top_p, 0.0) * static_cast<double>(all)));
     return x < 1 ? 1 : x > all ? all : x;
   };
   auto drawn = [&](uint64_t all) -> uint64_t {
-    // (u below 1: the product is below the sum but for its rounding)
+    // (u below 1: the product is below the sum but for its rounding; NaN: as 0)
     const double u = fmax(static_cast<double>(a.uniform[r]), 0.0) * static_cast<double>(all);
     const uint64_t x = u < static_cast<double>(all) ? static_cast<uint64_t>(u) : all - 1;
     return x < all ? x : all - 1;

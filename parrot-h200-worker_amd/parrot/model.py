@@ -891,13 +891,15 @@ def sample_torch(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor
     k = torch.where(greedy, 1.0, torch.where(k > 0, k, float(vocab)))
     w = torch.where(rank < k, w, 0.0)
     before = torch.cumsum(w, -1) - w
-    w = torch.where((before < p * w.sum(-1, keepdim=True)) | (p >= 1) | (rank == 0), w, 0.0)
-    w = torch.where(w >= m.clamp_max(1.0), w, 0.0)
+    w = torch.where((before < p * w.sum(-1, keepdim=True)) | ~(p < 1) | (rank == 0), w, 0.0)
+    w = torch.where(w >= m.nan_to_num(0.0).clamp_max(1.0), w, 0.0)
     w = torch.zeros_like(w).scatter_(1, order, w)
     reach = torch.cumsum(w, -1)
     total = reach[:, -1:]
-    target = uniform.reshape(-1, 1).double() * total
-    token = torch.searchsorted(reach, target, right=True).clamp_max(vocab - 1)
+    target = uniform.reshape(-1, 1).double().nan_to_num(0.0) * total
+    # (the last that was kept, where the product is not below the sum)
+    token = torch.minimum(torch.searchsorted(reach, target, right=True),
+                          torch.searchsorted(reach, total.contiguous()))
     none = top == -float("inf")
     prob = torch.where(none, 0.0, w.gather(1, token) / total)
     token = torch.where(none, -1, token)

@@ -143,6 +143,35 @@ def test_tiny_temperatures(vocab, temperature):
         _check(x, u, temperature=temperature, **kw)
 
 
+@pytest.mark.parametrize("vocab", [100, 1000, 3001, 6000, 12001, 29000, 40001])
+def test_parameters_that_are_not_numbers(vocab):
+    """As sample_torch has them: a NaN counts as no restriction, a temperature of 0, a
+    uniform number of 0; at an infinite temperature every logit is alike, the largest
+    and the smallest too."""
+    from parrot import hip_moe
+    from parrot.model import sample_torch
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(6, vocab, generator=g) * 4
+    x[1, vocab // 2:] = -math.inf
+    u = torch.rand(6, generator=g)
+    nan, inf, one = (torch.full((6,), v) for v in (math.nan, math.inf, 1.0))
+    # the largest numbers; infinities (which numpy's form above does not take at an
+    # infinite temperature)
+    ends = (torch.rand(6, vocab, generator=g) - 0.5) * 6.8e38
+    cases = [(x, u, {"temperature": nan}), (x, u, {"temperature": inf}), (x, u, {"top_p": nan}),
+             (x, u, {"min_p": nan, "top_k": 20}), (x, nan, {"top_k": 9}), (x, one, {"top_k": 9}),
+             (x, u, {"temperature": inf, "top_k": 600, "top_p": 0.5})]
+    for y in (ends, ends.nan_to_num()):
+        cases += [(y, torch.rand(6, generator=g), {"temperature": math.inf, **kw})
+                  for kw in ({}, {"top_k": 20}, {"top_p": 0.5})]
+    for y, v, kw in cases:
+        want = sample_torch(y, v, **kw)
+        token, prob = hip_moe.sample(y.cuda(), v.cuda(), **{
+            n: p.cuda() if isinstance(p, torch.Tensor) else p for n, p in kw.items()})
+        assert torch.equal(token.cpu(), want[0]), kw
+        assert ((prob.cpu() - want[1]).abs() <= 2.0 ** -23 * want[1] + 2.0 ** -30).all()
+
+
 def test_a_row_does_not_depend_on_the_others():
     from parrot import hip_moe
     g = torch.Generator().manual_seed(3)

@@ -55,6 +55,29 @@ def test_sample_torch():
             assert abs(prob[r].item() - share) <= 1e-6
 
 
+def test_parameters_that_are_not_numbers():
+    """A NaN counts as no restriction, a temperature of 0, a uniform number of 0; an
+    infinite temperature makes every logit alike; a uniform number of 1 is the last
+    that was kept."""
+    from parrot.model import sample_torch
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(6, 200, generator=g) * 4
+    x[:, 150:] = -math.inf
+    u = torch.rand(6, generator=g)
+    nan, inf = torch.full((6,), math.nan), torch.full((6,), math.inf)
+    for kw, same in (({"temperature": nan}, {"temperature": 0.0}), ({"top_p": nan}, {"top_p": 1.0}),
+                     ({"min_p": nan, "top_k": 20}, {"min_p": 0.0, "top_k": 20})):
+        for got, want in zip(sample_torch(x, u, **kw), sample_torch(x, u, **same)):
+            assert torch.equal(got, want), kw
+    for got, want in zip(sample_torch(x, nan, top_k=9), sample_torch(x, 0 * u, top_k=9)):
+        assert torch.equal(got, want)
+    token, prob = sample_torch(x, u, temperature=inf)
+    assert torch.equal(token[:, 0], (u.double() * 150).floor().long())
+    assert torch.equal(prob, torch.full((6, 1), 1 / 150))
+    token, _ = sample_torch(x, torch.ones(6), top_k=9)
+    assert torch.equal(token[:, 0], x.topk(9).indices.amax(-1))
+
+
 def test_decode_sample_on_the_pytorch_backend():
     from parrot import Parrot
     from parrot.model import sample_torch
