@@ -635,17 +635,17 @@ SAMPLE_MAX_VOCAB = 1 << 20
 
 
 def _sample_parameter(x, what: str, rows: int, device: torch.device, dtype: torch.dtype,
-                      most: float = math.inf):
+                      least: float, most: float):
     """(pointer, number) of one sampling parameter: a tensor of one value per
-    row, or a number from 0 to ``most`` for every row."""
+    row, or a number from ``least`` to ``most`` for every row."""
     if isinstance(x, Tensor):
         if x.dtype is not dtype or x.device != device or x.numel() != rows or \
                 not x.is_contiguous():
             raise RuntimeError(f"{what} must be a number or a contiguous {dtype} tensor of one "
                                "value per row on the logits' device")
         return x.data_ptr(), 0
-    if not 0 <= x <= most:
-        raise RuntimeError(f"{what} must lie between 0 and {most}")
+    if not least <= x <= most:
+        raise RuntimeError(f"{what} must lie between {least} and {most}")
     return None, x
 
 
@@ -657,7 +657,7 @@ def sample(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor = 1.0
     [..., 1] and their fp32 probabilities [..., 1] among the tokens that were kept.
 
     The weights are w = exp((logits - max) / temperature).  Of the ``top_k``
-    largest (equal ones by their index; 0: all), the shortest prefix that holds
+    largest (equal ones by their index; 0 or less: all), the shortest prefix that holds
     ``top_p`` of their sum is kept (never fewer than one), and of it the weights
     of at least ``min_p``; the token is the first, by index, at which the sum of
     the kept weights passes ``uniform`` times the whole.  A temperature of 0 (or
@@ -686,10 +686,11 @@ def sample(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor = 1.0
             not uniform.is_contiguous()):
         raise RuntimeError("uniform must be a contiguous fp32 tensor of one number per row on the "
                            "logits' device")
-    t, t_all = _sample_parameter(temperature, "temperature", rows, device, torch.float32)
-    k, k_all = _sample_parameter(top_k, "top_k", rows, device, torch.int32, 2 ** 31 - 1)
-    p, p_all = _sample_parameter(top_p, "top_p", rows, device, torch.float32, 1)
-    m, m_all = _sample_parameter(min_p, "min_p", rows, device, torch.float32, 1)
+    t, t_all = _sample_parameter(temperature, "temperature", rows, device, torch.float32,
+                                 -math.inf, math.inf)
+    k, k_all = _sample_parameter(top_k, "top_k", rows, device, torch.int32, -2 ** 31, 2 ** 31 - 1)
+    p, p_all = _sample_parameter(top_p, "top_p", rows, device, torch.float32, 0, 1)
+    m, m_all = _sample_parameter(min_p, "min_p", rows, device, torch.float32, 0, 1)
     lead.append(1)
     if out is None:
         out = token = torch.empty(lead, dtype=torch.int64, device=device)

@@ -172,6 +172,17 @@ def test_parameters_that_are_not_numbers(vocab):
         assert ((prob.cpu() - want[1]).abs() <= 2.0 ** -23 * want[1] + 2.0 ** -30).all()
 
 
+def test_numbers_below_zero():
+    """A temperature below 0 takes the largest, a top_k below 0 is none, as numbers and
+    as tensors."""
+    g = torch.Generator().manual_seed(8)
+    x, u = torch.randn(5, 3000, generator=g), torch.rand(5, generator=g)
+    for t in (-0.5, -math.inf, torch.full((5,), -2.0)):
+        _check(x, u, temperature=t)
+    for k in (-1, -2 ** 31, torch.full((5,), -7, dtype=torch.int32)):
+        _check(x, u, top_k=k)
+
+
 def test_a_row_does_not_depend_on_the_others():
     from parrot import hip_moe
     g = torch.Generator().manual_seed(3)

@@ -103,3 +103,33 @@ def test_hip_sample_refuses_cpu_tensors():
     from parrot import hip_moe
     with torch.no_grad(), pytest.raises(RuntimeError):
         hip_moe.sample(torch.zeros(2, 5), torch.zeros(2))
+
+
+def test_sample_parameters():
+    """A temperature of 0 or less and a top_k of 0 or less are numbers like any other, as
+    in a tensor and on the pytorch backend."""
+    from parrot import hip_moe
+    from parrot.model import sample_torch
+
+    def sample(**kw):  # as far as its arguments' checks, which come before the launch
+        parameter, given = hip_moe._sample_parameter, {}
+        with pytest.MonkeyPatch.context() as patch, torch.no_grad():
+            patch.setattr(hip_moe, "_require", lambda *_: None)
+            patch.setattr(hip_moe, "_on", lambda _: (_ for _ in ()).throw(InterruptedError))
+            patch.setattr(hip_moe, "_sample_parameter", lambda x, what, *a: given.setdefault(
+                what, parameter(x, what, *a)))
+            with pytest.raises(InterruptedError):
+                hip_moe.sample(torch.zeros(2, 5), torch.zeros(2), **kw)
+        return given
+    assert sample(temperature=-0.5)["temperature"] == (None, -0.5)
+    assert sample(temperature=math.inf)["temperature"] == (None, math.inf)
+    for k in (-1, -2 ** 31, 0, 2 ** 31 - 1):
+        assert sample(top_k=k)["top_k"] == (None, k)
+    for bad in ({"temperature": math.nan}, {"top_k": 2 ** 31}, {"top_k": -2 ** 31 - 1},
+                {"top_p": -0.1}, {"top_p": 1.1}, {"top_p": math.nan}, {"min_p": 2.0},
+                {"min_p": math.nan}, {"min_p": -1.0}):
+        with pytest.raises(RuntimeError):
+            sample(**bad)
+    x, u = torch.randn(3, 50, generator=torch.Generator().manual_seed(0)), torch.full((3,), 0.7)
+    assert torch.equal(sample_torch(x, u, temperature=-0.5)[0][:, 0], x.argmax(-1))
+    assert torch.equal(sample_torch(x, u, top_k=-1)[0], sample_torch(x, u)[0])
