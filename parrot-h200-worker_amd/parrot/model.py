@@ -1432,6 +1432,9 @@ class Parrot(nn.Module):
                 output = hip_moe.sample(logits, _draw[0], out=_out, **_draw[1])[0]
             else:
                 output = sample_torch(logits, _draw[0], **_draw[1])[0]
+            # A row of nothing but NaN draws -1, which is no token: the first is, as for
+            # decode_next (an embedding of -1 would be a read out of range).
+            output.clamp_(min=0)
         else:
             logits = self._head(h, None if _next_token_only else _out)
             output = logits.argmax(-1) if _next_token_only else logits
@@ -1454,7 +1457,8 @@ class Parrot(nn.Module):
                       top_p: float | Tensor = 1.0,
                       min_p: float | Tensor = 0.0) -> tuple[Tensor, GenerationState]:
         """Append one token and draw the next [batch, 1] by the given numbers
-        ``uniform`` [batch] in [0, 1) (see hip_moe.sample for the parameters)."""
+        ``uniform`` [batch] in [0, 1) (see hip_moe.sample for the parameters).  Where
+        all logits are NaN it is token 0."""
         kw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         return self.decode_step(input_ids, state, _next_token_only=True, _draw=(uniform, kw))
 

@@ -179,6 +179,34 @@ def test_generation_that_draws():
             DecodeGraph(model, state, logits=True, sampling=kw)
 
 
+@pytest.mark.parametrize("batch,kw", [(3, {}), (17, {}), (3, {"residual": "standard"})])
+def test_rows_of_nan_draw_a_token(batch, kw):
+    """Logits that are all NaN draw token 0, eagerly and captured, also where the next
+    step's embedding is looked up by itself (more than 16 sequences, no depth mixes)."""
+    from parrot.decode_graph import DecodeGraph
+    model = _model(**kw)
+    ids = torch.randint(0, model.config.vocab_size, (batch, 20),
+                        generator=torch.Generator().manual_seed(1)).cuda()
+    u = torch.linspace(0, 0.9, batch, device="cuda")
+    with torch.inference_mode():
+        _, state = model.prefill(ids)
+        weight = model.final_norm.weight.clone()
+        model.final_norm.weight.fill_(float("nan"))
+        token = ids[:, -1:].contiguous()
+        for _ in range(2):
+            token, state = model.decode_sample(token, state, u, top_k=5)
+            assert token.shape == (batch, 1) and not token.any()
+        graph = DecodeGraph(model, state, sampling=dict(temperature=0.8))
+        for _ in range(3):
+            token = graph.step(token, u)
+            assert not token.any()
+        model.final_norm.weight.copy_(weight)
+        want, _ = model.decode_sample(token.clone(), state, u, temperature=0.8)
+        state.position -= 1
+        state.position_device.sub_(1)
+        assert torch.equal(graph.step(token, u), want) and (want >= 0).all()
+
+
 def _greedy(model, ids, token, steps):
     _, state = model.prefill(ids)
     out = []

@@ -133,3 +133,18 @@ def test_sample_parameters():
     x, u = torch.randn(3, 50, generator=torch.Generator().manual_seed(0)), torch.full((3,), 0.7)
     assert torch.equal(sample_torch(x, u, temperature=-0.5)[0][:, 0], x.argmax(-1))
     assert torch.equal(sample_torch(x, u, top_k=-1)[0], sample_torch(x, u)[0])
+
+
+def test_a_row_of_nan_draws_a_token():
+    """Logits that are all NaN draw a token that the next step takes."""
+    from parrot import Parrot
+    torch.manual_seed(0)
+    model = Parrot(tiny_model_config()).eval()
+    ids = torch.randint(0, model.config.vocab_size, (2, 9))
+    _, state = model.prefill(ids)
+    with torch.no_grad():
+        model.final_norm.weight.fill_(math.nan)
+    token = ids[:, -1:]
+    for kw in ({}, {"temperature": 0.0}, {"top_k": 3}):
+        token, state = model.decode_sample(token, state, torch.tensor([0.2, 0.9]), **kw)
+        assert not token.any() and token.shape == (2, 1)
