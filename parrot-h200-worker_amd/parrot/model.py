@@ -1350,6 +1350,10 @@ class Parrot(nn.Module):
                         raise IndexError("decode_step token id out of range of the "
                                          f"{weight.shape[0]}-row embedding")
                 return x, (input_ids, weight)
+        if input_ids.is_cuda and torch.cuda.is_current_stream_capturing():
+            # A replay's ids (a graph's own, or what hip_moe.sample wrote there) are
+            # clamped as that launch does, not read from outside the table.
+            input_ids = input_ids.clamp(0, self.embedding.weight.shape[0] - 1)
         return self.embedding(input_ids), None
 
     @torch.inference_mode()

@@ -207,6 +207,33 @@ def test_rows_of_nan_draw_a_token(batch, kw):
         assert torch.equal(graph.step(token, u), want) and (want >= 0).all()
 
 
+@pytest.mark.parametrize("batch,kw", [(3, {}), (17, {}), (3, {"residual": "standard"})])
+def test_captured_ids_outside_the_vocabulary(batch, kw):
+    """A captured step takes ids outside the embedding as its nearest row, such as the
+    -1 that hip_moe.sample writes into a graph's ids for a row of NaN."""
+    from parrot import hip_moe
+    from parrot.decode_graph import DecodeGraph
+    model = _model(**kw)
+    vocab = model.config.vocab_size
+    ids = torch.randint(0, vocab, (batch, 20), generator=torch.Generator().manual_seed(1)).cuda()
+    with torch.inference_mode():
+        _, state = model.prefill(ids)
+        graph = DecodeGraph(model, state, logits=True)
+        u = torch.zeros(batch, device="cuda")
+        nothing = torch.full((batch, vocab), float("nan"), device="cuda")
+
+        def step(token):
+            state.position = 20
+            state.position_device.fill_(20)
+            return graph.step(token).clone()
+        for far, near in ((-1, 0), (vocab, vocab - 1), (2 ** 40, vocab - 1)):
+            want = step(torch.full((batch, 1), near, device="cuda"))
+            assert torch.equal(step(torch.full((batch, 1), far, device="cuda")), want)
+            if far == -1:
+                hip_moe.sample(nothing, u, out=graph.ids)
+                assert (graph.ids == -1).all() and torch.equal(step(graph.ids), want)
+
+
 def _greedy(model, ids, token, steps):
     _, state = model.prefill(ids)
     out = []
