@@ -16,7 +16,7 @@
 //
 // (and the same on v_mfma_f32_16x16x32_bf16 for tiles of 16 rows).
 //
-// 8-bit rows enter the products unrounded: K as q 2^x (exact in bf16), V as q
+// 8-bit rows enter the products unrounded: K as q 2^x (exact in bf16; int8: 2^(x - 2)), V as q
 // with its power of two on the probability instead (one power per key, and a
 // piece of V holds eight keys).  P is rounded to bf16 once, which the matrix
 // instructions ask for: half a step of 2^-8 on each probability, 1.9 to 2.3e-3 of the output
@@ -44,7 +44,7 @@ struct AttendArgs {
   int heads, rep;
   int window;  // INT_MAX: none
   int sinks;
-  float scale_log2;  // |scale| log2(e)
+  float scale_log2;  // |scale| log2(e), times kUnit
   uint32_t q_sign;   // 0x80008000 for a negative scale (q is negated), else 0
   int splits, whole;
   float* part;       // [rows * heads][splits][D], unnormalised
@@ -99,6 +99,21 @@ __device__ __forceinline__ Visible visible_to(int query, int stored, int window,
   const int last = min(query, stored - 1);
   const int first = query >= window ? query - window + 1 : 0;
   return {first, static_cast<uint32_t>(max(last - first + 1, 0)), min(sinks, last + 1)};
+}
+
+// int8 rows are multiplied by a quarter of their power of two, because the bias that their
+// conversion takes off, 128 times the power, is no number for the two largest powers
+// (rows past 2^127); the scale of scores, or the end of a sum, has the 4.
+template <int TYPE>
+constexpr float kUnit = TYPE == kPagedInt8 ? 4.0f : 1.0f;
+
+// 2^(byte - 127) / kUnit; of a row that is not finite what makes every product NaN.
+template <int TYPE>
+__device__ __forceinline__ float piece_power(uint32_t byte) {
+  if constexpr (TYPE == kPagedInt8)
+    return byte == kPagedNotFinite ? INFINITY : __uint_as_float((max(byte, 2u) - 2u) << 23);
+  else
+    return __uint_as_float(byte << 23);
 }
 
 // A piece (8 values) of a page as bf16: K's values are times `power`, V's are

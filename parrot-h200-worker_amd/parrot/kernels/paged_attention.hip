@@ -160,7 +160,8 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   a.rep = heads / cache.kv_heads;
   a.window = window;
   a.sinks = sinks;
-  a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
+  a.scale_log2 = fabsf(scale) * 1.4426950408889634f *
+                 (type == kPagedInt8 ? kUnit<kPagedInt8> : 1.0f);
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.out = out;
   const Plan p = plan(type, batch.batch, batch.rows, heads, cache.kv_heads, cache.page, batch.width,

@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
       f32x16 sc;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
-      const float power = TYPE == kPagedBf16 ? 1.0f : __uint_as_float(kbyte << 23);
+      const float power = TYPE == kPagedBf16 ? 1.0f : piece_power<TYPE>(kbyte);
 #pragma unroll
       for (int u = 0; u < KU; ++u)
         sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(piece_bf16<TYPE>(k[u], power), qf[u], sc, 0, 0,

@@ -53,7 +53,7 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     sc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const float power = TYPE == kPagedBf16 ? 1.0f : __uint_as_float(b.kbytes[n] << 23);
+    const float power = TYPE == kPagedBf16 ? 1.0f : piece_power<TYPE>(b.kbytes[n]);
 #pragma unroll
     for (int s = 0; s < S; ++s)
       sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(piece_bf16<TYPE>(b.k[n * S + s], power), qf[s],

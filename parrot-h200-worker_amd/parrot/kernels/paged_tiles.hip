@@ -28,7 +28,7 @@ namespace paged {
 
 namespace {
 
-// A V piece with its positions' powers of two (int8: shift = -128 times the power).
+// A V piece with its positions' powers of two over kUnit (int8: shift = -128 times the power).
 template <int TYPE>
 __device__ __forceinline__ bf16x8 value_piece(uint2 w, const float (&power)[8],
                                               const float (&shift)[8]) {
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
           float power[8], shift[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            power[e] = __uint_as_float(((bytes[e >> 2] >> (8 * (e & 3))) & 0xffu) << 23);
+            power[e] = piece_power<TYPE>((bytes[e >> 2] >> (8 * (e & 3))) & 0xffu);
             shift[e] = -128.0f * power[e];
           }
 #pragma unroll
@@ -179,8 +179,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
             const int at = (kWave * u + lane) * 16;
             const uint32_t b = at >= 16 * D ? bytes[1] : bytes[0];
             bf16x8* const p = reinterpret_cast<bf16x8*>(to + at + (at >= 16 * D ? kHalf : 0));
-            p[0] = piece_bf16<TYPE>(make_uint2(got[u].x, got[u].y), __uint_as_float((b & 0xffu) << 23));
-            p[1] = piece_bf16<TYPE>(make_uint2(got[u].z, got[u].w), __uint_as_float((b >> 8) << 23));
+            p[0] = piece_bf16<TYPE>(make_uint2(got[u].x, got[u].y), piece_power<TYPE>(b & 0xffu));
+            p[1] = piece_bf16<TYPE>(make_uint2(got[u].z, got[u].w), piece_power<TYPE>(b >> 8));
           }
         }
       }
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
   const int64_t to = static_cast<int64_t>(mine.token) * a.heads + mine.head;
   if (share.whole) {
     if (a.splits > 1 && half == 0) a.part_ml[to * a.splits] = make_float2(0.0f, kWhole);
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    const float f = l == 0.0f ? 0.0f : kUnit<TYPE> / l;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -379,7 +379,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
           *reinterpret_cast<float4*>(a.part + at * D + 32 * t + 8 * (e >> 2) + 4 * half) =
-              make_float4(st.o[t][e], st.o[t][e + 1], st.o[t][e + 2], st.o[t][e + 3]);
+              make_float4(st.o[t][e] * kUnit<TYPE>, st.o[t][e + 1] * kUnit<TYPE>,
+                          st.o[t][e + 2] * kUnit<TYPE>, st.o[t][e + 3] * kUnit<TYPE>);
     }
   }
 }

@@ -498,6 +498,35 @@ def test_tables_shorter_than_the_lengths(dtype, new, window, sinks):
     run.attend(8, [new], run.batch([new]), window=window, sinks=sinks, gone=[(0, 2048, 3200)])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+# tiles of 16 rows, of 32, and of 128, as above
+@pytest.mark.parametrize("n,copies", [(1, 1), (15, 1), (73, 1), (73, 128)])
+def test_largest_rows(dtype, n, copies):
+    """Keys and values up to the largest bf16 numbers, zeros among them: scores by
+    queries as small, values where a row sees one key."""
+    run = Run(dtype, 2, 64, 32, [[150]])
+    g = run.g
+    large = torch.randint(-3, 4, (150, 2, 64), generator=g) / 3 * 3.3e38
+    large[::3] = torch.randint(-2, 3, (50, 2, 64), generator=g) * 2.0 ** 126
+    large[1::5] = torch.randint(-1, 2, (30, 2, 64), generator=g) * 2.0 ** 127
+    large, usual = large.bfloat16(), _rows(g, 150, 2, 64)
+    assert torch.isfinite(large).all()
+    q = (torch.randint(-3, 4, (n, 8, 64), generator=g) * 2.0 ** -125).bfloat16()
+    for k, v, kw in ((large, usual, {}), (large, usual, {"window": 40, "sinks": 3}),
+                     (usual, large, {"window": 1}), (large, large, {"window": 1})):
+        run.lengths = [0]
+        run.plain = Plain(dtype, 2, 64, 1)
+        run.append([150], k, v)
+        lengths, tables = run.lengths, run.tables
+        run.tables, run.lengths = tables * copies, lengths * copies
+        got = run.cache.attend(q.cuda().repeat(copies, 1, 1), run.batch([n] * copies), scale=0.1,
+                               **kw).view(copies, n, -1)
+        run.tables, run.lengths = tables, lengths
+        assert torch.equal(got, got[:1].expand_as(got))
+        ref, bound = run.plain.attend(q, [n], 0.1, kw.get("window"), kw.get("sinks", 0))
+        assert ((got[0].double().cpu() - ref).abs() <= bound).all(), kw
+
+
 # ---------------------------------------------------------------------------
 # streams and graphs
 # ---------------------------------------------------------------------------
