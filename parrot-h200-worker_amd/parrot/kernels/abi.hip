@@ -856,7 +856,8 @@ int parrot_paged_attention_bf16(const parrot_paged_cache* cache, const parrot_pa
                                 void* stream) {
   if (int rc = check_paged(cache, batch)) return rc;
   if (int rc = check_paged_heads(rows, heads, cache->kv_heads)) return rc;
-  if (sinks < 0 || !(scale - scale == 0.0f) || scale == 0.0f) return PARROT_ERR_BAD_SHAPE;
+  // (times log2(e), and 4 for int8, it is a number still)
+  if (sinks < 0 || !(fabsf(scale) <= 0x1p125f) || scale == 0.0f) return PARROT_ERR_BAD_SHAPE;
   if (rows == 0 || batch->batch == 0) return PARROT_OK;
   const int64_t q_strides[3] = {q_row, q_head, 0};
   if (int rc = check_paged_rows(q, q_strides, 8)) return rc;

@@ -263,7 +263,8 @@ class PagedKVCache:
         """Attention of the new rows q [rows, heads, head_dim] (bf16, any row and
         head strides) over their sequences, their own keys and values appended
         before: softmax(q k^T * scale) v with key j visible to the row at position i
-        iff j <= i and (j > i - window or j < sinks).  Query head h reads kv head
+        iff j <= i and (j > i - window or j < sinks); scale not 0, up to 2^125 either
+        way.  Query head h reads kv head
         h // (heads // kv_heads).  Returns [rows, heads * head_dim] bf16, the
         layout of the output projection's input.  A row that sees no key is 0;
         rows of no sequence are left as they are in ``out`` (a contiguous tensor

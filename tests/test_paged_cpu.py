@@ -143,3 +143,15 @@ def test_stored_forms():
         q = (x.double() / step).float()
         q = q.to(dtype) if dtype == torch.float8_e4m3fn else q.round()
         assert torch.equal(q.double() * step, y)
+
+
+def test_scales_that_attention_refuses():
+    """A scale whose product with log2(e), and 4 for int8 pages, is no fp32 number."""
+    from parrot import _abi
+    lib, ref, c, b = _abi.load(), ctypes.byref, _cache(), _batch()
+    for scale, status in ((2.0 ** 126, -2), (-3e38, -2), (float("-inf"), -2), (2.0 ** 125, -1),
+                          (-(2.0 ** 125), -1), (1e-30, -1)):  # (-1: no query rows)
+        for type in range(3):
+            c.type = type
+            assert lib.parrot_paged_attention_bf16(ref(c), ref(b), None, 192, 96, 4, 8, 0, 0, scale,
+                                                   FAKE, FAKE, 1 << 40, None) == status, scale
