@@ -1362,7 +1362,7 @@ class Parrot(nn.Module):
                     _draw: tuple[Tensor, dict] | None = None) -> tuple[Tensor, GenerationState]:
         """Append one token per sequence to an existing generation state.
         ``_out``: the tensor that the logits, or (with ``_next_token_only``,
-        int64 [batch, 1]) the greedy tokens, are written into and returned as.
+        int64 [batch, 1]) the next tokens, are written into and returned as.
         ``_draw``: uniform numbers and parameters to draw the tokens by instead."""
         cfg = self.config
         if self.training:
@@ -1436,6 +1436,8 @@ class Parrot(nn.Module):
                 output = hip_moe.sample(logits, _draw[0], out=_out, **_draw[1])[0]
             else:
                 output = sample_torch(logits, _draw[0], **_draw[1])[0]
+                if _out is not None:
+                    output = _out.copy_(output)
             # A row of nothing but NaN draws -1, which is no token: the first is, as for
             # decode_next (an embedding of -1 would be a read out of range).
             output.clamp_(min=0)

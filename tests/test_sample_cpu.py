@@ -148,3 +148,18 @@ def test_a_row_of_nan_draws_a_token():
     for kw in ({}, {"temperature": 0.0}, {"top_k": 3}):
         token, state = model.decode_sample(token, state, torch.tensor([0.2, 0.9]), **kw)
         assert not token.any() and token.shape == (2, 1)
+
+
+def test_drawn_tokens_land_in_the_given_tensor():
+    """decode_step's output tensor takes drawn tokens as it does greedy ones."""
+    from parrot import Parrot
+    torch.manual_seed(0)
+    model = Parrot(tiny_model_config()).eval()
+    ids = torch.randint(0, model.config.vocab_size, (2, 9))
+    u, out = torch.tensor([0.3, 0.6]), torch.full((2, 1), -7)
+    _, state = model.prefill(ids)
+    want, _ = model.decode_sample(ids[:, -1:], state, u, temperature=0.9)
+    _, state = model.prefill(ids)
+    got, _ = model.decode_step(ids[:, -1:], state, _next_token_only=True, _out=out,
+                               _draw=(u, {"temperature": 0.9}))
+    assert got is out and torch.equal(out, want)
