@@ -518,12 +518,16 @@ class LocalGQA(nn.Module):
         sequences of their own lengths, over a paged cache that the rows' keys and
         values are appended to (one token or a chunk of a prompt per sequence; a
         window's first ``sinks`` positions stay visible).  HIP backend only.  Rows
-        of no sequence hold anything."""
+        of no sequence hold anything.  Positions end at max_seq_len: a table with a
+        page past it is refused; lengths, which only the device knows, are the
+        caller's to keep below it (RoPE takes later ones as the last)."""
         c = self.cfg
         if not self._hip(x) or x.ndim != 2:
             raise RuntimeError("a paged extension takes bf16 rows [rows, dim] on the HIP backend")
         if (cache.kv_heads, cache.head_dim) != (c.n_kv_heads, c.head_dim):
             raise RuntimeError("the cache's heads do not match the layer's")
+        if (batch.table.shape[1] - 1) * cache.page_size >= c.max_seq_len:
+            raise ValueError("RoPE position exceeds max_seq_len")
         from . import hip_moe
         if x.shape[0] == 0:
             return x if addend is None else addend

@@ -126,6 +126,19 @@ def test_layer_extended_in_chunks(dtype, sinks):
                 assert err < 1.2 * base
 
 
+def test_layer_refuses_pages_past_its_positions():
+    """A table may end inside the page that max_seq_len ends in, not behind it."""
+    from parrot import PagedBatch, PagedKVCache
+    cfg = _hip_config(max_seq_len=100, window_size=50)
+    layer = _layer(cfg)
+    cache = PagedKVCache(6, 32, cfg.n_kv_heads, cfg.head_dim)
+    x = torch.randn(3, cfg.dim, device="cuda").bfloat16()
+    with torch.no_grad():
+        layer.extend(x, cache, PagedBatch.from_lists([[0, 1, 2, 3]], [100], [3]))
+        with pytest.raises(ValueError, match="max_seq_len"):
+            layer.extend(x, cache, PagedBatch.from_lists([[0, 1, 2, 3, 4]], [131], [3]))
+
+
 def _model(seed=0, **kw):
     from parrot import Parrot
     torch.manual_seed(seed)
