@@ -99,12 +99,13 @@ class PagedKVCache:
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
         self._check(pages, page_size, kv_heads, head_dim, dtype)
-        def zeros(*shape):
-            return torch.zeros(shape, dtype=torch.uint8, device=device)
+        # (8 bits as bytes that are viewed: no tensor beside those that are kept)
+        byte = torch.uint8 if dtype.itemsize == 1 else dtype
         shape = (pages, kv_heads, page_size // PAGE_BLOCK, PAGE_BLOCK * head_dim)
-        rows = [zeros(*shape).to(dtype) for _ in range(2)]
+        rows = [torch.zeros(shape, dtype=byte, device=device).view(dtype) for _ in range(2)]
         exponents = [None, None] if dtype == torch.bfloat16 else \
-            [zeros(pages, kv_heads, page_size) for _ in range(2)]
+            [torch.zeros((pages, kv_heads, page_size), dtype=torch.uint8, device=device)
+             for _ in range(2)]
         self._describe(*rows, *exponents)
 
     @classmethod

@@ -527,6 +527,20 @@ def test_largest_rows(dtype, n, copies):
         assert ((got[0].double().cpu() - ref).abs() <= bound).all(), kw
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+def test_a_cache_takes_its_own_memory_only(dtype):
+    """No tensor beside the four that are kept is made, not for a moment either."""
+    from parrot import PagedKVCache
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    cache = PagedKVCache(4096, 64, 2, 128, dtype)
+    size = sum(x.numel() * x.element_size() for x in (
+        cache.key, cache.value, cache.key_exponent, cache.value_exponent) if x is not None)
+    assert torch.cuda.max_memory_allocated() - before <= size + 4096
+    assert not cache.key.view(torch.uint8).any() and not cache.value.view(torch.uint8).any()
+
+
 # ---------------------------------------------------------------------------
 # streams and graphs
 # ---------------------------------------------------------------------------
