@@ -63,6 +63,10 @@ class PagedBatch:
             self.table.data_ptr(), self.lengths.data_ptr(), self.starts.data_ptr(), b, width))
         object.__setattr__(self, "_at", ctypes.addressof(self._struct))
 
+    # (copies and pickles are of the tensors, not of their addresses)
+    def __reduce__(self):
+        return type(self), (self.table, self.lengths, self.starts)
+
     @classmethod
     def from_lists(cls, pages: list[list[int]], lengths: list[int], new: list[int],
                    device="cuda") -> "PagedBatch":
@@ -130,6 +134,10 @@ class PagedKVCache:
         self = cls.__new__(cls)
         self._describe(key, value, *(exponents or (None, None)))
         return self
+
+    # (as PagedBatch)
+    def __reduce__(self):
+        return type(self).from_pages, self._tensors
 
     @staticmethod
     def _check(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype) -> None:

@@ -155,3 +155,32 @@ def test_scales_that_attention_refuses():
             c.type = type
             assert lib.parrot_paged_attention_bf16(ref(c), ref(b), None, 192, 96, 4, 8, 0, 0, scale,
                                                    FAKE, FAKE, 1 << 40, None) == status, scale
+
+
+def test_copies_and_pickles():
+    """Of a cache and a batch: tensors of their own, whose addresses the calls get."""
+    import copy
+    import pickle
+    from parrot import PagedBatch, PagedKVCache
+    for dtype in (torch.bfloat16, torch.float8_e4m3fn, torch.int8):
+        c = PagedKVCache(3, 64, 2, 64, dtype, device="cpu")
+        c.key.view(torch.uint8).random_(0, 100)
+        copies = [copy.deepcopy(c), copy.deepcopy({"cache": c})["cache"]]
+        if dtype != torch.float8_e4m3fn:  # (torch itself does not unpickle such a tensor)
+            copies.append(pickle.loads(pickle.dumps(c)))
+        for d in copies:
+            assert (d.page_size, d.kv_heads, d.head_dim, d.dtype) == (64, 2, 64, dtype)
+            for x, y, at in zip(c._tensors, d._tensors, ("key", "value", "key_exponent",
+                                                         "value_exponent")):
+                if x is None:
+                    assert y is None
+                    continue
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+                assert getattr(d._struct, at) == y.data_ptr() != x.data_ptr()
+            assert d._at == ctypes.addressof(d._struct) and d._struct.type == c._struct.type
+        assert copy.copy(c).key is c.key
+    b = PagedBatch.from_lists([[0, 2], [1]], [70, 3], [1, 2], device="cpu")
+    for d in (copy.deepcopy(b), pickle.loads(pickle.dumps(b))):
+        assert torch.equal(b.table, d.table) and torch.equal(b.lengths, d.lengths)
+        assert d._struct.table == d.table.data_ptr() != b.table.data_ptr()
+        assert d._at == ctypes.addressof(d._struct)
