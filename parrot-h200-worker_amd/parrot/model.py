@@ -881,9 +881,8 @@ def sample_torch(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor
     x = logits.reshape(-1, vocab).double()
     rows = x.shape[0]
 
-    def column(v):
-        v = torch.as_tensor(v, device=x.device)
-        return v.double().reshape(-1, 1).expand(rows, 1)
+    def column(v):  # (a number in 64 bits, as hip_moe.sample takes it)
+        return torch.as_tensor(v, dtype=torch.float64, device=x.device).reshape(-1, 1).expand(rows, 1)
     t, k, p, m = (column(v) for v in (temperature, top_k, top_p, min_p))
     x = torch.where(x.isnan(), -float("inf"), x)
     x, order = torch.sort(x, dim=-1, descending=True, stable=True)

@@ -183,6 +183,14 @@ def test_numbers_below_zero():
         _check(x, u, top_k=k)
 
 
+def test_numbers_are_taken_in_64_bits():
+    """0.1 of 40 equal weights is four of them; as fp32, in a tensor, a fifth."""
+    x, u = torch.zeros(3, 40), torch.tensor([0.0, 0.5, 0.99])
+    for p, kept in ((0.1, 4), (torch.full((3,), 0.1), 5)):
+        token = _check(x, u, top_p=p)
+        assert token.flatten().tolist() == [int(kept * v) for v in (0.0, 0.5, 0.99)]
+
+
 def test_a_row_does_not_depend_on_the_others():
     from parrot import hip_moe
     g = torch.Generator().manual_seed(3)

@@ -163,3 +163,16 @@ def test_drawn_tokens_land_in_the_given_tensor():
     got, _ = model.decode_step(ids[:, -1:], state, _next_token_only=True, _out=out,
                                _draw=(u, {"temperature": 0.9}))
     assert got is out and torch.equal(out, want)
+
+
+def test_numbers_are_taken_in_64_bits():
+    """0.1 of 40 equal weights is four of them, as the definition and the kernel have it;
+    rounded to fp32 it would be a fifth."""
+    from parrot.model import sample_torch
+    x, u = torch.zeros(3, 40), torch.tensor([0.0, 0.5, 0.99])
+    for p, kept in ((0.1, 4), (torch.full((3,), 0.1), 5)):
+        token, prob = sample_torch(x, u, top_p=p)
+        assert token.flatten().tolist() == [int(kept * v) for v in (0.0, 0.5, 0.99)]
+        assert torch.equal(prob, torch.full((3, 1), 1 / kept))
+    token, prob = sample_torch(torch.tensor([[0.0, -1.0]]), torch.zeros(1), temperature=0.3)
+    assert prob.item() == torch.tensor(1 / (1 + math.exp(-1 / 0.3))).item()
