@@ -107,13 +107,10 @@ __device__ __forceinline__ Visible visible_to(int query, int stored, int window,
 template <int TYPE>
 constexpr float kUnit = TYPE == kPagedInt8 ? 4.0f : 1.0f;
 
-// 2^(byte - 127) / kUnit; of a row that is not finite what makes every product NaN.
+// 2^(byte - 127) / kUnit; infinite for a row that is not finite, which makes it NaN.
 template <int TYPE>
 __device__ __forceinline__ float piece_power(uint32_t byte) {
-  if constexpr (TYPE == kPagedInt8)
-    return byte == kPagedNotFinite ? INFINITY : __uint_as_float((max(byte, 2u) - 2u) << 23);
-  else
-    return __uint_as_float(byte << 23);
+  return __uint_as_float(byte << 23) * (1.0f / kUnit<TYPE>);
 }
 
 // A piece (8 values) of a page as bf16: K's values are times `power`, V's are

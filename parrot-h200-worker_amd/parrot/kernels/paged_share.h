@@ -29,6 +29,11 @@ constexpr int kStepRows = 16;              // rows of a workgroup's tile, few pe
 constexpr int kTileRows = kWaves * kRows;  // ... many
 constexpr int kMaxSplits = 64;             // a lane each in the join
 
+// (by value: with std::min's references the compiler orders the kernels otherwise, 115.6 us
+// for 114.9 for 4 prompts of 4096 in e4m3, 8 heads on 2 of 96)
+PARROT_EXTENT int lesser(int a, int b) { return a < b ? a : b; }
+PARROT_EXTENT int greater(int a, int b) { return a > b ? a : b; }
+
 // The key blocks that a tile's rows see, in order: the first `sinks` blocks,
 // then those from `lo` on.
 struct Blocks {
@@ -38,12 +43,12 @@ struct Blocks {
 
 PARROT_EXTENT Blocks tile_blocks(int first, int last, int stored, int window, int sinks) {
   Blocks r{0, 0, 0};
-  last = std::min(last, stored - 1);
+  last = lesser(last, stored - 1);
   if (last < 0) return r;
   // (a window past the first position reaches every key; first - window + 1 fits)
-  r.lo = first >= window ? std::min((first - window + 1) / kPagedBlock, last / kPagedBlock + 1) : 0;
+  r.lo = first >= window ? lesser((first - window + 1) / kPagedBlock, last / kPagedBlock + 1) : 0;
   // sinks > 0 only count where the window has left them
-  r.sinks = std::min(
+  r.sinks = lesser(
       static_cast<int>((static_cast<int64_t>(sinks) + kPagedBlock - 1) / kPagedBlock), r.lo);
   r.count = r.sinks + last / kPagedBlock - r.lo + 1;
   return r;
@@ -71,13 +76,13 @@ PARROT_EXTENT Share split_share(const PagedSequence& s, int rows, int tile, int 
   const int row0 = (rows - 1) / tile * tile;
   const Blocks last = tile_blocks(s.length - s.count + row0 / rep, s.length - 1, s.stored, window,
                                   sinks);
-  const int most = std::max(last.count, blocks.count);
+  const int most = greater(last.count, blocks.count);
   if (splits == 1) return {0, blocks.count, true, most};
   const int even = ((most + splits - 1) / splits + kWaves - 1) / kWaves * kWaves;
-  const int share = most <= whole ? most : std::max(even, kMinShare);
-  const int begin = std::min(split * share, blocks.count);
-  return {begin, std::min(begin + share, blocks.count), blocks.count <= share,
-          std::min(share, most)};
+  const int share = most <= whole ? most : greater(even, kMinShare);
+  const int begin = lesser(split * share, blocks.count);
+  return {begin, lesser(begin + share, blocks.count), blocks.count <= share,
+          lesser(share, most)};
 }
 
 struct Plan {
