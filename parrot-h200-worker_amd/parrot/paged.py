@@ -197,7 +197,7 @@ class PagedKVCache:
     def append(self, key: Tensor, value: Tensor, batch: PagedBatch) -> None:
         """Writes the new rows key and value [rows, kv_heads, head_dim] (bf16, any
         row and head strides) into their sequences' pages.  Other positions stay
-        as they are.  A page that is written must belong to one sequence."""
+        as they are.  A page that is written must belong to one sequence, once."""
         key = self._new_rows(key, self.kv_heads, "HIP paged append", 4)
         value = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
         if key.shape != value.shape:
@@ -258,9 +258,10 @@ class PagedKVCache:
             for x in out:
                 if x.dtype != torch.bfloat16 or x.device != self.device or x.shape != shape or \
                         x.stride(3) != 1 or any(st % 4 for st in x.stride()[:3]) or \
+                        any(st == 0 and n > 1 for st, n in zip(x.stride(), shape)) or \
                         x.data_ptr() % 8:
                     raise RuntimeError(f"out must be two bf16 tensors {list(shape)} on the cache's "
-                                       "device, strides multiples of 4")
+                                       "device, strides multiples of 4, no element in two places")
         with _on(self.device):
             _abi.check(_abi.load().parrot_paged_read_bf16(
                 self._at, b, positions, key.data_ptr(), *key.stride()[:3], value.data_ptr(),

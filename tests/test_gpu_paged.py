@@ -541,6 +541,21 @@ def test_a_cache_takes_its_own_memory_only(dtype):
     assert not cache.key.view(torch.uint8).any() and not cache.value.view(torch.uint8).any()
 
 
+def test_read_refuses_outputs_that_it_cannot_write():
+    """Of another shape, type or device, strides that are not multiples of 4, one place for
+    two positions."""
+    run = Run(torch.int8, 2, 64, 32, [[40, 9]])
+    batch = run.append([40, 9])
+    good = torch.empty(2, 2, 40, 64, dtype=torch.bfloat16, device="cuda")
+    run.cache.read(batch, 40, out=(good, good.clone()))
+    for bad in (good[:, :, :39], good.float(), good.cpu(), good.repeat(1, 1, 1, 2)[..., ::2],
+                torch.empty(2, 2, 40, 66, dtype=torch.bfloat16, device="cuda")[..., :64],
+                good[:, :, :1].expand(2, 2, 40, 64), good[:1].expand(2, 2, 40, 64)):
+        for pair in ((good, bad), (bad, good)):
+            with pytest.raises(RuntimeError):
+                run.cache.read(batch, 40, out=pair)
+
+
 # ---------------------------------------------------------------------------
 # streams and graphs
 # ---------------------------------------------------------------------------
