@@ -10,7 +10,9 @@
 //
 // What bounds it: bytes for many rows, the chain starts - table - page for few.
 // Measured, 2 heads of 96: 16384 rows into e4m3 pages 6.1 us (19 MB, 3.1 TB/s), read back
-// 6.4 us (3.0 TB/s); one row of one sequence 4.1 us either way, of which 3 are a launch's.
+// 6.2 us (3.0 TB/s), bf16 6.1 and 5.7 (25 MB, 4.1 and 4.4 TB/s); with RoPE and 8 query heads 16.9
+// and 16.6 (71 and 77 MB, 4.2 and 4.6 TB/s); one row of one sequence 4.0 us, in bf16 3.3 and
+// 2.9, with RoPE 6.3 and 5.6, of which 2.5 to 3 are a launch's.
 #include <algorithm>
 #include <type_traits>
 

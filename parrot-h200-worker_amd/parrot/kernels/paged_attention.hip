@@ -1,5 +1,5 @@
-// The launches of paged attention (paged_attention.h): which tiles, how many workgroups
-// a tile's keys are split over, and the join of what those found.
+// The launches of paged attention by its plan (paged_share.h), and the join of what the
+// workgroups found that a tile's keys were split over.
 #include <algorithm>
 
 #include "paged_attention.h"

@@ -7,15 +7,15 @@
 // K's second half lies 128 bytes further, so that the 16 lanes of a read's phase, which
 // take eight keys of each half, fall into different banks.
 //
-// What bounds it: a wavefront's chain of LDS reads, products and softmax, some 4300
-// clocks a pair of blocks (770 the products, 1000 the exponentials and sums, the rest
-// reads, the copies' issue and waits), which three wavefronts a SIMD overlap in part and
-// whose registers leave no fourth.  So a pair that every row sees whole
+// What bounds it: a wavefront's chain of LDS reads, products and softmax, some 4340
+// clocks a pair of blocks (760 the products, 970 the vector instructions, the rest
+// reads, the copies' issue and waits), which three wavefronts a SIMD (2.2 on average)
+// overlap in part and whose registers leave no fourth.  So a pair that every row sees whole
 // takes one step of the softmax and no mask (4 prompts of 4096, 8 heads on 2 of 96 in
 // bf16, window 2048: 114 us without, 102 with), and wavefronts step back for those with
-// more left (99).  Measured there 93 us in a trace, 0.83 PFLOP/s of the visible pairs'
-// products; 2 prompts of 4096, 8 heads of 64 in int8, 75 us and 6.8 for the join; 3 chunks
-// of 512 after up to 3500 keys 21.9 and 5.5.  Not kept: two blocks' scores ahead of the
+// more left (99).  Measured there 96 us in a trace and 88 to 92 among others, 0.84 to
+// 0.88 PFLOP/s of the visible pairs' products; 2 prompts of 4096, 8 heads of 64 in int8, 74 us
+// with the join (76 and 6.4 in a trace); 3 chunks of 512 after up to 3500 keys 21.8 and 5.6.  Not kept: two blocks' scores ahead of the
 // softmax (no change at three workgroups a CU, 130 us where registers leave two),
 // workgroups that take a second, short tile (the registers leave two a CU), odd shares in
 // reverse order (no change), sums of P by dot products of bf16 (eight instructions a block
