@@ -899,7 +899,7 @@ def sample_torch(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor
     w = torch.zeros_like(w).scatter_(1, order, w)
     reach = torch.cumsum(w, -1)
     total = reach[:, -1:]
-    target = uniform.reshape(-1, 1).double().nan_to_num(0.0) * total
+    target = uniform.reshape(-1, 1).double().nan_to_num(0.0).clamp_min(0.0) * total
     # (the last that was kept, where the product is not below the sum)
     token = torch.minimum(torch.searchsorted(reach, target, right=True),
                           torch.searchsorted(reach, total.contiguous()))

@@ -183,6 +183,18 @@ def test_numbers_below_zero():
         _check(x, u, top_k=k)
 
 
+@pytest.mark.parametrize("vocab", [5, 1500, 5000, 40000])
+def test_uniform_numbers_outside_their_range(vocab):
+    """Below 0 the first token that was kept, from 1 on the last."""
+    from parrot import hip_moe
+    x = torch.zeros(6, vocab)
+    x[:, 1], x[:, 2], x[:, 3] = 5.0, 1.0, 6.0
+    u = torch.tensor([-1.0, -math.inf, -0.0, 1.0, 2.0, math.inf])
+    for kw in ({"top_k": 2}, {"min_p": 0.3}):
+        token, _ = hip_moe.sample(x.cuda(), u.cuda(), **kw)
+        assert token.flatten().tolist() == [1, 1, 1, 3, 3, 3]
+
+
 def test_numbers_are_taken_in_64_bits():
     """0.1 of 40 equal weights is four of them; as fp32, in a tensor, a fifth."""
     x, u = torch.zeros(3, 40), torch.tensor([0.0, 0.5, 0.99])

@@ -176,3 +176,14 @@ def test_numbers_are_taken_in_64_bits():
         assert torch.equal(prob, torch.full((3, 1), 1 / kept))
     token, prob = sample_torch(torch.tensor([[0.0, -1.0]]), torch.zeros(1), temperature=0.3)
     assert prob.item() == torch.tensor(1 / (1 + math.exp(-1 / 0.3))).item()
+
+
+def test_uniform_numbers_outside_their_range():
+    """Below 0 the first token that was kept, from 1 on the last, never one that was not."""
+    from parrot.model import sample_torch
+    x = torch.tensor([[0.0, 5.0, 1.0, 6.0, 2.0]]).expand(6, 5)
+    u = torch.tensor([-1.0, -math.inf, -0.0, 1.0, 2.0, math.inf])
+    token, prob = sample_torch(x, u, top_k=2)
+    assert token.flatten().tolist() == [1, 1, 1, 3, 3, 3]
+    share = 1 / (1 + math.exp(-1.0))
+    assert (prob.flatten() - torch.tensor([1 - share] * 3 + [share] * 3)).abs().max() <= 1e-6
