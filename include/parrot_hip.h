@@ -898,9 +898,10 @@ size_t parrot_paged_attention_workspace_bytes(const parrot_paged_cache* cache,
  * head h / (heads / kv_heads).  A row that sees no key is 0; rows of no sequence
  * are left as they are.  What a row does not see cannot reach it, infinities and
  * NaN included.  Probabilities (times up to 2^8) times values are summed in fp32 before
- * they are divided, so values past 2^120 over the number of keys may overflow.  q bf16 [rows, heads, head_dim] with the given element strides of
- * rows and heads (multiples of 8, 16-byte aligned); out 8-byte aligned;
- * scale not 0, 2^125 in magnitude at most; workspace 16-byte aligned.
+ * they are divided, so values past 2^120 over the number of keys may overflow.  q bf16
+ * [rows, heads, head_dim] with the given element strides of rows and heads (multiples
+ * of 8, 16-byte aligned); out 8-byte aligned; scale not 0, 2^125 in magnitude at most;
+ * workspace 16-byte aligned.
  * New beside parrot_causal_attention_bf16 and parrot_decode_attention_bf16
  * (parrot/model.py:239-262, 264-295). */
 int parrot_paged_attention_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,

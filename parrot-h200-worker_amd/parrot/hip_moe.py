@@ -666,8 +666,9 @@ def sample(logits: Tensor, uniform: Tensor, *, temperature: float | Tensor = 1.0
     top_k; a NaN there counts as a temperature of 0, a top_p of 1, a min_p or
     uniform number of 0).  At an infinite temperature every logit but -infinity
     weighs 1.  A NaN logit counts as -infinity; a row of nothing else gives token
-    -1 with probability 0 (not an id that an embedding takes).  ``out``: a contiguous int64 tensor of one id per row to
-    write the tokens into (a decode graph's input ids).
+    -1 with probability 0 (not an id that an embedding takes).  ``out``: a
+    contiguous int64 tensor of one id per row to write the tokens into (a decode
+    graph's input ids).
 
     The arithmetic behind the borders is in 64 bits (see sample.hip), so a row's
     token does not depend on the other rows of the call."""

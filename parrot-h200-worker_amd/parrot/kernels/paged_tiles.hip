@@ -15,11 +15,11 @@
 // bf16, window 2048: 114 us without, 102 with), and wavefronts step back for those with
 // more left (99).  Measured there 96 us in a trace and 88 to 92 among others, 0.84 to
 // 0.88 PFLOP/s of the visible pairs' products; 2 prompts of 4096, 8 heads of 64 in int8, 74 us
-// with the join (76 and 6.4 in a trace); 3 chunks of 512 after up to 3500 keys 21.8 and 5.6.  Not kept: two blocks' scores ahead of the
-// softmax (no change at three workgroups a CU, 130 us where registers leave two),
-// workgroups that take a second, short tile (the registers leave two a CU), odd shares in
-// reverse order (no change), sums of P by dot products of bf16 (eight instructions a block
-// fewer, no change).
+// with the join (76 and 6.4 in a trace); 3 chunks of 512 after up to 3500 keys 21.8 and 5.6.
+// Not kept: two blocks' scores ahead of the softmax (no change at three workgroups a CU,
+// 130 us where registers leave two), workgroups that take a second, short tile (the
+// registers leave two a CU), odd shares in reverse order (no change), sums of P by dot
+// products of bf16 (eight instructions a block fewer, no change).
 #include "attention_lds.h"
 #include "paged_attention.h"
 
