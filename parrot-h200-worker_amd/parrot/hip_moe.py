@@ -607,7 +607,8 @@ def vocab_argmax(h: Tensor, weight: Tensor, advance: Tensor | None = None,
     parrot/kernels/moe_bf16.metal:1541-1621).  ``advance``: an int32 device
     counter the same launch increments by one (a decode step's position).
     ``out``: a contiguous int64 tensor of one id per row to write them into
-    (a decode graph's input ids, so the next replay reads them in place)."""
+    (a decode graph's input ids, so the next replay reads them in place).  A NaN
+    counts as less than any logit; a row of nothing else gives 0."""
     if advance is not None and (advance.dtype != torch.int32 or advance.device != h.device):
         raise RuntimeError("advance must be an int32 tensor on h's device")
     if out is not None and (out.dtype != torch.int64 or out.device != h.device or

@@ -259,7 +259,7 @@ __global__ __launch_bounds__(256) void vocab_argmax_reduce_kernel(
   if (tid == 0) {
 #pragma unroll
     for (int w = 1; w < 4; ++w) keep_better(vs[w], is[w], v, i);
-    out[r] = i;
+    out[r] = i == 0x7fffffff ? 0 : i;  // (no logit but NaN: the first, a token still)
     // The decode step's last launch: it advances the device position the
     // step's attention kernels read (no kernel of this launch reads it).
     if (r == 0 && advance != nullptr) *advance += 1;

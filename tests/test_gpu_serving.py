@@ -220,6 +220,40 @@ def test_rows_of_nan_draw_a_token(batch, kw):
         assert torch.equal(graph.step(token, u), want) and (want >= 0).all()
 
 
+@pytest.mark.parametrize("rows,vocab,dim", [(1, 300, 768), (16, 32768, 768), (5, 1001, 200)])
+def test_greedy_rows_of_nan(rows, vocab, dim):
+    """A row whose logits are all NaN gives token 0, the others theirs."""
+    from parrot import hip_moe
+    g = torch.Generator().manual_seed(3)
+    h = torch.randn(rows, dim, generator=g).bfloat16().cuda()
+    w = torch.randn(vocab, dim, generator=g).bfloat16().cuda()
+    with torch.no_grad():
+        want = hip_moe.vocab_argmax(h, w)
+        h[rows // 2] = float("nan")
+        want[rows // 2] = 0
+        assert torch.equal(hip_moe.vocab_argmax(h, w), want)
+
+
+@pytest.mark.parametrize("batch,kw", [(3, {}), (17, {}), (3, {"residual": "standard"})])
+def test_greedy_steps_of_nan(batch, kw):
+    """Greedy tokens of logits that are all NaN are tokens that the next step takes."""
+    from parrot.decode_graph import DecodeGraph
+    model = _model(**kw)
+    ids = torch.randint(0, model.config.vocab_size, (batch, 20),
+                        generator=torch.Generator().manual_seed(1)).cuda()
+    with torch.inference_mode():
+        _, state = model.prefill(ids)
+        model.final_norm.weight.fill_(float("nan"))
+        token = ids[:, -1:].contiguous()
+        for _ in range(2):
+            token, state = model.decode_next(token, state)
+            assert not token.any()
+        graph = DecodeGraph(model, state)
+        for _ in range(3):
+            token = graph.step(token)
+            assert not token.any()
+
+
 @pytest.mark.parametrize("batch,kw", [(3, {}), (17, {}), (3, {"residual": "standard"})])
 def test_captured_ids_outside_the_vocabulary(batch, kw):
     """A captured step takes ids outside the embedding as its nearest row, such as the
