@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define PARROT_ABI_VERSION 16
+#define PARROT_ABI_VERSION 17
 
 #define PARROT_OK 0
 #define PARROT_ERR_NULL_POINTER (-1)
@@ -809,6 +809,7 @@ int parrot_grouped_experts_static_bf16(const void* x, int64_t tokens, int32_t di
 #define PARROT_PAGED_BF16 0
 #define PARROT_PAGED_E4M3 1 /* OCP e4m3 (no infinities) */
 #define PARROT_PAGED_INT8 2
+#define PARROT_PAGED_E2M1 4 /* OCP e2m1, two to a byte */
 
 /* A paged KV cache (this struct lies in host memory, its pointers are device
  * pointers).  key and value: [pages, kv_heads, page / 32, 32 head_dim] elements,
@@ -820,7 +821,17 @@ int parrot_grouped_experts_static_bf16(const void* x, int64_t tokens, int32_t di
  * value_exponent [pages, kv_heads, page] (4-byte aligned): the smallest power of
  * two, 2^-100 at least, that brings the row's largest magnitude inside the type's
  * range (448, 127); q is rounded to nearest even.  x = 255: the row held a NaN
- * or an infinity, and reads back as NaN.  page a multiple of 32; head_dim 64, 96
+ * or an infinity, and reads back as NaN.
+ * e2m1: the values of a block lie eight to a 32-bit word, the first in the lowest bits,
+ * K as [4][16][2][head_dim / 32] words ([g][c][n][s]: position 16 n + c, dimensions
+ * 32 s + 8 g to 32 s + 8 g + 7), V as [4][16][2][head_dim / 32] ([g][c][o][u]: dimension
+ * 32 u + 16 o + c, positions 4 g to 4 g + 3 and 16 + 4 g to 16 + 4 g + 3).  Each 32
+ * dimensions of a key have a byte of their own: key_exponent is [pages, kv_heads,
+ * page / 32, head_dim], a block's bytes as [16][2][head_dim / 32] ([c][n][s]); a value
+ * row has one, as above (both 8-byte aligned).  The power of two, 2^-100 to 2^125, leaves
+ * the largest magnitude of those values above 3.5 and not above 7; what is above 6 then is
+ * stored as 6.  x = 255 as above, for the 32 dimensions of a key alone.
+ * page a multiple of 32; head_dim 64, 96
  * or 128; pages * kv_heads * page / 32 below 2^31. */
 typedef struct parrot_paged_cache {
   void* key;
@@ -853,7 +864,7 @@ typedef struct parrot_paged_batch {
 /* Writes the new rows k and v, bf16 [rows, kv_heads, head_dim] with the given
  * element strides of rows and heads (multiples of 4; unit stride inside a row,
  * 8-byte aligned), into their sequences' pages, quantised where the cache holds
- * 8 bits.  A page that is written belongs to one sequence.
+ * 8 or 4 bits.  A page that is written belongs to one sequence.
  * New beside parrot_decode_attention_bf16's store into a contiguous cache
  * (LocalGQA.decode, parrot/model.py:239-262). */
 int parrot_paged_append_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
@@ -878,8 +889,8 @@ int parrot_paged_append_rope_bf16(const parrot_paged_cache* cache, const parrot_
 /* Reads positions 0 .. positions - 1 of every sequence back: k and v, bf16
  * [batch, kv_heads, positions, head_dim] with the given element strides of
  * sequences, heads and positions (multiples of 4), zero from a sequence's length
- * on and where no page is named.  starts is not read.  8-bit values are exact in
- * bf16. */
+ * on and where no page is named.  starts is not read.  8-bit and 4-bit values are exact
+ * in bf16. */
 int parrot_paged_read_bf16(const parrot_paged_cache* cache, const parrot_paged_batch* batch,
                            int32_t positions, void* k, int64_t k_sequence, int64_t k_head,
                            int64_t k_position, void* v, int64_t v_sequence, int64_t v_head,

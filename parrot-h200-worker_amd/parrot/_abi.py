@@ -13,7 +13,7 @@ from pathlib import Path
 import torch  # noqa: F401  (maps PyTorch's HIP runtime before the library)
 
 LIBRARY = Path(__file__).resolve().parent / "_lib" / "libparrot_hip.so"
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32

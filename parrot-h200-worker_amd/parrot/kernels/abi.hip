@@ -50,10 +50,11 @@ int check_paged(const parrot_paged_cache* c, const parrot_paged_batch* b) {
   if (c->page % 32 || c->kv_heads > 65535 || b->batch > 65535 ||
       !parrot::paged_head_dim_supported(c->head_dim))
     return PARROT_ERR_UNSUPPORTED;
-  if (c->type != PARROT_PAGED_BF16 && c->type != PARROT_PAGED_E4M3 && c->type != PARROT_PAGED_INT8)
+  if (c->type != PARROT_PAGED_BF16 && c->type != PARROT_PAGED_E4M3 &&
+      c->type != PARROT_PAGED_INT8 && c->type != PARROT_PAGED_E2M1)
     return PARROT_ERR_UNSUPPORTED;
   // positions are 32-bit numbers, and so are the cache's blocks of 32 of them (which
-  // are 4 KiB or more: 2^31 of them fit no memory)
+  // are 1 KiB of 4 bits or more: 2^31 of them fit no memory)
   if (static_cast<int64_t>(b->width) * c->page > INT32_MAX - 64) return PARROT_ERR_BAD_SHAPE;
   if (c->pages > INT32_MAX / (c->page / 32) / c->kv_heads) return PARROT_ERR_BAD_SHAPE;
   const bool bytes = c->type != PARROT_PAGED_BF16;
@@ -63,7 +64,8 @@ int check_paged(const parrot_paged_cache* c, const parrot_paged_batch* b) {
     return PARROT_ERR_NULL_POINTER;
   if (!aligned16(c->key) || !aligned16(c->value) ||
       (bytes && ((reinterpret_cast<uintptr_t>(c->key_exponent) |
-                  reinterpret_cast<uintptr_t>(c->value_exponent)) & 3u)))
+                  reinterpret_cast<uintptr_t>(c->value_exponent)) &
+                 (c->type == PARROT_PAGED_E2M1 ? 7u : 3u))))
     return PARROT_ERR_ALIGNMENT;
   return PARROT_OK;
 }

@@ -43,6 +43,9 @@ template <int TYPE>
 __device__ __forceinline__ uint32_t exponent_byte(uint32_t amax) {
   const int e = static_cast<int>(amax >> 7), m = static_cast<int>(amax & 0x7f);
   if (e == 255) return kPagedNotFinite;
+  // (6 2^125 is the largest that e2m1 holds below 2^128)
+  if (TYPE == kPagedE2m1)
+    return static_cast<uint32_t>(min(max(e - 129 + (m > 96), kPagedMinExponent), 125) + 127);
   const int power = TYPE == kPagedE4m3 ? e - 135 + (m > 96) : e - 133 + (m > 126);
   return static_cast<uint32_t>(max(power, kPagedMinExponent) + 127);
 }
@@ -103,6 +106,127 @@ __device__ __forceinline__ uint32_t row_amax(uint32_t a) {
   return a;
 }
 
+// Four bf16 values over 2^(byte - 127) as 4 bits each, nearest even (one conversion, which
+// keeps what is above 6 at 6); zeros for a byte of kPagedNotFinite.
+__device__ __forceinline__ uint32_t quantise4_e2m1(uint2 x, uint32_t byte) {
+  if (byte == kPagedNotFinite) return 0;
+  const float power = __uint_as_float(byte << 23);
+  const uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(
+      0, __builtin_bit_cast(bf16x2_t, x.x), power, 0);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x.y), power, 1);
+}
+
+// Where a block of 4-bit values lies, and what this thread has of it.  Rows: eight threads
+// a row, thread `part` of row p with dims 32 j + 4 part .. of each group j.  V, which the
+// records hold by positions, by quads: words (o, u) of records (g, c0 .. c0 + 3), D threads
+// in all; in LDS the rows' four-value pieces, piece 8 u + 4 o + c0 / 4 of eight rows.
+template <int D>
+struct BlockE2m1 {
+  static constexpr int S = D / 32, kLd = D / 4 + 2;
+  uint8_t* k;             // 16-bit pieces of the thread's row: k + 4 j
+  uint32_t* v;            // words of the thread's quad: v + 2 S i
+  uint8_t* key_bytes;     // of the row's groups
+  uint8_t* value_byte;
+  int g, piece;           // of the quad; -1: none
+  __device__ __forceinline__ BlockE2m1(const PagedCache& c, int64_t block) {
+    const int p = threadIdx.x >> 3, part = threadIdx.x & 7, n = p >> 4, row = p & 15;
+    k = static_cast<uint8_t*>(c.key) + block * (16 * D) +
+        (((part >> 1) * 16 + row) * 2 * S + n * S) * 4 + 2 * (part & 1);
+    key_bytes = c.key_exponent + block * D + (2 * row + n) * S;
+    value_byte = c.value_exponent + block * kPagedBlock + p;
+    const int quad = threadIdx.x / (2 * S), w = threadIdx.x - quad * 2 * S;
+    const int o = w >= S, u = w - o * S;
+    g = quad >> 2;
+    piece = threadIdx.x < D ? 8 * u + 4 * o + (quad & 3) : -1;
+    v = static_cast<uint32_t*>(c.value) + block * (4 * D) + quad * 4 * 2 * S + w;
+  }
+  // The position of the e-th value of the quad's words.
+  __device__ __forceinline__ int position(int e) const { return (e >> 2) * 16 + 4 * g + (e & 3); }
+};
+
+// Rows lo .. hi - 1 of a block written (kw, vw: the thread's row); the others stay.
+template <int D>
+__device__ __forceinline__ void append_e2m1(const PagedCache& c, int64_t block,
+                                            const uint2 (&kw)[D / 32], const uint2 (&vw)[D / 32],
+                                            int lo, int hi, uint16_t (*v_s)[BlockE2m1<D>::kLd]) {
+  constexpr int S = D / 32;
+  const int p = threadIdx.x >> 3, part = threadIdx.x & 7;
+  const bool fresh = p >= lo && p < hi;
+  const BlockE2m1<D> at(c, block);
+  // Words that hold other positions too are read before they are written.
+  uint32_t keep = 0, old[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (at.position(e) < lo || at.position(e) >= hi) keep |= 0xfu << (4 * e);
+  const bool writes = at.piece >= 0 && keep != ~0u;
+  if (writes && keep != 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) old[i] = at.v[2 * S * i];
+  }
+  auto largest = [](uint2 w) {
+    return max(max(w.x & 0x7fffu, (w.x >> 16) & 0x7fffu), max(w.y & 0x7fffu, (w.y >> 16) & 0x7fffu));
+  };
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < S; ++j) {
+    const uint32_t byte = exponent_byte<kPagedE2m1>(row_amax(largest(kw[j])));
+    if (fresh) {
+      *reinterpret_cast<uint16_t*>(at.k + 4 * j) =
+          static_cast<uint16_t>(quantise4_e2m1(kw[j], byte));
+      if (part == 0) at.key_bytes[j] = static_cast<uint8_t>(byte);
+    }
+    most = max(most, largest(vw[j]));
+  }
+  const uint32_t byte = exponent_byte<kPagedE2m1>(row_amax(most));
+  if (fresh && part == 0) *at.value_byte = static_cast<uint8_t>(byte);
+#pragma unroll
+  for (int j = 0; j < S; ++j)
+    v_s[p][8 * j + part] = static_cast<uint16_t>(quantise4_e2m1(vw[j], byte));
+  __syncthreads();
+  if (!writes) return;
+  uint32_t y[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t x = v_s[at.position(e)][at.piece];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] |= ((x >> (4 * i)) & 0xfu) << (4 * e);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) at.v[2 * S * i] = (y[i] & ~keep) | (old[i] & keep);
+}
+
+// The thread's row of a block.
+template <int D>
+__device__ __forceinline__ void read_e2m1(const PagedCache& c, int64_t block, uint2 (&kw)[D / 32],
+                                          uint2 (&vw)[D / 32],
+                                          uint16_t (*v_s)[BlockE2m1<D>::kLd]) {
+  constexpr int S = D / 32;
+  const int p = threadIdx.x >> 3, part = threadIdx.x & 7;
+  const BlockE2m1<D> at(c, block);
+  if (at.piece >= 0) {
+    uint32_t y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = at.v[2 * S * i];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint32_t x = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x |= ((y[i] >> (4 * e)) & 0xfu) << (4 * i);
+      v_s[at.position(e)][at.piece] = static_cast<uint16_t>(x);
+    }
+  }
+  // (a byte of kPagedNotFinite makes the conversion's results NaN)
+  const uint32_t byte = *at.value_byte;
+#pragma unroll
+  for (int j = 0; j < S; ++j)
+    kw[j] = e2m1_bf16x4<0>(*reinterpret_cast<const uint16_t*>(at.k + 4 * j),
+                           __uint_as_float(static_cast<uint32_t>(at.key_bytes[j]) << 23));
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < S; ++j)
+    vw[j] = e2m1_bf16x4<0>(v_s[p][8 * j + part], __uint_as_float(byte << 23));
+}
+
 struct Rows {
   const uint16_t* k;
   const uint16_t* v;
@@ -127,6 +251,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c, Pa
   constexpr int S = D / 32;
   constexpr int kLd = D + 16 / sizeof(E);
   __shared__ __attribute__((aligned(16))) E v_s[kPagedBlock][kLd];
+  static_assert(2 * BlockE2m1<D>::kLd <= sizeof(E) * kLd, "a block's 4-bit values fit");
 
   // Blocks that new rows fall into.
   auto units_of = [&](const PagedSequence& s) {
@@ -185,6 +310,11 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedCache c, Pa
 #pragma unroll
       for (int j = 0; j < S; ++j) kw[j] = rotated(kw[j], rows.rope, angles, 32 * j + 4 * part);
     }
+  }
+  if constexpr (TYPE == kPagedE2m1) {
+    append_e2m1<D>(c, at * per_page + blk % per_page, kw, vw, lo, hi,
+                   reinterpret_cast<uint16_t(*)[BlockE2m1<D>::kLd]>(&v_s[0][0]));
+    return;
   }
   uint32_t kb = 0, vb = 0;
   if constexpr (TYPE != kPagedBf16) {
@@ -281,7 +411,14 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedCache c, Page
   uint2 kw[S], vw[S];
 #pragma unroll
   for (int j = 0; j < S; ++j) kw[j] = vw[j] = make_uint2(0, 0);
-  if (page >= 0) {  // (uniform)
+  if (TYPE == kPagedE2m1 && page >= 0) {
+    read_e2m1<D>(c, (static_cast<int64_t>(page) * c.kv_heads + head) * per_page + blk % per_page, kw,
+                 vw, reinterpret_cast<uint16_t(*)[BlockE2m1<D>::kLd]>(&v_s[0][0]));
+    if (!there) {
+#pragma unroll
+      for (int j = 0; j < S; ++j) kw[j] = vw[j] = make_uint2(0, 0);
+    }
+  } else if (page >= 0) {  // (uniform)
     const int64_t at = static_cast<int64_t>(page) * c.kv_heads + head;
     const E* const kp =
         static_cast<const E*>(c.key) + (at * per_page + blk % per_page) * (kPagedBlock * D);
@@ -370,6 +507,7 @@ hipError_t launch_paged_append(const PagedCache& cache, int type, int head_dim,
   };
   if (type == kPagedBf16) return run(std::integral_constant<int, kPagedBf16>{});
   if (type == kPagedE4m3) return run(std::integral_constant<int, kPagedE4m3>{});
+  if (type == kPagedE2m1) return run(std::integral_constant<int, kPagedE2m1>{});
   return run(std::integral_constant<int, kPagedInt8>{});
 }
 
@@ -388,6 +526,7 @@ hipError_t launch_paged_read(const PagedCache& cache, int type, int head_dim,
   };
   if (type == kPagedBf16) return run(std::integral_constant<int, kPagedBf16>{});
   if (type == kPagedE4m3) return run(std::integral_constant<int, kPagedE4m3>{});
+  if (type == kPagedE2m1) return run(std::integral_constant<int, kPagedE2m1>{});
   return run(std::integral_constant<int, kPagedInt8>{});
 }
 

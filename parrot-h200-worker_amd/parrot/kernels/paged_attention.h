@@ -16,7 +16,7 @@
 //
 // (and the same on v_mfma_f32_16x16x32_bf16 for tiles of 16 rows).
 //
-// 8-bit rows enter the products unrounded: K as q 2^x (exact in bf16; int8: 2^(x - 2)), V as q
+// 8-bit and 4-bit rows enter the products unrounded: K as q 2^x (exact in bf16; int8: 2^(x - 2)), V as q
 // with its power of two on the probability instead (one power per key, and a
 // piece of V holds eight keys).  P is rounded to bf16 once, which the matrix
 // instructions ask for: half a step of 2^-8 on each probability, 1.9 to 2.3e-3 of the output
@@ -32,7 +32,6 @@ namespace parrot {
 namespace paged {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 static_assert(kMaxSplits == kWave, "a share a lane");
 
@@ -123,6 +122,21 @@ template <>
 struct Piece<kPagedBf16> {
   using raw = uint4;
 };
+template <>
+struct Piece<kPagedE2m1> {
+  using raw = uint32_t;
+};
+
+// N consecutive words (of a record of 4-bit values), with as few loads as there can be.
+template <int N>
+__device__ __forceinline__ void load_words(const uint32_t* from, uint32_t (&to)[N]) {
+  struct __attribute__((aligned(N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4))) Words {
+    uint32_t w[N];
+  };
+  const Words x = *reinterpret_cast<const Words*>(from);
+#pragma unroll
+  for (int i = 0; i < N; ++i) to[i] = x.w[i];
+}
 
 __device__ __forceinline__ uint32_t bits(bf16x2_t v) { return __builtin_bit_cast(uint32_t, v); }
 
@@ -149,6 +163,9 @@ __device__ __forceinline__ bf16x8 piece_bf16(typename Piece<TYPE>::raw w, float 
     y.z = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, power, false));
     y.w = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, power, true));
     return __builtin_bit_cast(bf16x8, y);
+  } else if constexpr (TYPE == kPagedE2m1) {
+    const uint2 lo = e2m1_bf16x4<0>(w, power), hi = e2m1_bf16x4<1>(w, power);
+    return __builtin_bit_cast(bf16x8, make_uint4(lo.x, lo.y, hi.x, hi.y));
   } else {
     // (known to be 1, the compiler subtracts in whole numbers first: twice the work)
     asm("" : "+v"(power));
@@ -379,6 +396,7 @@ hipError_t by_type_and_width(int type, int head_dim, F f) {
   };
   if (type == kPagedBf16) return by_width(std::integral_constant<int, kPagedBf16>{});
   if (type == kPagedE4m3) return by_width(std::integral_constant<int, kPagedE4m3>{});
+  if (type == kPagedE2m1) return by_width(std::integral_constant<int, kPagedE2m1>{});
   return by_width(std::integral_constant<int, kPagedInt8>{});
 }
 

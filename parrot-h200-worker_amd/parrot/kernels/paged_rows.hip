@@ -16,6 +16,23 @@ namespace paged {
 
 namespace {
 
+// A block's 4-bit values as a lane needs them: to[2 t + h] the t-th word of half `part`
+// of record `record` + 32 h.
+template <int D>
+__device__ __forceinline__ void two_records(const void* pages, int block, int record, int part,
+                                            uint32_t (&to)[D / 16]) {
+  const uint32_t* from = static_cast<const uint32_t*>(pages) +
+                         int64_t{block} * (kPagedBlock * D / 8) + record * (D / 16) +
+                         part * (D / 32);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w[D / 32];
+    load_words(from + 32 * (D / 16) * h, w);
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) to[2 * t + h] = w[t];
+  }
+}
+
 template <int TYPE, int D>
 __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArgs a) {
   constexpr int KU = D / 16, DT = D / 32;
@@ -56,21 +73,33 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
     uint32_t kbyte = 0, vbytes[4] = {0, 0, 0, 0};
     auto load_keys = [&] {
       if (block < 0) return;
-      const raw* from = static_cast<const raw*>(a.cache.key) +
-                        int64_t{block} * (kPagedBlock * D / 8) + k_off;
+      if constexpr (TYPE == kPagedE2m1) {
+        two_records<D>(a.cache.key, block, half * 16 + kc, kn, k);
+        const uint8_t* e = a.cache.key_exponent + int64_t{block} * D + (2 * kc + kn) * DT;
+        kbyte = 0;
 #pragma unroll
-      for (int u = 0; u < KU; ++u) k[u] = from[32 * u];
-      if constexpr (TYPE != kPagedBf16)
-        kbyte = a.cache.key_exponent[int64_t{block} * kPagedBlock + 16 * kn + kc];
+        for (int i = 0; i < DT; ++i) kbyte |= static_cast<uint32_t>(e[i]) << (8 * i);
+      } else {
+        const raw* from = static_cast<const raw*>(a.cache.key) +
+                          int64_t{block} * (kPagedBlock * D / 8) + k_off;
+#pragma unroll
+        for (int u = 0; u < KU; ++u) k[u] = from[32 * u];
+        if constexpr (TYPE != kPagedBf16)
+          kbyte = a.cache.key_exponent[int64_t{block} * kPagedBlock + 16 * kn + kc];
+      }
     };
     auto load_values = [&] {
       if (block < 0) return;
-      const raw* from = static_cast<const raw*>(a.cache.value) +
-                        int64_t{block} * (kPagedBlock * D / 8) + v_off;
+      if constexpr (TYPE == kPagedE2m1) {
+        two_records<D>(a.cache.value, block, half * 16 + (col & 15), col >> 4, v);
+      } else {
+        const raw* from = static_cast<const raw*>(a.cache.value) +
+                          int64_t{block} * (kPagedBlock * D / 8) + v_off;
 #pragma unroll
-      for (int t = 0; t < DT; ++t)
+        for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) v[2 * t + h] = from[128 * t + 32 * h];
+          for (int h = 0; h < 2; ++h) v[2 * t + h] = from[128 * t + 32 * h];
+      }
       if constexpr (TYPE != kPagedBf16) {
         const uint8_t* e = a.cache.value_exponent + int64_t{block} * kPagedBlock + 4 * half;
 #pragma unroll
@@ -102,11 +131,12 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
       f32x16 sc;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
-      const float power = TYPE == kPagedBf16 ? 1.0f : piece_power<TYPE>(kbyte);
+      const float power = TYPE == kPagedBf16 || TYPE == kPagedE2m1 ? 1.0f : piece_power<TYPE>(kbyte);
 #pragma unroll
       for (int u = 0; u < KU; ++u)
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(piece_bf16<TYPE>(k[u], power), qf[u], sc, 0, 0,
-                                                     0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            piece_bf16<TYPE>(k[u], TYPE == kPagedE2m1 ? e2m1_power(kbyte, u / 2) : power), qf[u], sc,
+            0, 0, 0);
       if (more) {
         block = at.find(i + kWaves);
         load_keys();
@@ -135,7 +165,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
           if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              if (byte_of(e) == kPagedNotFinite) {  // (such an int8 row holds zeros)
+              if (byte_of(e) == kPagedNotFinite) {  // (such a row of int8 or e2m1 holds zeros)
                 bytes[e >> 2] &= ~(0xffu << (8 * (e & 3)));
 #pragma unroll
                 for (int t = 0; t < DT; ++t)

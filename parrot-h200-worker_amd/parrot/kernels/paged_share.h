@@ -10,7 +10,7 @@
 
 namespace parrot {
 
-enum PagedType { kPagedBf16 = 0, kPagedE4m3 = 1, kPagedInt8 = 2 };
+enum PagedType { kPagedBf16 = 0, kPagedE4m3 = 1, kPagedInt8 = 2, kPagedE2m1 = 4 };
 
 constexpr int kPagedBlock = 32;  // positions of a block
 

@@ -28,7 +28,7 @@ struct StepBlock {
   using raw = typename Piece<TYPE>::raw;
   static constexpr int N = D / 16;  // pieces of K, and of V, per lane
   raw k[N], v[N];
-  uint32_t kbytes[2], vbytes[2];  // exponents of the lane's key rows; of its 8 scores
+  uint32_t kbytes[2], vbytes[2];  // exponents of the lane's key rows (e2m1: S each); of its 8 scores
   int at;                         // which block of the cache; -1: none
 };
 
@@ -53,11 +53,13 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     sc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const float power = TYPE == kPagedBf16 ? 1.0f : piece_power<TYPE>(b.kbytes[n]);
+    const float power = TYPE == kPagedBf16 || TYPE == kPagedE2m1 ? 1.0f
+                                                                 : piece_power<TYPE>(b.kbytes[n]);
 #pragma unroll
     for (int s = 0; s < S; ++s)
-      sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(piece_bf16<TYPE>(b.k[n * S + s], power), qf[s],
-                                                      sc[n], 0, 0, 0);
+      sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+          piece_bf16<TYPE>(b.k[n * S + s], TYPE == kPagedE2m1 ? e2m1_power(b.kbytes[n], s) : power),
+          qf[s], sc[n], 0, 0, 0);
   }
   then();
   auto key_of = [&](int e) { return k0 + 16 * (e >> 2) + 4 * g + (e & 3); };
@@ -93,14 +95,15 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
 
   bf16x8 vf[T];
 #pragma unroll
-  for (int t = 0; t < T; ++t) vf[t] = piece_bf16<TYPE>(b.v[t], 1.0f);
+  for (int t = 0; t < T; ++t)  // (a record's words of 4 bits: dims 32 u + 16 o)
+    vf[t] = piece_bf16<TYPE>(b.v[TYPE == kPagedE2m1 ? (t & 1) * S + t / 2 : t], 1.0f);
   uint32_t bytes[2] = {b.vbytes[0], b.vbytes[1]};
   auto byte_of = [&](int e) { return (bytes[e >> 2] >> (8 * (e & 3))) & 0xffu; };
   // Values that some row must not see: times a probability of 0 an infinity or a NaN
   // is not 0.  They are left out and added to the rows that see them.
   bool odd = false;
   if (!whole) {
-    bool mine = has_nonfinite(vf);
+    bool mine = TYPE != kPagedE2m1 && has_nonfinite(vf);
     if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) mine |= byte_of(e) == kPagedNotFinite;
@@ -110,7 +113,7 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
       if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (byte_of(e) == kPagedNotFinite) {  // (such an int8 row holds zeros)
+          if (byte_of(e) == kPagedNotFinite) {  // (such a row of int8 or e2m1 holds zeros)
             bytes[e >> 2] &= ~(0xffu << (8 * (e & 3)));
 #pragma unroll
             for (int t = 0; t < T; ++t) vf[t][e] = __builtin_bit_cast(__bf16, uint16_t{0x7fc0});
@@ -188,9 +191,15 @@ __global__ __launch_bounds__(kWaves * kWave, D < 128 ? 3 : 2) void paged_step_ke
                     auto key) {
       if (b.at < 0) return;
       const raw* from = static_cast<const raw*>(pages) + int64_t{b.at} * (kPagedBlock * D / 8);
+      if constexpr (TYPE == kPagedE2m1) {
+        load_words(from + T * lane, to);
+      } else {
 #pragma unroll
-      for (int u = 0; u < T; ++u) to[u] = from[kWave * u + lane];
-      if constexpr (TYPE != kPagedBf16) {
+        for (int u = 0; u < T; ++u) to[u] = from[kWave * u + lane];
+      }
+      if constexpr (TYPE == kPagedE2m1 && decltype(key)::value) {
+        e2m1_key_bytes<D>(exponents + int64_t{b.at} * D, col, bytes);
+      } else if constexpr (TYPE != kPagedBf16) {
         const uint8_t* e = exponents + int64_t{b.at} * kPagedBlock;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {

@@ -30,7 +30,7 @@ namespace {
 
 // A V piece with its positions' powers of two over kUnit (int8: shift = -128 times the power).
 template <int TYPE>
-__device__ __forceinline__ bf16x8 value_piece(uint2 w, const float (&power)[8],
+__device__ __forceinline__ bf16x8 value_piece(typename Piece<TYPE>::raw w, const float (&power)[8],
                                               const float (&shift)[8]) {
   float x[8];
   if constexpr (TYPE == kPagedE4m3) {
@@ -43,6 +43,14 @@ __device__ __forceinline__ bf16x8 value_piece(uint2 w, const float (&power)[8],
       x[4 * i] = lo[0] * power[4 * i], x[4 * i + 1] = lo[1] * power[4 * i + 1];
       x[4 * i + 2] = hi[0] * power[4 * i + 2], x[4 * i + 3] = hi[1] * power[4 * i + 3];
     }
+  } else if constexpr (TYPE == kPagedE2m1) {
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    const f32x2_t y[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3)};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = y[e >> 1][e & 1] * power[e];
   } else {
     int8_values(w, x);
 #pragma unroll
@@ -62,8 +70,9 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
   constexpr int kHalf = 64;                                  // elements between K's halves
   constexpr int kK = kPagedBlock * D + kHalf;                // elements of K, then of V
   constexpr int kBlock = kK + kPagedBlock * D;
-  constexpr int kBytes = TYPE == kPagedBf16 ? 2 : 1;
-  constexpr int kLoads = kPagedBlock * D * kBytes / (16 * kWave);  // 1 KB pieces of a matrix
+  constexpr int kMatrix = TYPE == kPagedBf16 ? 64 * D : TYPE == kPagedE2m1 ? 16 * D : 32 * D;
+  // 1 KB pieces of a matrix (4 bits: a record a lane, with the first of four quarters)
+  constexpr int kLoads = TYPE == kPagedE2m1 ? 4 : kMatrix / (16 * kWave);
   __shared__ __attribute__((aligned(16))) uint16_t stage[2][2][kBlock];  // [buffer][block]
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -117,6 +126,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
     int at0 = -1, at1 = -1;            // of the stage that is brought
     __amdgpu_buffer_rsrc_t from;       // what this wavefront brings of it
     uint4 got[kLoads];                 // 8-bit types
+    uint32_t record[D / 16];           // 4 bits
     uint32_t bytes[2] = {0, 0};
     auto aim = [&](int i) {  // at blocks i and i + 1 (past the share: at nothing)
       const int j = (i - begin) % kWave;
@@ -127,15 +137,17 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
       at0 = i < end ? __builtin_amdgcn_readlane(ids, j) : -1;
       at1 = i < end ? __builtin_amdgcn_readlane(ids, j + 1) : -1;
       const int at = which ? at1 : at0;
-      from = make_rsrc(matrix + int64_t{max(at, 0)} * (kPagedBlock * D * kBytes),
-                       at < 0 ? 0 : kPagedBlock * D * kBytes);
+      from = make_rsrc(matrix + int64_t{max(at, 0)} * kMatrix, at < 0 ? 0 : kMatrix);
       if constexpr (TYPE != kPagedBf16) {
         if (at < 0) return;
         const int64_t e = int64_t{at} * kPagedBlock;
         if (brings_v) {  // positions 4 g .. + 3 and 16 + 4 g .. + 3 of the lane's pieces
-          const uint8_t* x = a.cache.value_exponent + e + 4 * ((lane >> 3) & 3);
+          const uint8_t* x =
+              a.cache.value_exponent + e + 4 * (TYPE == kPagedE2m1 ? lane >> 4 : (lane >> 3) & 3);
           bytes[0] = *reinterpret_cast<const uint32_t*>(x);
           bytes[1] = *reinterpret_cast<const uint32_t*>(x + 16);
+        } else if constexpr (TYPE == kPagedE2m1) {
+          e2m1_key_bytes<D>(a.cache.key_exponent + int64_t{at} * D, lane & 15, bytes);
         } else {  // keys c, c + 1 of either half
           const uint8_t* x = a.cache.key_exponent + e + ((2 * lane) & 15);
           bytes[0] = *reinterpret_cast<const uint16_t*>(x);
@@ -151,12 +163,20 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
           buffer_to_lds16(from, &stage[buf][which][brings_v ? kK : 0] + 512 * u +
                                     (!brings_v && u >= S ? kHalf : 0),
                           lane * 16u, 1024u * u);
-        else
+        else if constexpr (TYPE == kPagedE2m1) {
+          if (u > 0) continue;
+#pragma unroll
+          for (int w = 0; w < D / 16; w += 2) {
+            const auto x = __builtin_amdgcn_raw_buffer_load_b64(from, lane * (D / 4u), 4u * w, 0);
+            record[w] = x[0];
+            record[w + 1] = x[1];
+          }
+        } else
           got[u] = __builtin_bit_cast(
               uint4, __builtin_amdgcn_raw_buffer_load_b128(from, lane * 16u, 1024u * u, 0));
       }
     };
-    auto put = [&](int buf) {  // 8-bit types: what was brought, as bf16
+    auto put = [&](int buf) {  // 8-bit and 4-bit types: what was brought, as bf16
       if constexpr (TYPE != kPagedBf16) {
         if ((which ? at1 : at0) < 0) return;
         uint16_t* const to = &stage[buf][which][brings_v ? kK : 0];
@@ -167,12 +187,24 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
             power[e] = piece_power<TYPE>((bytes[e >> 2] >> (8 * (e & 3))) & 0xffu);
             shift[e] = -128.0f * power[e];
           }
+          if constexpr (TYPE == kPagedE2m1) {  // word (o, u): dims 32 u + 16 o ..
 #pragma unroll
-          for (int u = 0; u < kLoads; ++u) {
-            bf16x8* const p = reinterpret_cast<bf16x8*>(to + (kWave * u + lane) * 16);
-            p[0] = value_piece<TYPE>(make_uint2(got[u].x, got[u].y), power, shift);
-            p[1] = value_piece<TYPE>(make_uint2(got[u].z, got[u].w), power, shift);
+            for (int t = 0; t < D / 16; ++t)
+              *reinterpret_cast<bf16x8*>(to + (kWave * t + lane) * 8) =
+                  value_piece<TYPE>(record[(t & 1) * S + t / 2], power, shift);
+          } else {
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u) {
+              bf16x8* const p = reinterpret_cast<bf16x8*>(to + (kWave * u + lane) * 16);
+              p[0] = value_piece<TYPE>(make_uint2(got[u].x, got[u].y), power, shift);
+              p[1] = value_piece<TYPE>(make_uint2(got[u].z, got[u].w), power, shift);
+            }
           }
+        } else if constexpr (TYPE == kPagedE2m1) {  // word (n, s): dims 32 s ..
+#pragma unroll
+          for (int w = 0; w < D / 16; ++w)
+            *reinterpret_cast<bf16x8*>(to + (kWave * w + lane) * 8 + (w >= S ? kHalf : 0)) =
+                piece_bf16<TYPE>(record[w], e2m1_power(bytes[w / S], w % S));
         } else {
 #pragma unroll
           for (int u = 0; u < kLoads; ++u) {

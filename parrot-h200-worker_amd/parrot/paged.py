@@ -1,7 +1,7 @@
 """A paged KV cache of the MI355X backend, and attention over it.
 
 ``PagedKVCache`` holds one layer's keys and values for many sequences in pages,
-in bf16 or in 8 bits (quantised as they are written); ``PagedBatch`` says which
+in bf16, or in 8 or 4 bits (quantised as they are written); ``PagedBatch`` says which
 pages, lengths and new rows belong to which sequence of a call.  A step of a
 layer appends the new rows and attends from them::
 
@@ -25,7 +25,9 @@ from torch import Tensor
 from . import _abi
 from .hip_moe import ATTENTION_HEAD_DIMS, _on, _require, _stream
 
-PAGE_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2}
+PAGE_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2,
+              torch.float4_e2m1fn_x2: 4}
+FOUR_BITS = torch.float4_e2m1fn_x2  # an element of such a tensor is two values
 PAGE_BLOCK = 32  # a page is a whole number of blocks of so many positions
 
 
@@ -91,44 +93,58 @@ class PagedKVCache:
     """Pages of keys and values of one layer.
 
     ``key`` / ``value`` [pages, kv_heads, page_size / 32, 32 head_dim] of ``dtype``
-    (bf16, float8_e4m3fn or int8) hold blocks of 32 positions in the order in
+    (bf16, float8_e4m3fn, int8 or float4_e2m1fn_x2, half as many elements) hold blocks of 32 positions in the order in
     which the attention kernels read them (include/parrot_hip.h); ``read`` gives
     rows.  8-bit rows are scaled by a power of two of their own, one byte per
     position and head in ``key_exponent`` / ``value_exponent`` [pages, kv_heads,
     page_size], so that a stored value is exact in bf16.  What that costs, for
     normally distributed rows of 96: 2.7 % of the row's norm in e4m3 (whatever
     the row holds: its error goes with the value), 0.9 % in int8.  A row with a
-    NaN or an infinity reads back as NaN."""
+    NaN or an infinity reads back as NaN.
+
+    4 bits (e2m1): a power of two for 32 dims of a key each, ``key_exponent`` [pages,
+    kv_heads, page_size / 32, head_dim], and one for a value row as above; it leaves the
+    largest magnitude above 3.5 and not above 7, which becomes 6.  11.2 % of a normal
+    key's norm, 11.4 % of a value's, in 99 bytes for both of 96 (int8: 194).  32 dims with
+    a NaN or an infinity read back as NaN."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
         self._check(pages, page_size, kv_heads, head_dim, dtype)
         # (8 bits as bytes that are viewed: no tensor beside those that are kept)
         byte = torch.uint8 if dtype.itemsize == 1 else dtype
-        shape = (pages, kv_heads, page_size // PAGE_BLOCK, PAGE_BLOCK * head_dim)
+        shape = (pages, kv_heads, page_size // PAGE_BLOCK,
+                 PAGE_BLOCK * head_dim // (2 if dtype == FOUR_BITS else 1))
         rows = [torch.zeros(shape, dtype=byte, device=device).view(dtype) for _ in range(2)]
         exponents = [None, None] if dtype == torch.bfloat16 else \
-            [torch.zeros((pages, kv_heads, page_size), dtype=torch.uint8, device=device)
-             for _ in range(2)]
+            [torch.zeros(x, dtype=torch.uint8, device=device)
+             for x in self._exponent_shapes(*shape[:3], head_dim, dtype)]
         self._describe(*rows, *exponents)
+
+    @staticmethod
+    def _exponent_shapes(pages: int, kv_heads: int, blocks: int, head_dim: int, dtype):
+        rows = (pages, kv_heads, blocks * PAGE_BLOCK)
+        return ((pages, kv_heads, blocks, head_dim) if dtype == FOUR_BITS else rows), rows
 
     @classmethod
     def from_pages(cls, key: Tensor, value: Tensor, key_exponent: Tensor | None = None,
                    value_exponent: Tensor | None = None) -> "PagedKVCache":
         """A cache over tensors that are there already, laid out as above."""
-        if key.ndim != 4 or key.shape[3] % PAGE_BLOCK:
-            raise RuntimeError("pages are [pages, kv_heads, page_size / 32, 32 head_dim]")
+        per_dim = PAGE_BLOCK // 2 if key.dtype == FOUR_BITS else PAGE_BLOCK
+        if key.ndim != 4 or key.shape[3] % per_dim:
+            raise RuntimeError("pages are [pages, kv_heads, page_size / 32, 32 head_dim] (4 bits: "
+                               "16 head_dim)")
         pages, kv_heads, blocks, width = key.shape
-        cls._check(pages, blocks * PAGE_BLOCK, kv_heads, width // PAGE_BLOCK, key.dtype)
+        cls._check(pages, blocks * PAGE_BLOCK, kv_heads, width // per_dim, key.dtype)
         exponents = () if key.dtype == torch.bfloat16 else (key_exponent, value_exponent)
         if value.shape != key.shape or value.dtype != key.dtype or \
                 not (key.is_contiguous() and value.is_contiguous()):
             raise RuntimeError("key and value pages must be contiguous, of one shape and type")
-        for x in exponents:
-            if x is None or x.dtype != torch.uint8 or not x.is_contiguous() or \
-                    x.shape != (pages, kv_heads, blocks * PAGE_BLOCK):
-                raise RuntimeError("8-bit pages need contiguous uint8 exponents "
-                                   "[pages, kv_heads, page_size]")
+        for x, shape in zip(exponents, cls._exponent_shapes(pages, kv_heads, blocks,
+                                                            width // per_dim, key.dtype)):
+            if x is None or x.dtype != torch.uint8 or not x.is_contiguous() or x.shape != shape:
+                raise RuntimeError("8-bit and 4-bit pages need contiguous uint8 exponents "
+                                   f"{list(shape)}")
         if any(x.device != key.device for x in (value, *exponents)):
             raise RuntimeError("a cache's tensors must be on one device")
         self = cls.__new__(cls)
@@ -153,7 +169,8 @@ class PagedKVCache:
         self._tensors = tensors
         pages, kv_heads, blocks, width = self.key.shape
         self.page_size, self.kv_heads = blocks * PAGE_BLOCK, kv_heads
-        self.head_dim, self.dtype, self.device = width // PAGE_BLOCK, self.key.dtype, self.key.device
+        self.dtype, self.device = self.key.dtype, self.key.device
+        self.head_dim = width * (2 if self.dtype == FOUR_BITS else 1) // PAGE_BLOCK
         self._struct = _abi.PagedCacheStruct(
             self.key.data_ptr(), self.value.data_ptr(), _abi.ptr(self.key_exponent),
             _abi.ptr(self.value_exponent), pages, self.page_size, kv_heads, self.head_dim,
