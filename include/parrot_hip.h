@@ -896,6 +896,43 @@ int parrot_paged_read_bf16(const parrot_paged_cache* cache, const parrot_paged_b
                            int64_t k_position, void* v, int64_t v_sequence, int64_t v_head,
                            int64_t v_position, void* stream);
 
+/* Pages that are handed out and taken back on the GPU (host memory, a device pointer):
+ * uses [pages], 16-byte aligned, says how many tables name each page; those with 0 or less are free.
+ * pages 2^30 at most, page (positions) a multiple of 32. */
+typedef struct parrot_paged_pool {
+  int32_t* uses;
+  int64_t pages;
+  int32_t page;
+} parrot_paged_pool;
+
+/* Bytes of workspace that parrot_paged_extend needs for a batch of that many sequences. */
+size_t parrot_paged_extend_workspace_bytes(int32_t batch);
+
+/* Gives sequence i new_rows[i] new positions (below 0: none) and the pages for them: writes
+ * lengths, starts and table of the batch (of device memory that may be written) and uses.
+ * The sequences are served in order: with need_i the pages that sequence i is short of,
+ * sequence i gets its positions, all or none, iff its table has room for them, the
+ * new_rows of it and those before it (whose tables have room) come to no more than `rows`,
+ * and need_i is 0 or the need of it and those before it (likewise) come to no more than
+ * there are free pages.  The lowest free pages go first, to the sequences in order.  A page
+ * that is handed out has a use of 1.  A sequence that gets none stays as it is.
+ * slots [rows] and positions [rows]: of each new row the place in the pool, table[i, p /
+ * page] * page + p % page, and its position p; -1 for rows past the last (slots too where a table names
+ * no page).  Sequences' table columns past their lengths are taken to name no page of the
+ * pool.  workspace 16-byte aligned.
+ * New: parrot/model.py has contiguous caches of one length (model.py:772-788). */
+int parrot_paged_extend(const parrot_paged_pool* pool, const parrot_paged_batch* batch,
+                        const int32_t* new_rows, int32_t rows, int64_t* slots,
+                        int32_t* positions, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Takes positions back: sequence i keeps its first lengths[i] (NULL, or more than it has: all),
+ * and pages wholly past them lose a use and their table entry (-1).  window > 0: so do pages
+ * of which no later query (from its length on) sees a position, those with all positions
+ * j <= length - window and j >= sinks.  starts is not read. */
+int parrot_paged_release(const parrot_paged_pool* pool, const parrot_paged_batch* batch,
+                         const int32_t* lengths, int32_t window, int32_t sinks, void* stream);
+
 /* Bytes of workspace that parrot_paged_attention_bf16 needs for these sizes (0
  * where it needs none, or for sizes that it does not take). */
 size_t parrot_paged_attention_workspace_bytes(const parrot_paged_cache* cache,

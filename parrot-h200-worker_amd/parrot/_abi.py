@@ -35,6 +35,11 @@ class PagedBatchStruct(ctypes.Structure):
     _fields_ = [("table", _p), ("lengths", _p), ("starts", _p), ("batch", _i32), ("width", _i32)]
 
 
+class PagedPoolStruct(ctypes.Structure):
+    """parrot_paged_pool."""
+    _fields_ = [("uses", _p), ("pages", _i64), ("page", _i32)]
+
+
 # name -> (restype, argtypes); mirrors include/parrot_hip.h
 SIGNATURES: dict[str, tuple] = {
     "parrot_abi_version": (ctypes.c_int, []),
@@ -164,6 +169,9 @@ SIGNATURES: dict[str, tuple] = {
                        _i32, _p, _p]),
     "parrot_paged_read_bf16": (
         ctypes.c_int, [_p, _p, _i32, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p]),
+    "parrot_paged_extend_workspace_bytes": (_sz, [_i32]),
+    "parrot_paged_extend": (ctypes.c_int, [_p, _p, _p, _i32, _p, _p, _p, _sz, _p]),
+    "parrot_paged_release": (ctypes.c_int, [_p, _p, _p, _i32, _i32, _p]),
     "parrot_paged_attention_workspace_bytes": (_sz, [_p, _p, _i32, _i32, _i32, _i32]),
     "parrot_paged_attention_bf16": (
         ctypes.c_int, [_p, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _f32, _p, _p, _sz, _p]),

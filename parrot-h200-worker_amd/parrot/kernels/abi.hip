@@ -878,6 +878,54 @@ int parrot_paged_attention_bf16(const parrot_paged_cache* cache, const parrot_pa
       scale, workspace, static_cast<uint16_t*>(out), as_stream(stream)));
 }
 
+namespace {
+
+int check_pool(const parrot_paged_pool* p, const parrot_paged_batch* b) {
+  if (!p || !b) return PARROT_ERR_NULL_POINTER;
+  if (p->pages < 0 || p->page <= 0 || b->batch < 0 || b->width < 0) return PARROT_ERR_BAD_SHAPE;
+  if (p->page % 32 || b->batch > 65535) return PARROT_ERR_UNSUPPORTED;
+  if (p->pages > (1 << 30) || static_cast<int64_t>(b->width) * p->page > INT32_MAX - 64)
+    return PARROT_ERR_BAD_SHAPE;
+  if ((p->pages > 0 && !p->uses) || !b->starts || (b->batch > 0 && !b->lengths) ||
+      (b->batch > 0 && b->width > 0 && !b->table))
+    return PARROT_ERR_NULL_POINTER;
+  return aligned16(p->uses) ? PARROT_OK : PARROT_ERR_ALIGNMENT;
+}
+
+}  // namespace
+
+size_t parrot_paged_extend_workspace_bytes(int32_t batch) {
+  return batch < 0 || batch > 65535 ? 0 : parrot::paged_extend_workspace_bytes(batch);
+}
+
+int parrot_paged_extend(const parrot_paged_pool* pool, const parrot_paged_batch* batch,
+                        const int32_t* new_rows, int32_t rows, int64_t* slots,
+                        int32_t* positions, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  if (int rc = check_pool(pool, batch)) return rc;
+  if (rows < 0 || rows > (1 << 30)) return PARROT_ERR_BAD_SHAPE;
+  if ((batch->batch > 0 && !new_rows) || (rows > 0 && (!slots || !positions)))
+    return PARROT_ERR_NULL_POINTER;
+  const size_t need = parrot::paged_extend_workspace_bytes(batch->batch);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need) return PARROT_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return PARROT_ERR_ALIGNMENT;
+  }
+  return status(parrot::launch_paged_extend({pool->uses, pool->pages, pool->page},
+                                            paged_batch(batch, rows), new_rows, slots, positions,
+                                            workspace, as_stream(stream)));
+}
+
+int parrot_paged_release(const parrot_paged_pool* pool, const parrot_paged_batch* batch,
+                         const int32_t* lengths, int32_t window, int32_t sinks, void* stream) {
+  if (int rc = check_pool(pool, batch)) return rc;
+  if (sinks < 0) return PARROT_ERR_BAD_SHAPE;
+  return status(parrot::launch_paged_release({pool->uses, pool->pages, pool->page},
+                                             paged_batch(batch, 0), lengths,
+                                             window > 0 ? window : INT32_MAX, sinks,
+                                             as_stream(stream)));
+}
+
 int parrot_sample(const void* logits, int32_t type, int64_t rows, int32_t vocab, int64_t stride,
                   const float* uniform, const float* temperature, double temperature_all,
                   const int32_t* top_k, int32_t top_k_all, const float* top_p, double top_p_all,

@@ -50,6 +50,13 @@ struct PagedCache {
   int page, kv_heads;
 };
 
+// Pages that sequences share out among themselves: those with a use of 0 or less are free.
+struct PagedPool {
+  int32_t* uses;  // [pages]
+  int64_t pages;
+  int page;
+};
+
 // Sequence i: its pages table[i, :width], its whole length lengths[i] (new
 // rows included), its new rows starts[i] .. starts[i + 1] of `rows`.
 struct PagedBatch {
@@ -228,6 +235,11 @@ hipError_t launch_paged_append(const PagedCache& cache, int type, int head_dim,
 hipError_t launch_paged_read(const PagedCache& cache, int type, int head_dim,
                              const PagedBatch& batch, int positions, uint16_t* k, uint16_t* v,
                              const int64_t* k_strides, const int64_t* v_strides, hipStream_t s);
+size_t paged_extend_workspace_bytes(int batch);
+hipError_t launch_paged_extend(const PagedPool& pool, const PagedBatch& batch, const int32_t* fresh,
+                               int64_t* slots, int32_t* positions, void* workspace, hipStream_t s);
+hipError_t launch_paged_release(const PagedPool& pool, const PagedBatch& batch, const int32_t* to,
+                                int window, int sinks, hipStream_t s);
 int paged_attention_splits(int type, int batch, int rows, int heads, int kv_heads, int page,
                            int width, int window, int sinks);
 size_t paged_attention_workspace_bytes(int splits, int rows, int heads, int head_dim);

@@ -89,6 +89,113 @@ class PagedBatch:
                    torch.tensor(starts, dtype=torch.int32).to(device))
 
 
+class PagePool:
+    """The pages of one or more caches, handed to sequences and taken back on the GPU.
+
+    ``uses`` int32 [pages] says how many tables name each page; a page with 0 (or less) is
+    free.  ``extend`` and ``release`` keep it, and the table, lengths and starts of a
+    ``PagedBatch``, so a serving loop whose sequences grow needs no number from the GPU,
+    and its step can be captured whole::
+
+        slots, positions = pool.extend(batch, new, rows)
+        cache.append(k, v, batch)                  # of every layer
+        y = cache.attend(q, batch, ...)
+        pool.release(batch, window=2048, sinks=4)  # what the window has left
+
+    Calls on one pool or batch belong on one stream, or in order.  A program that lets a
+    sequence begin with pages of another adds one to their ``uses`` (and new rows must not
+    fall into them, so whole pages are shared)."""
+
+    def __init__(self, pages: int, page_size: int, device="cuda"):
+        if pages < 0:
+            raise RuntimeError("a pool has no negative number of pages")
+        self._describe(torch.zeros(pages, dtype=torch.int32, device=device), page_size)
+
+    @classmethod
+    def from_uses(cls, uses: Tensor, page_size: int) -> "PagePool":
+        """A pool over a tensor that is there already."""
+        self = cls.__new__(cls)
+        self._describe(uses, page_size)
+        return self
+
+    def _describe(self, uses: Tensor, page_size: int) -> None:
+        if uses.dtype != torch.int32 or uses.ndim != 1 or not uses.is_contiguous() or \
+                uses.data_ptr() % 16:
+            raise RuntimeError("uses must be a contiguous int32 tensor [pages], 16-byte aligned")
+        if page_size < 1 or page_size % PAGE_BLOCK:
+            raise RuntimeError(f"a page is a multiple of {PAGE_BLOCK} positions")
+        self._uses, self.page_size, self.device = uses, page_size, uses.device
+        self._struct = _abi.PagedPoolStruct(uses.data_ptr(), uses.shape[0], page_size)
+        self._at = ctypes.addressof(self._struct)
+
+    # (as PagedBatch)
+    def __reduce__(self):
+        return type(self).from_uses, (self._uses, self.page_size)
+
+    # The calls hand its address over.
+    uses = property(lambda self: self._uses)
+
+    def _numbers(self, x: Tensor, batch: PagedBatch, what: str) -> int:
+        if x.dtype != torch.int32 or x.device != self.device or not x.is_contiguous() or \
+                x.shape != batch.lengths.shape:
+            raise RuntimeError(f"{what} must be a contiguous int32 tensor [b] on the pool's device")
+        return x.data_ptr()
+
+    def _batch(self, batch: PagedBatch, what: str) -> int:
+        if self.device.type != "cuda":
+            raise RuntimeError(f"{what} requires a ROCm (cuda) pool, got {self.device}")
+        if batch.table.device != self.device:
+            raise RuntimeError("the batch must be on the pool's device")
+        return batch._at
+
+    def extend(self, batch: PagedBatch, new: Tensor, rows: int) -> tuple[Tensor, Tensor]:
+        """Gives each sequence ``new`` [b] (int32, below 0: none) more positions and the
+        pages for them, in place: ``batch.lengths`` grow, ``batch.starts`` are this step's
+        rows, ``batch.table`` names the pages, of which ``uses`` become 1.
+
+        The sequences are served in order, each with all of its rows or none: it gets them
+        iff its table has room, the new rows up to it come to no more than ``rows`` (what
+        the step's operands hold), and it needs no page or the pages needed up to it come
+        to no more than are free (what does not fit its own table asks for nothing; what is
+        refused otherwise still counts, so that nobody is overtaken).  A sequence that is
+        refused stays as it is, without new rows.  The lowest free pages go first.
+
+        Returns ``slots`` int64 [rows], each new row's place in the pool (page *
+        page_size + position in it), and ``positions`` int32 [rows]; both -1 past the last
+        row, and a slot -1 where the table names no page of the pool."""
+        at = self._batch(batch, "HIP page pool")
+        fresh = self._numbers(new, batch, "new")
+        slots = torch.empty(rows, dtype=torch.int64, device=self.device)
+        positions = torch.empty(rows, dtype=torch.int32, device=self.device)
+        lib = _abi.load()
+        nbytes = lib.parrot_paged_extend_workspace_bytes(new.shape[0])
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        with _on(self.device):
+            _abi.check(lib.parrot_paged_extend(
+                self._at, at, fresh, rows, slots.data_ptr(), positions.data_ptr(), _abi.ptr(ws),
+                nbytes, _stream(self.device)), "parrot_paged_extend")
+        return slots, positions
+
+    def release(self, batch: PagedBatch, lengths: Tensor | None = None, *,
+                window: int | None = None, sinks: int = 0) -> None:
+        """Takes positions back, in place: each sequence keeps its first ``lengths`` [b]
+        (int32; 0 ends it, more than it has changes nothing; None: all of each), and pages
+        wholly past them lose a use and their entry in the table, which becomes -1.  With a
+        ``window`` so do the pages that no later position sees, all but those of the first
+        ``sinks`` positions.  ``batch.starts`` stay as they are."""
+        at = self._batch(batch, "HIP page pool")
+        to = None if lengths is None else self._numbers(lengths, batch, "lengths")
+        if window is not None and window < 1:
+            raise RuntimeError("window must be positive, or None")
+        if sinks < 0:
+            raise RuntimeError("sinks must not be negative")
+        window = 0 if window is None else min(window, 2 ** 31 - 1)
+        with _on(self.device):
+            _abi.check(_abi.load().parrot_paged_release(
+                self._at, at, to, window, min(sinks, 2 ** 31 - 1), _stream(self.device)),
+                "parrot_paged_release")
+
+
 class PagedKVCache:
     """Pages of keys and values of one layer.
 
