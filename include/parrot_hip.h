@@ -905,8 +905,10 @@ typedef struct parrot_paged_pool {
   int32_t page;
 } parrot_paged_pool;
 
-/* Bytes of workspace that parrot_paged_extend needs for a batch of that many sequences. */
-size_t parrot_paged_extend_workspace_bytes(int32_t batch);
+/* Bytes of workspace that parrot_paged_extend needs for a pool of that many pages and a
+ * batch of that many sequences and rows (0 where it needs none, or for sizes that it does
+ * not take). */
+size_t parrot_paged_extend_workspace_bytes(int64_t pages, int32_t batch, int32_t rows);
 
 /* Gives sequence i new_rows[i] new positions (below 0: none) and the pages for them: writes
  * lengths, starts and table of the batch (of device memory that may be written) and uses.
@@ -919,7 +921,7 @@ size_t parrot_paged_extend_workspace_bytes(int32_t batch);
  * slots [rows] and positions [rows]: of each new row the place in the pool, table[i, p /
  * page] * page + p % page, and its position p; -1 for rows past the last (slots too where a table names
  * no page).  Sequences' table columns past their lengths are taken to name no page of the
- * pool.  workspace 16-byte aligned.
+ * pool.  slots, positions and workspace 16-byte aligned.
  * New: parrot/model.py has contiguous caches of one length (model.py:772-788). */
 int parrot_paged_extend(const parrot_paged_pool* pool, const parrot_paged_batch* batch,
                         const int32_t* new_rows, int32_t rows, int64_t* slots,

@@ -169,7 +169,7 @@ SIGNATURES: dict[str, tuple] = {
                        _i32, _p, _p]),
     "parrot_paged_read_bf16": (
         ctypes.c_int, [_p, _p, _i32, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p]),
-    "parrot_paged_extend_workspace_bytes": (_sz, [_i32]),
+    "parrot_paged_extend_workspace_bytes": (_sz, [_i64, _i32, _i32]),
     "parrot_paged_extend": (ctypes.c_int, [_p, _p, _p, _i32, _p, _p, _p, _sz, _p]),
     "parrot_paged_release": (ctypes.c_int, [_p, _p, _p, _i32, _i32, _p]),
     "parrot_paged_attention_workspace_bytes": (_sz, [_p, _p, _i32, _i32, _i32, _i32]),

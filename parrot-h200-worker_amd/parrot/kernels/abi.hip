@@ -894,8 +894,11 @@ int check_pool(const parrot_paged_pool* p, const parrot_paged_batch* b) {
 
 }  // namespace
 
-size_t parrot_paged_extend_workspace_bytes(int32_t batch) {
-  return batch < 0 || batch > 65535 ? 0 : parrot::paged_extend_workspace_bytes(batch);
+size_t parrot_paged_extend_workspace_bytes(int64_t pages, int32_t batch, int32_t rows) {
+  if (pages < 0 || pages > (1 << 30) || batch < 0 || batch > 65535 || rows < 0 ||
+      rows > (1 << 30))
+    return 0;
+  return parrot::paged_extend_workspace_bytes(pages, batch, rows);
 }
 
 int parrot_paged_extend(const parrot_paged_pool* pool, const parrot_paged_batch* batch,
@@ -906,7 +909,8 @@ int parrot_paged_extend(const parrot_paged_pool* pool, const parrot_paged_batch*
   if (rows < 0 || rows > (1 << 30)) return PARROT_ERR_BAD_SHAPE;
   if ((batch->batch > 0 && !new_rows) || (rows > 0 && (!slots || !positions)))
     return PARROT_ERR_NULL_POINTER;
-  const size_t need = parrot::paged_extend_workspace_bytes(batch->batch);
+  if (!aligned16(slots) || !aligned16(positions)) return PARROT_ERR_ALIGNMENT;
+  const size_t need = parrot::paged_extend_workspace_bytes(pool->pages, batch->batch, rows);
   if (need > 0) {
     if (!workspace || workspace_bytes < need) return PARROT_ERR_WORKSPACE;
     if (!aligned16(workspace)) return PARROT_ERR_ALIGNMENT;

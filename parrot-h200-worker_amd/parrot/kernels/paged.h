@@ -235,7 +235,7 @@ hipError_t launch_paged_append(const PagedCache& cache, int type, int head_dim,
 hipError_t launch_paged_read(const PagedCache& cache, int type, int head_dim,
                              const PagedBatch& batch, int positions, uint16_t* k, uint16_t* v,
                              const int64_t* k_strides, const int64_t* v_strides, hipStream_t s);
-size_t paged_extend_workspace_bytes(int batch);
+size_t paged_extend_workspace_bytes(int64_t pages, int batch, int rows);
 hipError_t launch_paged_extend(const PagedPool& pool, const PagedBatch& batch, const int32_t* fresh,
                                int64_t* slots, int32_t* positions, void* workspace, hipStream_t s);
 hipError_t launch_paged_release(const PagedPool& pool, const PagedBatch& batch, const int32_t* to,

@@ -25,6 +25,8 @@ from torch import Tensor
 from . import _abi
 from .hip_moe import ATTENTION_HEAD_DIMS, _on, _require, _stream
 
+_current_device = torch._C._cuda_getDevice  # (torch.cuda.current_device() without its checks)
+
 PAGE_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2,
               torch.float4_e2m1fn_x2: 4}
 FOUR_BITS = torch.float4_e2m1fn_x2  # an element of such a tensor is two values
@@ -127,6 +129,9 @@ class PagePool:
         self._uses, self.page_size, self.device = uses, page_size, uses.device
         self._struct = _abi.PagedPoolStruct(uses.data_ptr(), uses.shape[0], page_size)
         self._at = ctypes.addressof(self._struct)
+        self._cuda = self.device.type == "cuda"
+        self._slot = torch.empty(0, dtype=torch.int64, device=self.device)
+        self._sizes: dict[tuple, int] = {}
 
     # (as PagedBatch)
     def __reduce__(self):
@@ -142,7 +147,7 @@ class PagePool:
         return x.data_ptr()
 
     def _batch(self, batch: PagedBatch, what: str) -> int:
-        if self.device.type != "cuda":
+        if not self._cuda:
             raise RuntimeError(f"{what} requires a ROCm (cuda) pool, got {self.device}")
         if batch.table.device != self.device:
             raise RuntimeError("the batch must be on the pool's device")
@@ -165,15 +170,17 @@ class PagePool:
         row, and a slot -1 where the table names no page of the pool."""
         at = self._batch(batch, "HIP page pool")
         fresh = self._numbers(new, batch, "new")
-        slots = torch.empty(rows, dtype=torch.int64, device=self.device)
-        positions = torch.empty(rows, dtype=torch.int32, device=self.device)
-        lib = _abi.load()
-        nbytes = lib.parrot_paged_extend_workspace_bytes(new.shape[0])
+        slots, positions = self._slot.new_empty(rows), new.new_empty(rows)
+        b = len(new)
+        nbytes = self._sizes.get((b, rows))
+        if nbytes is None:
+            if len(self._sizes) >= 256:
+                self._sizes.clear()
+            nbytes = self._sizes[b, rows] = _abi.load().parrot_paged_extend_workspace_bytes(
+                len(self._uses), b, rows)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
-        with _on(self.device):
-            _abi.check(lib.parrot_paged_extend(
-                self._at, at, fresh, rows, slots.data_ptr(), positions.data_ptr(), _abi.ptr(ws),
-                nbytes, _stream(self.device)), "parrot_paged_extend")
+        _run(self.device, "parrot_paged_extend", self._at, at, fresh, rows, slots.data_ptr(),
+             positions.data_ptr(), _abi.ptr(ws), nbytes)
         return slots, positions
 
     def release(self, batch: PagedBatch, lengths: Tensor | None = None, *,
@@ -190,10 +197,19 @@ class PagePool:
         if sinks < 0:
             raise RuntimeError("sinks must not be negative")
         window = 0 if window is None else min(window, 2 ** 31 - 1)
-        with _on(self.device):
-            _abi.check(_abi.load().parrot_paged_release(
-                self._at, at, to, window, min(sinks, 2 ** 31 - 1), _stream(self.device)),
-                "parrot_paged_release")
+        _run(self.device, "parrot_paged_release", self._at, at, to, window, min(sinks, 2 ** 31 - 1))
+
+
+def _run(device: torch.device, name: str, *args) -> None:
+    """A call of the library on the device's current stream."""
+    call = getattr(_abi.load(), name)
+    if device.index == _current_device():
+        status = call(*args, _stream(device))
+    else:
+        with _on(device):
+            status = call(*args, _stream(device))
+    if status:
+        _abi.check(status, name)
 
 
 class PagedKVCache:
@@ -277,6 +293,7 @@ class PagedKVCache:
         pages, kv_heads, blocks, width = self.key.shape
         self.page_size, self.kv_heads = blocks * PAGE_BLOCK, kv_heads
         self.dtype, self.device = self.key.dtype, self.key.device
+        self._cuda = self.device.type == "cuda"
         self.head_dim = width * (2 if self.dtype == FOUR_BITS else 1) // PAGE_BLOCK
         self._struct = _abi.PagedCacheStruct(
             self.key.data_ptr(), self.value.data_ptr(), _abi.ptr(self.key_exponent),
@@ -307,30 +324,32 @@ class PagedKVCache:
             raise RuntimeError("the batch must be on the cache's device")
         return batch._at
 
-    def _new_rows(self, x: Tensor, heads: int, what: str, step: int) -> Tensor:
-        _require(x, what)
-        if x.ndim != 3 or x.shape[1] != heads or x.shape[2] != self.head_dim or \
-                x.device != self.device:
+    def _new_rows(self, x: Tensor, heads: int, what: str, step: int):
+        """The rows as the kernels read them: tensor, address, row and head strides."""
+        shape = x.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or \
+                x.dtype != torch.bfloat16 or x.device != self.device or not self._cuda or \
+                torch.is_grad_enabled():
+            _require(x, what)
             raise RuntimeError(f"{what} takes rows [rows, {heads}, {self.head_dim}] on the "
                                "cache's device")
-        sr, sh, sd = x.stride()
-        if sd != 1 or sr % step or sh % step or x.data_ptr() % (2 * step):
+        row, head, one = x.stride()
+        at = x.data_ptr()
+        if one != 1 or row % step or head % step or at % (2 * step):
             x = x.clone(memory_format=torch.contiguous_format)
-        return x
+            (row, head, _), at = x.stride(), x.data_ptr()
+        return x, at, row, head
 
     def append(self, key: Tensor, value: Tensor, batch: PagedBatch) -> None:
         """Writes the new rows key and value [rows, kv_heads, head_dim] (bf16, any
         row and head strides) into their sequences' pages.  Other positions stay
         as they are.  A page that is written must belong to one sequence, once."""
-        key = self._new_rows(key, self.kv_heads, "HIP paged append", 4)
-        value = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
-        if key.shape != value.shape:
+        key, *k = self._new_rows(key, self.kv_heads, "HIP paged append", 4)
+        value, *v = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
+        rows = len(key)
+        if rows != len(value):
             raise RuntimeError("as many rows of values as of keys")
-        b, (kr, kh, _), (vr, vh, _) = self._batch(batch), key.stride(), value.stride()
-        with _on(self.device):
-            _abi.check(_abi.load().parrot_paged_append_bf16(
-                self._at, b, key.data_ptr(), kr, kh, value.data_ptr(), vr, vh, key.shape[0],
-                _stream(self.device)), "parrot_paged_append_bf16")
+        _run(self.device, "parrot_paged_append_bf16", self._at, self._batch(batch), *k, *v, rows)
 
     def append_rope(self, q: Tensor, key: Tensor, value: Tensor, batch: PagedBatch, cos: Tensor,
                     sin: Tensor) -> Tensor:
@@ -338,14 +357,15 @@ class PagedKVCache:
         pairs; fp32 tables [positions, head_dim / 2], past them by the last row), in
         the same launch.  Returns the query rows q [rows, heads, head_dim] rotated in
         the same way, a new tensor.  Rows of no sequence hold anything in it."""
-        key = self._new_rows(key, self.kv_heads, "HIP paged append", 4)
-        value = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
+        key, *k = self._new_rows(key, self.kv_heads, "HIP paged append", 4)
+        value, *v = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
         heads = q.shape[1] if q.ndim == 3 else 0
         if heads < 1 or heads % self.kv_heads:
             raise RuntimeError("HIP paged append takes query rows [rows, heads, head_dim] of a "
                                "multiple of the cache's kv heads")
-        q = self._new_rows(q, heads, "HIP paged append", 4)
-        if not key.shape[0] == value.shape[0] == q.shape[0]:
+        q, *query = self._new_rows(q, heads, "HIP paged append", 4)
+        rows = len(key)
+        if not rows == len(value) == len(q):
             raise RuntimeError("as many rows of queries and values as of keys")
         for x in (cos, sin):
             if x.dtype != torch.float32 or x.device != self.device or not x.is_contiguous() or \
@@ -353,13 +373,8 @@ class PagedKVCache:
                 raise RuntimeError("RoPE tables must be contiguous fp32 [positions, head_dim / 2] "
                                    "on the cache's device")
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        b = self._batch(batch)
-        (kr, kh, _), (vr, vh, _), (qr, qh, _) = key.stride(), value.stride(), q.stride()
-        with _on(self.device):
-            _abi.check(_abi.load().parrot_paged_append_rope_bf16(
-                self._at, b, key.data_ptr(), kr, kh, value.data_ptr(), vr, vh, key.shape[0],
-                cos.data_ptr(), sin.data_ptr(), cos.shape[0], q.data_ptr(), qr, qh, heads,
-                out.data_ptr(), _stream(self.device)), "parrot_paged_append_rope_bf16")
+        _run(self.device, "parrot_paged_append_rope_bf16", self._at, self._batch(batch), *k, *v, rows,
+             cos.data_ptr(), sin.data_ptr(), cos.shape[0], *query, heads, out.data_ptr())
         return out
 
     def read(self, batch: PagedBatch, positions: int,
@@ -370,13 +385,16 @@ class PagedKVCache:
         ``LocalKVCache.key[:, :, :positions]``; strides that are multiples of 4)."""
         if torch.is_grad_enabled():
             raise RuntimeError("HIP paged read is inference-only; disable gradients")
-        if self.device.type != "cuda":
+        if not self._cuda:
             raise RuntimeError(f"HIP paged read requires a ROCm (cuda) cache, got {self.device}")
         b = self._batch(batch)
         shape = (batch.table.shape[0], self.kv_heads, positions, self.head_dim)
         if out is None:
             key = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
             value = torch.empty_like(key)
+            strides = key.stride()[:3]
+            _run(self.device, "parrot_paged_read_bf16", self._at, b, positions, key.data_ptr(),
+                 *strides, value.data_ptr(), *strides)
         else:
             key, value = out
             for x in out:
@@ -386,10 +404,8 @@ class PagedKVCache:
                         x.data_ptr() % 8:
                     raise RuntimeError(f"out must be two bf16 tensors {list(shape)} on the cache's "
                                        "device, strides multiples of 4, no element in two places")
-        with _on(self.device):
-            _abi.check(_abi.load().parrot_paged_read_bf16(
-                self._at, b, positions, key.data_ptr(), *key.stride()[:3], value.data_ptr(),
-                *value.stride()[:3], _stream(self.device)), "parrot_paged_read_bf16")
+            _run(self.device, "parrot_paged_read_bf16", self._at, b, positions, key.data_ptr(),
+                 *key.stride()[:3], value.data_ptr(), *value.stride()[:3])
         return key, value
 
     def attend(self, q: Tensor, batch: PagedBatch, *, scale: float, window: int | None = None,
@@ -403,16 +419,16 @@ class PagedKVCache:
         layout of the output projection's input.  A row that sees no key is 0;
         rows of no sequence are left as they are in ``out`` (a contiguous tensor
         of that shape) and hold anything otherwise."""
-        heads = q.shape[1] if q.ndim == 3 else 0
+        rows, heads = q.shape[:2] if q.ndim == 3 else (0, 0)
         if heads < 1 or heads % self.kv_heads:
             raise RuntimeError("HIP paged attention takes rows [rows, heads, head_dim] of a "
                                "multiple of the cache's kv heads")
-        q = self._new_rows(q, heads, "HIP paged attention", 8)
+        q, *query = self._new_rows(q, heads, "HIP paged attention", 8)
         if window is not None and window < 1:
             raise RuntimeError("window must be positive, or None")
         if sinks < 0:
             raise RuntimeError("sinks must not be negative")
-        rows, device = q.shape[0], self.device
+        device = self.device
         b = self._batch(batch)
         if out is None:
             out = q.new_empty((rows, heads * self.head_dim))
@@ -425,10 +441,6 @@ class PagedKVCache:
         nbytes = self._workspace_bytes(*batch.table.shape, rows, heads, window, sinks)
         # a fresh one per call: calls on several streams share nothing
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        row, head, _ = q.stride()
-        with _on(device):
-            _abi.check(_abi.load().parrot_paged_attention_bf16(
-                self._at, b, q.data_ptr(), row, head, rows, heads, window, sinks, scale,
-                out.data_ptr(), _abi.ptr(ws), nbytes, _stream(device)),
-                "parrot_paged_attention_bf16")
+        _run(device, "parrot_paged_attention_bf16", self._at, b, *query, rows, heads, window, sinks,
+             scale, out.data_ptr(), _abi.ptr(ws), nbytes)
         return out

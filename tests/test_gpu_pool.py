@@ -78,6 +78,7 @@ class Both:
     (65, 9, 32, 700, 200, 40, 3), (65, 9, 32, 300, 200, 100, 4), (400, 20, 64, 9000, 1000, 7, 5),
     (1025, 3, 32, 3000, 64, 33, 6), (1025, 3, 32, 700, 40, 33, 7), (5000, 2, 32, 9000, 50, 20, 8),
     (5000, 2, 32, 1500, 10, 60, 9), (70, 130, 32, 5000, 2000, 2000, 10),
+    (6, 40, 32, 70001, 900, 300, 11), (40, 700, 64, 140000, 30000, 9000, 12),
 ])
 def test_extend_and_release(b, width, page, pages, most, new, seed):
     rng = random.Random(seed)

@@ -41,12 +41,16 @@ def test_arguments():
     assert extend(pool(), batch(), FAKE, rows=-1) == -2
     assert extend(pool(), batch(), FAKE, rows=(1 << 30) + 1) == -2
     assert release(pool(), batch()) == -2  # sinks below 0
+    assert extend(pool(), batch(), FAKE, slots=FAKE + 8) == -5
+    assert extend(pool(), batch(), FAKE, positions=FAKE + 4) == -5
     size = lib.parrot_paged_extend_workspace_bytes
-    assert size(0) == 0 and size(-1) == 0 and size(70000) == 0 and size(60000) > 0
-    many = batch(batch=60000)
-    assert extend(pool(), many, FAKE, ws=None, wsb=size(60000)) == -4
-    assert extend(pool(), many, FAKE, ws=FAKE, wsb=size(60000) - 1) == -4
-    assert extend(pool(), many, FAKE, ws=FAKE + 8, wsb=size(60000)) == -5
+    assert size(100, 0, 0) == 0 and size(100, -1, 5) == 0 and size(100, 70000, 5) == 0
+    assert size(-1, 5, 50000) == 0 and size(100, 5, -1) == 0 and size(100, 5, 50000) > 0
+    many, need = batch(batch=60000), size(100, 60000, 5)
+    assert need > 0
+    assert extend(pool(), many, FAKE, ws=None, wsb=need) == -4
+    assert extend(pool(), many, FAKE, ws=FAKE, wsb=need - 1) == -4
+    assert extend(pool(), many, FAKE, ws=FAKE + 8, wsb=need) == -5
 
 
 def test_pool_checks():
