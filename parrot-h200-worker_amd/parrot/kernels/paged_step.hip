@@ -186,11 +186,12 @@ __global__ __launch_bounds__(kWaves * kWave, D < 128 ? 3 : 2) void paged_step_ke
   for (int t = 0; t < T; ++t) st.o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (begin + wave < end) {
     WaveBlocks at(a, sequence, kvh, blocks, begin, end);
-    StepBlock<TYPE, D> b = {};
-    auto load = [&](const void* pages, const uint8_t* exponents, raw(&to)[T], uint32_t(&bytes)[2],
-                    auto key) {
-      if (b.at < 0) return;
-      const raw* from = static_cast<const raw*>(pages) + int64_t{b.at} * (kPagedBlock * D / 8);
+    constexpr int kAhead = TYPE == kPagedE2m1 ? 2 : 1;
+    StepBlock<TYPE, D> ahead[kAhead] = {};
+    auto load = [&](int at, const void* pages, const uint8_t* exponents, raw(&to)[T],
+                    uint32_t(&bytes)[2], auto key) {
+      if (at < 0) return;
+      const raw* from = static_cast<const raw*>(pages) + int64_t{at} * (kPagedBlock * D / 8);
       if constexpr (TYPE == kPagedE2m1) {
         load_words(from + T * lane, to);
       } else {
@@ -198,9 +199,9 @@ __global__ __launch_bounds__(kWaves * kWave, D < 128 ? 3 : 2) void paged_step_ke
         for (int u = 0; u < T; ++u) to[u] = from[kWave * u + lane];
       }
       if constexpr (TYPE == kPagedE2m1 && decltype(key)::value) {
-        e2m1_key_bytes<D>(exponents + int64_t{b.at} * D, col, bytes);
+        e2m1_key_bytes<D>(exponents + int64_t{at} * D, col, bytes);
       } else if constexpr (TYPE != kPagedBf16) {
-        const uint8_t* e = exponents + int64_t{b.at} * kPagedBlock;
+        const uint8_t* e = exponents + int64_t{at} * kPagedBlock;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           if constexpr (decltype(key)::value) bytes[n] = e[16 * n + col];
@@ -208,15 +209,19 @@ __global__ __launch_bounds__(kWaves * kWave, D < 128 ? 3 : 2) void paged_step_ke
         }
       }
     };
-    auto load_keys = [&] {
-      load(a.cache.key, a.cache.key_exponent, b.k, b.kbytes, std::true_type{});
+    auto load_keys = [&](StepBlock<TYPE, D>& b) {
+      load(b.at, a.cache.key, a.cache.key_exponent, b.k, b.kbytes, std::true_type{});
     };
-    auto load_values = [&] {
-      load(a.cache.value, a.cache.value_exponent, b.v, b.vbytes, std::false_type{});
+    auto load_values = [&](StepBlock<TYPE, D>& b) {
+      load(b.at, a.cache.value, a.cache.value_exponent, b.v, b.vbytes, std::false_type{});
     };
-    b.at = at.find(begin + wave);
-    load_keys();
-    load_values();
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (begin + wave + u * kWaves >= end) break;
+      ahead[u].at = at.find(begin + wave + u * kWaves);
+      load_keys(ahead[u]);
+      load_values(ahead[u]);
+    }
     bf16x8 qf[S];
     {
       const uint16_t* row = a.q + mine.token * a.qs[0] + mine.head * a.qs[1] + 8 * g;
@@ -230,17 +235,23 @@ __global__ __launch_bounds__(kWaves * kWave, D < 128 ? 3 : 2) void paged_step_ke
         qf[u] = __builtin_bit_cast(bf16x8, v);
       }
     }
-    for (int i = begin + wave; i < end; i += kWaves) {
-      const bool more = i + kWaves < end;
-      // (of a block without a page no row sees a key)
-      step_block<TYPE, D>(st, b, qf, blocks.at(i) * kPagedBlock, mine.position, first, last,
-                          b.at >= 0 ? s.stored : 0, a,
-                          reinterpret_cast<uint16_t*>(&o_s[wave][0][0]), [&] {
-                            if (!more) return;
-                            b.at = at.find(i + kWaves);
-                            load_keys();
-                          });
-      if (more) load_values();
+    for (int i0 = begin + wave; i0 < end; i0 += kAhead * kWaves) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * kWaves;
+        if (i >= end) break;
+        StepBlock<TYPE, D>& b = ahead[u];
+        const bool more = i + kAhead * kWaves < end;
+        // (of a block without a page no row sees a key)
+        step_block<TYPE, D>(st, b, qf, blocks.at(i) * kPagedBlock, mine.position, first, last,
+                            b.at >= 0 ? s.stored : 0, a,
+                            reinterpret_cast<uint16_t*>(&o_s[wave][0][0]), [&] {
+                              if (!more) return;
+                              b.at = at.find(i + kAhead * kWaves);
+                              load_keys(b);
+                            });
+        if (more) load_values(b);
+      }
     }
   }
   float l = st.l + __shfl_xor(st.l, 16);
