@@ -182,19 +182,19 @@ __device__ __forceinline__ bool paged_find_last(const PagedBatch& b, int page, i
   return false;
 }
 
-// Four-bit keys: the powers' bytes of a lane's two positions, kbytes[n] those of
-// position 16 n + c in its lowest D / 32 bytes (what is above them is anything).
-// bytes: the block's.
+// Four-bit keys: the powers' bytes of positions c and 16 + c, D / 32 each, in memory's order
+// (what is above them is anything).  Words as they are loaded: whoever puts them together
+// here waits for them here.
 template <int D>
 __device__ __forceinline__ void e2m1_key_bytes(const uint8_t* bytes, int c, uint32_t (&to)[2]) {
   if constexpr (D == 64) {
     to[0] = *reinterpret_cast<const uint32_t*>(bytes + 4 * c);
-    to[1] = to[0] >> 16;
   } else if constexpr (D == 96) {
-    const uint16_t* const w = reinterpret_cast<const uint16_t*>(bytes + 6 * c);
-    const uint32_t x = w[0], y = w[1], z = w[2];
-    to[0] = x | (y << 16);
-    to[1] = (y >> 8) | (z << 8);
+    struct __attribute__((packed, aligned(2))) Word {
+      uint32_t w;
+    };
+    to[0] = reinterpret_cast<const Word*>(bytes + 6 * c)->w;
+    to[1] = *reinterpret_cast<const uint16_t*>(bytes + 6 * c + 4);
   } else {
     const uint2 w = *reinterpret_cast<const uint2*>(bytes + 8 * c);
     to[0] = w.x;
@@ -202,10 +202,11 @@ __device__ __forceinline__ void e2m1_key_bytes(const uint8_t* bytes, int c, uint
   }
 }
 
-// 2^(byte s of bytes - 127) as the conversions of 4-bit values take it: they read the
-// eight bits of the exponent (255: NaN) and no others.
-__device__ __forceinline__ float e2m1_power(uint32_t bytes, int s) {
-  return __uint_as_float(s < 3 ? bytes << (23 - 8 * s) : bytes >> 1);
+// 2^(byte i - 127) as the conversions of 4-bit values take it: they read the eight bits of
+// the exponent (255: NaN) and no others.
+__device__ __forceinline__ float e2m1_power(const uint32_t (&bytes)[2], int i) {
+  const uint32_t w = bytes[i / 4];
+  return __uint_as_float(i % 4 < 3 ? w << (23 - 8 * (i % 4)) : w >> 1);
 }
 
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));

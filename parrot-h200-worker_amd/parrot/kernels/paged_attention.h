@@ -246,25 +246,25 @@ __device__ __forceinline__ TileRow tile_row(const PagedSequence& s, int row, int
   return {s.length - s.count + token, s.first + token, kv_head * rep + (r - token * rep)};
 }
 
-// The four wavefronts' shares of a tile of R rows, each in the units of its own
+// The W wavefronts' shares of a tile of R rows, each in the units of its own
 // maximum, joined: to the output, or to the split's partial sums.
-template <int D, int R>
-__device__ __forceinline__ void merge_tile(const AttendArgs& a, const float (&o_s)[kWaves][R][D + 4],
-                                           const float (&ml_s)[kWaves][2][R],
+template <int D, int R, int W>
+__device__ __forceinline__ void merge_tile(const AttendArgs& a, const float (&o_s)[W][R][D + 4],
+                                           const float (&ml_s)[W][2][R],
                                            const PagedSequence& s, int row0, int rows, int kvh,
                                            int split, const Share& share) {
-  constexpr int kThreads = kWaves * kWave, kPieces = R * (D / 4);
+  constexpr int kThreads = W * kWave, kPieces = R * (D / 4);
 #pragma unroll
   for (int k = 0; k < (kPieces + kThreads - 1) / kThreads; ++k) {
     const int i = threadIdx.x + k * kThreads;
     const int r = min(i / (D / 4), R - 1), d = 4 * (i % (D / 4));
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml_s[w][0][r]);
+    for (int w = 0; w < W; ++w) m = fmaxf(m, ml_s[w][0][r]);
     float sum = 0.0f;
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float mw = ml_s[w][0][r], lw = ml_s[w][1][r];
       // A wavefront that saw nothing adds nothing (its maximum is -inf, its sum
       // 0; a NaN sum has to come through).
@@ -382,6 +382,8 @@ __device__ __forceinline__ void raise(State<D>& st, float mx, float scale_log2) 
 }
 
 hipError_t launch_step(const AttendArgs& a, int type, int head_dim, dim3 grid, hipStream_t s);
+hipError_t launch_step4(const AttendArgs& a, int head_dim, int tile, bool wide, dim3 grid,
+                        hipStream_t s);
 hipError_t launch_rows(const AttendArgs& a, int type, int head_dim, dim3 grid, hipStream_t s);
 hipError_t launch_tiles(const AttendArgs& a, int type, int head_dim, dim3 grid, hipStream_t s);
 

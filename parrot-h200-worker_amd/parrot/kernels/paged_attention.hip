@@ -172,12 +172,15 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   a.part = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part +
                                         static_cast<size_t>(splits) * batch.rows * heads * head_dim);
-  // ceil(n rep / tile) tiles a sequence
-  const int64_t tiles = static_cast<int64_t>(batch.rows) * a.rep / tile +
-                        std::min(batch.batch, batch.rows);
+  // ceil(n rep / tile) tiles a sequence of n rows, which is no more than one more than its
+  // rows fill and no more than those of each row alone
+  const int64_t tiles = std::min<int64_t>(
+      static_cast<int64_t>(batch.rows) * a.rep / tile + std::min(batch.batch, batch.rows),
+      static_cast<int64_t>(batch.rows) * ((a.rep + tile - 1) / tile));
   const dim3 grid(static_cast<uint32_t>(tiles), cache.kv_heads, splits);
   const dim3 tile_grid(static_cast<uint32_t>(tiles * cache.kv_heads), 1, splits);
-  const hipError_t e = tile == kStepRows ? launch_step(a, type, head_dim, grid, s)
+  const hipError_t e = tile < kStepRows    ? launch_step4(a, head_dim, tile, p.wide, grid, s)
+                       : tile == kStepRows ? launch_step(a, type, head_dim, grid, s)
                        : tile == kRows  ? launch_rows(a, type, head_dim, grid, s)
                                         : launch_tiles(a, type, head_dim, tile_grid, s);
   if (e != hipSuccess || splits == 1) return e;

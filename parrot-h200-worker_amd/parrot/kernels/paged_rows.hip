@@ -70,22 +70,21 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
     WaveBlocks at(a, sequence, kvh, blocks, begin, end);
     int block = -1;
     raw k[KU] = {}, v[2 * DT] = {};
-    uint32_t kbyte = 0, vbytes[4] = {0, 0, 0, 0};
+    uint32_t kbytes[TYPE == kPagedE2m1 ? DT : 1] = {}, vbytes[4] = {0, 0, 0, 0};
     auto load_keys = [&] {
       if (block < 0) return;
       if constexpr (TYPE == kPagedE2m1) {
         two_records<D>(a.cache.key, block, half * 16 + kc, kn, k);
         const uint8_t* e = a.cache.key_exponent + int64_t{block} * D + (2 * kc + kn) * DT;
-        kbyte = 0;
 #pragma unroll
-        for (int i = 0; i < DT; ++i) kbyte |= static_cast<uint32_t>(e[i]) << (8 * i);
+        for (int i = 0; i < DT; ++i) kbytes[i] = e[i];
       } else {
         const raw* from = static_cast<const raw*>(a.cache.key) +
                           int64_t{block} * (kPagedBlock * D / 8) + k_off;
 #pragma unroll
         for (int u = 0; u < KU; ++u) k[u] = from[32 * u];
         if constexpr (TYPE != kPagedBf16)
-          kbyte = a.cache.key_exponent[int64_t{block} * kPagedBlock + 16 * kn + kc];
+          kbytes[0] = a.cache.key_exponent[int64_t{block} * kPagedBlock + 16 * kn + kc];
       }
     };
     auto load_values = [&] {
@@ -131,12 +130,14 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
       f32x16 sc;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
-      const float power = TYPE == kPagedBf16 || TYPE == kPagedE2m1 ? 1.0f : piece_power<TYPE>(kbyte);
+      const float power = TYPE == kPagedBf16 || TYPE == kPagedE2m1
+                              ? 1.0f
+                              : piece_power<TYPE>(kbytes[0]);
 #pragma unroll
       for (int u = 0; u < KU; ++u)
         sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            piece_bf16<TYPE>(k[u], TYPE == kPagedE2m1 ? e2m1_power(kbyte, u / 2) : power), qf[u], sc,
-            0, 0, 0);
+            piece_bf16<TYPE>(k[u], TYPE == kPagedE2m1 ? __uint_as_float(kbytes[u / 2] << 23) : power),
+            qf[u], sc, 0, 0, 0);
       if (more) {
         block = at.find(i + kWaves);
         load_keys();

@@ -28,6 +28,7 @@ constexpr int kRows = 32;                  // rows of a wavefront's tile
 constexpr int kStepRows = 16;              // rows of a workgroup's tile, few per sequence
 constexpr int kTileRows = kWaves * kRows;  // ... many
 constexpr int kMaxSplits = 64;             // a lane each in the join
+constexpr int kWideWaves = 8;
 
 // (by value: with std::min's references the compiler orders the kernels otherwise, 115.6 us
 // for 114.9 for 4 prompts of 4096 in e4m3, 8 heads on 2 of 96)
@@ -87,6 +88,7 @@ PARROT_EXTENT Share split_share(const PagedSequence& s, int rows, int tile, int 
 
 struct Plan {
   int tile, splits, whole;
+  bool wide;  // workgroups of kWideWaves wavefronts (tiles of fewer than 16 rows)
 };
 
 // Tiles: of 16 rows where a sequence has no more than 32 on average (most of a larger
@@ -109,6 +111,15 @@ struct Plan {
 // least (384: 24.5 and, of 32 rows with a window, 12.8 for 12.7); for larger tiles about
 // 1024, which evens out the causal ones (2 prompts of 4096 92.5 us, of 768 102), each with
 // 384 keys (3 chunks of 512 rows after 3500 keys 32.2 us, of 256 keys 35.5, of 512 33.2).
+// Of 4-bit pages: tiles of 8 rows where a sequence has no more than 8 on average (two key
+// blocks a step, paged_step4.hip), and wide workgroups, with four blocks a step for up to 4
+// rows, where one of them is as fast as the split and its join (us, 8 heads on 2 of 96, wide /
+// split: 1 sequence of 1536 keys 9.1 / 9.4, 3072 11.8 / 9.7; 16 of 2048 10.8 / 10.8, 3072 12.9 /
+// 11.3; 32 of 2048 10.9 / 12.5, 4096 15.6 / 14.9; 64 of 4096 15.9 / 20.4, 8000 27.5 / 26.5; 128 of
+// 16000 76 / 82; 16 heads on 2 of 128: 4 of 1024 8.6 / 9.6, 2048 11.6 / 9.8, 32 of 2048 12.0 / 13.0).
+// One fills a CU, so from three quarters of the CUs on the question is how full their last
+// round is.  Short sequences leave most of its wavefronts nothing (512 of 129 keys 22.4 us,
+// by four wavefronts 12.1).
 inline Plan plan(int type, int batch, int rows, int heads, int kv_heads, int page, int width,
                  int window, int sinks) {
   const int rep = heads / kv_heads;
@@ -121,19 +132,30 @@ inline Plan plan(int type, int batch, int rows, int heads, int kv_heads, int pag
   const int64_t all = static_cast<int64_t>(rows) * rep, n = std::max(std::min(batch, rows), 1);
   const int64_t work = n * ((all + n * kRows - 1) / (n * kRows)) * kv_heads *
                        ((keys_of(kRows) + kPagedBlock - 1) / kPagedBlock);
-  const int tile = all <= 2 * kStepRows * n                          ? kStepRows
+  const bool few = type == kPagedE2m1 && all <= kStepRows / 2 * n;
+  if (few) {
+    const bool fewer = all <= kStepRows / 4 * n;
+    const int tile = fewer ? kStepRows / 4 : kStepRows / 2;
+    const int64_t keys = keys_of(tile), tiles = std::max<int64_t>((all + tile - 1) / tile, n);
+    const int64_t units = tiles * kv_heads, rounds = (units + 255) / 256;
+    const int64_t most = (fewer ? 2176 : 1152) + 16 * units;
+    if (keys > 768 && units < 768 && (units < 192 ? keys <= most : 4 * units >= 768 * rounds))
+      return {tile, 1, static_cast<int>(keys / kPagedBlock + 1), true};
+  }
+  const int tile = few                                               ? kStepRows / 2
+                   : all <= 2 * kStepRows * n                        ? kStepRows
                    : work <= (type == kPagedBf16 ? 4096 : 8192) ? kRows
                                                                      : kTileRows;
   const int64_t keys = keys_of(tile);
   const int64_t tiles = (static_cast<int64_t>(rows) * rep + tile - 1) / tile;
   const int64_t units = std::max<int64_t>({tiles, std::min(batch, rows), 1}) * kv_heads;
   const int64_t line = tile == kTileRows ? std::min<int64_t>(384 + 4 * units, 1024) : 768;
-  const bool step = tile == kStepRows;
+  const bool step = tile <= kStepRows;
   const int64_t want = step ? std::max<int64_t>(768 / units, 1) : (1024 + units - 1) / units;
   const int64_t least = step ? 256 : 384;
   const int64_t splits =
       keys <= line ? 1 : std::min<int64_t>({want, (keys + least - 1) / least, kMaxSplits});
-  return {tile, static_cast<int>(splits), static_cast<int>(line / kPagedBlock)};
+  return {tile, static_cast<int>(splits), static_cast<int>(line / kPagedBlock), false};
 }
 
 }  // namespace paged

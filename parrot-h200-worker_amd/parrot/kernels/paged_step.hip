@@ -28,7 +28,7 @@ struct StepBlock {
   using raw = typename Piece<TYPE>::raw;
   static constexpr int N = D / 16;  // pieces of K, and of V, per lane
   raw k[N], v[N];
-  uint32_t kbytes[2], vbytes[2];  // exponents of the lane's key rows (e2m1: S each); of its 8 scores
+  uint32_t kbytes[2], vbytes[2];  // exponents of the lane's key rows (e2m1: 2 S bytes); of its 8 scores
   int at;                         // which block of the cache; -1: none
 };
 
@@ -58,7 +58,7 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
 #pragma unroll
     for (int s = 0; s < S; ++s)
       sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-          piece_bf16<TYPE>(b.k[n * S + s], TYPE == kPagedE2m1 ? e2m1_power(b.kbytes[n], s) : power),
+          piece_bf16<TYPE>(b.k[n * S + s], TYPE == kPagedE2m1 ? e2m1_power(b.kbytes, n * S + s) : power),
           qf[s], sc[n], 0, 0, 0);
   }
   then();

@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
 #pragma unroll
           for (int w = 0; w < D / 16; ++w)
             *reinterpret_cast<bf16x8*>(to + (kWave * w + lane) * 8 + (w >= S ? kHalf : 0)) =
-                piece_bf16<TYPE>(record[w], e2m1_power(bytes[w / S], w % S));
+                piece_bf16<TYPE>(record[w], e2m1_power(bytes, w));
         } else {
 #pragma unroll
           for (int u = 0; u < kLoads; ++u) {
