@@ -25,7 +25,10 @@ from torch import Tensor
 from . import _abi
 from .hip_moe import ATTENTION_HEAD_DIMS, _on, _require, _stream
 
-_current_device = torch._C._cuda_getDevice  # (torch.cuda.current_device() without its checks)
+# (torch.cuda.current_device() and current_stream().cuda_stream without their checks)
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_grads = torch.is_grad_enabled
 
 PAGE_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2,
               torch.float4_e2m1fn_x2: 4}
@@ -66,6 +69,8 @@ class PagedBatch:
         object.__setattr__(self, "_struct", _abi.PagedBatchStruct(
             self.table.data_ptr(), self.lengths.data_ptr(), self.starts.data_ptr(), b, width))
         object.__setattr__(self, "_at", ctypes.addressof(self._struct))
+        object.__setattr__(self, "_device", self.table.device)
+        object.__setattr__(self, "_sizes", (b, width))
 
     # (copies and pickles are of the tensors, not of their addresses)
     def __reduce__(self):
@@ -89,6 +94,18 @@ class PagedBatch:
                              dtype=torch.int32).view(len(pages), width)
         return cls(table.to(device), torch.tensor(lengths, dtype=torch.int32).to(device),
                    torch.tensor(starts, dtype=torch.int32).to(device))
+
+
+def _run(name: str, device: torch.device, *args) -> None:
+    """A call of the library on the device's current stream."""
+    call, index = getattr(_abi.load(), name), device.index
+    if index == _current_device():
+        status = call(*args, _raw_stream(index))
+    else:
+        with _on(device):
+            status = call(*args, _raw_stream(index))
+    if status:
+        _abi.check(status, name)
 
 
 class PagePool:
@@ -142,14 +159,14 @@ class PagePool:
 
     def _numbers(self, x: Tensor, batch: PagedBatch, what: str) -> int:
         if x.dtype != torch.int32 or x.device != self.device or not x.is_contiguous() or \
-                x.shape != batch.lengths.shape:
+                x.shape != batch._sizes[:1]:
             raise RuntimeError(f"{what} must be a contiguous int32 tensor [b] on the pool's device")
         return x.data_ptr()
 
     def _batch(self, batch: PagedBatch, what: str) -> int:
         if not self._cuda:
             raise RuntimeError(f"{what} requires a ROCm (cuda) pool, got {self.device}")
-        if batch.table.device != self.device:
+        if batch._device != self.device:
             raise RuntimeError("the batch must be on the pool's device")
         return batch._at
 
@@ -171,16 +188,16 @@ class PagePool:
         at = self._batch(batch, "HIP page pool")
         fresh = self._numbers(new, batch, "new")
         slots, positions = self._slot.new_empty(rows), new.new_empty(rows)
-        b = len(new)
+        b = batch._sizes[0]
         nbytes = self._sizes.get((b, rows))
         if nbytes is None:
             if len(self._sizes) >= 256:
                 self._sizes.clear()
             nbytes = self._sizes[b, rows] = _abi.load().parrot_paged_extend_workspace_bytes(
-                len(self._uses), b, rows)
+                self._uses.shape[0], b, rows)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
-        _run(self.device, "parrot_paged_extend", self._at, at, fresh, rows, slots.data_ptr(),
-             positions.data_ptr(), _abi.ptr(ws), nbytes)
+        _run("parrot_paged_extend", self.device, self._at, at, fresh, rows, slots.data_ptr(),
+             positions.data_ptr(), ws.data_ptr() if nbytes else None, nbytes)
         return slots, positions
 
     def release(self, batch: PagedBatch, lengths: Tensor | None = None, *,
@@ -197,19 +214,7 @@ class PagePool:
         if sinks < 0:
             raise RuntimeError("sinks must not be negative")
         window = 0 if window is None else min(window, 2 ** 31 - 1)
-        _run(self.device, "parrot_paged_release", self._at, at, to, window, min(sinks, 2 ** 31 - 1))
-
-
-def _run(device: torch.device, name: str, *args) -> None:
-    """A call of the library on the device's current stream."""
-    call = getattr(_abi.load(), name)
-    if device.index == _current_device():
-        status = call(*args, _stream(device))
-    else:
-        with _on(device):
-            status = call(*args, _stream(device))
-    if status:
-        _abi.check(status, name)
+        _run("parrot_paged_release", self.device, self._at, at, to, window, min(sinks, 2 ** 31 - 1))
 
 
 class PagedKVCache:
@@ -294,6 +299,7 @@ class PagedKVCache:
         self.page_size, self.kv_heads = blocks * PAGE_BLOCK, kv_heads
         self.dtype, self.device = self.key.dtype, self.key.device
         self._cuda = self.device.type == "cuda"
+        self._row = torch.empty(0, dtype=torch.bfloat16, device=self.device)
         self.head_dim = width * (2 if self.dtype == FOUR_BITS else 1) // PAGE_BLOCK
         self._struct = _abi.PagedCacheStruct(
             self.key.data_ptr(), self.value.data_ptr(), _abi.ptr(self.key_exponent),
@@ -320,16 +326,16 @@ class PagedKVCache:
         return nbytes
 
     def _batch(self, batch: PagedBatch) -> int:
-        if batch.table.device != self.device:
+        if batch._device != self.device:
             raise RuntimeError("the batch must be on the cache's device")
         return batch._at
 
     def _new_rows(self, x: Tensor, heads: int, what: str, step: int):
-        """The rows as the kernels read them: tensor, address, row and head strides."""
+        """The rows as the kernels read them: their number, the tensor, its address, row and
+        head strides."""
         shape = x.shape
         if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or \
-                x.dtype != torch.bfloat16 or x.device != self.device or not self._cuda or \
-                torch.is_grad_enabled():
+                x.dtype != torch.bfloat16 or x.device != self.device or not self._cuda or _grads():
             _require(x, what)
             raise RuntimeError(f"{what} takes rows [rows, {heads}, {self.head_dim}] on the "
                                "cache's device")
@@ -338,18 +344,18 @@ class PagedKVCache:
         if one != 1 or row % step or head % step or at % (2 * step):
             x = x.clone(memory_format=torch.contiguous_format)
             (row, head, _), at = x.stride(), x.data_ptr()
-        return x, at, row, head
+        return shape[0], x, at, row, head
 
     def append(self, key: Tensor, value: Tensor, batch: PagedBatch) -> None:
         """Writes the new rows key and value [rows, kv_heads, head_dim] (bf16, any
         row and head strides) into their sequences' pages.  Other positions stay
         as they are.  A page that is written must belong to one sequence, once."""
-        key, *k = self._new_rows(key, self.kv_heads, "HIP paged append", 4)
-        value, *v = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
-        rows = len(key)
-        if rows != len(value):
+        rows, key, k, kr, kh = self._new_rows(key, self.kv_heads, "HIP paged append", 4)
+        values, value, v, vr, vh = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
+        if rows != values:
             raise RuntimeError("as many rows of values as of keys")
-        _run(self.device, "parrot_paged_append_bf16", self._at, self._batch(batch), *k, *v, rows)
+        _run("parrot_paged_append_bf16", self.device, self._at, self._batch(batch), k, kr, kh, v, vr,
+             vh, rows)
 
     def append_rope(self, q: Tensor, key: Tensor, value: Tensor, batch: PagedBatch, cos: Tensor,
                     sin: Tensor) -> Tensor:
@@ -357,15 +363,14 @@ class PagedKVCache:
         pairs; fp32 tables [positions, head_dim / 2], past them by the last row), in
         the same launch.  Returns the query rows q [rows, heads, head_dim] rotated in
         the same way, a new tensor.  Rows of no sequence hold anything in it."""
-        key, *k = self._new_rows(key, self.kv_heads, "HIP paged append", 4)
-        value, *v = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
+        rows, key, *k = self._new_rows(key, self.kv_heads, "HIP paged append", 4)
+        values, value, *v = self._new_rows(value, self.kv_heads, "HIP paged append", 4)
         heads = q.shape[1] if q.ndim == 3 else 0
         if heads < 1 or heads % self.kv_heads:
             raise RuntimeError("HIP paged append takes query rows [rows, heads, head_dim] of a "
                                "multiple of the cache's kv heads")
-        q, *query = self._new_rows(q, heads, "HIP paged append", 4)
-        rows = len(key)
-        if not rows == len(value) == len(q):
+        queries, q, *query = self._new_rows(q, heads, "HIP paged append", 4)
+        if not rows == values == queries:
             raise RuntimeError("as many rows of queries and values as of keys")
         for x in (cos, sin):
             if x.dtype != torch.float32 or x.device != self.device or not x.is_contiguous() or \
@@ -373,7 +378,7 @@ class PagedKVCache:
                 raise RuntimeError("RoPE tables must be contiguous fp32 [positions, head_dim / 2] "
                                    "on the cache's device")
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _run(self.device, "parrot_paged_append_rope_bf16", self._at, self._batch(batch), *k, *v, rows,
+        _run("parrot_paged_append_rope_bf16", self.device, self._at, self._batch(batch), *k, *v, rows,
              cos.data_ptr(), sin.data_ptr(), cos.shape[0], *query, heads, out.data_ptr())
         return out
 
@@ -383,18 +388,19 @@ class PagedKVCache:
         [b, kv_heads, positions, head_dim], zero from a sequence's length on and
         where it has no page.  ``out``: the two tensors to write them into (such as
         ``LocalKVCache.key[:, :, :positions]``; strides that are multiples of 4)."""
-        if torch.is_grad_enabled():
+        if _grads():
             raise RuntimeError("HIP paged read is inference-only; disable gradients")
         if not self._cuda:
             raise RuntimeError(f"HIP paged read requires a ROCm (cuda) cache, got {self.device}")
         b = self._batch(batch)
-        shape = (batch.table.shape[0], self.kv_heads, positions, self.head_dim)
+        heads, d = self.kv_heads, self.head_dim
+        shape = (batch._sizes[0], heads, positions, d)
         if out is None:
-            key = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            key = self._row.new_empty(shape)
             value = torch.empty_like(key)
-            strides = key.stride()[:3]
-            _run(self.device, "parrot_paged_read_bf16", self._at, b, positions, key.data_ptr(),
-                 *strides, value.data_ptr(), *strides)
+            step = positions * d
+            _run("parrot_paged_read_bf16", self.device, self._at, b, positions, key.data_ptr(),
+                 heads * step, step, d, value.data_ptr(), heads * step, step, d)
         else:
             key, value = out
             for x in out:
@@ -404,7 +410,7 @@ class PagedKVCache:
                         x.data_ptr() % 8:
                     raise RuntimeError(f"out must be two bf16 tensors {list(shape)} on the cache's "
                                        "device, strides multiples of 4, no element in two places")
-            _run(self.device, "parrot_paged_read_bf16", self._at, b, positions, key.data_ptr(),
+            _run("parrot_paged_read_bf16", self.device, self._at, b, positions, key.data_ptr(),
                  *key.stride()[:3], value.data_ptr(), *value.stride()[:3])
         return key, value
 
@@ -419,11 +425,12 @@ class PagedKVCache:
         layout of the output projection's input.  A row that sees no key is 0;
         rows of no sequence are left as they are in ``out`` (a contiguous tensor
         of that shape) and hold anything otherwise."""
-        rows, heads = q.shape[:2] if q.ndim == 3 else (0, 0)
+        shape = q.shape
+        heads = shape[1] if len(shape) == 3 else 0
         if heads < 1 or heads % self.kv_heads:
             raise RuntimeError("HIP paged attention takes rows [rows, heads, head_dim] of a "
                                "multiple of the cache's kv heads")
-        q, *query = self._new_rows(q, heads, "HIP paged attention", 8)
+        rows, q, query, row, head = self._new_rows(q, heads, "HIP paged attention", 8)
         if window is not None and window < 1:
             raise RuntimeError("window must be positive, or None")
         if sinks < 0:
@@ -438,9 +445,10 @@ class PagedKVCache:
                                f"{heads * self.head_dim}] on the cache's device")
         window = 0 if window is None else min(window, 2 ** 31 - 1)
         sinks = min(sinks, 2 ** 31 - 1)
-        nbytes = self._workspace_bytes(*batch.table.shape, rows, heads, window, sinks)
+        nbytes = self._workspace_bytes(*batch._sizes, rows, heads, window, sinks)
         # a fresh one per call: calls on several streams share nothing
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        _run(device, "parrot_paged_attention_bf16", self._at, b, *query, rows, heads, window, sinks,
-             scale, out.data_ptr(), _abi.ptr(ws), nbytes)
+        # (of bf16: two bytes an element)
+        ws = self._row.new_empty((nbytes + 1) // 2) if nbytes else None
+        _run("parrot_paged_attention_bf16", device, self._at, b, query, row, head, rows, heads,
+             window, sinks, scale, out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes)
         return out
