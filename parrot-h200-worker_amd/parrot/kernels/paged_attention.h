@@ -299,11 +299,9 @@ __device__ __forceinline__ int tile_key(int k0, int e) {
          4 * (2 * (e >> 3) + (static_cast<int>(threadIdx.x & (kWave - 1)) >> 5)) + (e & 3);
 }
 
-// Scores that the lane's row does not see become -infinity.  True where the block
-// holds a value that is not finite.
-template <int D>
-__device__ __forceinline__ bool mask_block(f32x16& sc, const bf16x8 (&vf)[D / 16], int k0,
-                                           int query, int stored, const AttendArgs& a) {
+// Scores that the lane's row does not see become -infinity.
+__device__ __forceinline__ void mask_scores(f32x16& sc, int k0, int query, int stored,
+                                            const AttendArgs& a) {
   const Visible sees = visible_to(query, stored, a.window, a.sinks);
   if (k0 < a.sinks) {
 #pragma unroll
@@ -312,6 +310,13 @@ __device__ __forceinline__ bool mask_block(f32x16& sc, const bf16x8 (&vf)[D / 16
 #pragma unroll
     for (int e = 0; e < 16; ++e) sc[e] = sees.window(tile_key(k0, e)) ? sc[e] : -INFINITY;
   }
+}
+
+// ... and true where the block holds a value that is not finite.
+template <int D>
+__device__ __forceinline__ bool mask_block(f32x16& sc, const bf16x8 (&vf)[D / 16], int k0,
+                                           int query, int stored, const AttendArgs& a) {
+  mask_scores(sc, k0, query, stored, a);
   return __ballot(has_nonfinite(vf)) != 0;
 }
 

@@ -33,6 +33,25 @@ __device__ __forceinline__ void two_records(const void* pages, int block, int re
   }
 }
 
+// The bytes of a 4-bit key's N groups, as words that are used as they come (e2m1_key_bytes).
+template <int N>
+__device__ __forceinline__ void load_row_bytes(const uint8_t* from, uint32_t (&to)[2]) {
+  if constexpr (N == 4) {
+    to[0] = *reinterpret_cast<const uint32_t*>(from);
+  } else {
+    struct __attribute__((packed, aligned(1))) Two {
+      uint16_t w;
+    };
+    to[0] = reinterpret_cast<const Two*>(from)->w;
+    if constexpr (N == 3) to[1] = from[2];
+  }
+}
+
+template <int N>
+__device__ __forceinline__ float row_power(const uint32_t (&bytes)[2], int i) {
+  return e2m1_power(bytes, N == 3 && i == 2 ? 4 : i);
+}
+
 template <int TYPE, int D>
 __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArgs a) {
   constexpr int KU = D / 16, DT = D / 32;
@@ -70,14 +89,12 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
     WaveBlocks at(a, sequence, kvh, blocks, begin, end);
     int block = -1;
     raw k[KU] = {}, v[2 * DT] = {};
-    uint32_t kbytes[TYPE == kPagedE2m1 ? DT : 1] = {}, vbytes[4] = {0, 0, 0, 0};
+    uint32_t kbytes[2] = {0, 0}, vbytes[4] = {0, 0, 0, 0};
     auto load_keys = [&] {
       if (block < 0) return;
       if constexpr (TYPE == kPagedE2m1) {
         two_records<D>(a.cache.key, block, half * 16 + kc, kn, k);
-        const uint8_t* e = a.cache.key_exponent + int64_t{block} * D + (2 * kc + kn) * DT;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) kbytes[i] = e[i];
+        load_row_bytes<DT>(a.cache.key_exponent + int64_t{block} * D + (2 * kc + kn) * DT, kbytes);
       } else {
         const raw* from = static_cast<const raw*>(a.cache.key) +
                           int64_t{block} * (kPagedBlock * D / 8) + k_off;
@@ -136,8 +153,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
 #pragma unroll
       for (int u = 0; u < KU; ++u)
         sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            piece_bf16<TYPE>(k[u], TYPE == kPagedE2m1 ? __uint_as_float(kbytes[u / 2] << 23) : power),
-            qf[u], sc, 0, 0, 0);
+            piece_bf16<TYPE>(k[u], TYPE == kPagedE2m1 ? row_power<DT>(kbytes, u / 2) : power), qf[u],
+            sc, 0, 0, 0);
       if (more) {
         block = at.find(i + kWaves);
         load_keys();
@@ -153,8 +170,15 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
                          (last - k0 < a.window || k0 + 31 < a.sinks);
       // Values that some row must not see: times a probability of 0 an infinity or a
       // NaN is not 0.  They are left out and added to the rows that see them.
+      // (4-bit values are finite themselves: a power of 0 is enough)
       bool odd = false;
-      if (!whole) {
+      if (TYPE == kPagedE2m1 && !whole) {
+        mask_scores(sc, k0, mine.position, stored, a);
+        const Visible sees = visible_to(mine.position, stored, a.window, a.sinks);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!sees(tile_key(k0, e))) bytes[e >> 2] &= ~(0xffu << (8 * (e & 3)));
+      } else if (!whole) {
         odd = mask_block<D>(sc, vf, k0, mine.position, stored, a);
         if constexpr (TYPE != kPagedBf16) {
           bool bad = false;
@@ -166,7 +190,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
           if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              if (byte_of(e) == kPagedNotFinite) {  // (such a row of int8 or e2m1 holds zeros)
+              if (byte_of(e) == kPagedNotFinite) {  // (such an int8 row holds zeros)
                 bytes[e >> 2] &= ~(0xffu << (8 * (e & 3)));
 #pragma unroll
                 for (int t = 0; t < DT; ++t)

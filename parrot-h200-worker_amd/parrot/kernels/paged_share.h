@@ -119,7 +119,10 @@ struct Plan {
 // 16000 76 / 82; 16 heads on 2 of 128: 4 of 1024 8.6 / 9.6, 2048 11.6 / 9.8, 32 of 2048 12.0 / 13.0).
 // One fills a CU, so from three quarters of the CUs on the question is how full their last
 // round is.  Short sequences leave most of its wavefronts nothing (512 of 129 keys 22.4 us,
-// by four wavefronts 12.1).
+// by four wavefronts 12.1).  Tiles of 16 rows up to 96 on average: their registers are two
+// blocks ahead, and the third conversion of what two larger tiles convert twice costs less
+// than the rows that those leave empty (5 sequences of 9000 keys, 48 rows, 16 heads on 2 of 128
+// 18.3 / 22.8 in tiles of 32; 5 x 96 rows 21.1 / 23.8, of 128; 2 x 128 rows after 4000 15.0 / 13.3).
 inline Plan plan(int type, int batch, int rows, int heads, int kv_heads, int page, int width,
                  int window, int sinks) {
   const int rep = heads / kv_heads;
@@ -142,8 +145,8 @@ inline Plan plan(int type, int batch, int rows, int heads, int kv_heads, int pag
     if (keys > 768 && units < 768 && (units < 192 ? keys <= most : 4 * units >= 768 * rounds))
       return {tile, 1, static_cast<int>(keys / kPagedBlock + 1), true};
   }
-  const int tile = few                                               ? kStepRows / 2
-                   : all <= 2 * kStepRows * n                        ? kStepRows
+  const int tile = few                                                   ? kStepRows / 2
+                   : all <= (type == kPagedE2m1 ? 6 : 2) * kStepRows * n ? kStepRows
                    : work <= (type == kPagedBf16 ? 4096 : 8192) ? kRows
                                                                      : kTileRows;
   const int64_t keys = keys_of(tile);

@@ -101,9 +101,15 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
   auto byte_of = [&](int e) { return (bytes[e >> 2] >> (8 * (e & 3))) & 0xffu; };
   // Values that some row must not see: times a probability of 0 an infinity or a NaN
   // is not 0.  They are left out and added to the rows that see them.
+  // (4-bit values are finite themselves: a power of 0 is enough)
   bool odd = false;
-  if (!whole) {
-    bool mine = TYPE != kPagedE2m1 && has_nonfinite(vf);
+  if (TYPE == kPagedE2m1 && !whole) {
+    const Visible sees = visible_to(query, stored, a.window, a.sinks);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (!sees(key_of(e))) bytes[e >> 2] &= ~(0xffu << (8 * (e & 3)));
+  } else if (!whole) {
+    bool mine = has_nonfinite(vf);
     if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) mine |= byte_of(e) == kPagedNotFinite;
@@ -113,7 +119,7 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
       if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (byte_of(e) == kPagedNotFinite) {  // (such a row of int8 or e2m1 holds zeros)
+          if (byte_of(e) == kPagedNotFinite) {  // (such an int8 row holds zeros)
             bytes[e >> 2] &= ~(0xffu << (8 * (e & 3)));
 #pragma unroll
             for (int t = 0; t < T; ++t) vf[t][e] = __builtin_bit_cast(__bf16, uint16_t{0x7fc0});
