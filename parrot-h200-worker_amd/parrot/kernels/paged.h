@@ -209,6 +209,25 @@ __device__ __forceinline__ float e2m1_power(const uint32_t (&bytes)[2], int i) {
   return __uint_as_float(i % 4 < 3 ? w << (23 - 8 * (i % 4)) : w >> 1);
 }
 
+// The bytes of a 4-bit key's N groups, as words that are used as they come (e2m1_key_bytes).
+template <int N>
+__device__ __forceinline__ void load_row_bytes(const uint8_t* from, uint32_t (&to)[2]) {
+  if constexpr (N == 4) {
+    to[0] = *reinterpret_cast<const uint32_t*>(from);
+  } else {
+    struct __attribute__((packed, aligned(1))) Two {
+      uint16_t w;
+    };
+    to[0] = reinterpret_cast<const Two*>(from)->w;
+    if constexpr (N == 3) to[1] = from[2];
+  }
+}
+
+template <int N>
+__device__ __forceinline__ float row_power(const uint32_t (&bytes)[2], int i) {
+  return e2m1_power(bytes, N == 3 && i == 2 ? 4 : i);
+}
+
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 // Bytes 0 and 1, or 2 and 3, of a word of 4-bit values times a power, as bf16 (exact).

@@ -33,25 +33,6 @@ __device__ __forceinline__ void two_records(const void* pages, int block, int re
   }
 }
 
-// The bytes of a 4-bit key's N groups, as words that are used as they come (e2m1_key_bytes).
-template <int N>
-__device__ __forceinline__ void load_row_bytes(const uint8_t* from, uint32_t (&to)[2]) {
-  if constexpr (N == 4) {
-    to[0] = *reinterpret_cast<const uint32_t*>(from);
-  } else {
-    struct __attribute__((packed, aligned(1))) Two {
-      uint16_t w;
-    };
-    to[0] = reinterpret_cast<const Two*>(from)->w;
-    if constexpr (N == 3) to[1] = from[2];
-  }
-}
-
-template <int N>
-__device__ __forceinline__ float row_power(const uint32_t (&bytes)[2], int i) {
-  return e2m1_power(bytes, N == 3 && i == 2 ? 4 : i);
-}
-
 template <int TYPE, int D>
 __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArgs a) {
   constexpr int KU = D / 16, DT = D / 32;

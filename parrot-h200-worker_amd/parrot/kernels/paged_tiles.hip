@@ -1,8 +1,9 @@
 // Paged attention of many rows per sequence (prompts and their chunks): a wavefront has
 // 32 rows, the four of a workgroup share key blocks through LDS.
 //
-// Each wavefront brings one of a stage's four matrices (K and V of two blocks) from
-// the pages while the stage before is computed: bf16 straight into LDS, 8-bit pages
+// Each wavefront brings one of a stage's four matrices (K and V of two blocks; of 4 bits,
+// whose values take four times as many instructions as keys, half of K and of V of a block)
+// from the pages while the stage before is computed: bf16 straight into LDS, 8-bit pages
 // into registers, from which they are written as bf16, converted once for 128 rows.
 // K's second half lies 128 bytes further, so that the 16 lanes of a read's phase, which
 // take eight keys of each half, fall into different banks.
@@ -65,7 +66,7 @@ __device__ __forceinline__ bf16x8 value_piece(typename Piece<TYPE>::raw w, const
 }
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kWaves * kWave, TYPE == kPagedE2m1 && D == 96 ? 3 : 2) void paged_tile_kernel(AttendArgs a) {
   constexpr int KU = D / 16, DT = D / 32, S = D / 32;
   constexpr int kHalf = 64;                                  // elements between K's halves
   constexpr int kK = kPagedBlock * D + kHalf;                // elements of K, then of V
@@ -126,7 +127,8 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
     int at0 = -1, at1 = -1;            // of the stage that is brought
     __amdgpu_buffer_rsrc_t from;       // what this wavefront brings of it
     uint4 got[kLoads];                 // 8-bit types
-    uint32_t record[D / 16];           // 4 bits
+    uint32_t k_words[S], v_words[S];   // 4 bits
+    uint32_t k_bytes[2];
     uint32_t bytes[2] = {0, 0};
     auto aim = [&](int i) {  // at blocks i and i + 1 (past the share: at nothing)
       const int j = (i - begin) % kWave;
@@ -138,16 +140,20 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
       at1 = i < end ? __builtin_amdgcn_readlane(ids, j + 1) : -1;
       const int at = which ? at1 : at0;
       from = make_rsrc(matrix + int64_t{max(at, 0)} * kMatrix, at < 0 ? 0 : kMatrix);
-      if constexpr (TYPE != kPagedBf16) {
+      if constexpr (TYPE == kPagedE2m1) {
+        if (at < 0) return;
+        load_row_bytes<S>(
+            a.cache.key_exponent + int64_t{at} * D + (2 * (lane & 15) + brings_v) * S, k_bytes);
+        const uint8_t* x = a.cache.value_exponent + int64_t{at} * kPagedBlock + 4 * (lane >> 4);
+        bytes[0] = *reinterpret_cast<const uint32_t*>(x);
+        bytes[1] = *reinterpret_cast<const uint32_t*>(x + 16);
+      } else if constexpr (TYPE != kPagedBf16) {
         if (at < 0) return;
         const int64_t e = int64_t{at} * kPagedBlock;
         if (brings_v) {  // positions 4 g .. + 3 and 16 + 4 g .. + 3 of the lane's pieces
-          const uint8_t* x =
-              a.cache.value_exponent + e + 4 * (TYPE == kPagedE2m1 ? lane >> 4 : (lane >> 3) & 3);
+          const uint8_t* x = a.cache.value_exponent + e + 4 * ((lane >> 3) & 3);
           bytes[0] = *reinterpret_cast<const uint32_t*>(x);
           bytes[1] = *reinterpret_cast<const uint32_t*>(x + 16);
-        } else if constexpr (TYPE == kPagedE2m1) {
-          e2m1_key_bytes<D>(a.cache.key_exponent + int64_t{at} * D, lane & 15, bytes);
         } else {  // keys c, c + 1 of either half
           const uint8_t* x = a.cache.key_exponent + e + ((2 * lane) & 15);
           bytes[0] = *reinterpret_cast<const uint16_t*>(x);
@@ -164,13 +170,11 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
                                     (!brings_v && u >= S ? kHalf : 0),
                           lane * 16u, 1024u * u);
         else if constexpr (TYPE == kPagedE2m1) {
-          if (u > 0) continue;
-#pragma unroll
-          for (int w = 0; w < D / 16; w += 2) {
-            const auto x = __builtin_amdgcn_raw_buffer_load_b64(from, lane * (D / 4u), 4u * w, 0);
-            record[w] = x[0];
-            record[w + 1] = x[1];
-          }
+          const int at = which ? at1 : at0;
+          if (u > 0 || at < 0) continue;
+          const int64_t word = int64_t{at} * (4 * D) + lane * (D / 16) + brings_v * S;
+          load_words(static_cast<const uint32_t*>(a.cache.key) + word, k_words);
+          load_words(static_cast<const uint32_t*>(a.cache.value) + word, v_words);
         } else
           got[u] = __builtin_bit_cast(
               uint4, __builtin_amdgcn_raw_buffer_load_b128(from, lane * 16u, 1024u * u, 0));
@@ -179,19 +183,25 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
     auto put = [&](int buf) {  // 8-bit and 4-bit types: what was brought, as bf16
       if constexpr (TYPE != kPagedBf16) {
         if ((which ? at1 : at0) < 0) return;
-        uint16_t* const to = &stage[buf][which][brings_v ? kK : 0];
-        if (brings_v) {
+        uint16_t* const to = &stage[buf][which][brings_v && TYPE != kPagedE2m1 ? kK : 0];
+        if (brings_v || TYPE == kPagedE2m1) {
           float power[8], shift[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             power[e] = piece_power<TYPE>((bytes[e >> 2] >> (8 * (e & 3))) & 0xffu);
             shift[e] = -128.0f * power[e];
           }
-          if constexpr (TYPE == kPagedE2m1) {  // word (o, u): dims 32 u + 16 o ..
+          if constexpr (TYPE == kPagedE2m1) {
+            const int half = brings_v;  // words (n, s): dims 32 s ..; (o, u): dims 32 u + 16 o ..
+            uint16_t* const k_to = to + half * (16 * D + kHalf) + lane * 8;
+            uint16_t* const v_to = to + kK + half * 512 + lane * 8;
 #pragma unroll
-            for (int t = 0; t < D / 16; ++t)
-              *reinterpret_cast<bf16x8*>(to + (kWave * t + lane) * 8) =
-                  value_piece<TYPE>(record[(t & 1) * S + t / 2], power, shift);
+            for (int i = 0; i < S; ++i) {
+              *reinterpret_cast<bf16x8*>(k_to + 512 * i) =
+                  piece_bf16<TYPE>(k_words[i], row_power<S>(k_bytes, i));
+              *reinterpret_cast<bf16x8*>(v_to + 1024 * i) =
+                  value_piece<TYPE>(v_words[i], power, shift);
+            }
           } else {
 #pragma unroll
             for (int u = 0; u < kLoads; ++u) {
@@ -200,12 +210,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_tile_kernel(AttendArg
               p[1] = value_piece<TYPE>(make_uint2(got[u].z, got[u].w), power, shift);
             }
           }
-        } else if constexpr (TYPE == kPagedE2m1) {  // word (n, s): dims 32 s ..
-#pragma unroll
-          for (int w = 0; w < D / 16; ++w)
-            *reinterpret_cast<bf16x8*>(to + (kWave * w + lane) * 8 + (w >= S ? kHalf : 0)) =
-                piece_bf16<TYPE>(record[w], e2m1_power(bytes, w));
-        } else {
+        } else if constexpr (TYPE != kPagedE2m1) {
 #pragma unroll
           for (int u = 0; u < kLoads; ++u) {
             const int at = (kWave * u + lane) * 16;
