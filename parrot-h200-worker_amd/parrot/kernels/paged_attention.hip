@@ -172,11 +172,7 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   a.part = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part +
                                         static_cast<size_t>(splits) * batch.rows * heads * head_dim);
-  // ceil(n rep / tile) tiles a sequence of n rows, which is no more than one more than its
-  // rows fill and no more than those of each row alone
-  const int64_t tiles = std::min<int64_t>(
-      static_cast<int64_t>(batch.rows) * a.rep / tile + std::min(batch.batch, batch.rows),
-      static_cast<int64_t>(batch.rows) * ((a.rep + tile - 1) / tile));
+  const int64_t tiles = grid_tiles(batch.rows, batch.batch, a.rep, tile);
   const dim3 grid(static_cast<uint32_t>(tiles), cache.kv_heads, splits);
   const dim3 tile_grid(static_cast<uint32_t>(tiles * cache.kv_heads), 1, splits);
   const hipError_t e = tile < kStepRows    ? launch_step4(a, head_dim, tile, p.wide, grid, s)

@@ -118,7 +118,7 @@ struct Plan {
 // 11.3; 32 of 2048 10.9 / 12.5, 4096 15.6 / 14.9; 64 of 4096 15.9 / 20.4, 8000 27.5 / 26.5; 128 of
 // 16000 76 / 82; 16 heads on 2 of 128: 4 of 1024 8.6 / 9.6, 2048 11.6 / 9.8, 32 of 2048 12.0 / 13.0).
 // One fills a CU, so from three quarters of the CUs on the question is how full their last
-// round is.  Short sequences leave most of its wavefronts nothing (512 of 129 keys 22.4 us,
+// round is (to 8192 keys: a table so wide may hold one sequence as long and many short ones).  Short sequences leave most of its wavefronts nothing (512 of 129 keys 22.4 us,
 // by four wavefronts 12.1).  Tiles of 16 rows up to 96 on average: their registers are two
 // blocks ahead, and the third conversion of what two larger tiles convert twice costs less
 // than the rows that those leave empty (5 sequences of 9000 keys, 48 rows, 16 heads on 2 of 128
@@ -142,7 +142,8 @@ inline Plan plan(int type, int batch, int rows, int heads, int kv_heads, int pag
     const int64_t keys = keys_of(tile), tiles = std::max<int64_t>((all + tile - 1) / tile, n);
     const int64_t units = tiles * kv_heads, rounds = (units + 255) / 256;
     const int64_t most = (fewer ? 2176 : 1152) + 16 * units;
-    if (keys > 768 && units < 768 && (units < 192 ? keys <= most : 4 * units >= 768 * rounds))
+    if (keys > 768 && units < 768 &&
+        (units < 192 ? keys <= most : 4 * units >= 768 * rounds && keys <= 8192))
       return {tile, 1, static_cast<int>(keys / kPagedBlock + 1), true};
   }
   const int tile = few                                                   ? kStepRows / 2
@@ -159,6 +160,15 @@ inline Plan plan(int type, int batch, int rows, int heads, int kv_heads, int pag
   const int64_t splits =
       keys <= line ? 1 : std::min<int64_t>({want, (keys + least - 1) / least, kMaxSplits});
   return {tile, static_cast<int>(splits), static_cast<int>(line / kPagedBlock), false};
+}
+
+// Workgroups for the tiles of all sequences, ceil(n rep / tile) for one of n rows: no more
+// than one each besides those that all rows fill, and no more than those of each row alone
+// (those without a tile end at once, but take room until they do: 8 sequences of 32000 keys by
+// eight empty ones beside eight 21.6 us, without 15.9).
+inline int64_t grid_tiles(int rows, int batch, int rep, int tile) {
+  return std::min(static_cast<int64_t>(rows) * rep / tile + std::min(batch, rows),
+                  static_cast<int64_t>(rows) * ((rep + tile - 1) / tile));
 }
 
 }  // namespace paged

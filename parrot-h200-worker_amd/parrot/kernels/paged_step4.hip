@@ -88,7 +88,7 @@ void paged_step4_kernel(AttendArgs a) {
     // lies in the cache (-1: nowhere).
     int held = -1;
     int at[G];  // of the step whose blocks are in registers, or on their way
-    uint32_t k[G][T], v[G][T], kbytes[G][2], vbytes[2];
+    uint32_t k[G][T], v[G][T], kbytes[G][2], vbytes[2] = {0, 0};
     int there = -1;  // `at` of this lane's group
     auto aim = [&](int j) {
       const int slot = j % kWave;
@@ -111,7 +111,8 @@ void paged_step4_kernel(AttendArgs a) {
                  v[b]);
     };
     auto load_powers = [&] {
-      const uint8_t* e = a.cache.value_exponent + int64_t{max(there, 0)} * kPagedBlock + 4 * g;
+      if (there < 0) return;
+      const uint8_t* e = a.cache.value_exponent + int64_t{there} * kPagedBlock + 4 * g;
       vbytes[0] = *reinterpret_cast<const uint32_t*>(e);
       vbytes[1] = *reinterpret_cast<const uint32_t*>(e + 16);
     };

@@ -266,6 +266,21 @@ def test_rows_without_keys(n, copies):
                 assert ((y[i, 0, n - some:].double().cpu() - ref).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("n,copies", [(1, 1), (2, 1), (6, 1), (75, 1), (75, 40), (1, 100)])
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_a_cache_without_pages(d, n, copies):
+    """Nothing is stored, so nothing is read: 0 everywhere."""
+    from parrot import PagedBatch, PagedKVCache
+    cache = PagedKVCache(0, 32, 2, d, E2M1)
+    b = copies
+    batch = PagedBatch(i32([[0, -1, 5, 2 ** 31 - 1] * 20] * b), i32([1200 + n] * b),
+                       i32(range(0, n * b + 1, n)))
+    rows = torch.ones(n * b, 12, d, dtype=torch.bfloat16, device="cuda")
+    cache.append(rows[:, :2], rows[:, 2:4], batch)
+    assert not cache.attend(rows[:, 4:], batch, scale=0.1).any()
+    assert not any(x.any() for x in cache.read(batch, 70))
+
+
 @pytest.mark.parametrize("n,copies", [(1, 1), (6, 1), (75, 1), (75, 40)])
 def test_pages_missing_inside(n, copies):
     """Pages that are not there between pages that are: their positions are not seen, in
