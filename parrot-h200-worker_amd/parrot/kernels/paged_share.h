@@ -112,17 +112,22 @@ struct Plan {
 // 1024, which evens out the causal ones (2 prompts of 4096 92.5 us, of 768 102), each with
 // 384 keys (3 chunks of 512 rows after 3500 keys 32.2 us, of 256 keys 35.5, of 512 33.2).
 // Of 4-bit pages: tiles of 8 rows where a sequence has no more than 8 on average (two key
-// blocks a step, paged_step4.hip), and wide workgroups, with four blocks a step for up to 4
-// rows, where one of them is as fast as the split and its join (us, 8 heads on 2 of 96, wide /
-// split: 1 sequence of 1536 keys 9.1 / 9.4, 3072 11.8 / 9.7; 16 of 2048 10.8 / 10.8, 3072 12.9 /
-// 11.3; 32 of 2048 10.9 / 12.5, 4096 15.6 / 14.9; 64 of 4096 15.9 / 20.4, 8000 27.5 / 26.5; 128 of
-// 16000 76 / 82; 16 heads on 2 of 128: 4 of 1024 8.6 / 9.6, 2048 11.6 / 9.8, 32 of 2048 12.0 / 13.0).
-// One fills a CU, so from three quarters of the CUs on the question is how full their last
-// round is (to 8192 keys: a table so wide may hold one sequence as long and many short ones).  Short sequences leave most of its wavefronts nothing (512 of 129 keys 22.4 us,
-// by four wavefronts 12.1).  Tiles of 16 rows up to 96 on average: their registers are two
-// blocks ahead, and the third conversion of what two larger tiles convert twice costs less
-// than the rows that those leave empty (5 sequences of 9000 keys, 48 rows, 16 heads on 2 of 128
-// 18.3 / 22.8 in tiles of 32; 5 x 96 rows 21.1 / 23.8, of 128; 2 x 128 rows after 4000 15.0 / 13.3).
+// blocks a step, paged_step4.hip), and workgroups of eight wavefronts, with four blocks a step
+// for up to 4 rows, where one of them is as fast as the split and its join (us, 8 heads on 2 of
+// 96, one wide / split: 1 sequence of 1536 keys 9.1 / 9.4; 16 of 2048 10.8 / 10.8; 32 of 2048
+// 10.9 / 12.5, 4096 15.6 / 14.9; 64 of 4096 15.9 / 20.4, 8000 27.5 / 26.5; 128 of 16000 76 / 82;
+// 16 heads on 2 of 128: 4 of 1024 8.6 / 9.6, 2048 11.6 / 9.8, 32 of 2048 12.0 / 13.0).  One fills
+// a CU, so from three quarters of the CUs on the question is how full their last round is (to
+// 8192 keys: a table so wide may hold one sequence as long and many short ones).  Short
+// sequences leave most of its wavefronts nothing (512 of 129 keys 22.4 us, by four 12.1).
+// Splits are as wide where each CU's one has 512 keys or more and few are left over (join
+// included, wide / four wavefronts: 8 sequences of 4000 keys 10.2 / 9.3, 8000 10.3 / 10.6, 16000
+// 12.9 / 15.6, 32000 17.1 / 18.5, 64000 24.4 / 25.8; 32 of 16000 24.3 / 26.3, 48, which leave 64
+// CUs none, 34.4 / 32.2; 1 of 8000 9.8 / 9.0; 16 heads on 2 of 128: 4 of 8000 10.9 / 9.9, of 20000
+// 12.6 / 14.7).  Tiles of 16 rows up to 96 on average: their registers are two blocks ahead, and
+// the third conversion of what two larger tiles convert twice costs less than the rows that
+// those leave empty (5 sequences of 9000 keys, 48 rows, 16 heads on 2 of 128 18.3 / 22.8 in tiles
+// of 32; 5 x 96 rows 21.1 / 23.8, of 128; 2 x 128 rows after 4000 15.0 / 13.3).
 inline Plan plan(int type, int batch, int rows, int heads, int kv_heads, int page, int width,
                  int window, int sinks) {
   const int rep = heads / kv_heads;
@@ -155,11 +160,14 @@ inline Plan plan(int type, int batch, int rows, int heads, int kv_heads, int pag
   const int64_t units = std::max<int64_t>({tiles, std::min(batch, rows), 1}) * kv_heads;
   const int64_t line = tile == kTileRows ? std::min<int64_t>(384 + 4 * units, 1024) : 768;
   const bool step = tile <= kStepRows;
-  const int64_t want = step ? std::max<int64_t>(768 / units, 1) : (1024 + units - 1) / units;
-  const int64_t least = step ? 256 : 384;
+  const bool wide = few && units <= 64 && keys * units >= 1 << 17;
+  const int64_t want = wide   ? 256 / units
+                       : step ? std::max<int64_t>(768 / units, 1)
+                              : (1024 + units - 1) / units;
+  const int64_t least = wide ? 512 : step ? 256 : 384;
   const int64_t splits =
       keys <= line ? 1 : std::min<int64_t>({want, (keys + least - 1) / least, kMaxSplits});
-  return {tile, static_cast<int>(splits), static_cast<int>(line / kPagedBlock), false};
+  return {tile, static_cast<int>(splits), static_cast<int>(line / kPagedBlock), wide};
 }
 
 // Workgroups for the tiles of all sequences, ceil(n rep / tile) for one of n rows: no more

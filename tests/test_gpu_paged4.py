@@ -215,6 +215,17 @@ def test_attend_long(d, steps, page, window, sinks):
         run.attend(8, new, batch, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("heads,d", [(8, 64), (16, 96), (64, 128)])
+@pytest.mark.parametrize("new,window,sinks", [([1, 1, 1, 1], None, 0), ([1, 1, 0, 1], 4064, 0),
+                                              ([1, 1, 1, 1], 4032, 20)])
+def test_attend_long_of_many_heads(heads, d, new, window, sinks):
+    """Splits of as many keys as eight wavefronts take, beside sequences that need none."""
+    run = Run4(8, d, 64, [[4130, 700, 4099, 0], new])
+    for now in ([4130, 700, 4099, 0], new):
+        batch = run.append(now)
+    run.attend(heads, new, batch, window=window, sinks=sinks)
+
+
 def test_attend_scales_and_strides():
     """Negative and large scales; rows of a packed projection, strides that the kernels do
     not read in place, an offset that is not aligned."""

@@ -12,7 +12,7 @@ def test_every_batch(tmp_path):
     return std::min(static_cast<int>(std::exp(u(rng))), high);
   };
   const int layouts[][2] = {{8, 2}, {8, 8}, {16, 2}, {12, 4}, {4, 1}, {6, 2}, {5, 1}, {32, 32}, {7, 1}};
-  int tiles[129] = {0}, wide = 0;
+  int tiles[129] = {0}, wide = 0, wide_splits = 0;
   for (int run = 0; run < 8000; ++run) {
     Walk w;
     w.type = 4;
@@ -21,7 +21,7 @@ def test_every_batch(tmp_path):
     w.window = rng() % 4 == 0 ? INT32_MAX : pick(1, 4096);
     w.sinks = rng() % 2 ? 0 : pick(1, 300);
     const int batch = pick(1, 300), most = rng() % 3 ? pick(1, 4) : pick(1, std::max(1, 8192 / batch));
-    const int context = pick(1, 12000);
+    const int context = pick(1, rng() % 4 ? 12000 : 100000);
     int longest = 0, rows = 0;
     for (int i = 0; i < batch; ++i) {
       w.news.push_back(rng() % 5 ? static_cast<int>(rng() % most) + 1 : rng() % 2 ? most : 0);
@@ -38,13 +38,15 @@ def test_every_batch(tmp_path):
     int64_t all = 0;
     for (int n : w.news) all += (static_cast<int64_t>(n) * rep + p.tile - 1) / p.tile;
     if (all > grid_tiles(rows, batch, rep, p.tile)) return 3;
-    if (p.wide && (p.splits != 1 || p.tile > 8)) return 4;
+    if (p.wide && (p.tile > 8 || (p.tile == 4 && p.splits != 1))) return 4;
+    wide_splits += p.wide && p.splits > 1;
     ++tiles[p.tile];
     wide += p.wide;
   }
   for (int t : {4, 8, 16, 32, 128})
     if (tiles[t] < 20) return 5;
-  return split > 10000 && wide > 100 && wide < 4000 ? 0 : 2;""")
+  std::printf("%d shares, %d wide, %d of them split\\n", split, wide, wide_splits);
+  return split > 10000 && wide > 100 && wide < 4000 && wide_splits >= 20 ? 0 : 2;""")
 
 
 def test_grids(tmp_path):
