@@ -8,7 +8,9 @@
 // to four blocks between, and for 8-bit pages their conversion (some 2.7 instructions
 // a value of int8, for 32 rows).  Measured, five chunks of 6 tokens after up to 9000 keys,
 // 16 heads on 2 of 128 in int8: 17.2 us for 16 MB and 3.2 to 3.9 for the join; in tiles of 16
-// rows (three conversions in place of two) 27.8 in all, of 128 22.7.
+// rows (three conversions in place of two) 27.8 in all, of 128 22.7.  Of 4-bit pages (from 97 rows
+// on: their conversion is one instruction for two values of a key) a lane's two records of a
+// block come as two loads, and their words are taken in the order of the products.
 #include "paged_attention.h"
 
 namespace parrot {

@@ -16,6 +16,11 @@
 // in a window of 2048 8.3 us for 23 MB and 3.9; one sequence of 129 keys in bf16 4.6 us.  Not
 // kept: registers of two blocks at a time (33 us for the first), four workgroups a CU
 // (the registers spill).
+//
+// Of 4-bit pages (9 to 96 rows a sequence; paged_step4.hip has fewer) a block is a quarter of
+// the registers, and two are on their way ahead of the one in hand: 8 sequences of 32000 keys
+// 14.8 us, with one 17.1.  5 sequences of 48 rows over up to 9000 keys, 16 heads on 2 of 128: 12.4
+// us at three blocks a wavefront, and the join 4.0.
 #include "paged_attention.h"
 
 namespace parrot {

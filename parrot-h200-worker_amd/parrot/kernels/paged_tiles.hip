@@ -21,6 +21,12 @@
 // 130 us where registers leave two), workgroups that take a second, short tile (the
 // registers leave two a CU), odd shares in reverse order (no change), sums of P by dot
 // products of bf16 (eight instructions a block fewer, no change).
+// In 4 bits: 2 prompts of 4096, 8 heads of 64, 68.5 us and 6.8 of join (0.50 PFLOP/s; 3970
+// clocks a pair of blocks, 500 the products, 1140 the vector instructions; where a wavefront
+// brings one whole matrix 70.4), 4 of 4096, 8 heads on 2 of 96, 144 to 150, 3 chunks of 512 24.5
+// and 5.6.  Not kept: S from products that take 4-bit keys and their powers as they are, Q as
+// two parts of 8 bits (66.5, but 32 or, of fewer workgroups, 24.1 for the chunks, whose
+// registers spill, and 91 for 84 at heads of 128); odd shares in reverse order (69).
 #include "attention_lds.h"
 #include "paged_attention.h"
 
@@ -65,8 +71,11 @@ __device__ __forceinline__ bf16x8 value_piece(typename Piece<TYPE>::raw w, const
   return __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
 }
 
+// (4 bits at 96: three workgroups a CU, for which eight registers spill; the two together
+// took 4 prompts of 4096 from 155 us to 150)
 template <int TYPE, int D>
-__global__ __launch_bounds__(kWaves * kWave, TYPE == kPagedE2m1 && D == 96 ? 3 : 2) void paged_tile_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kWaves * kWave, TYPE == kPagedE2m1 && D == 96 ? 3 : 2)
+void paged_tile_kernel(AttendArgs a) {
   constexpr int KU = D / 16, DT = D / 32, S = D / 32;
   constexpr int kHalf = 64;                                  // elements between K's halves
   constexpr int kK = kPagedBlock * D + kHalf;                // elements of K, then of V

@@ -221,8 +221,9 @@ class PagedKVCache:
     """Pages of keys and values of one layer.
 
     ``key`` / ``value`` [pages, kv_heads, page_size / 32, 32 head_dim] of ``dtype``
-    (bf16, float8_e4m3fn, int8 or float4_e2m1fn_x2, half as many elements) hold blocks of 32 positions in the order in
-    which the attention kernels read them (include/parrot_hip.h); ``read`` gives
+    (bf16, float8_e4m3fn, int8, or float4_e2m1fn_x2, whose elements are two values, half
+    as many) hold blocks of 32 positions in the order in which the attention kernels read
+    them (include/parrot_hip.h); ``read`` gives
     rows.  8-bit rows are scaled by a power of two of their own, one byte per
     position and head in ``key_exponent`` / ``value_exponent`` [pages, kv_heads,
     page_size], so that a stored value is exact in bf16.  What that costs, for
@@ -233,7 +234,7 @@ class PagedKVCache:
     4 bits (e2m1): a power of two for 32 dims of a key each, ``key_exponent`` [pages,
     kv_heads, page_size / 32, head_dim], and one for a value row as above; it leaves the
     largest magnitude above 3.5 and not above 7, which becomes 6.  11.2 % of a normal
-    key's norm, 11.4 % of a value's, in 99 bytes for both of 96 (int8: 194).  32 dims with
+    key's norm, 11.4 % of a value's, in 100 bytes for both of 96 (int8: 194).  32 dims with
     a NaN or an infinity read back as NaN."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int,
