@@ -16,8 +16,8 @@
 //
 // (and the same on v_mfma_f32_16x16x32_bf16 for tiles of 16 rows).
 //
-// 8-bit and 4-bit rows enter the products unrounded: K as q 2^x (exact in bf16; int8: 2^(x - 2)), V as q
-// with its power of two on the probability instead (one power per key, and a
+// 8-bit and 4-bit rows enter the products unrounded: K as q 2^x (exact in bf16; int8:
+// 2^(x - 2)), V as q with its power of two on the probability instead (one power per key, and a
 // piece of V holds eight keys).  P is rounded to bf16 once, which the matrix
 // instructions ask for: half a step of 2^-8 on each probability, 1.9 to 2.3e-3 of the output
 // beside its own rounding's 1.6e-3 (in two parts, with twice the products: 1.6e-3, decode
@@ -59,8 +59,25 @@ __device__ __forceinline__ int cache_block(const AttendArgs& a, int sequence, in
   return page < 0 ? -1 : (page * a.cache.kv_heads + kvh) * per_page + block - at * per_page;
 }
 
+// Which tile, kv head and share a workgroup has: of a grid of these, or of a line with the
+// tiles slowest (tiles_last; the same, where there is one kv head and one share).
+struct GridPlace {
+  int tile, kvh, split;
+  __device__ __forceinline__ explicit GridPlace(const AttendArgs& a) {
+    if (gridDim.y * gridDim.z > 1) {
+      tile = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
+      return;
+    }
+    const int x = blockIdx.x, t = x / a.splits;
+    split = x - t * a.splits;
+    tile = t / a.cache.kv_heads;
+    kvh = t - tile * a.cache.kv_heads;
+  }
+};
+
 // Where a wavefront's key blocks (every fourth of its workgroup's share) lie among the
 // cache's: lane j holds the j-th of the last 64.
+
 struct WaveBlocks {
   const AttendArgs& a;
   const int sequence, kvh;

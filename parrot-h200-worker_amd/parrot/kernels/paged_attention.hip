@@ -173,12 +173,15 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
   a.part_ml = reinterpret_cast<float2*>(a.part +
                                         static_cast<size_t>(splits) * batch.rows * heads * head_dim);
   const int64_t tiles = grid_tiles(batch.rows, batch.batch, a.rep, tile);
-  const dim3 grid(static_cast<uint32_t>(tiles), cache.kv_heads, splits);
-  const dim3 tile_grid(static_cast<uint32_t>(tiles * cache.kv_heads), 1, splits);
+  const int64_t units = tiles * cache.kv_heads, all = units * splits;
+  const dim3 grid = tiles_last(type, batch.batch, batch.rows, a.rep, all)
+                        ? dim3(static_cast<uint32_t>(all))
+                        : dim3(static_cast<uint32_t>(tiles), cache.kv_heads, splits);
+  const dim3 tile_grid(static_cast<uint32_t>(units), 1, splits);
   const hipError_t e = tile < kStepRows    ? launch_step4(a, head_dim, tile, p.wide, grid, s)
                        : tile == kStepRows ? launch_step(a, type, head_dim, grid, s)
-                       : tile == kRows  ? launch_rows(a, type, head_dim, grid, s)
-                                        : launch_tiles(a, type, head_dim, tile_grid, s);
+                       : tile == kRows     ? launch_rows(a, type, head_dim, grid, s)
+                                           : launch_tiles(a, type, head_dim, tile_grid, s);
   if (e != hipSuccess || splits == 1) return e;
   return by_type_and_width(type, head_dim, [&](auto, auto d) {
     constexpr int D = decltype(d)::value, kPer = 256 / (D / 4);

@@ -45,12 +45,13 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
-  const int kvh = blockIdx.y, split = blockIdx.z;
+  const GridPlace place(a);
+  const int kvh = place.kvh, split = place.split;
 
   auto units_of = [&](const PagedSequence& s) { return (s.count * a.rep + kRows - 1) / kRows; };
   int sequence, tile;
   PagedSequence s;
-  if (!paged_find(a.batch, a.cache.page, blockIdx.x, units_of, sequence, tile, s)) return;
+  if (!paged_find(a.batch, a.cache.page, place.tile, units_of, sequence, tile, s)) return;
   const int rows = s.count * a.rep;
   const int row0 = tile * kRows;
   const TileRow mine = tile_row(s, row0 + col, rows, a.rep, kvh);

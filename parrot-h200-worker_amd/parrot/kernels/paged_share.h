@@ -179,5 +179,24 @@ inline int64_t grid_tiles(int rows, int batch, int rep, int tile) {
                   static_cast<int64_t>(rows) * ((rep + tile - 1) / tile));
 }
 
+// Whether the workgroups lie in a line with the shares fastest and the tiles slowest, so that
+// those without a tile come last, in place of a grid with the tiles fastest: in that they take
+// the room of workgroups that have one.  For batches that may have such tiles: of several rows
+// a sequence, of 8 and 16 bits more than one tile's (us, grid / line, 8 kv heads of 64, or 8 or 16
+// heads on 2: 16 x 2 rows after 4000 of 96 in 4 bits 12.9 / 10.1, 64 x 2 in a window of 2048 11.3 /
+// 11.4, 16 x 8 after 4000 of 64 18.2 / 14.9, 16 x 6 after 9000 of 128 31.5 / 24.8, 5 ragged ones of 6
+// 14.3 / 15.1; 16 x 5 after 2000 of 96 in bf16 16.0 / 11.3, e4m3 12.8 / 11.1, int8 14.3 / 12.3; 64 x 5 in
+// a window of 2048 36.7 / 24.3, 24.7 / 22.4, 26.2 / 27.5; 8 x 4 after 16000 of 128 47.4 / 35.2, 28.9 /
+// 23.5, 31.2 / 28.2; 2 x 60 after 3000 of 64 in tiles of 32 12.1 / 10.2, 12.2 / 10.7, 13.1 / 11.4; but,
+// a tile each, 16 x 8 after 4000 of 64 26.3 / 27.4, 18.6 / 19.0, 20.3 / 20.7 and 8 x 3 after 16000, 8 heads
+// on 4 of 128, 46.8 / 52.4, 27.8 / 29.1, 30.0 / 30.7).  One row a sequence has no tile too many (in 4
+// bits 8 of 32000 keys 17.1 / 17.8).  A line is as long as a grid may be; past 2^20
+// workgroups the order is nothing.  Tiles of 128 keep theirs, longest first (2 prompts of 4096 68.8 /
+// 75.7).
+inline bool tiles_last(int type, int batch, int rows, int rep, int64_t workgroups) {
+  return rows > batch && workgroups <= 1 << 20 &&
+         (type == kPagedE2m1 || static_cast<int64_t>(rows) * rep > int64_t{kStepRows} * batch);
+}
+
 }  // namespace paged
 }  // namespace parrot

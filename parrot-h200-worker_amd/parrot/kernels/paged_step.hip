@@ -33,7 +33,8 @@ struct StepBlock {
   using raw = typename Piece<TYPE>::raw;
   static constexpr int N = D / 16;  // pieces of K, and of V, per lane
   raw k[N], v[N];
-  uint32_t kbytes[2], vbytes[2];  // exponents of the lane's key rows (e2m1: 2 S bytes); of its 8 scores
+  uint32_t kbytes[2], vbytes[2];  // exponents of the lane's key rows (4 bits: 2 S bytes); of its
+                                  // 8 scores
   int at;                         // which block of the cache; -1: none
 };
 
@@ -173,14 +174,15 @@ __global__ __launch_bounds__(kWaves * kWave, D < 128 ? 3 : 2) void paged_step_ke
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  const int kvh = blockIdx.y, split = blockIdx.z;
+  const GridPlace place(a);
+  const int kvh = place.kvh, split = place.split;
 
   auto units_of = [&](const PagedSequence& s) {
     return (s.count * a.rep + kStepRows - 1) / kStepRows;
   };
   int sequence, tile;
   PagedSequence s;
-  if (!paged_find(a.batch, a.cache.page, blockIdx.x, units_of, sequence, tile, s)) return;
+  if (!paged_find(a.batch, a.cache.page, place.tile, units_of, sequence, tile, s)) return;
   const int rows = s.count * a.rep;
   const int row0 = tile * kStepRows;
   const TileRow mine = tile_row(s, row0 + col, rows, a.rep, kvh);

@@ -71,12 +71,13 @@ void paged_step4_kernel(AttendArgs a) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15, group = col / R, r = col % R;
-  const int kvh = blockIdx.y, split = blockIdx.z;
+  const GridPlace place(a);
+  const int kvh = place.kvh, split = place.split;
 
   auto units_of = [&](const PagedSequence& s) { return (s.count * a.rep + R - 1) / R; };
   int sequence, tile;
   PagedSequence s;
-  if (!paged_find(a.batch, a.cache.page, blockIdx.x, units_of, sequence, tile, s)) return;
+  if (!paged_find(a.batch, a.cache.page, place.tile, units_of, sequence, tile, s)) return;
   const int rows = s.count * a.rep;
   const int row0 = tile * R;
   const TileRow mine = tile_row(s, row0 + r, rows, a.rep, kvh);
