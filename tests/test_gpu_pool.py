@@ -265,6 +265,41 @@ def test_a_captured_loop(dtype):
     assert not pool.uses.any()
 
 
+def test_captured_steps_of_many_rows():
+    """Steps whose rows a second launch places, of two pools in two graphs that are
+    replayed in turn: each as the plain form."""
+    rng = random.Random(8)
+    sides = []
+    for b, width, page, pages, rows in ((60, 90, 32, 5000, 9000), (1100, 3, 64, 3000, 20000)):
+        both = Both.filled(rng, b, width, page, pages, 70)
+        new, keep = i32([0] * b), i32(both.plain.lengths)
+
+        def step():
+            places = both.pool.extend(both.batch, new, rows)
+            both.pool.release(both.batch, keep)
+            return places
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        sides.append((both, new, keep, rows, graph, out))
+    for t in range(6):
+        for both, new, keep, rows, graph, out in sides:
+            b = len(both.plain.lengths)
+            news = [rng.choice([0, 1, rng.randint(2, 400)]) for _ in range(b)]
+            keeps = [rng.choice([0, n, n + 9, n + 500]) for n in both.plain.lengths]
+            new.copy_(i32(news))
+            keep.copy_(i32(keeps))
+            torch.zeros(1 << 20, device="cuda").sum().item()  # eager work in between
+            graph.replay()
+            want = both.plain.extend(news, rows)
+            assert both.batch.starts.tolist() == both.plain.starts, t
+            assert out[0].tolist() == want[0] and out[1].tolist() == want[1], t
+            both.plain.release(keeps)
+            both.check()
+
+
 def test_slots_index_what_lies_by_page():
     """A per-token tensor [pages * page_size, ...] written and read by slots."""
     from parrot import PagedBatch, PagePool
