@@ -280,9 +280,16 @@ class PagedKVCache:
         self._describe(key, value, *(exponents or (None, None)))
         return self
 
-    # (as PagedBatch)
+    # (as PagedBatch; 4 bits as bytes, since pickle knows no tensors of that type)
     def __reduce__(self):
-        return type(self).from_pages, self._tensors
+        if self.dtype != FOUR_BITS:
+            return type(self).from_pages, self._tensors
+        return type(self)._from_bytes, (*(x.view(torch.uint8) for x in self._tensors[:2]),
+                                        *self._tensors[2:])
+
+    @classmethod
+    def _from_bytes(cls, key: Tensor, value: Tensor, *exponents: Tensor) -> "PagedKVCache":
+        return cls.from_pages(key.view(FOUR_BITS), value.view(FOUR_BITS), *exponents)
 
     @staticmethod
     def _check(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype) -> None:

@@ -2,6 +2,8 @@
 and the plain form that the GPU tests compare with."""
 import copy
 import ctypes
+import io
+import pickle
 
 import pytest
 import torch
@@ -93,3 +95,23 @@ def test_stored_forms():
         assert torch.equal(want.flatten(-2), y)
         # what the documentation says of normal rows: their error is 11 % of the norm
         assert 0.108 < ((y - x.double()).norm(dim=-1) / x.double().norm(dim=-1)).mean() < 0.117
+
+
+def test_pickles():
+    """Caches of 4 bits are pickled and saved as those of the other types are; a copy is over
+    the same memory."""
+    from parrot import PagedKVCache
+    c = PagedKVCache(4, 64, 2, 96, E2M1, device="cpu")
+    for x in c._tensors:
+        x.view(torch.uint8).random_(0, 256)
+    saved = io.BytesIO()
+    torch.save(c, saved)
+    saved.seek(0)
+    for d in (pickle.loads(pickle.dumps(c)), torch.load(saved, weights_only=False)):
+        assert d.dtype == E2M1 and (d.page_size, d.kv_heads, d.head_dim) == (64, 2, 96)
+        for x, y in zip(c._tensors, d._tensors):
+            assert x.dtype == y.dtype and x.data_ptr() != y.data_ptr()
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+        assert d._struct.key == d.key.data_ptr() and d._struct.type == 4
+    for x, y in zip(c._tensors, copy.copy(c)._tensors):
+        assert x.data_ptr() == y.data_ptr()
