@@ -34,6 +34,7 @@ PAGE_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2,
               torch.float4_e2m1fn_x2: 4}
 FOUR_BITS = torch.float4_e2m1fn_x2  # an element of such a tensor is two values
 PAGE_BLOCK = 32  # a page is a whole number of blocks of so many positions
+MOST_ROWS = 2 ** 30  # of a step that a pool places
 
 
 @dataclass(frozen=True, eq=False)
@@ -185,6 +186,8 @@ class PagePool:
         Returns ``slots`` int64 [rows], each new row's place in the pool (page *
         page_size + position in it), and ``positions`` int32 [rows]; both -1 past the last
         row, and a slot -1 where the table names no page of the pool."""
+        if not 0 <= rows <= MOST_ROWS:  # (before memory is taken for them)
+            raise RuntimeError(f"a step of a page pool has 0 to {MOST_ROWS} rows, got {rows}")
         at = self._batch(batch, "HIP page pool")
         fresh = self._numbers(new, batch, "new")
         slots, positions = self._slot.new_empty(rows), new.new_empty(rows)

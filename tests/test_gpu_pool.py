@@ -317,3 +317,18 @@ def test_slots_index_what_lies_by_page():
             p = torch.arange(int(batch.lengths[i]), device="cuda")
             at = batch.table[i][p // 32].long() * 32 + p % 32
             assert torch.equal(latents[at], torch.cat(kept[i]))
+
+
+def test_refused_rows_take_no_memory():
+    from parrot import PagedBatch, PagePool
+    pool = PagePool(9, 32)
+    batch = PagedBatch.from_lists([[0], [1]], [5, 6], [1, 1])
+    new = i32([1, 1])
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for rows in ((1 << 30) + 1, 1 << 32, (1 << 32) + 2):
+        with pytest.raises(RuntimeError, match="rows"):
+            pool.extend(batch, new, rows)
+    assert torch.cuda.max_memory_allocated() == before
+    assert batch.lengths.tolist() == [5, 6] and batch.starts.tolist() == [0, 1, 2]

@@ -95,3 +95,14 @@ def test_the_plain_form():
     assert p.table == [[1, 0, -1], [2, -1, -1], [-1, -1, -1]] and p.uses == [1, 1, 1, 0, 0, 0]
     p.release(window=33)
     assert p.table[0] == [-1, 0, -1] and p.uses == [1, 0, 1, 0, 0, 0] and p.lengths == [64, 32, 0]
+
+
+def test_rows_of_a_step_are_bounded():
+    """Numbers of rows that the library has no 32 bits for are refused before anything is
+    allocated for them (the check comes before that for a GPU)."""
+    from parrot import PagedBatch, PagePool
+    p = PagePool(4, 64, device="cpu")
+    b = PagedBatch.from_lists([[0]], [5], [1], device="cpu")
+    for rows in (-1, 2 ** 30 + 1, 2 ** 31, 2 ** 32, 2 ** 32 + 7, 2 ** 64 + 1):
+        with pytest.raises(RuntimeError, match="rows"):
+            p.extend(b, torch.ones(1, dtype=torch.int32), rows)
