@@ -931,7 +931,9 @@ int parrot_paged_extend(const parrot_paged_pool* pool, const parrot_paged_batch*
 /* Takes positions back: sequence i keeps its first lengths[i] (NULL, or more than it has: all),
  * and pages wholly past them lose a use and their table entry (-1).  window > 0: so do pages
  * of which no later query (from its length on) sees a position, those with all positions
- * j <= length - window and j >= sinks.  starts is not read. */
+ * j <= length - window and j >= sinks, by the length that this call leaves.  They are gone: a
+ * sequence that a later call shortens lacks their keys, so rows that may be refused are taken
+ * back before, or in the same call.  starts is not read. */
 int parrot_paged_release(const parrot_paged_pool* pool, const parrot_paged_batch* batch,
                          const int32_t* lengths, int32_t window, int32_t sinks, void* stream);
 

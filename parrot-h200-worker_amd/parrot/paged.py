@@ -118,9 +118,14 @@ class PagePool:
     and its step can be captured whole::
 
         slots, positions = pool.extend(batch, new, rows)
-        cache.append(k, v, batch)                  # of every layer
+        cache.append(k, v, batch)                        # of every layer
         y = cache.attend(q, batch, ...)
-        pool.release(batch, window=2048, sinks=4)  # what the window has left
+        pool.release(batch, kept, window=2048, sinks=4)  # refused rows, and what the window
+                                                         # of the others has left
+
+    What a window has left is gone: a later call that takes positions back does not bring
+    it, and then lacks keys that the shorter sequence sees.  So positions that may be taken
+    back are, before their window is released or in the same call.
 
     Calls on one pool or batch belong on one stream, or in order.  A program that lets a
     sequence begin with pages of another adds one to their ``uses`` (and new rows must not
@@ -183,6 +188,9 @@ class PagePool:
         refused otherwise still counts, so that nobody is overtaken).  A sequence that is
         refused stays as it is, without new rows.  The lowest free pages go first.
 
+        Columns of the table past a sequence's length must name no page (-1): what stands
+        there is overwritten, and a use that it had is never given back.
+
         Returns ``slots`` int64 [rows], each new row's place in the pool (page *
         page_size + position in it), and ``positions`` int32 [rows]; both -1 past the last
         row, and a slot -1 where the table names no page of the pool."""
@@ -208,8 +216,10 @@ class PagePool:
         """Takes positions back, in place: each sequence keeps its first ``lengths`` [b]
         (int32; 0 ends it, more than it has changes nothing; None: all of each), and pages
         wholly past them lose a use and their entry in the table, which becomes -1.  With a
-        ``window`` so do the pages that no later position sees, all but those of the first
-        ``sinks`` positions.  ``batch.starts`` stay as they are."""
+        ``window`` so do the pages that no later position sees, from the kept lengths on, all
+        but those of the first ``sinks`` positions: lengths that no call may shorten again
+        (rows that may still be refused are not to be counted; give ``lengths`` without them
+        in the same call).  ``batch.starts`` stay as they are."""
         at = self._batch(batch, "HIP page pool")
         to = None if lengths is None else self._numbers(lengths, batch, "lengths")
         if window is not None and window < 1:

@@ -332,3 +332,65 @@ def test_refused_rows_take_no_memory():
             pool.extend(batch, new, rows)
     assert torch.cuda.max_memory_allocated() == before
     assert batch.lengths.tolist() == [5, 6] and batch.starts.tolist() == [0, 1, 2]
+
+
+@pytest.mark.parametrize("one_call", [True, False])
+def test_refused_rows_beside_a_window(one_call):
+    """Drafts that are turned down after the window has left pages, at lengths around the
+    edges where it does: with the positions taken back before their window is released, or
+    in the same call, each captured step is the same calls on pages that all stay."""
+    from parrot import PagedBatch, PagedKVCache, PagePool
+    b, heads, kv_heads, d, page, width, rows = 4, 8, 2, 96, 32, 16, 28
+    window, sinks = 70, 33
+    g = torch.Generator().manual_seed(16)
+    rng = random.Random(16)
+    pool, cache = PagePool(40, page), PagedKVCache(40, page, kv_heads, d)
+    whole = PagedKVCache(b * width, page, kv_heads, d)
+    tables = [list(range(i * width, (i + 1) * width)) for i in range(b)]
+    batch = PagedBatch(i32([[-1] * width] * b), i32([0] * b), i32([0] * (b + 1)))
+    k, v, q = (torch.zeros(rows, h, d, dtype=torch.bfloat16, device="cuda")
+               for h in (kv_heads, kv_heads, heads))
+    new, kept = i32([0] * b), i32([0] * b)
+
+    def step():
+        pool.extend(batch, new, rows)
+        cache.append(k, v, batch)
+        y = cache.attend(q, batch, scale=0.1, window=window, sinks=sinks)
+        if one_call:
+            pool.release(batch, kept, window=window, sinks=sinks)
+        else:
+            pool.release(batch, kept)
+            pool.release(batch, window=window, sinks=sinks)
+        return y
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    lengths, plain = [0] * b, PlainPool([0] * 40, page, [[-1] * width] * b, [0] * b)
+    left = crossed = 0
+    while min(lengths) < width * page - 7:
+        # drafts of up to 7 tokens, of which some stay; the last sequence never waits
+        news = [min(n, width * page - length) for n, length in
+                zip([1, 7, rng.randint(1, 7), 6], lengths)]
+        keeps = [length + n - rng.randint(0, max(n - 1, 0)) for n, length in zip(news, lengths)]
+        keeps[3] = lengths[3] + news[3] - (0 if rng.random() < 0.3 else max(news[3] - 1, 0))
+        grown = [n + length for n, length in zip(news, lengths)]
+        for n, to in zip(grown, keeps):  # pages that all of the rows would leave, the kept ones not
+            crossed += (n - window + 1) // page > max(to - window + 1, 0) // page >= 2
+        fresh = [torch.randn(rows, h, d, generator=g).bfloat16() for h in (kv_heads, kv_heads, heads)]
+        for x, y in zip((k, v, q, new, kept), (*fresh, i32(news), i32(keeps))):
+            x.copy_(y)
+        graph.replay()
+        byhand = PagedBatch.from_lists(tables, grown, news)
+        whole.append(k, v, byhand)
+        want = whole.attend(q, byhand, scale=0.1, window=window, sinks=sinks)
+        total = sum(news)
+        assert torch.equal(out[:total], want[:total]), lengths
+        plain.extend(news, rows)
+        plain.release(keeps, window=window, sinks=sinks)
+        assert batch.lengths.tolist() == plain.lengths == keeps
+        assert batch.table.tolist() == plain.table and pool.uses.tolist() == plain.uses
+        lengths = keeps
+        left += sum(row[2] == -1 for row in plain.table)
+    assert left > 0 and crossed > 10
