@@ -394,3 +394,24 @@ def test_refused_rows_beside_a_window(one_call):
         lengths = keeps
         left += sum(row[2] == -1 for row in plain.table)
     assert left > 0 and crossed > 10
+
+
+def test_a_step_and_back():
+    """extend, then release to the lengths before: the table and the lengths are as they
+    were, and so are the uses (of pages that a use below 0 made free, 0 is left)."""
+    rng = random.Random(5)
+    for negative in (False, True):
+        both = Both.filled(rng, 300, 40, 32, 9000, 600)
+        if not negative:
+            both.pool.uses.clamp_(min=0)
+        assert (both.pool.uses < 0).any() == negative
+        new = i32([rng.randint(0, 500) for _ in range(300)])
+        state = (both.batch.table, both.batch.lengths, both.pool.uses)
+        before = [x.clone() for x in state]
+        for _ in range(3):
+            both.pool.extend(both.batch, new, 80000)
+            assert not torch.equal(state[0], before[0]) and not torch.equal(state[1], before[1])
+            both.pool.release(both.batch, before[1])
+            assert torch.equal(state[0], before[0]) and torch.equal(state[1], before[1])
+            assert torch.equal(state[2].clamp_min(0), before[2].clamp_min(0))
+            assert negative or torch.equal(state[2], before[2])
