@@ -72,6 +72,7 @@ class PagedBatch:
         object.__setattr__(self, "_at", ctypes.addressof(self._struct))
         object.__setattr__(self, "_device", self.table.device)
         object.__setattr__(self, "_sizes", (b, width))
+        object.__setattr__(self, "_pool", None)  # the last PagePool that handed it pages
 
     # (copies and pickles are of the tensors, not of their addresses)
     def __reduce__(self):
@@ -127,6 +128,9 @@ class PagePool:
     it, and then lacks keys that the shorter sequence sees.  So positions that may be taken
     back are, before their window is released or in the same call.
 
+    The caches have pages of the pool's size, and as many at least: their calls refuse a
+    batch that a pool of another size, or of pages that they lack, was called with last.
+
     Calls on one pool or batch belong on one stream, or in order.  A program that lets a
     sequence begin with pages of another adds one to their ``uses`` (and new rows must not
     fall into them, so whole pages are shared)."""
@@ -174,6 +178,7 @@ class PagePool:
             raise RuntimeError(f"{what} requires a ROCm (cuda) pool, got {self.device}")
         if batch._device != self.device:
             raise RuntimeError("the batch must be on the pool's device")
+        object.__setattr__(batch, "_pool", self)
         return batch._at
 
     def extend(self, batch: PagedBatch, new: Tensor, rows: int) -> tuple[Tensor, Tensor]:
@@ -349,6 +354,11 @@ class PagedKVCache:
     def _batch(self, batch: PagedBatch) -> int:
         if batch._device != self.device:
             raise RuntimeError("the batch must be on the cache's device")
+        pool = batch._pool
+        if pool is not None and (pool.page_size != self.page_size or
+                                 pool._struct.pages > self._struct.pages):
+            raise RuntimeError(f"the batch's pool has {pool._struct.pages} pages of {pool.page_size} "
+                               f"positions, the cache {self._struct.pages} of {self.page_size}")
         return batch._at
 
     def _new_rows(self, x: Tensor, heads: int, what: str, step: int):

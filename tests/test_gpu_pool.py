@@ -415,3 +415,28 @@ def test_a_step_and_back():
             assert torch.equal(state[0], before[0]) and torch.equal(state[1], before[1])
             assert torch.equal(state[2].clamp_min(0), before[2].clamp_min(0))
             assert negative or torch.equal(state[2], before[2])
+
+
+def test_pools_and_caches_of_other_sizes():
+    """Pages that a cache does not have, or of another size: refused by its calls, where
+    rows would be dropped or go astray; taken once a fitting pool has the batch."""
+    from parrot import PagedBatch, PagedKVCache, PagePool
+    cache = PagedKVCache(6, 64, 2, 96)
+    rows = torch.randn(3, 12, 96, device="cuda").bfloat16()
+    k, v, q = rows[:, :2], rows[:, 2:4], rows[:, 4:]
+    table = torch.ones(64, 48, device="cuda")
+    for pool in (PagePool(7, 64), PagePool(6, 32), PagePool(6, 128)):
+        batch = PagedBatch(i32([[-1, -1]]), i32([0]), i32([0, 0]))
+        pool.extend(batch, i32([3]), 3)
+        before = [x.clone() for x in cache._tensors[:2]]
+        for call in (lambda: cache.append(k, v, batch), lambda: cache.read(batch, 3),
+                     lambda: cache.append_rope(q, k, v, batch, table, table),
+                     lambda: cache.attend(q, batch, scale=0.1)):
+            with pytest.raises(RuntimeError, match="pool"):
+                call()
+        assert all(torch.equal(x, y) for x, y in zip(before, cache._tensors))
+        pool.release(batch, i32([0]))
+        PagePool(5, 64).extend(batch, i32([3]), 3)
+        cache.append(k, v, batch)
+        assert torch.equal(cache.read(batch, 3)[0][0], k.transpose(0, 1))
+        cache.attend(q, batch, scale=0.1)

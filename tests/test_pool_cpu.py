@@ -106,3 +106,21 @@ def test_rows_of_a_step_are_bounded():
     for rows in (-1, 2 ** 30 + 1, 2 ** 31, 2 ** 32, 2 ** 32 + 7, 2 ** 64 + 1):
         with pytest.raises(RuntimeError, match="rows"):
             p.extend(b, torch.ones(1, dtype=torch.int32), rows)
+
+
+def test_caches_know_their_pool():
+    """A cache takes a batch that nobody or a fitting pool handed pages to, and no other; copies
+    of a batch are nobody's."""
+    from parrot import PagedBatch, PagedKVCache, PagePool
+    cache = PagedKVCache(9, 64, 2, 96, device="cpu")
+    b = PagedBatch.from_lists([[0]], [5], [1], device="cpu")
+    assert cache._batch(b) == b._at
+    for pages, page, fits in ((9, 64, True), (10, 64, False), (9, 32, False), (4, 128, False),
+                              (3, 64, True)):
+        object.__setattr__(b, "_pool", PagePool(pages, page, device="cpu"))
+        if fits:
+            assert cache._batch(b) == b._at
+        else:
+            with pytest.raises(RuntimeError, match=f"{pages} pages of {page}"):
+                cache._batch(b)
+            assert cache._batch(copy.copy(b))
