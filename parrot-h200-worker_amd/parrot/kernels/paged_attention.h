@@ -123,10 +123,20 @@ __device__ __forceinline__ Visible visible_to(int query, int stored, int window,
 template <int TYPE>
 constexpr float kUnit = TYPE == kPagedInt8 ? 4.0f : 1.0f;
 
-// 2^(byte - 127) / kUnit; infinite for a row that is not finite, which makes it NaN.
+// 2^(byte - 127) / kUnit as the factor of a piece of K; infinite for a row that is not
+// finite, which the piece's conversion makes NaN.
 template <int TYPE>
 __device__ __forceinline__ float piece_power(uint32_t byte) {
   return __uint_as_float(byte << 23) * (1.0f / kUnit<TYPE>);
+}
+
+// 2^(byte i of a word - 127) as a factor of probabilities or values; NaN for 255, so that a
+// row that is not finite is NaN whatever values stand in it (an infinity would leave those
+// that are not 0 infinite).  One conversion of 1, which reads a float's eight exponent bits and
+// no others.
+__device__ __forceinline__ float byte_power(uint32_t word, int i) {
+  const uint32_t w = i < 3 ? word << (23 - 8 * i) : word >> 1;
+  return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(2u, __uint_as_float(w), 0)[0];
 }
 
 // A piece (8 values) of a page as bf16: K's values are times `power`, V's are

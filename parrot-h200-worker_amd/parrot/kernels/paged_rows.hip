@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
           if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              if (byte_of(e) == kPagedNotFinite) {  // (such an int8 row holds zeros)
+              if (byte_of(e) == kPagedNotFinite) {  // (whatever values such a row holds)
                 bytes[e >> 2] &= ~(0xffu << (8 * (e & 3)));
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
       raise(st, largest(sc), a.scale_log2);
       bf16x8 pf[2];
       probabilities(st, sc, a.scale_log2, pf, [&](float p, int e) {
-        return TYPE == kPagedBf16 ? p : p * __uint_as_float(byte_of(e) << 23);
+        return TYPE == kPagedBf16 ? p : p * byte_power(bytes[e >> 2], e & 3);
       });
 #pragma unroll
       for (int h = 0; h < 2; ++h)

@@ -125,7 +125,7 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
       if constexpr (TYPE != kPagedBf16) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (byte_of(e) == kPagedNotFinite) {  // (such an int8 row holds zeros)
+          if (byte_of(e) == kPagedNotFinite) {  // (whatever values such a row holds)
             bytes[e >> 2] &= ~(0xffu << (8 * (e & 3)));
 #pragma unroll
             for (int t = 0; t < T; ++t) vf[t][e] = __builtin_bit_cast(__bf16, uint16_t{0x7fc0});
@@ -140,7 +140,7 @@ __device__ __forceinline__ void step_block(StepState<TYPE, D>& st, const StepBlo
   bf16x8 pf;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float y = TYPE == kPagedBf16 ? p[e] : p[e] * __uint_as_float(byte_of(e) << 23);
+    const float y = TYPE == kPagedBf16 ? p[e] : p[e] * byte_power(bytes[e >> 2], e & 3);
     pf[e] = static_cast<__bf16>(y);
   }
 #pragma unroll

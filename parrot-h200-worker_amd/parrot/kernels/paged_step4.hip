@@ -27,9 +27,9 @@
 // is left is the launch, the first loads (sequence, table, block: some 4 us), and the last.
 // Not kept: 16 wavefronts of two blocks a step (12.0 us for the first).
 //
-// The stored values are finite whatever a row held (its power of two, byte 255, makes the
-// products NaN), so a row that is not seen takes 0 in place of its power and cannot reach
-// anything.
+// The stored values are finite whatever a row held (its power of two, which is NaN for byte
+// 255, makes the products NaN), so a row that is not seen takes 0 in place of its power and
+// cannot reach anything.
 #include "paged_attention.h"
 
 namespace parrot {
@@ -183,7 +183,7 @@ void paged_step4_kernel(AttendArgs a) {
       float power[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        power[e] = __uint_as_float(((vbytes[e >> 2] >> (8 * (e & 3))) & 0xffu) << 23);
+        power[e] = byte_power(vbytes[e >> 2], e & 3);
       if (more) load_powers();
       bool whole = i >= whole0 && i + (G - 1) * W < whole1;
 #pragma unroll

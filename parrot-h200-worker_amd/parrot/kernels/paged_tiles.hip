@@ -197,7 +197,7 @@ void paged_tile_kernel(AttendArgs a) {
           float power[8], shift[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            power[e] = piece_power<TYPE>((bytes[e >> 2] >> (8 * (e & 3))) & 0xffu);
+            power[e] = byte_power(bytes[e >> 2], e & 3) * (1.0f / kUnit<TYPE>);
             shift[e] = -128.0f * power[e];
           }
           if constexpr (TYPE == kPagedE2m1) {
