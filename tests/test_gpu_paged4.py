@@ -162,6 +162,52 @@ def test_append_rope():
         assert torch.equal(got.double(), stored(x, group))
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 96), (4, 4, 64), (12, 2, 128), (5, 1, 64), (16, 1, 128)])
+@pytest.mark.parametrize("page,steps", [(64, [[1, 1, 0], [1, 1, 1]]), (32, [[33, 0, 95], [32, 5, 1], [0, 64, 33]]),
+                                        (96, [[100, 96, 3], [1, 1, 3]]), (128, [[257, 600, 0], [1, 40, 7]])])
+def test_append_rope_in_steps(heads, kv_heads, d, page, steps):
+    """Chunks at every offset of a block, tables shorter than the positions, rows of a packed
+    projection and rows of nobody: keys as append stores what a cache in bf16 rotated,
+    values and queries as they are there."""
+    from parrot import PagedBatch, PagedKVCache
+    run = Run4(kv_heads, d, page, steps)
+    plain = PagedKVCache(run.cache.key.shape[0], page, kv_heads, d)
+    angle = torch.arange(300.0)[:, None] * 10000.0 ** (-torch.arange(0, d, 2) / d)
+    cos, sin = angle.cos().cuda(), angle.sin().cuda()
+    for new in steps:
+        run.lengths = [a + b for a, b in zip(run.lengths, new)]
+        batch = run.batch(new)
+        rows = sum(new)
+        packed = _rows(run.g, rows + 4, heads + 2 * kv_heads, d).cuda()
+        packed[rows:] = math.nan  # (nobody's)
+        q, k, v = packed.split((heads, kv_heads, kv_heads), 1)
+        print(f"{new} after {run.lengths}", flush=True)
+        want = plain.append_rope(q, k, v, batch, cos, sin)
+        got = run.cache.append_rope(q, k, v, batch, cos, sin)
+        assert torch.equal(got[:rows], want[:rows])
+        longest = max(run.lengths)
+        key, value = plain.read(batch, longest)
+        for got, x, group in zip(run.cache.read(batch, longest), (key, value), (32, d)):
+            assert torch.equal(got.double(), stored(x, group))
+    # into a captured graph, replayed for other rows
+    new = [1] * len(run.lengths)
+    batch = PagedBatch(batch.table, batch.lengths, i32(range(len(new) + 1)))
+    q, k, v = (_rows(run.g, len(new), h, d).cuda() for h in (heads, kv_heads, kv_heads))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = run.cache.append_rope(q, k, v, batch, cos, sin)
+    for _ in range(3):
+        for x in (q, k, v):
+            x.copy_(_rows(run.g, *x.shape))
+        graph.replay()
+        assert torch.equal(out, plain.append_rope(q, k, v, batch, cos, sin))
+        key, value = plain.read(batch, longest)
+        for got, x, group in zip(run.cache.read(batch, longest), (key, value), (32, d)):
+            assert torch.equal(got.double(), stored(x, group))
+        torch.zeros(1 << 20, device="cuda").sum().item()  # eager work in between
+
+
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
