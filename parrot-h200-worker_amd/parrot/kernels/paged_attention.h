@@ -59,21 +59,14 @@ __device__ __forceinline__ int cache_block(const AttendArgs& a, int sequence, in
   return page < 0 ? -1 : (page * a.cache.kv_heads + kvh) * per_page + block - at * per_page;
 }
 
-// Which tile, kv head and share a workgroup has: of a grid of these, or of a line with the
-// tiles slowest (tiles_last; the same, where there is one kv head and one share).
-struct GridPlace {
-  int tile, kvh, split;
-  __device__ __forceinline__ explicit GridPlace(const AttendArgs& a) {
-    if (gridDim.y * gridDim.z > 1) {
-      tile = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
-      return;
-    }
-    const int x = blockIdx.x, t = x / a.splits;
-    split = x - t * a.splits;
-    tile = t / a.cache.kv_heads;
-    kvh = t - tile * a.cache.kv_heads;
-  }
-};
+// What a workgroup has: its place in the grid, or in a line (tiles_last; the same, where
+// there is one kv head and one share).
+__device__ __forceinline__ Place place_of(const AttendArgs& a) {
+  if (gridDim.y * gridDim.z > 1)
+    return {static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.y),
+            static_cast<int>(blockIdx.z)};
+  return line_place(static_cast<int>(blockIdx.x), a.cache.kv_heads, a.splits);
+}
 
 // Where a wavefront's key blocks (every fourth of its workgroup's share) lie among the
 // cache's: lane j holds the j-th of the last 64.

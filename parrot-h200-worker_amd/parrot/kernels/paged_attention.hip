@@ -174,7 +174,8 @@ hipError_t launch_paged_attention(const PagedCache& cache, int type, int head_di
                                         static_cast<size_t>(splits) * batch.rows * heads * head_dim);
   const int64_t tiles = grid_tiles(batch.rows, batch.batch, a.rep, tile);
   const int64_t units = tiles * cache.kv_heads, all = units * splits;
-  const dim3 grid = tiles_last(type, batch.batch, batch.rows, a.rep, all)
+  const dim3 grid = tiles_last(p, type, batch.batch, batch.rows, a.rep, cache.kv_heads,
+                               batch.width * cache.page, window, sinks, all)
                         ? dim3(static_cast<uint32_t>(all))
                         : dim3(static_cast<uint32_t>(tiles), cache.kv_heads, splits);
   const dim3 tile_grid(static_cast<uint32_t>(units), 1, splits);

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void paged_rows_kernel(AttendArg
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
-  const GridPlace place(a);
+  const Place place = place_of(a);
   const int kvh = place.kvh, split = place.split;
 
   auto units_of = [&](const PagedSequence& s) { return (s.count * a.rep + kRows - 1) / kRows; };

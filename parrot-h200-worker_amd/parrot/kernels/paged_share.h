@@ -71,6 +71,10 @@ struct Share {
   int most;  // key blocks of the longest share of the tile and the sequence's last rows
 };
 
+PARROT_EXTENT int even_share(int blocks, int splits) {
+  return greater(((blocks + splits - 1) / splits + kWaves - 1) / kWaves * kWaves, kMinShare);
+}
+
 PARROT_EXTENT Share split_share(const PagedSequence& s, int rows, int tile, int rep,
                                 const Blocks& blocks, int split, int splits, int whole,
                                 int window, int sinks) {
@@ -79,8 +83,7 @@ PARROT_EXTENT Share split_share(const PagedSequence& s, int rows, int tile, int 
                                   sinks);
   const int most = greater(last.count, blocks.count);
   if (splits == 1) return {0, blocks.count, true, most};
-  const int even = ((most + splits - 1) / splits + kWaves - 1) / kWaves * kWaves;
-  const int share = most <= whole ? most : greater(even, kMinShare);
+  const int share = most <= whole ? most : even_share(most, splits);
   const int begin = lesser(split * share, blocks.count);
   return {begin, lesser(begin + share, blocks.count), blocks.count <= share,
           lesser(share, most)};
@@ -179,23 +182,55 @@ inline int64_t grid_tiles(int rows, int batch, int rep, int tile) {
                   static_cast<int64_t>(rows) * ((rep + tile - 1) / tile));
 }
 
-// Whether the workgroups lie in a line with the shares fastest and the tiles slowest, so that
-// those without a tile come last, in place of a grid with the tiles fastest: in that they take
-// the room of workgroups that have one.  For batches that may have such tiles: of several rows
-// a sequence, of 8 and 16 bits more than one tile's (us, grid / line, 8 kv heads of 64, or 8 or 16
-// heads on 2: 16 x 2 rows after 4000 of 96 in 4 bits 12.9 / 10.1, 64 x 2 in a window of 2048 11.3 /
-// 11.4, 16 x 8 after 4000 of 64 18.2 / 14.9, 16 x 6 after 9000 of 128 31.5 / 24.8, 5 ragged ones of 6
-// 14.3 / 15.1; 16 x 5 after 2000 of 96 in bf16 16.0 / 11.3, e4m3 12.8 / 11.1, int8 14.3 / 12.3; 64 x 5 in
-// a window of 2048 36.7 / 24.3, 24.7 / 22.4, 26.2 / 27.5; 8 x 4 after 16000 of 128 47.4 / 35.2, 28.9 /
-// 23.5, 31.2 / 28.2; 2 x 60 after 3000 of 64 in tiles of 32 12.1 / 10.2, 12.2 / 10.7, 13.1 / 11.4; but,
-// a tile each, 16 x 8 after 4000 of 64 26.3 / 27.4, 18.6 / 19.0, 20.3 / 20.7 and 8 x 3 after 16000, 8 heads
-// on 4 of 128, 46.8 / 52.4, 27.8 / 29.1, 30.0 / 30.7).  One row a sequence has no tile too many (in 4
-// bits 8 of 32000 keys 17.1 / 17.8).  A line is as long as a grid may be; past 2^20
-// workgroups the order is nothing.  Tiles of 128 keep theirs, longest first (2 prompts of 4096 68.8 /
-// 75.7).
-inline bool tiles_last(int type, int batch, int rows, int rep, int64_t workgroups) {
-  return rows > batch && workgroups <= 1 << 20 &&
-         (type == kPagedE2m1 || static_cast<int64_t>(rows) * rep > int64_t{kStepRows} * batch);
+// A tile, kv head and share.
+struct Place {
+  int tile, kvh, split;
+};
+
+// Workgroup x of a line: the shares fastest, then the kv heads, the tiles slowest.
+PARROT_EXTENT Place line_place(int x, int kv_heads, int splits) {
+  const int t = x / splits, tile = t / kv_heads;
+  return {tile, t - tile * kv_heads, x - t * splits};
+}
+
+// Whether the workgroups lie in a line, in place of a grid with the tiles fastest and the
+// shares slowest.  Workgroups go to the eight XCDs in turn, so where a tile has a multiple of
+// eight of them, the same share of a sequence's tiles is on one XCD, whose L2 then has the keys
+// for the second; and those without a tile come last, in place of taking the room of others.
+// For batches of several rows a sequence, of 8 and 16 bits more than one tile's (us, grid / line;
+// 8 kv heads of 64, or 8 or 16 heads on 2 of 96 or 128):
+//              16 x 5 rows   64 x 5 in a   8 x 4 after   2 x 60 after  16 x 24 after  16 x 6 after
+//              after 2000    window of     16000 of 128  3000 of 64    4000 of 64     9000 of 128
+//                            3000
+//     bf16     16.0 / 11.5   49.1 / 29.1   46.4 / 34.7   11.6 / 10.2   43.6 / 26.8    (128 rows a tile)
+//     e4m3     13.0 / 11.2   31.7 / 24.9   28.5 / 23.0   12.3 / 10.6   26.9 / 20.9    (128)
+//     int8     14.3 / 12.3   34.4 / 30.7   30.9 / 27.4   13.2 / 11.4   28.8 / 25.9    (128)
+//     4 bits   11.8 / 10.8   23.7 / 22.1   21.9 / 20.1   12.4 / 11.5   20.8 / 19.2    31.3 / 24.2
+// (but, a tile each, 16 x 8 after 4000 of 64 26.3 / 27.4 in bf16, 18.6 / 19.0, 20.3 / 20.7 and 8 x 3
+// after 16000, 8 heads on 4 of 128, 46.8 / 52.4, 27.8 / 29.1, 30.0 / 30.7; in 4 bits 16 x 2 after 4000
+// of 96 12.9 / 10.1).  Ragged contexts go either way in 4 bits (5, 6 and 12 chunks of 6 rows of
+// up to 9000, 9000 and 5000, 16 heads on 2 of 128: 14.2 / 14.9, 16.5 / 15.3, 19.0 / 16.8).
+// A window cuts shares of unlike length, and the grid has the short ones last.  So with one, and
+// two tiles a sequence in 4 bits, the line needs the gain of the L2 (tiles of other numbers of
+// workgroups: 32 x 5 in one of 2048 of 96 23.9 / 23.8 in bf16, 19.4 / 20.2, 21.3 / 22.2 and 16.8 / 17.1
+// in 4 bits; 32 x 4 in one of 1000, 16 heads on 2 of 128, 19.2 / 20.4, 13.9 / 15.6, 15.3 / 17.1, 13.4 /
+// 14.1), and below 16 bits, which have less to gain, shares that all have blocks (64 x 5 in one of 1000,
+// four shares of 12, 12, 9 and no blocks, 22.6 / 18.7 in bf16, 17.1 / 17.9, 18.4 / 20.8, 14.1 / 16.1; in
+// one of 2048, 20 to 5 blocks, 36.4 / 24.1, 24.7 / 22.3, 26.3 / 26.8, 19.7 / 19.7).  In 4 bits of one tile
+// a sequence, or three and more, windows gain (64 x 3 in one of 2048 15.1 / 14.6, 64 x 5, 16 heads on
+// 2 of 128, 26.9 / 24.5).
+// One row a sequence has no tile too many (in 4 bits 8 of 32000 keys 17.1 / 17.8).  A line is as
+// long as a grid may be; past 2^20 workgroups the order is nothing.  Tiles of 128 keep theirs,
+// longest first (2 prompts of 4096 68.8 / 75.7).
+inline bool tiles_last(const Plan& p, int type, int batch, int rows, int rep, int kv_heads,
+                       int positions, int window, int sinks, int64_t workgroups) {
+  const int64_t all = static_cast<int64_t>(rows) * rep, one = int64_t{kStepRows} * batch;
+  if (rows <= batch || workgroups > 1 << 20 || (type != kPagedE2m1 && all <= one)) return false;
+  if (window >= positions || (type == kPagedE2m1 && (all <= one || all > 2 * one))) return true;
+  if (p.splits * kv_heads % 8 != 0 || type == kPagedBf16) return p.splits * kv_heads % 8 == 0;
+  const int blocks =
+      static_cast<int>((int64_t{window} + sinks + kPagedBlock - 1) / kPagedBlock + 1);
+  return (p.splits - 1) * even_share(blocks, p.splits) < blocks;
 }
 
 }  // namespace paged

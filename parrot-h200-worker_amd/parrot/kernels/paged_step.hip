@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kWaves * kWave, D < 128 ? 3 : 2) void paged_step_ke
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  const GridPlace place(a);
+  const Place place = place_of(a);
   const int kvh = place.kvh, split = place.split;
 
   auto units_of = [&](const PagedSequence& s) {

@@ -71,7 +71,7 @@ void paged_step4_kernel(AttendArgs a) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15, group = col / R, r = col % R;
-  const GridPlace place(a);
+  const Place place = place_of(a);
   const int kvh = place.kvh, split = place.split;
 
   auto units_of = [&](const PagedSequence& s) { return (s.count * a.rep + R - 1) / R; };

@@ -143,3 +143,58 @@ def test_every_batch(tmp_path):
     if (!w.covered(&split)) return 1;
   }
   return split > 10000 ? 0 : 2;""")
+
+
+def test_lines(tmp_path):
+    """A line of workgroups is every tile, kv head and share once, the tiles in order."""
+    _run(tmp_path, """
+  for (int tiles : {1, 2, 5, 36, 191})
+    for (int kv_heads : {1, 2, 3, 8, 32})
+      for (int splits : {1, 2, 7, 8, 25, 64}) {
+        std::vector<int> seen(static_cast<size_t>(tiles) * kv_heads * splits, 0);
+        int before = 0;
+        for (int x = 0; x < tiles * kv_heads * splits; ++x) {
+          const Place p = line_place(x, kv_heads, splits);
+          if (p.tile < before || p.tile >= tiles || p.kvh < 0 || p.kvh >= kv_heads || p.split < 0 ||
+              p.split >= splits || seen[(p.tile * kv_heads + p.kvh) * splits + p.split]++)
+            return 1;
+          before = p.tile;
+        }
+      }
+  return split;""")
+
+
+def test_which_batches_lie_in_a_line(tmp_path):
+    """Those for which it was faster than a grid, and none for which it was slower: one row a
+    sequence, one tile a sequence of 8 and 16 bits, and windows that make shares of unlike
+    length without a tile's multiple of eight of them, or (below 16 bits) with empty ones."""
+    _run(tmp_path, """
+  struct Case { int b, n, context, page, heads, kv_heads, window, lines; };
+  // lines: bits of bf16, e4m3, int8, 4 bits
+  const Case cases[] = {
+      {16, 5, 2000, 64, 8, 2, 0, 15},     {64, 5, 4096, 64, 8, 2, 3000, 15},
+      {8, 4, 16000, 64, 16, 2, 0, 15},    {2, 60, 3000, 64, 8, 8, 0, 15},
+      {16, 24, 4000, 64, 8, 8, 0, 15},    {64, 5, 4096, 64, 8, 2, 5000, 15},
+      {32, 20, 4000, 64, 8, 8, 1000, 15}, {64, 1, 4096, 64, 8, 2, 0, 0},
+      {64, 1, 4096, 64, 8, 2, 2048, 0},   {16, 8, 4000, 64, 8, 8, 0, 8},
+      {64, 3, 4096, 64, 8, 2, 2048, 8},   {64, 5, 4096, 64, 16, 2, 2048, 8},
+      {64, 5, 4096, 64, 8, 2, 1000, 1},   {8, 24, 4000, 64, 8, 8, 2048, 1},
+      {32, 5, 4096, 64, 8, 2, 2048, 0},   {48, 5, 4096, 64, 8, 2, 2048, 0},
+      {32, 4, 4096, 64, 16, 2, 1000, 0},  {128, 5, 4096, 64, 8, 2, 2048, 0},
+  };
+  const int types[] = {0, 1, 2, 4};
+  for (const Case& c : cases)
+    for (int i = 0; i < 4; ++i) {
+      const int rows = c.b * c.n, width = (c.context + c.n + c.page - 1) / c.page;
+      const int window = c.window ? c.window : INT32_MAX;
+      const Plan p = plan(types[i], c.b, rows, c.heads, c.kv_heads, c.page, width, window, 0);
+      if (p.tile == kTileRows) continue;  // (these have an order of their own)
+      const bool line = tiles_last(p, types[i], c.b, rows, c.heads / c.kv_heads, c.kv_heads,
+                                   width * c.page, window, 0, 1000);
+      if (line != ((c.lines >> i & 1) != 0)) {
+        std::printf("%d x %d after %d, window %d, type %d: %d\\n", c.b, c.n, c.context, c.window,
+                    types[i], line);
+        ++split;
+      }
+    }
+  return split;""")
