@@ -70,7 +70,6 @@ __device__ __forceinline__ Place place_of(const AttendArgs& a) {
 
 // Where a wavefront's key blocks (every fourth of its workgroup's share) lie among the
 // cache's: lane j holds the j-th of the last 64.
-
 struct WaveBlocks {
   const AttendArgs& a;
   const int sequence, kvh;
@@ -116,8 +115,8 @@ __device__ __forceinline__ Visible visible_to(int query, int stored, int window,
 template <int TYPE>
 constexpr float kUnit = TYPE == kPagedInt8 ? 4.0f : 1.0f;
 
-// 2^(byte - 127) / kUnit as the factor of a piece of K; infinite for a row that is not
-// finite, which the piece's conversion makes NaN.
+// 2^(byte - 127) / kUnit as the factor of a conversion (of K's pieces, and of int8's V);
+// infinite for a row that is not finite, which the conversion makes NaN.
 template <int TYPE>
 __device__ __forceinline__ float piece_power(uint32_t byte) {
   return __uint_as_float(byte << 23) * (1.0f / kUnit<TYPE>);

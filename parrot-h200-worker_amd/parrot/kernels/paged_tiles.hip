@@ -71,8 +71,10 @@ __device__ __forceinline__ bf16x8 value_piece(typename Piece<TYPE>::raw w, const
   return __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
 }
 
-// (4 bits at 96: three workgroups a CU, for which eight registers spill; the two together
-// took 4 prompts of 4096 from 155 us to 150)
+// (4 bits at 96: three workgroups a CU, for which eight registers spill, where the other forms'
+// registers leave two: us with two / three, 8 heads on 2, 4 prompts of 4096 130.7 / 126.6, in a window
+// of 2048 110 / 97.8, 16 of them 470 / 429, 3 chunks of 512 36.5 / 32.5; where CUs stay empty, the other
+// way: 2 prompts 82.1 / 87.1, 8 chunks of 512 77.3 / 78.8)
 template <int TYPE, int D>
 __global__ __launch_bounds__(kWaves * kWave, TYPE == kPagedE2m1 && D == 96 ? 3 : 2)
 void paged_tile_kernel(AttendArgs a) {
@@ -80,7 +82,7 @@ void paged_tile_kernel(AttendArgs a) {
   constexpr int kHalf = 64;                                  // elements between K's halves
   constexpr int kK = kPagedBlock * D + kHalf;                // elements of K, then of V
   constexpr int kBlock = kK + kPagedBlock * D;
-  constexpr int kMatrix = TYPE == kPagedBf16 ? 64 * D : TYPE == kPagedE2m1 ? 16 * D : 32 * D;
+  constexpr int kMatrix = TYPE == kPagedBf16 ? 64 * D : 32 * D;  // (4 bits: by plain loads)
   // 1 KB pieces of a matrix (4 bits: a record a lane, with the first of four quarters)
   constexpr int kLoads = TYPE == kPagedE2m1 ? 4 : kMatrix / (16 * kWave);
   __shared__ __attribute__((aligned(16))) uint16_t stage[2][2][kBlock];  // [buffer][block]
@@ -148,7 +150,8 @@ void paged_tile_kernel(AttendArgs a) {
       at0 = i < end ? __builtin_amdgcn_readlane(ids, j) : -1;
       at1 = i < end ? __builtin_amdgcn_readlane(ids, j + 1) : -1;
       const int at = which ? at1 : at0;
-      from = make_rsrc(matrix + int64_t{max(at, 0)} * kMatrix, at < 0 ? 0 : kMatrix);
+      if constexpr (TYPE != kPagedE2m1)
+        from = make_rsrc(matrix + int64_t{max(at, 0)} * kMatrix, at < 0 ? 0 : kMatrix);
       if constexpr (TYPE == kPagedE2m1) {
         if (at < 0) return;
         load_row_bytes<S>(
@@ -197,7 +200,11 @@ void paged_tile_kernel(AttendArgs a) {
           float power[8], shift[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            power[e] = byte_power(bytes[e >> 2], e & 3) * (1.0f / kUnit<TYPE>);
+            // (int8 values are NaN for an infinity too, as those of K are: 73.8 us for 74.6 for
+            // 2 prompts of 4096, 8 heads of 64)
+            power[e] = TYPE == kPagedInt8
+                           ? piece_power<TYPE>((bytes[e >> 2] >> (8 * (e & 3))) & 0xffu)
+                           : byte_power(bytes[e >> 2], e & 3);
             shift[e] = -128.0f * power[e];
           }
           if constexpr (TYPE == kPagedE2m1) {
