@@ -25,14 +25,17 @@ from torch import Tensor
 from . import _abi
 from .hip_moe import ATTENTION_HEAD_DIMS, _on, _require, _stream
 
-# (torch.cuda.current_device() and current_stream().cuda_stream without their checks)
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# (torch.cuda.current_device() and current_stream().cuda_stream without their checks; a
+# PyTorch without GPU support has neither, and calls neither)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _grads = torch.is_grad_enabled
 
-PAGE_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2,
-              torch.float4_e2m1fn_x2: 4}
-FOUR_BITS = torch.float4_e2m1fn_x2  # an element of such a tensor is two values
+PAGE_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1, torch.int8: 2}
+# an element of such a tensor is two values (None: a PyTorch that does not know the type)
+FOUR_BITS = getattr(torch, "float4_e2m1fn_x2", None)
+if FOUR_BITS is not None:
+    PAGE_TYPES[FOUR_BITS] = 4
 PAGE_BLOCK = 32  # a page is a whole number of blocks of so many positions
 MOST_ROWS = 2 ** 30  # of a step that a pool places
 

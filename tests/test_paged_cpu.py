@@ -1,6 +1,10 @@
 """Argument checks of the paged KV cache, of attention over it and of sampling
 (no GPU)."""
 import ctypes
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -184,3 +188,22 @@ def test_copies_and_pickles():
         assert torch.equal(b.table, d.table) and torch.equal(b.lengths, d.lengths)
         assert d._struct.table == d.table.data_ptr() != b.table.data_ptr()
         assert d._at == ctypes.addressof(d._struct)
+
+
+def test_import_without_gpu_support():
+    """The package is imported, and its caches of the other types described, by a PyTorch
+    that has no GPU support and does not know 4-bit floats."""
+    code = """
+import torch
+for name in [x for x in dir(torch._C) if x.startswith("_cuda_")]:
+    delattr(torch._C, name)
+del torch.float4_e2m1fn_x2
+from parrot import ModelConfig, PagedBatch, PagedKVCache, PagePool, Parrot
+cache = PagedKVCache(2, 64, 2, 96, torch.int8, device="cpu")
+assert cache._batch(PagedBatch.from_lists([[0]], [5], [1], device="cpu")) and PagePool(3, 32, device="cpu")
+"""
+    import parrot
+    path = str(Path(parrot.__file__).resolve().parent.parent)
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
+                          env={**os.environ, "PYTHONPATH": path})
+    assert done.returncode == 0, done.stderr
