@@ -18,8 +18,10 @@
 // (the registers spill).
 //
 // Of 4-bit pages (9 to 96 rows a sequence; paged_step4.hip has fewer) a block is a quarter of
-// the registers, and two are on their way ahead of the one in hand: 8 sequences of 32000 keys
-// 14.8 us, with one 17.1.  5 sequences of 48 rows over up to 9000 keys, 16 heads on 2 of 128: 12.4
+// the registers, and two are on their way ahead of the one in hand.  Measured, join included, two
+// / one: 8 sequences of 32 rows after 32000 keys, 8 heads on 2 of 96, 24.4 / 25.1 us, 5 of 96 rows after
+// 9000, 16 heads on 2 of 128, 19.8 / 20.1, 5 ragged of 48 14.7 / 15.0, 8 of 32 after 16000 20.6 / 20.5, but
+// 64 of 20 after 4096, 8 heads on 2 of 96, 26.9 / 25.2.  5 sequences of 48 rows over up to 9000 keys, 16 heads on 2 of 128: 12.4
 // us at three blocks a wavefront, and the join 4.0.
 #include "paged_attention.h"
 
